@@ -628,6 +628,36 @@ int tc_fused_compiled(uint64_t* count);
  * reference's interface: a diagnostic and tuning hook, for tests. */
 int tc_fused_resident(uint64_t limit, uint64_t* resident, uint64_t* current_limit);
 
+/* ---- layer norm ----------------------------------------------------------
+ *
+ * This and the sections below are operators that a network trained on tokens
+ * needs beside its products and its optimizer.  The reference has none of
+ * them; they follow this header's conventions.  Steps between rows are in
+ * elements; rows may start at any element, and a base pointer need only be
+ * aligned to its element. */
+
+/* Of each of the `rows` rows x of `cols` elements, `x_step` apart:
+ *   y = (x - mean) * scale * weight + bias,
+ *   scale = 1 / sqrt(variance + epsilon), the variance the population's
+ * in f32, rounded to `dtype` once.  `weight` and `bias` hold `cols` elements
+ * of `weight_dtype` (`dtype`, or TC_F32); either may be null (1, or 0).
+ * `means` and `scales` receive each row's f32 statistics for the backward
+ * pass, and may be null.  y may be x itself (with the same step), not
+ * otherwise overlap it.  Rows of no elements are refused. */
+int tc_layer_norm(uint32_t dtype, uint32_t weight_dtype, const void* x, uint64_t x_step, uint64_t rows, uint64_t cols,
+                  const void* weight, const void* bias, float epsilon, void* y, uint64_t y_step, float* means,
+                  float* scales);
+
+/* The gradients from `dy` and the forward pass's `x`, `means` and `scales`:
+ * `dx` (which may be `dy` itself, with the same step), and the sums over all
+ * rows `dweight` and `dbias`, of `cols` elements of `weight_dtype`.  Any of
+ * the three may be null and is then left out; `weight` null is a weight of 1.
+ * The sums are taken in an order that depends on the shape alone.  With no
+ * rows, `dweight` and `dbias` are zeros. */
+int tc_layer_norm_backward(uint32_t dtype, uint32_t weight_dtype, const void* dy, uint64_t dy_step, const void* x,
+                           uint64_t x_step, uint64_t rows, uint64_t cols, const void* weight, const float* means,
+                           const float* scales, void* dx, uint64_t dx_step, void* dweight, void* dbias);
+
 #ifdef __cplusplus
 }
 #endif

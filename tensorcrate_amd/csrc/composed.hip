@@ -30,23 +30,10 @@
 
 #include <string.h>
 
-#include "common.hpp"
+#include "rows.hpp"
 
 namespace tc {
 namespace {
-
-// A scratch block freed when it leaves scope (stream order keeps it alive
-// until the queued work has read it).
-struct Scratch {
-    void* ptr = nullptr;
-    int status = TC_OK;
-    explicit Scratch(uint64_t bytes) { status = tc_alloc(bytes, &ptr); }
-    ~Scratch() {
-        if (ptr != nullptr) tc_free(ptr);
-    }
-    Scratch(const Scratch&) = delete;
-    Scratch& operator=(const Scratch&) = delete;
-};
 
 int fill_nan(uint32_t dtype, void* out, uint64_t n) {
     if (n == 0) return TC_OK;

@@ -1,0 +1,605 @@
+// Layer norm of rows and its gradients.
+//
+// Forward, of a row x of n elements, with weight w and bias b:
+//   m = mean(x),  s = 1 / sqrt(mean((x - m)^2) + epsilon),  y = (x - m) s w + b
+// Backward, with u = (x - m) s and g = dy w:
+//   dx = s (g - mean(g) - u mean(g u)),  dw = sum over rows dy u,
+//   db = sum over rows dy
+// Both are bound by memory: the forward pass reads x once and writes y once,
+// the backward pass reads dy and x once and writes dx once.  So a row is held
+// in registers from its one read on, by 16 lanes, a wave or a block, and the
+// variance is the second sum over those registers (exact about the mean, where
+// a sum of squares would cancel).  A group of lanes walks rows a grid apart
+// with the next row's words already in flight, and keeps its columns' weights.
+//
+// dw and db are sums over all rows: a lane sums its columns over the rows of
+// its walk in registers, each block writes those sums once, and a second
+// kernel adds the blocks' in block order, so the result does not depend on
+// timing.  Everything is summed in f32 and rounded to its type once.
+
+#include "rows.hpp"
+
+namespace tc {
+namespace {
+
+constexpr uint32_t kMostLanes = 1024;  // of a block
+constexpr int kMostHeld = 16;          // elements of a row that one lane holds
+
+template <typename W, int E, int VECTORS>
+struct Columns {
+    Words<W, E> words[VECTORS];
+
+    __device__ __forceinline__ void load(const W* from, const Run<E> (&runs)[VECTORS]) {
+#pragma unroll
+        for (int v = 0; v < VECTORS; v++) {
+            if (runs[v].live()) runs[v].template load<false>(from, words[v]);
+        }
+    }
+};
+
+// LANES lanes a row: 16 or 64, several rows a block, or 0 for the block.
+template <typename S, typename W, int LANES, int VECTORS, bool NT>
+__global__ void __launch_bounds__(LANES ? 256 : kMostLanes)
+    norm_kernel(const S* x, uint64_t x_step, uint64_t rows, uint64_t cols, const W* weight, const W* bias,
+                float epsilon, S* y, uint64_t y_step, float* means, float* scales) {
+    constexpr int E = kWordElements<S>;
+    __shared__ float shared[2][kMostWaves];
+    const uint32_t lanes = LANES ? LANES : blockDim.x;
+    const uint32_t lane = threadIdx.x % lanes;
+    const uint64_t groups = static_cast<uint64_t>(gridDim.x) * (blockDim.x / lanes);
+    uint64_t row = static_cast<uint64_t>(blockIdx.x) * (blockDim.x / lanes) + threadIdx.x / lanes;
+    if (row >= rows) return;  // the whole group
+
+    Run<E> runs[VECTORS];
+#pragma unroll
+    for (int v = 0; v < VECTORS; v++) runs[v] = Run<E>(lane + static_cast<uint64_t>(v) * lanes, cols);
+    Columns<W, E, VECTORS> w, b;
+    if (weight != nullptr) w.load(weight, runs);
+    if (bias != nullptr) b.load(bias, runs);
+
+    const float count = static_cast<float>(cols);
+    Words<S, E> next[VECTORS];
+#pragma unroll
+    for (int v = 0; v < VECTORS; v++) {
+        if (runs[v].live()) runs[v].template load<NT>(x + row * x_step, next[v]);
+    }
+    for (; row < rows; row += groups) {
+        float value[VECTORS][E];
+        float sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < VECTORS; v++) {
+            if (!runs[v].live()) continue;
+            next[v].get(value[v]);
+            float part = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; e++) part += value[v][e];
+            if (runs[v].partial()) {
+                part = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; e++) part += runs[v].own(e) ? value[v][e] : 0.0f;
+            }
+            sum += part;
+        }
+        if (row + groups < rows) {
+#pragma unroll
+            for (int v = 0; v < VECTORS; v++) {
+                if (runs[v].live()) runs[v].template load<NT>(x + (row + groups) * x_step, next[v]);
+            }
+        }
+        const float mean = row_join<LANES, Added>(sum, shared[0]) / count;
+        float squares = 0.0f;
+#pragma unroll
+        for (int v = 0; v < VECTORS; v++) {
+            if (!runs[v].live()) continue;
+            float part = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                value[v][e] -= mean;
+                part = fmaf(value[v][e], value[v][e], part);
+            }
+            if (runs[v].partial()) {
+                part = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; e++) part += runs[v].own(e) ? value[v][e] * value[v][e] : 0.0f;
+            }
+            squares += part;
+        }
+        const float scale = 1.0f / sqrtf(row_join<LANES, Added>(squares, shared[1]) / count + epsilon);
+#pragma unroll
+        for (int v = 0; v < VECTORS; v++) {
+            if (!runs[v].live()) continue;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                value[v][e] *= scale;
+                if (weight != nullptr) value[v][e] *= w.words[v].at(e);
+                if (bias != nullptr) value[v][e] += b.words[v].at(e);
+            }
+            runs[v].template store<NT>(y + row * y_step, value[v]);
+        }
+        if (lane == 0) {
+            if (means != nullptr) means[row] = mean;
+            if (scales != nullptr) scales[row] = scale;
+        }
+    }
+}
+
+// Rows longer than a block's registers: a block a row, which it reads three
+// times (from the caches, mostly).  Elements are read and written one by one
+// at a row's ragged end, so that y may be x.
+template <typename S, typename W>
+__global__ void __launch_bounds__(kMostLanes)
+    norm_long_kernel(const S* x, uint64_t x_step, uint64_t rows, uint64_t cols, const W* weight, const W* bias,
+                     float epsilon, S* y, uint64_t y_step, float* means, float* scales) {
+    constexpr int E = kWordElements<S>;
+    __shared__ float shared[2][kMostWaves];
+    const uint64_t whole = cols / E * E;
+    const float count = static_cast<float>(cols);
+    for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const S* from = x + row * x_step;
+        S* to = y + row * y_step;
+        const auto each = [&](auto&& body) {
+            for (uint64_t at = static_cast<uint64_t>(threadIdx.x) * E; at < whole; at += uint64_t{blockDim.x} * E) {
+                Words<S, E> words;
+                words.template load<false>(from + at);
+                float v[E];
+                words.get(v);
+                body(at, v, E);
+            }
+            if (threadIdx.x < cols - whole) {
+                float v[E] = {Elem<S>::widen(from[whole + threadIdx.x])};
+                body(whole + threadIdx.x, v, 1);
+            }
+        };
+        float sum = 0.0f;
+        each([&](uint64_t, float (&v)[E], int n) {
+#pragma unroll
+            for (int e = 0; e < E; e++) sum += e < n ? v[e] : 0.0f;
+        });
+        const float mean = block_join<Added>(sum, shared[0]) / count;
+        float squares = 0.0f;
+        each([&](uint64_t, float (&v)[E], int n) {
+#pragma unroll
+            for (int e = 0; e < E; e++) squares += e < n ? (v[e] - mean) * (v[e] - mean) : 0.0f;
+        });
+        const float scale = 1.0f / sqrtf(block_join<Added>(squares, shared[1]) / count + epsilon);
+        each([&](uint64_t at, float (&v)[E], int n) {
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                if (e >= n) continue;
+                v[e] = (v[e] - mean) * scale;
+                if (weight != nullptr) v[e] *= Elem<W>::widen(weight[at + e]);
+                if (bias != nullptr) v[e] += Elem<W>::widen(bias[at + e]);
+            }
+            if (n == E) {
+                Words<S, E> words;
+                words.put(v);
+                words.template store<false>(to + at);
+            } else {
+                to[at] = Elem<S>::narrow(v[0]);
+            }
+        });
+        if (threadIdx.x == 0) {
+            if (means != nullptr) means[row] = mean;
+            if (scales != nullptr) scales[row] = scale;
+        }
+    }
+}
+
+// The gradients.  `partial` (null if neither dw nor db is wanted) holds, for
+// each block, cols sums of dy u and then cols sums of dy.
+template <typename S, typename W, int LANES, int VECTORS, bool NT>
+__global__ void __launch_bounds__(LANES ? 256 : kMostLanes)
+    norm_back_kernel(const S* dy, uint64_t dy_step, const S* x, uint64_t x_step,
+                     uint64_t rows, uint64_t cols, const W* weight, const float* __restrict__ means,
+                     const float* __restrict__ scales, S* dx, uint64_t dx_step, float* __restrict__ partial) {
+    constexpr int E = kWordElements<S>;
+    __shared__ float shared[2][2][kMostWaves];
+    const uint32_t lanes = LANES ? LANES : blockDim.x;
+    const uint32_t lane = threadIdx.x % lanes;
+    const uint64_t groups = static_cast<uint64_t>(gridDim.x) * (blockDim.x / lanes);
+    uint64_t row = static_cast<uint64_t>(blockIdx.x) * (blockDim.x / lanes) + threadIdx.x / lanes;
+
+    Run<E> runs[VECTORS];
+#pragma unroll
+    for (int v = 0; v < VECTORS; v++) runs[v] = Run<E>(lane + static_cast<uint64_t>(v) * lanes, cols);
+    Columns<W, E, VECTORS> w;
+    if (weight != nullptr) w.load(weight, runs);
+    float dw[VECTORS][E] = {}, db[VECTORS][E] = {};
+
+    Words<S, E> next_x[VECTORS], next_dy[VECTORS];
+    float next_mean = 0.0f, next_scale = 0.0f;
+    const auto fetch = [&](uint64_t at) {
+#pragma unroll
+        for (int v = 0; v < VECTORS; v++) {
+            if (!runs[v].live()) continue;
+            runs[v].template load<NT>(x + at * x_step, next_x[v]);
+            runs[v].template load<NT>(dy + at * dy_step, next_dy[v]);
+        }
+        next_mean = means[at];
+        next_scale = scales[at];
+    };
+    // The next row's words are in flight while this one's are worked on,
+    // where the registers allow both.
+    constexpr bool AHEAD = VECTORS == 1;
+    if (AHEAD && row < rows) fetch(row);
+    int turn = 0;
+    for (; row < rows; row += groups) {
+        if (!AHEAD) fetch(row);
+        const float mean = next_mean, scale = next_scale;
+        float u[VECTORS][E], g[VECTORS][E];
+        float sum = 0.0f, along = 0.0f;
+#pragma unroll
+        for (int v = 0; v < VECTORS; v++) {
+            if (!runs[v].live()) continue;
+            next_x[v].get(u[v]);
+            next_dy[v].get(g[v]);
+            if (runs[v].partial()) {
+                // Neighbours' elements and those past a short row: nothing
+                // to the sums, and mean(g) is all that dx needs of them.
+                float one = 0.0f, two = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    u[v][e] = (u[v][e] - mean) * scale;
+                    if (runs[v].own(e)) {
+                        dw[v][e] = fmaf(g[v][e], u[v][e], dw[v][e]);
+                        db[v][e] += g[v][e];
+                    }
+                    if (weight != nullptr) g[v][e] *= w.words[v].at(e);
+                    if (runs[v].own(e)) {
+                        one += g[v][e];
+                        two = fmaf(g[v][e], u[v][e], two);
+                    }
+                }
+                sum += one;
+                along += two;
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    u[v][e] = (u[v][e] - mean) * scale;
+                    dw[v][e] = fmaf(g[v][e], u[v][e], dw[v][e]);
+                    db[v][e] += g[v][e];
+                    if (weight != nullptr) g[v][e] *= w.words[v].at(e);
+                    sum += g[v][e];
+                    along = fmaf(g[v][e], u[v][e], along);
+                }
+            }
+        }
+        if (AHEAD && row + groups < rows) fetch(row + groups);
+        if (dx == nullptr) continue;
+        if constexpr (LANES == 0) {
+            // Both sums past one barrier, in buffers that alternate.
+            sum = wave64<Added>(sum);
+            along = wave64<Added>(along);
+            const int waves = blockDim.x / 64;
+            if (waves > 1) {
+                float(&at)[2][kMostWaves] = shared[turn];
+                turn ^= 1;
+                if (threadIdx.x % 64 == 0) {
+                    at[0][threadIdx.x / 64] = sum;
+                    at[1][threadIdx.x / 64] = along;
+                }
+                __syncthreads();
+                sum = at[0][0];
+                along = at[1][0];
+                for (int k = 1; k < waves; k++) {
+                    sum += at[0][k];
+                    along += at[1][k];
+                }
+            }
+        } else {
+            sum = row_join<LANES, Added>(sum, nullptr);
+            along = row_join<LANES, Added>(along, nullptr);
+        }
+        const float mean_g = sum / static_cast<float>(cols), mean_gu = along / static_cast<float>(cols);
+#pragma unroll
+        for (int v = 0; v < VECTORS; v++) {
+            if (!runs[v].live()) continue;
+#pragma unroll
+            for (int e = 0; e < E; e++) g[v][e] = scale * (g[v][e] - mean_g - u[v][e] * mean_gu);
+            runs[v].template store<NT>(dx + row * dx_step, g[v]);
+        }
+    }
+    if (partial == nullptr) return;
+
+    float* sums = partial + static_cast<uint64_t>(blockIdx.x) * 2 * cols;
+    if constexpr (LANES == 0) {
+#pragma unroll
+        for (int v = 0; v < VECTORS; v++) {
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                if (!runs[v].own(e)) continue;
+                sums[runs[v].start + e] = dw[v][e];
+                sums[cols + runs[v].start + e] = db[v][e];
+            }
+        }
+    } else {
+        // The block's groups hold the same columns: added in group order.
+        __shared__ float turns[256 * VECTORS * E];
+        const int groups_here = 256 / LANES;
+        for (int which = 0; which < 2; which++) {
+            if (which) __syncthreads();
+#pragma unroll
+            for (int v = 0; v < VECTORS; v++) {
+#pragma unroll
+                for (int e = 0; e < E; e++) turns[(v * E + e) * 256 + threadIdx.x] = which ? db[v][e] : dw[v][e];
+            }
+            __syncthreads();
+            // A group's lanes hold VECTORS x E values each: value k of lane l.
+            for (int at = threadIdx.x; at < LANES * VECTORS * E; at += 256) {
+                const int l = at % LANES, k = at / LANES;
+                const Run<E> run(l + static_cast<uint64_t>(k / E) * LANES, cols);
+                if (!run.own(k % E)) continue;
+                float all = 0.0f;
+                for (int q = 0; q < groups_here; q++) all += turns[k * 256 + q * LANES + l];
+                sums[which * cols + run.start + k % E] = all;
+            }
+        }
+    }
+}
+
+// Rows longer than a block's registers: dx, a block a row read twice.
+template <typename S, typename W>
+__global__ void __launch_bounds__(kMostLanes)
+    norm_back_long_kernel(const S* dy, uint64_t dy_step, const S* x, uint64_t x_step, uint64_t rows,
+                          uint64_t cols, const W* weight, const float* __restrict__ means,
+                          const float* __restrict__ scales, S* dx, uint64_t dx_step) {
+    __shared__ float shared[2][kMostWaves];
+    const float count = static_cast<float>(cols);
+    for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const float mean = means[row], scale = scales[row];
+        float sum = 0.0f, along = 0.0f;
+        for (uint64_t c = threadIdx.x; c < cols; c += blockDim.x) {
+            const float g = Elem<S>::widen(dy[row * dy_step + c]) * (weight != nullptr ? Elem<W>::widen(weight[c]) : 1.0f);
+            sum += g;
+            along += g * ((Elem<S>::widen(x[row * x_step + c]) - mean) * scale);
+        }
+        sum = block_join<Added>(sum, shared[0]) / count;
+        along = block_join<Added>(along, shared[1]) / count;
+        for (uint64_t c = threadIdx.x; c < cols; c += blockDim.x) {
+            const float g = Elem<S>::widen(dy[row * dy_step + c]) * (weight != nullptr ? Elem<W>::widen(weight[c]) : 1.0f);
+            const float u = (Elem<S>::widen(x[row * x_step + c]) - mean) * scale;
+            dx[row * dx_step + c] = Elem<S>::narrow(scale * (g - sum - u * along));
+        }
+        __syncthreads();  // the next row writes `shared` again
+    }
+}
+
+// ... and their dw and db: a lane a column, blockIdx.y a share of the rows.
+template <typename S>
+__global__ void __launch_bounds__(256)
+    norm_back_columns_kernel(const S* __restrict__ dy, uint64_t dy_step, const S* __restrict__ x, uint64_t x_step,
+                             uint64_t rows, uint64_t cols, const float* __restrict__ means,
+                             const float* __restrict__ scales, float* __restrict__ partial) {
+    const uint64_t c = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (c >= cols) return;
+    float dw = 0.0f, db = 0.0f;
+    for (uint64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+        const float g = Elem<S>::widen(dy[row * dy_step + c]);
+        dw = fmaf(g, (Elem<S>::widen(x[row * x_step + c]) - means[row]) * scales[row], dw);
+        db += g;
+    }
+    float* sums = partial + static_cast<uint64_t>(blockIdx.y) * 2 * cols;
+    sums[c] = dw;
+    sums[cols + c] = db;
+}
+
+// out[c] = the sum over `parts` of partial[part][c] in a fixed order, for the
+// 2 x cols columns: 16 lanes of every 64 columns each take every 16th part.
+template <typename W>
+__global__ void __launch_bounds__(1024)
+    add_parts_kernel(const float* __restrict__ partial, uint32_t parts, uint64_t cols, W* dweight, W* dbias) {
+    __shared__ float shared[16][64];
+    const uint64_t c = static_cast<uint64_t>(blockIdx.x) * 64 + threadIdx.x % 64;
+    const uint32_t turn = threadIdx.x / 64;
+    float sum = 0.0f;
+    if (c < 2 * cols) {
+#pragma unroll 8
+        for (uint32_t p = turn; p < parts; p += 16) sum += partial[static_cast<uint64_t>(p) * 2 * cols + c];
+    }
+    shared[turn][threadIdx.x % 64] = sum;
+    __syncthreads();
+    if (turn != 0 || c >= 2 * cols) return;
+#pragma unroll
+    for (int k = 1; k < 16; k++) sum += shared[k][threadIdx.x];
+    W* out = c < cols ? dweight : dbias;
+    if (out != nullptr) out[c < cols ? c : c - cols] = Elem<W>::narrow(sum);
+}
+
+// How the lanes are laid over rows of `cols` elements, `run` of them a
+// 16-byte word: the fewest words a lane.
+struct Layout {
+    int lanes = 0;         // 16, 64, or 0 for a block of `threads`
+    int vectors = 0;       // words a lane: 1, 2 or 4; 0 for rows too long for registers
+    uint32_t threads = 0;  // of a block
+};
+
+Layout layout_of(uint64_t cols, int run) {
+    const uint64_t words = (cols + run - 1) / run;
+    Layout out;
+    out.threads = 256;
+    if (words <= 64) {
+        out.lanes = words <= 16 ? 16 : 64;
+        out.vectors = 1;
+        return out;
+    }
+    out.vectors = 1;
+    while (words > uint64_t{kMostLanes} * out.vectors) {
+        out.vectors *= 2;
+        if (out.vectors * run > kMostHeld) {
+            out.vectors = 0, out.threads = kMostLanes;
+            return out;
+        }
+    }
+    out.threads = static_cast<uint32_t>(((words + out.vectors - 1) / out.vectors + 63) / 64 * 64);
+    return out;
+}
+
+uint32_t blocks_of(const Layout& layout, uint64_t rows, uint32_t threads_per_cu) {
+    const uint64_t per_block = layout.lanes ? 256 / layout.lanes : 1;
+    const uint64_t wanted = (rows + per_block - 1) / per_block;
+    const uint64_t most = static_cast<uint64_t>(compute_units()) * (threads_per_cu > layout.threads ? threads_per_cu / layout.threads : 1);
+    return static_cast<uint32_t>(wanted < most ? wanted : most);
+}
+
+// The body with LANES and VECTORS of the layout (four words a lane only for
+// f32, where they are 16 elements).
+#define TC_NORM_FORM(layout, S, ...)                                     \
+    if (layout.lanes == 16) {                                            \
+        constexpr int LANES = 16, VECTORS = 1; __VA_ARGS__;              \
+    } else if (layout.lanes == 64) {                                     \
+        constexpr int LANES = 64, VECTORS = 1; __VA_ARGS__;              \
+    } else if (layout.vectors == 1) {                                    \
+        constexpr int LANES = 0, VECTORS = 1; __VA_ARGS__;               \
+    } else if (layout.vectors == 2) {                                    \
+        constexpr int LANES = 0, VECTORS = 2; __VA_ARGS__;               \
+    } else {                                                             \
+        constexpr int LANES = 0, VECTORS = kMostHeld / kWordElements<S>; \
+        __VA_ARGS__;                                                     \
+    }
+
+template <typename S, typename W>
+int norm(const S* x, uint64_t x_step, uint64_t rows, uint64_t cols, const W* weight, const W* bias, float epsilon,
+         S* y, uint64_t y_step, float* means, float* scales) {
+    TC_STREAM(s);
+    const Layout layout = layout_of(cols, kWordElements<S>);
+    if (layout.vectors == 0) {
+        norm_long_kernel<S, W><<<grid_for(rows, 1, 2), kMostLanes, 0, s>>>(x, x_step, rows, cols, weight, bias,
+                                                                          epsilon, y, y_step, means, scales);
+        return check_launch("layer norm");
+    }
+    const uint32_t blocks = blocks_of(layout, rows, 2048);
+    const bool streams = 2 * sizeof(S) * rows * cols > kStreamBytes;
+    TC_NORM_FORM(layout, S, {
+        if (streams) {
+            norm_kernel<S, W, LANES, VECTORS, true><<<blocks, layout.threads, 0, s>>>(
+                x, x_step, rows, cols, weight, bias, epsilon, y, y_step, means, scales);
+        } else {
+            norm_kernel<S, W, LANES, VECTORS, false><<<blocks, layout.threads, 0, s>>>(
+                x, x_step, rows, cols, weight, bias, epsilon, y, y_step, means, scales);
+        }
+    })
+    return check_launch("layer norm");
+}
+
+template <typename S, typename W>
+int norm_back(const S* dy, uint64_t dy_step, const S* x, uint64_t x_step, uint64_t rows, uint64_t cols,
+              const W* weight, const float* means, const float* scales, S* dx, uint64_t dx_step, W* dweight,
+              W* dbias) {
+    TC_STREAM(s);
+    const bool columns = dweight != nullptr || dbias != nullptr;
+    const Layout layout = layout_of(cols, kWordElements<S>);
+    const uint32_t row_blocks =
+        layout.vectors == 0 ? grid_for(rows, 64, 1) : blocks_of(layout, rows, 1024);
+    const uint32_t parts = rows == 0 ? 0 : row_blocks;
+    Scratch partial(columns ? uint64_t{parts} * 2 * cols * sizeof(float) : 0);
+    if (partial.status != TC_OK) return partial.status;
+    float* sums = columns ? static_cast<float*>(partial.ptr) : nullptr;
+    int status = TC_OK;
+    if (rows > 0 && layout.vectors == 0) {
+        if (columns) {
+            const dim3 grid(static_cast<uint32_t>((cols + 255) / 256), parts);
+            norm_back_columns_kernel<S><<<grid, 256, 0, s>>>(dy, dy_step, x, x_step, rows, cols, means, scales, sums);
+            status = check_launch("layer norm, backward");
+        }
+        if (status == TC_OK && dx != nullptr) {
+            norm_back_long_kernel<S, W><<<grid_for(rows, 1, 2), kMostLanes, 0, s>>>(
+                dy, dy_step, x, x_step, rows, cols, weight, means, scales, dx, dx_step);
+            status = check_launch("layer norm, backward");
+        }
+    } else if (rows > 0) {
+        const bool streams = 3 * sizeof(S) * rows * cols > kStreamBytes;
+        TC_NORM_FORM(layout, S, {
+            if (streams) {
+                norm_back_kernel<S, W, LANES, VECTORS, true><<<row_blocks, layout.threads, 0, s>>>(
+                    dy, dy_step, x, x_step, rows, cols, weight, means, scales, dx, dx_step, sums);
+            } else {
+                norm_back_kernel<S, W, LANES, VECTORS, false><<<row_blocks, layout.threads, 0, s>>>(
+                    dy, dy_step, x, x_step, rows, cols, weight, means, scales, dx, dx_step, sums);
+            }
+        })
+        status = check_launch("layer norm, backward");
+    }
+    if (status != TC_OK || !columns) return status;
+    add_parts_kernel<W><<<static_cast<uint32_t>((2 * cols + 63) / 64), 1024, 0, s>>>(sums, parts, cols, dweight, dbias);
+    return check_launch("layer norm, backward");
+}
+
+// The checks both passes share.
+int check_norm(const char* what, uint32_t dtype, uint32_t weight_dtype, uint64_t rows, uint64_t cols,
+               std::initializer_list<uint64_t> steps) {
+    if (dtype_size(dtype) == 0 || dtype == TC_F64) {
+        return fail(TC_UNSUPPORTED, std::string(what) + ": no kernel for " + dtype_name(dtype));
+    }
+    if (weight_dtype != dtype && weight_dtype != TC_F32) {
+        return fail(TC_UNSUPPORTED, std::string(what) + ": no kernel for " + dtype_name(dtype) + " rows with a " +
+                                        dtype_name(weight_dtype) + " weight");
+    }
+    for (uint64_t step : steps) {
+        if (rows > 1 && step < cols) {
+            return fail(TC_INVALID, std::string(what) + ": rows of " + std::to_string(cols) + " elements " +
+                                        std::to_string(step) + " apart overlap");
+        }
+        if (rows > 0 && step > UINT64_MAX / 8 / rows) {
+            return fail(TC_INVALID, std::string(what) + ": " + std::to_string(rows) + " rows " +
+                                        std::to_string(step) + " apart reach past the address space");
+        }
+    }
+    if (cols != 0 && rows > UINT64_MAX / 8 / cols) {
+        return fail(TC_INVALID, std::string(what) + ": shape [" + std::to_string(rows) + ", " + std::to_string(cols) +
+                                    "] has more elements than fit in a usize");
+    }
+    if (cols > (uint64_t{1} << 31)) {
+        return fail(TC_UNSUPPORTED, std::string(what) + ": rows of " + std::to_string(cols) + " elements");
+    }
+    return TC_OK;
+}
+
+}  // namespace
+}  // namespace tc
+
+using namespace tc;
+
+// `f(S rows' type, W weight's type)` for the two type codes.
+#define TC_NORM_TYPES(dtype, weight_dtype, what, ...)                    \
+    TC_DISPATCH_FLOAT(dtype, what, S, {                                  \
+        if (weight_dtype == TC_F32) {                                    \
+            using W = float; __VA_ARGS__;                                \
+        } else {                                                         \
+            using W = S; __VA_ARGS__;                                    \
+        }                                                                \
+    })
+
+extern "C" {
+
+int tc_layer_norm(uint32_t dtype, uint32_t weight_dtype, const void* x, uint64_t x_step, uint64_t rows, uint64_t cols,
+                  const void* weight, const void* bias, float epsilon, void* y, uint64_t y_step, float* means,
+                  float* scales) {
+    const int status = check_norm("layer norm", dtype, weight_dtype, rows, cols, {x_step, y_step});
+    if (status != TC_OK) return status;
+    if (rows == 0) return TC_OK;
+    if (cols == 0) return fail(TC_INVALID, "layer norm: rows of no elements");
+    if (any_null({x, y})) return null_operand("layer norm");
+    TC_NORM_TYPES(dtype, weight_dtype, "layer norm",
+                  return norm<S, W>(static_cast<const S*>(x), x_step, rows, cols, static_cast<const W*>(weight),
+                                    static_cast<const W*>(bias), epsilon, static_cast<S*>(y), y_step, means, scales))
+    return TC_OK;
+}
+
+int tc_layer_norm_backward(uint32_t dtype, uint32_t weight_dtype, const void* dy, uint64_t dy_step, const void* x,
+                           uint64_t x_step, uint64_t rows, uint64_t cols, const void* weight, const float* means,
+                           const float* scales, void* dx, uint64_t dx_step, void* dweight, void* dbias) {
+    const char* what = "layer norm, backward";
+    const int status = check_norm(what, dtype, weight_dtype, rows, cols, {dy_step, x_step, dx != nullptr ? dx_step : cols});
+    if (status != TC_OK) return status;
+    if (cols == 0) return rows == 0 ? TC_OK : fail(TC_INVALID, std::string(what) + ": rows of no elements");
+    if (rows > 0 && any_null({dy, x, means, scales})) return null_operand(what);
+    if (dx == nullptr && dweight == nullptr && dbias == nullptr) return TC_OK;
+    if (rows == 0 && dweight == nullptr && dbias == nullptr) return TC_OK;
+    TC_NORM_TYPES(dtype, weight_dtype, what,
+                  return norm_back<S, W>(static_cast<const S*>(dy), dy_step, static_cast<const S*>(x), x_step, rows,
+                                         cols, static_cast<const W*>(weight), means, scales, static_cast<S*>(dx),
+                                         dx_step, static_cast<W*>(dweight), static_cast<W*>(dbias)))
+    return TC_OK;
+}
+
+}  // extern "C"

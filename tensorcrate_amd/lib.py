@@ -199,6 +199,8 @@ SIGNATURES = {
     "tc_matmul_epilogue": [u32, ctypes.POINTER(Encoded), u32, ctypes.POINTER(Place), u32, u64, u64, u64, vp, vp,
                            ctypes.POINTER(vp), ctypes.POINTER(u64), u32, ctypes.POINTER(vp), ctypes.POINTER(u64),
                            u32],
+    "tc_layer_norm": [u32, u32, vp, u64, u64, u64, vp, vp, f32, vp, u64, vp, vp],
+    "tc_layer_norm_backward": [u32, u32, vp, u64, vp, u64, u64, u64, vp, vp, vp, vp, u64, vp, vp],
 }
 
 

@@ -1,0 +1,84 @@
+"""Plain implementations of the language-model operators in 64 bits, written
+from their formulas, and what the tests of them share."""
+
+from __future__ import annotations
+
+import numpy as np
+
+from tensorcrate_amd import lib
+from tests.common import to_kind, widen
+
+# The relative rounding of one result to its type.
+ROUNDING = {lib.F32: 2.0**-24, lib.F16: 2.0**-11, lib.BF16: 2.0**-8}
+# The smallest steps of a type around zero, half of them a rounding's error.
+TINY = {lib.F32: 2.0**-149, lib.F16: 2.0**-25, lib.BF16: 2.0**-134}
+EPSILON_32 = 2.0**-24
+
+
+def stored(values, kind) -> np.ndarray:
+    """`values` as `kind` holds them, in 64 bits."""
+    return widen(kind, to_kind(np.asarray(values, np.float32), kind)).astype(np.float64)
+
+
+class Rows:
+    """Rows of one kind on the device, `gap` elements between them and `shift`
+    elements before the first, all of it filled with `around`."""
+
+    def __init__(self, values, kind, gap=0, shift=0, around=np.nan):
+        values = np.asarray(values, np.float32)
+        self.rows, self.cols = values.shape
+        self.kind, self.step, self.shift = kind, self.cols + gap, shift
+        self.whole = np.full(shift + self.rows * self.step + 8, around, np.float32)
+        for row in range(self.rows):
+            at = shift + row * self.step
+            self.whole[at:at + self.cols] = values[row]
+        self.buffer = lib.Buffer.of(to_kind(self.whole, kind))
+
+    @classmethod
+    def empty(cls, rows, cols, kind, gap=0, shift=0):
+        return cls(np.full((rows, cols), 7.0), kind, gap, shift, around=7.0)
+
+    @property
+    def ptr(self) -> int:
+        return self.buffer.ptr + self.shift * lib.DTYPE_SIZE[self.kind]
+
+    def read(self) -> np.ndarray:
+        """The rows; what lies around them has to be as it was."""
+        got = widen(self.kind, self.buffer.download(lib.NUMPY_TYPE[self.kind]))
+        inside = np.zeros(got.size, bool)
+        out = np.empty((self.rows, self.cols), np.float64)
+        for row in range(self.rows):
+            at = self.shift + row * self.step
+            inside[at:at + self.cols] = True
+            out[row] = got[at:at + self.cols]
+        before = widen(self.kind, to_kind(self.whole, self.kind))
+        assert np.array_equal(got[~inside], before[~inside], equal_nan=True), "written outside the rows"
+        return out
+
+
+def near(got, want, bound, what: str) -> None:
+    """Every value within its own bound; infinities and NaNs where they are wanted."""
+    got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
+    assert got.shape == want.shape, what
+    special = ~np.isfinite(want)
+    assert np.array_equal(got[special], want[special], equal_nan=True), what
+    off = np.abs(got - want)[~special]
+    most = np.broadcast_to(np.asarray(bound, np.float64), want.shape)[~special]
+    bad = ~(off <= most)
+    assert not bad.any(), f"{what}: {bad.sum()} of {bad.size} off, by up to {np.nanmax(off[bad] / np.maximum(most[bad], 1e-300)):.3g} bounds"
+
+
+# ---- layer norm -------------------------------------------------------------
+
+
+def layer_norm(x, weight, bias, epsilon):
+    mean = x.mean(1, keepdims=True)
+    scale = 1.0 / np.sqrt(((x - mean) ** 2).mean(1, keepdims=True) + epsilon)
+    return (x - mean) * scale * weight + bias, mean[:, 0], scale[:, 0]
+
+
+def layer_norm_backward(dy, x, weight, mean, scale):
+    u = (x - mean[:, None]) * scale[:, None]
+    g = dy * weight
+    dx = scale[:, None] * (g - g.mean(1, keepdims=True) - u * (g * u).mean(1, keepdims=True))
+    return dx, (dy * u).sum(0), dy.sum(0)

@@ -1,0 +1,37 @@
+"""What the language-model operators refuse, on the host and before any device
+work (no test here touches a device)."""
+
+from tensorcrate_amd import lib
+
+
+def refused(name, *args):
+    loaded = lib.load()
+    status = getattr(loaded, name)(*args)
+    return status, loaded.tc_last_error().decode()
+
+
+def test_layer_norm():
+    F, E = lib.F32, 1e-5
+    assert refused("tc_layer_norm", lib.F64, F, 64, 8, 2, 8, None, None, E, 64, 8, None, None) == (
+        lib.UNSUPPORTED, "layer norm: no kernel for f64")
+    assert refused("tc_layer_norm", 9, F, 64, 8, 2, 8, None, None, E, 64, 8, None, None)[0] == lib.UNSUPPORTED
+    assert refused("tc_layer_norm", lib.F16, lib.BF16, 64, 8, 2, 8, None, None, E, 64, 8, None, None) == (
+        lib.UNSUPPORTED, "layer norm: no kernel for f16 rows with a bf16 weight")
+    assert refused("tc_layer_norm", F, F, 64, 7, 2, 8, None, None, E, 64, 8, None, None) == (
+        lib.INVALID, "layer norm: rows of 8 elements 7 apart overlap")
+    assert refused("tc_layer_norm", F, F, 64, 8, 2, 8, None, None, E, 64, 5, None, None)[0] == lib.INVALID
+    assert refused("tc_layer_norm", F, F, 64, 0, 2, 0, None, None, E, 64, 0, None, None) == (
+        lib.INVALID, "layer norm: rows of no elements")
+    assert refused("tc_layer_norm", F, F, None, 8, 2, 8, None, None, E, 64, 8, None, None) == (
+        lib.INVALID, "layer norm: a null operand")
+    assert refused("tc_layer_norm", F, F, 64, 8, 2, 8, None, None, E, None, 8, None, None)[0] == lib.INVALID
+    assert refused("tc_layer_norm", F, F, 64, 2**40, 2**40, 2**30, None, None, E, 64, 2**40, None, None)[0] == lib.INVALID
+    back = "tc_layer_norm_backward"
+    assert refused(back, F, F, 64, 8, 64, 8, 2, 8, None, None, 64, 64, 8, None, None) == (
+        lib.INVALID, "layer norm, backward: a null operand")
+    assert refused(back, F, F, 64, 8, 64, 4, 2, 8, None, 64, 64, 64, 8, None, None)[0] == lib.INVALID
+    assert refused(back, F, F, 64, 8, 64, 8, 2, 8, None, 64, 64, 64, 7, None, None)[0] == lib.INVALID
+    assert refused(back, F, F, 64, 0, 64, 0, 2, 0, None, 64, 64, 64, 0, None, None) == (
+        lib.INVALID, "layer norm, backward: rows of no elements")
+    # Nothing wanted, or nothing there: nothing is done, and no device is needed.
+    assert refused(back, F, F, 64, 8, 64, 8, 2, 8, None, 64, 64, None, 8, None, None)[0] == lib.OK
