@@ -23,16 +23,44 @@ namespace tc {
 namespace {
 
 constexpr uint32_t kMostLanes = 1024;  // of a block
-constexpr int kMostHeld = 16;          // elements of a row that one lane holds
+constexpr uint32_t kBackThreads = 512;  // at most, backward, whose sums over rows fill the registers
+// Elements of a row that one lane of a block holds at most.
+constexpr int kForwardHeld = 16, kBackHeld = 32;
 
-template <typename W, int E, int VECTORS>
-struct Columns {
-    Words<W, E> words[VECTORS];
+// The columns that one lane of a row holds: VECTORS words a row's lanes apart.
+// The layout leaves no word but a lane's last one ragged or past the row's
+// end, so that only the last is checked.
+template <int E, int VECTORS>
+struct Held {
+    uint64_t first;   // column of the lane's first word
+    uint64_t apart;   // columns between its words
+    Run<E> last;
 
-    __device__ __forceinline__ void load(const W* from, const Run<E> (&runs)[VECTORS]) {
+    __device__ __forceinline__ Held(uint32_t lane, uint32_t lanes, uint64_t cols)
+        : first(uint64_t{lane} * E),
+          apart(uint64_t{lanes} * E),
+          last(lane + uint64_t{lanes} * (VECTORS - 1), cols) {}
+    __device__ __forceinline__ bool live(int v) const { return v < VECTORS - 1 || last.live(); }
+    __device__ __forceinline__ bool partial(int v) const { return v == VECTORS - 1 && last.partial(); }
+    __device__ __forceinline__ bool own(int v, int e) const { return v < VECTORS - 1 || last.own(e); }
+    __device__ __forceinline__ uint64_t column(int v) const {
+        return v < VECTORS - 1 ? first + v * apart : last.start;
+    }
+
+    template <bool NT, typename T>
+    __device__ __forceinline__ void load(const T* row, Words<T, E> (&words)[VECTORS]) const {
 #pragma unroll
-        for (int v = 0; v < VECTORS; v++) {
-            if (runs[v].live()) runs[v].template load<false>(from, words[v]);
+        for (int v = 0; v < VECTORS - 1; v++) words[v].template load<NT>(row + first + v * apart);
+        if (last.live()) last.template load<NT>(row, words[VECTORS - 1]);
+    }
+    template <bool NT, typename T>
+    __device__ __forceinline__ void store(T* row, int v, const float (&value)[E]) const {
+        if (v < VECTORS - 1) {
+            Words<T, E> words;
+            words.put(value);
+            words.template store<NT>(row + first + v * apart);
+        } else {
+            last.template store<NT>(row, value);
         }
     }
 };
@@ -50,71 +78,61 @@ __global__ void __launch_bounds__(LANES ? 256 : kMostLanes)
     uint64_t row = static_cast<uint64_t>(blockIdx.x) * (blockDim.x / lanes) + threadIdx.x / lanes;
     if (row >= rows) return;  // the whole group
 
-    Run<E> runs[VECTORS];
-#pragma unroll
-    for (int v = 0; v < VECTORS; v++) runs[v] = Run<E>(lane + static_cast<uint64_t>(v) * lanes, cols);
-    Columns<W, E, VECTORS> w, b;
-    if (weight != nullptr) w.load(weight, runs);
-    if (bias != nullptr) b.load(bias, runs);
+    const Held<E, VECTORS> held(lane, lanes, cols);
+    Words<W, E> w[VECTORS], b[VECTORS];
+    if (weight != nullptr) held.template load<false>(weight, w);
+    if (bias != nullptr) held.template load<false>(bias, b);
 
     const float count = static_cast<float>(cols);
     Words<S, E> next[VECTORS];
-#pragma unroll
-    for (int v = 0; v < VECTORS; v++) {
-        if (runs[v].live()) runs[v].template load<NT>(x + row * x_step, next[v]);
-    }
+    held.template load<NT>(x + row * x_step, next);
     for (; row < rows; row += groups) {
         float value[VECTORS][E];
         float sum = 0.0f;
 #pragma unroll
         for (int v = 0; v < VECTORS; v++) {
-            if (!runs[v].live()) continue;
+            if (!held.live(v)) continue;
             next[v].get(value[v]);
             float part = 0.0f;
 #pragma unroll
             for (int e = 0; e < E; e++) part += value[v][e];
-            if (runs[v].partial()) {
+            if (held.partial(v)) {
                 part = 0.0f;
 #pragma unroll
-                for (int e = 0; e < E; e++) part += runs[v].own(e) ? value[v][e] : 0.0f;
+                for (int e = 0; e < E; e++) part += held.own(v, e) ? value[v][e] : 0.0f;
             }
             sum += part;
         }
-        if (row + groups < rows) {
-#pragma unroll
-            for (int v = 0; v < VECTORS; v++) {
-                if (runs[v].live()) runs[v].template load<NT>(x + (row + groups) * x_step, next[v]);
-            }
-        }
+        if (row + groups < rows) held.template load<NT>(x + (row + groups) * x_step, next);
         const float mean = row_join<LANES, Added>(sum, shared[0]) / count;
         float squares = 0.0f;
 #pragma unroll
         for (int v = 0; v < VECTORS; v++) {
-            if (!runs[v].live()) continue;
+            if (!held.live(v)) continue;
             float part = 0.0f;
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 value[v][e] -= mean;
                 part = fmaf(value[v][e], value[v][e], part);
             }
-            if (runs[v].partial()) {
+            if (held.partial(v)) {
                 part = 0.0f;
 #pragma unroll
-                for (int e = 0; e < E; e++) part += runs[v].own(e) ? value[v][e] * value[v][e] : 0.0f;
+                for (int e = 0; e < E; e++) part += held.own(v, e) ? value[v][e] * value[v][e] : 0.0f;
             }
             squares += part;
         }
         const float scale = 1.0f / sqrtf(row_join<LANES, Added>(squares, shared[1]) / count + epsilon);
 #pragma unroll
         for (int v = 0; v < VECTORS; v++) {
-            if (!runs[v].live()) continue;
+            if (!held.live(v)) continue;
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 value[v][e] *= scale;
-                if (weight != nullptr) value[v][e] *= w.words[v].at(e);
-                if (bias != nullptr) value[v][e] += b.words[v].at(e);
+                if (weight != nullptr) value[v][e] *= w[v].at(e);
+                if (bias != nullptr) value[v][e] += b[v].at(e);
             }
-            runs[v].template store<NT>(y + row * y_step, value[v]);
+            held.template store<NT>(y + row * y_step, v, value[v]);
         }
         if (lane == 0) {
             if (means != nullptr) means[row] = mean;
@@ -188,7 +206,7 @@ __global__ void __launch_bounds__(kMostLanes)
 // The gradients.  `partial` (null if neither dw nor db is wanted) holds, for
 // each block, cols sums of dy u and then cols sums of dy.
 template <typename S, typename W, int LANES, int VECTORS, bool NT>
-__global__ void __launch_bounds__(LANES ? 256 : kMostLanes)
+__global__ void __launch_bounds__(kBackThreads)
     norm_back_kernel(const S* dy, uint64_t dy_step, const S* x, uint64_t x_step,
                      uint64_t rows, uint64_t cols, const W* weight, const float* __restrict__ means,
                      const float* __restrict__ scales, S* dx, uint64_t dx_step, float* __restrict__ partial) {
@@ -199,55 +217,87 @@ __global__ void __launch_bounds__(LANES ? 256 : kMostLanes)
     const uint64_t groups = static_cast<uint64_t>(gridDim.x) * (blockDim.x / lanes);
     uint64_t row = static_cast<uint64_t>(blockIdx.x) * (blockDim.x / lanes) + threadIdx.x / lanes;
 
-    Run<E> runs[VECTORS];
+    const Held<E, VECTORS> held(lane, lanes, cols);
+    // The weight's columns: in registers, or for a wave's longer rows in LDS,
+    // the same for every wave.
+    constexpr bool SHARED_WEIGHT = LANES == 64 && VECTORS > 2;
+    __shared__ uint4 weights[SHARED_WEIGHT ? VECTORS * Words<W, E>::kCount * 64 : 1];
+    Words<W, E> w[SHARED_WEIGHT ? 1 : VECTORS];
+    if constexpr (SHARED_WEIGHT) {
+        if (weight != nullptr && threadIdx.x < 64) {
+            Words<W, E> all[VECTORS];
+            held.template load<false>(weight, all);
 #pragma unroll
-    for (int v = 0; v < VECTORS; v++) runs[v] = Run<E>(lane + static_cast<uint64_t>(v) * lanes, cols);
-    Columns<W, E, VECTORS> w;
-    if (weight != nullptr) w.load(weight, runs);
+            for (int v = 0; v < VECTORS; v++) {
+#pragma unroll
+                for (int k = 0; k < Words<W, E>::kCount; k++) {
+                    weights[(v * Words<W, E>::kCount + k) * 64 + lane] = all[v].w[k];
+                }
+            }
+        }
+        __syncthreads();
+    } else {
+        if (weight != nullptr) held.template load<false>(weight, w);
+    }
+    const auto weight_words = [&](int v) {
+        if constexpr (SHARED_WEIGHT) {
+            Words<W, E> out;
+#pragma unroll
+            for (int k = 0; k < Words<W, E>::kCount; k++) {
+                out.w[k] = weights[(v * Words<W, E>::kCount + k) * 64 + lane];
+            }
+            return out;
+        } else {
+            return w[v];
+        }
+    };
     float dw[VECTORS][E] = {}, db[VECTORS][E] = {};
 
     Words<S, E> next_x[VECTORS], next_dy[VECTORS];
     float next_mean = 0.0f, next_scale = 0.0f;
     const auto fetch = [&](uint64_t at) {
-#pragma unroll
-        for (int v = 0; v < VECTORS; v++) {
-            if (!runs[v].live()) continue;
-            runs[v].template load<NT>(x + at * x_step, next_x[v]);
-            runs[v].template load<NT>(dy + at * dy_step, next_dy[v]);
-        }
+        held.template load<NT>(x + at * x_step, next_x);
+        held.template load<NT>(dy + at * dy_step, next_dy);
         next_mean = means[at];
         next_scale = scales[at];
     };
-    // The next row's words are in flight while this one's are worked on,
-    // where the registers allow both.
-    constexpr bool AHEAD = VECTORS == 1;
-    if (AHEAD && row < rows) fetch(row);
+    // The next row's words are in flight while this one's are worked on.
+    constexpr bool KEPT = VECTORS * E > (LANES ? 32 : 16);
+    if (row < rows) fetch(row);
     int turn = 0;
     for (; row < rows; row += groups) {
-        if (!AHEAD) fetch(row);
         const float mean = next_mean, scale = next_scale;
-        float u[VECTORS][E], g[VECTORS][E];
+        // u and g of a word, from dy, x and the weight as they are stored.
+        // Where a lane holds many words it keeps those for the second pass
+        // rather than the 32-bit values, which would not fit its registers.
+        float u[KEPT ? 1 : VECTORS][E], g[KEPT ? 1 : VECTORS][E];
+        Words<S, E> now_x[KEPT ? VECTORS : 1], now_dy[KEPT ? VECTORS : 1];
         float sum = 0.0f, along = 0.0f;
 #pragma unroll
         for (int v = 0; v < VECTORS; v++) {
-            if (!runs[v].live()) continue;
-            next_x[v].get(u[v]);
-            next_dy[v].get(g[v]);
-            if (runs[v].partial()) {
-                // Neighbours' elements and those past a short row: nothing
-                // to the sums, and mean(g) is all that dx needs of them.
+            if (!held.live(v)) continue;
+            float(&uv)[E] = u[KEPT ? 0 : v];
+            float(&gv)[E] = g[KEPT ? 0 : v];
+            if constexpr (KEPT) now_x[v] = next_x[v], now_dy[v] = next_dy[v];
+            next_x[v].get(uv);
+            next_dy[v].get(gv);
+            Words<W, E> here;
+            if (weight != nullptr) here = weight_words(v);
+            if (held.partial(v)) {
+                // A neighbour's elements and those past a short row add
+                // nothing to the sums.
                 float one = 0.0f, two = 0.0f;
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    u[v][e] = (u[v][e] - mean) * scale;
-                    if (runs[v].own(e)) {
-                        dw[v][e] = fmaf(g[v][e], u[v][e], dw[v][e]);
-                        db[v][e] += g[v][e];
+                    uv[e] = (uv[e] - mean) * scale;
+                    if (held.own(v, e)) {
+                        dw[v][e] = fmaf(gv[e], uv[e], dw[v][e]);
+                        db[v][e] += gv[e];
                     }
-                    if (weight != nullptr) g[v][e] *= w.words[v].at(e);
-                    if (runs[v].own(e)) {
-                        one += g[v][e];
-                        two = fmaf(g[v][e], u[v][e], two);
+                    if (weight != nullptr) gv[e] *= here.at(e);
+                    if (held.own(v, e)) {
+                        one += gv[e];
+                        two = fmaf(gv[e], uv[e], two);
                     }
                 }
                 sum += one;
@@ -255,16 +305,16 @@ __global__ void __launch_bounds__(LANES ? 256 : kMostLanes)
             } else {
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    u[v][e] = (u[v][e] - mean) * scale;
-                    dw[v][e] = fmaf(g[v][e], u[v][e], dw[v][e]);
-                    db[v][e] += g[v][e];
-                    if (weight != nullptr) g[v][e] *= w.words[v].at(e);
-                    sum += g[v][e];
-                    along = fmaf(g[v][e], u[v][e], along);
+                    uv[e] = (uv[e] - mean) * scale;
+                    dw[v][e] = fmaf(gv[e], uv[e], dw[v][e]);
+                    db[v][e] += gv[e];
+                    if (weight != nullptr) gv[e] *= here.at(e);
+                    sum += gv[e];
+                    along = fmaf(gv[e], uv[e], along);
                 }
             }
         }
-        if (AHEAD && row + groups < rows) fetch(row + groups);
+        if (row + groups < rows) fetch(row + groups);
         if (dx == nullptr) continue;
         if constexpr (LANES == 0) {
             // Both sums past one barrier, in buffers that alternate.
@@ -293,46 +343,71 @@ __global__ void __launch_bounds__(LANES ? 256 : kMostLanes)
         const float mean_g = sum / static_cast<float>(cols), mean_gu = along / static_cast<float>(cols);
 #pragma unroll
         for (int v = 0; v < VECTORS; v++) {
-            if (!runs[v].live()) continue;
+            if (!held.live(v)) continue;
+            float(&uv)[E] = u[KEPT ? 0 : v];
+            float(&gv)[E] = g[KEPT ? 0 : v];
+            if constexpr (KEPT) {
+                now_x[v].get(uv);
+                now_dy[v].get(gv);
+                Words<W, E> here;
+                if (weight != nullptr) here = weight_words(v);
 #pragma unroll
-            for (int e = 0; e < E; e++) g[v][e] = scale * (g[v][e] - mean_g - u[v][e] * mean_gu);
-            runs[v].template store<NT>(dx + row * dx_step, g[v]);
+                for (int e = 0; e < E; e++) {
+                    uv[e] = (uv[e] - mean) * scale;
+                    if (weight != nullptr) gv[e] *= here.at(e);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < E; e++) gv[e] = scale * (gv[e] - mean_g - uv[e] * mean_gu);
+            held.template store<NT>(dx + row * dx_step, v, gv);
         }
     }
     if (partial == nullptr) return;
 
-    float* sums = partial + static_cast<uint64_t>(blockIdx.x) * 2 * cols;
-    if constexpr (LANES == 0) {
+    // The block's groups hold the same columns: halves added to halves.
+    if constexpr (LANES != 0) {
+        constexpr int HALF = kBackThreads / 2;
+        __shared__ float other[HALF * VECTORS * E];
+        for (int most = HALF; most >= LANES; most /= 2) {
+            for (int which = 0; which < 2; which++) {
+                __syncthreads();
+                if (threadIdx.x >= most && threadIdx.x < 2 * most) {
 #pragma unroll
-        for (int v = 0; v < VECTORS; v++) {
+                    for (int v = 0; v < VECTORS; v++) {
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                if (!runs[v].own(e)) continue;
-                sums[runs[v].start + e] = dw[v][e];
-                sums[cols + runs[v].start + e] = db[v][e];
+                        for (int e = 0; e < E; e++) {
+                            other[(v * E + e) * HALF + threadIdx.x - most] = which ? db[v][e] : dw[v][e];
+                        }
+                    }
+                }
+                __syncthreads();
+                if (threadIdx.x < most) {
+#pragma unroll
+                    for (int v = 0; v < VECTORS; v++) {
+#pragma unroll
+                        for (int e = 0; e < E; e++) {
+                            const float more = other[(v * E + e) * HALF + threadIdx.x];
+                            if (which) {
+                                db[v][e] += more;
+                            } else {
+                                dw[v][e] += more;
+                            }
+                        }
+                    }
+                }
             }
         }
-    } else {
-        // The block's groups hold the same columns: added in group order.
-        __shared__ float turns[256 * VECTORS * E];
-        const int groups_here = 256 / LANES;
-        for (int which = 0; which < 2; which++) {
-            if (which) __syncthreads();
+        if (threadIdx.x >= LANES) return;
+    }
+    float* sums = partial + static_cast<uint64_t>(blockIdx.x) * 2 * cols;
 #pragma unroll
-            for (int v = 0; v < VECTORS; v++) {
+    for (int v = 0; v < VECTORS; v++) {
+        if (!held.live(v)) continue;
 #pragma unroll
-                for (int e = 0; e < E; e++) turns[(v * E + e) * 256 + threadIdx.x] = which ? db[v][e] : dw[v][e];
-            }
-            __syncthreads();
-            // A group's lanes hold VECTORS x E values each: value k of lane l.
-            for (int at = threadIdx.x; at < LANES * VECTORS * E; at += 256) {
-                const int l = at % LANES, k = at / LANES;
-                const Run<E> run(l + static_cast<uint64_t>(k / E) * LANES, cols);
-                if (!run.own(k % E)) continue;
-                float all = 0.0f;
-                for (int q = 0; q < groups_here; q++) all += turns[k * 256 + q * LANES + l];
-                sums[which * cols + run.start + k % E] = all;
-            }
+        for (int e = 0; e < E; e++) {
+            if (!held.own(v, e)) continue;
+            sums[held.column(v) + e] = dw[v][e];
+            sums[cols + held.column(v) + e] = db[v][e];
         }
     }
 }
@@ -384,92 +459,119 @@ __global__ void __launch_bounds__(256)
 }
 
 // out[c] = the sum over `parts` of partial[part][c] in a fixed order, for the
-// 2 x cols columns: 16 lanes of every 64 columns each take every 16th part.
+// 2 x cols columns: 16 columns a block, of which each of 64 lanes takes every
+// 64th part; a wave's four sums are added in registers, then the waves'.
 template <typename W>
 __global__ void __launch_bounds__(1024)
     add_parts_kernel(const float* __restrict__ partial, uint32_t parts, uint64_t cols, W* dweight, W* dbias) {
-    __shared__ float shared[16][64];
-    const uint64_t c = static_cast<uint64_t>(blockIdx.x) * 64 + threadIdx.x % 64;
-    const uint32_t turn = threadIdx.x / 64;
+    __shared__ float shared[16][16];
+    const uint32_t column = threadIdx.x % 16, turn = threadIdx.x / 16;
+    const uint64_t c = static_cast<uint64_t>(blockIdx.x) * 16 + column;
     float sum = 0.0f;
     if (c < 2 * cols) {
 #pragma unroll 8
-        for (uint32_t p = turn; p < parts; p += 16) sum += partial[static_cast<uint64_t>(p) * 2 * cols + c];
+        for (uint32_t p = turn; p < parts; p += 64) sum += partial[static_cast<uint64_t>(p) * 2 * cols + c];
     }
-    shared[turn][threadIdx.x % 64] = sum;
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (threadIdx.x % 64 < 16) shared[threadIdx.x / 64][column] = sum;
     __syncthreads();
     if (turn != 0 || c >= 2 * cols) return;
 #pragma unroll
-    for (int k = 1; k < 16; k++) sum += shared[k][threadIdx.x];
+    for (int k = 1; k < 16; k++) sum += shared[k][column];
     W* out = c < cols ? dweight : dbias;
     if (out != nullptr) out[c < cols ? c : c - cols] = Elem<W>::narrow(sum);
 }
 
 // How the lanes are laid over rows of `cols` elements, `run` of them a
-// 16-byte word: the fewest words a lane.
+// 16-byte word.
 struct Layout {
     int lanes = 0;         // 16, 64, or 0 for a block of `threads`
-    int vectors = 0;       // words a lane: 1, 2 or 4; 0 for rows too long for registers
+    int vectors = 0;       // words a lane; 0 for rows too long for registers
     uint32_t threads = 0;  // of a block
 };
 
-Layout layout_of(uint64_t cols, int run) {
+// Rows of up to 64 x `wave` words take a wave, several rows to a block of
+// `block` threads; longer ones a block of at most `most` threads, two words a
+// lane at least and `held` elements at most.
+Layout layout_of(uint64_t cols, int run, uint32_t block, int wave, uint32_t most, int held) {
     const uint64_t words = (cols + run - 1) / run;
     Layout out;
-    out.threads = 256;
-    if (words <= 64) {
-        out.lanes = words <= 16 ? 16 : 64;
-        out.vectors = 1;
+    out.threads = block;
+    if (words <= 16) {
+        out.lanes = 16, out.vectors = 1;
         return out;
     }
-    out.vectors = 1;
-    while (words > uint64_t{kMostLanes} * out.vectors) {
-        out.vectors *= 2;
-        if (out.vectors * run > kMostHeld) {
-            out.vectors = 0, out.threads = kMostLanes;
-            return out;
-        }
+    if (words <= 64 * static_cast<uint64_t>(wave)) {
+        out.lanes = 64, out.vectors = static_cast<int>((words + 63) / 64);
+        return out;
     }
-    out.threads = static_cast<uint32_t>(((words + out.vectors - 1) / out.vectors + 63) / 64 * 64);
+    for (const int vectors : {2, 4, 6, 7, 8}) {
+        const uint64_t threads = ((words + vectors - 1) / vectors + 63) / 64 * 64;
+        // Only a lane's last word may lie past the row's end (`Held`).
+        if (vectors * run > held || threads > most || (vectors - 1) * threads >= words) continue;
+        out.vectors = vectors;
+        out.threads = static_cast<uint32_t>(threads);
+        return out;
+    }
+    out.vectors = 0, out.threads = kMostLanes;
     return out;
 }
 
+// As many blocks as `threads_per_cu` on every compute unit allow, or fewer
+// that have all the rows.
 uint32_t blocks_of(const Layout& layout, uint64_t rows, uint32_t threads_per_cu) {
-    const uint64_t per_block = layout.lanes ? 256 / layout.lanes : 1;
+    const uint64_t per_block = layout.lanes ? layout.threads / layout.lanes : 1;
     const uint64_t wanted = (rows + per_block - 1) / per_block;
-    const uint64_t most = static_cast<uint64_t>(compute_units()) * (threads_per_cu > layout.threads ? threads_per_cu / layout.threads : 1);
+    const uint64_t most = uint64_t{static_cast<uint32_t>(compute_units())} *
+                          (threads_per_cu > layout.threads ? threads_per_cu / layout.threads : 1);
     return static_cast<uint32_t>(wanted < most ? wanted : most);
 }
 
-// The body with LANES and VECTORS of the layout (four words a lane only for
-// f32, where they are 16 elements).
-#define TC_NORM_FORM(layout, S, ...)                                     \
+// The body with LANES and VECTORS of the layout of at most HELD elements a
+// lane.
+#define TC_NORM_FORM(layout, S, HELD, ...)                                    \
     if (layout.lanes == 16) {                                            \
         constexpr int LANES = 16, VECTORS = 1; __VA_ARGS__;              \
-    } else if (layout.lanes == 64) {                                     \
+    } else if (layout.lanes == 64 && layout.vectors == 1) {              \
         constexpr int LANES = 64, VECTORS = 1; __VA_ARGS__;              \
-    } else if (layout.vectors == 1) {                                    \
-        constexpr int LANES = 0, VECTORS = 1; __VA_ARGS__;               \
+    } else if (layout.lanes == 64 && layout.vectors == 2) {              \
+        constexpr int LANES = 64, VECTORS = 2; __VA_ARGS__;              \
+    } else if (layout.lanes == 64 && layout.vectors == 3) {              \
+        constexpr int LANES = 64, VECTORS = 3; __VA_ARGS__;              \
+    } else if (layout.lanes == 64 && layout.vectors == 4) {              \
+        constexpr int LANES = 64, VECTORS = 4; __VA_ARGS__;              \
+    } else if (layout.lanes == 64) {                                     \
+        constexpr int LANES = 64, VECTORS = 5; __VA_ARGS__;              \
     } else if (layout.vectors == 2) {                                    \
         constexpr int LANES = 0, VECTORS = 2; __VA_ARGS__;               \
-    } else {                                                             \
-        constexpr int LANES = 0, VECTORS = kMostHeld / kWordElements<S>; \
-        __VA_ARGS__;                                                     \
+    } else if (layout.vectors == 4) {                                    \
+        constexpr int LANES = 0, VECTORS = 4; __VA_ARGS__;               \
+    } else if constexpr (kWordElements<S> * 8 <= HELD) {                 \
+        if (layout.vectors == 6) {                                       \
+            constexpr int LANES = 0, VECTORS = 6; __VA_ARGS__;           \
+        } else if (layout.vectors == 7) {                                \
+            constexpr int LANES = 0, VECTORS = 7; __VA_ARGS__;           \
+        } else {                                                         \
+            constexpr int LANES = 0, VECTORS = 8; __VA_ARGS__;           \
+        }                                                                \
     }
 
 template <typename S, typename W>
 int norm(const S* x, uint64_t x_step, uint64_t rows, uint64_t cols, const W* weight, const W* bias, float epsilon,
          S* y, uint64_t y_step, float* means, float* scales) {
     TC_STREAM(s);
-    const Layout layout = layout_of(cols, kWordElements<S>);
+    const Layout layout = layout_of(cols, kWordElements<S>, 256, 5, kMostLanes, kForwardHeld);
     if (layout.vectors == 0) {
         norm_long_kernel<S, W><<<grid_for(rows, 1, 2), kMostLanes, 0, s>>>(x, x_step, rows, cols, weight, bias,
                                                                           epsilon, y, y_step, means, scales);
         return check_launch("layer norm");
     }
-    const uint32_t blocks = blocks_of(layout, rows, 2048);
-    const bool streams = 2 * sizeof(S) * rows * cols > kStreamBytes;
-    TC_NORM_FORM(layout, S, {
+    // Groups that need no barrier take a row each; blocks walk the rows, a
+    // compute unit's wavefronts half filled.
+    const uint32_t blocks = blocks_of(layout, rows, layout.lanes ? 1u << 30 : 1024);
+    const bool streams = 2 * sizeof(S) * rows * cols >= kStreamBytes;
+    TC_NORM_FORM(layout, S, kForwardHeld, {
         if (streams) {
             norm_kernel<S, W, LANES, VECTORS, true><<<blocks, layout.threads, 0, s>>>(
                 x, x_step, rows, cols, weight, bias, epsilon, y, y_step, means, scales);
@@ -487,9 +589,14 @@ int norm_back(const S* dy, uint64_t dy_step, const S* x, uint64_t x_step, uint64
               W* dbias) {
     TC_STREAM(s);
     const bool columns = dweight != nullptr || dbias != nullptr;
-    const Layout layout = layout_of(cols, kWordElements<S>);
-    const uint32_t row_blocks =
-        layout.vectors == 0 ? grid_for(rows, 64, 1) : blocks_of(layout, rows, 1024);
+    const Layout layout = layout_of(cols, kWordElements<S>, kBackThreads, 5, kBackThreads, kBackHeld);
+    // Every block writes 8 bytes a column at its end, so the fewer the better:
+    // half the wavefronts that a compute unit holds, but all of them where a
+    // lane holds so little that loads in flight are few.  Measured over 10007
+    // f16 rows of 2050: 512 threads 41 us, 1024 48; over 8192 f32 rows of 4096
+    // (8 elements a lane): 93 and 79.
+    const uint32_t per_cu = layout.lanes == 0 && layout.vectors * kWordElements<S> <= 8 ? 1024 : 512;
+    const uint32_t row_blocks = layout.vectors == 0 ? grid_for(rows, 64, 1) : blocks_of(layout, rows, per_cu);
     const uint32_t parts = rows == 0 ? 0 : row_blocks;
     Scratch partial(columns ? uint64_t{parts} * 2 * cols * sizeof(float) : 0);
     if (partial.status != TC_OK) return partial.status;
@@ -507,8 +614,8 @@ int norm_back(const S* dy, uint64_t dy_step, const S* x, uint64_t x_step, uint64
             status = check_launch("layer norm, backward");
         }
     } else if (rows > 0) {
-        const bool streams = 3 * sizeof(S) * rows * cols > kStreamBytes;
-        TC_NORM_FORM(layout, S, {
+        const bool streams = 3 * sizeof(S) * rows * cols >= kStreamBytes;
+        TC_NORM_FORM(layout, S, kBackHeld, {
             if (streams) {
                 norm_back_kernel<S, W, LANES, VECTORS, true><<<row_blocks, layout.threads, 0, s>>>(
                     dy, dy_step, x, x_step, rows, cols, weight, means, scales, dx, dx_step, sums);
@@ -520,7 +627,7 @@ int norm_back(const S* dy, uint64_t dy_step, const S* x, uint64_t x_step, uint64
         status = check_launch("layer norm, backward");
     }
     if (status != TC_OK || !columns) return status;
-    add_parts_kernel<W><<<static_cast<uint32_t>((2 * cols + 63) / 64), 1024, 0, s>>>(sums, parts, cols, dweight, dbias);
+    add_parts_kernel<W><<<static_cast<uint32_t>((2 * cols + 15) / 16), 1024, 0, s>>>(sums, parts, cols, dweight, dbias);
     return check_launch("layer norm, backward");
 }
 

@@ -23,7 +23,7 @@ EPSILON = 1e-5
 # form and one past them, many rows, long rows past a block's registers.
 SHAPES = [(1, 1), (3, 2), (5, 7), (4, 8), (4, 9), (33, 31), (17, 64), (65, 65), (9, 127), (9, 128), (100, 129),
           (31, 257), (7, 511), (7, 513), (300, 1000), (40, 1027), (5, 2050), (3, 4096), (3, 4099), (2, 8192),
-          (2, 8193), (2, 16384), (2, 16391), (3, 40003), (5000, 24), (2500, 200)]
+          (2, 8193), (2, 9300), (2, 12300), (2, 15000), (2, 16384), (2, 16391), (3, 40003), (5000, 24), (2500, 200)]
 
 
 def inputs(kind, weight_kind, rows, cols, seed):
