@@ -658,6 +658,38 @@ int tc_layer_norm_backward(uint32_t dtype, uint32_t weight_dtype, const void* dy
                            uint64_t x_step, uint64_t rows, uint64_t cols, const void* weight, const float* means,
                            const float* scales, void* dx, uint64_t dx_step, void* dweight, void* dbias);
 
+/* ---- log probabilities of tokens ------------------------------------------ */
+
+/* Of each of the `rows` rows of `cols` logits x, `step` elements apart, with
+ * p = softmax(x):
+ *   log_probabilities[row] = log p(tokens[row]),
+ *   normalizers[row] = log of the sum of exp x,
+ *   entropies[row] = -sum p log p, in nats;
+ * and the `top` (at most 64, at most `cols`) most probable tokens, highest
+ * first, equal logits by the lower token: their log probabilities and the
+ * tokens themselves, `top` a row.  All results are f32, from one read of the
+ * logits in f32.  `tokens` and `log_probabilities` are null together; each
+ * other result may be null (the last two with `top` 0).
+ *   A token of `cols` or more (such as -1 cast) is none: its log probability
+ * is 0.  A logit of -infinity is a token that cannot be: it has log
+ * probability -infinity and adds nothing.  A row of nothing else has the
+ * normalizer -infinity and the entropy 0.  A row with a NaN or +infinity has
+ * NaN statistics; a NaN comes after every other logit among the top. */
+int tc_log_probabilities(uint32_t dtype, const void* logits, uint64_t step, uint64_t rows, uint64_t cols,
+                         const uint32_t* tokens, float* log_probabilities, float* normalizers, float* entropies,
+                         uint32_t top, float* top_log_probabilities, uint32_t* top_tokens);
+
+/* The gradient of the logits, rows `d_step` apart, from those of the log
+ * probabilities (null: none; else with `tokens`) and of the entropies (null:
+ * none; else with `entropies`), and the forward pass's `normalizers`.  It
+ * may take the logits' place (`d_logits` the same pointer with the same
+ * step).  Rows without a token and without a gradient of their entropy get
+ * zeros, whatever their logits, and so do rows of -infinity alone. */
+int tc_log_probabilities_backward(uint32_t dtype, const void* logits, uint64_t step, uint64_t rows, uint64_t cols,
+                                  const uint32_t* tokens, const float* normalizers, const float* entropies,
+                                  const float* d_log_probabilities, const float* d_entropies, void* d_logits,
+                                  uint64_t d_step);
+
 #ifdef __cplusplus
 }
 #endif

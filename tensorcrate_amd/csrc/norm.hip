@@ -523,14 +523,16 @@ Layout layout_of(uint64_t cols, int run, uint32_t block, int wave, uint32_t most
 uint32_t blocks_of(const Layout& layout, uint64_t rows, uint32_t threads_per_cu) {
     const uint64_t per_block = layout.lanes ? layout.threads / layout.lanes : 1;
     const uint64_t wanted = (rows + per_block - 1) / per_block;
-    const uint64_t most = uint64_t{static_cast<uint32_t>(compute_units())} *
-                          (threads_per_cu > layout.threads ? threads_per_cu / layout.threads : 1);
+    uint64_t most = uint64_t{static_cast<uint32_t>(compute_units())} *
+                    (threads_per_cu > layout.threads ? threads_per_cu / layout.threads : 1);
+    // A dispatch holds fewer than 2^32 work-items.
+    if (most > 0xffffffffu / layout.threads) most = 0xffffffffu / layout.threads;
     return static_cast<uint32_t>(wanted < most ? wanted : most);
 }
 
 // The body with LANES and VECTORS of the layout of at most HELD elements a
 // lane.
-#define TC_NORM_FORM(layout, S, HELD, ...)                                    \
+#define TC_NORM_FORM(layout, S, HELD, ...)                               \
     if (layout.lanes == 16) {                                            \
         constexpr int LANES = 16, VECTORS = 1; __VA_ARGS__;              \
     } else if (layout.lanes == 64 && layout.vectors == 1) {              \
@@ -545,15 +547,17 @@ uint32_t blocks_of(const Layout& layout, uint64_t rows, uint32_t threads_per_cu)
         constexpr int LANES = 64, VECTORS = 5; __VA_ARGS__;              \
     } else if (layout.vectors == 2) {                                    \
         constexpr int LANES = 0, VECTORS = 2; __VA_ARGS__;               \
-    } else if (layout.vectors == 4) {                                    \
-        constexpr int LANES = 0, VECTORS = 4; __VA_ARGS__;               \
-    } else if constexpr (kWordElements<S> * 8 <= HELD) {                 \
-        if (layout.vectors == 6) {                                       \
-            constexpr int LANES = 0, VECTORS = 6; __VA_ARGS__;           \
-        } else if (layout.vectors == 7) {                                \
-            constexpr int LANES = 0, VECTORS = 7; __VA_ARGS__;           \
-        } else {                                                         \
-            constexpr int LANES = 0, VECTORS = 8; __VA_ARGS__;           \
+    } else if constexpr (kWordElements<S> * 4 <= HELD) {                 \
+        if (layout.vectors == 4) {                                       \
+            constexpr int LANES = 0, VECTORS = 4; __VA_ARGS__;           \
+        } else if constexpr (kWordElements<S> * 8 <= HELD) {             \
+            if (layout.vectors == 6) {                                   \
+                constexpr int LANES = 0, VECTORS = 6; __VA_ARGS__;       \
+            } else if (layout.vectors == 7) {                            \
+                constexpr int LANES = 0, VECTORS = 7; __VA_ARGS__;       \
+            } else {                                                     \
+                constexpr int LANES = 0, VECTORS = 8; __VA_ARGS__;       \
+            }                                                            \
         }                                                                \
     }
 

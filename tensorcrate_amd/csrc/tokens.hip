@@ -1,0 +1,627 @@
+// Log probabilities of tokens, their entropy and the most probable ones, and
+// the gradient of the logits.
+//
+// Of a row of logits x, with m the largest,
+//   s = sum exp(x - m),  t = sum (x - m) exp(x - m),
+//   l = m + log s                 the normalizer, log sum exp x
+//   log p(j) = (x_j - m) - log s
+//   H = log s - t / s             the entropy, -sum p log p
+// all from one read of the row: a lane keeps m, s and t of what it has read
+// and rescales s and t when m grows (t' = (t + s (m - m')) exp(m - m')), and
+// the lanes', waves' and blocks' states are joined the same way, in a fixed
+// order.
+//
+// The gradient, from g of log p(token) and h of H:
+//   d_j = g (j == token) - p_j (g + h (log p_j + H)),  p_j = exp(x_j - l)
+//
+// Both are bound by memory, the forward pass at one read of the logits, the
+// backward pass at one read and one write.  Rows are read in words that are
+// 16-byte aligned wherever the row starts, its first and last elements one by
+// one.  A block takes a row; few rows are split over several blocks each, and
+// a second kernel joins them.
+//
+// The most probable tokens are kept by a 64-bit key, the logit's bits in
+// order above the token's complement, so that equal logits go to the lowest
+// token and no two keys are equal.  A block collects the keys that beat the
+// last of its best so far in LDS and selects from them when they are many and
+// at the end.  However the logits lie they fit: of a batch that would not,
+// only keys at least as high as the k-th highest of the lanes' highest are
+// taken, and those are in k lanes.
+
+#include <type_traits>
+
+#include "rows.hpp"
+
+namespace tc {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBatch = 4;  // words a lane reads at a time
+constexpr uint32_t kMostTop = 64;
+constexpr uint64_t kMostParts = 64;  // of a row
+constexpr int kRoom = 3072;  // keys collected at most
+// Collected keys beyond which a block selects: kRoom less a batch's most,
+// kMostTop lanes of kBatch words of 8.
+constexpr int kFull = kRoom - static_cast<int>(kMostTop) * kBatch * 8;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// ---- a row's state ----------------------------------------------------------------
+
+struct State {
+    float most = -INFINITY;  // m
+    float sum = 0.0f;        // s
+    float mean = 0.0f;       // t
+};
+
+__device__ __forceinline__ float power(float v) { return __builtin_amdgcn_exp2f(v * kLog2e); }
+
+// The state with another m, not less than its own.
+// A state of nothing but -infinity holds zeros (or the NaN of a NaN logit),
+// which stay.
+__device__ __forceinline__ void move(State& s, float to) {
+    const float shift = s.most == -INFINITY ? 0.0f : s.most - to;
+    const float factor = power(shift);
+    s.mean = fmaf(s.sum, shift, s.mean) * factor;
+    s.sum *= factor;
+    s.most = to;
+}
+
+// Joined over the block, in every lane; `shared` holds three floats a wave.
+__device__ __forceinline__ State joined(State s, float (*shared)[kThreads / 64]) {
+    move(s, wave64<Largest>(s.most));
+    s.sum = wave64<Added>(s.sum);
+    s.mean = wave64<Added>(s.mean);
+    const int wave = threadIdx.x / 64;
+    if (threadIdx.x % 64 == 0) shared[0][wave] = s.most, shared[1][wave] = s.sum, shared[2][wave] = s.mean;
+    __syncthreads();
+    State all{shared[0][0], shared[1][0], shared[2][0]};
+    float most = all.most;
+    for (int w = 1; w < kThreads / 64; w++) most = fmaxf(most, shared[0][w]);
+    move(all, most);
+    for (int w = 1; w < kThreads / 64; w++) {
+        State other{shared[0][w], shared[1][w], shared[2][w]};
+        move(other, most);
+        all.sum += other.sum;
+        all.mean += other.mean;
+    }
+    return all;
+}
+
+// ---- the order of logits ------------------------------------------------------------
+
+// Whole numbers in the order of the floats, -0 as 0, a NaN below all.
+__device__ __forceinline__ uint32_t ordered(float v) {
+    const uint32_t bits = __float_as_uint(v + 0.0f);
+    if (v != v) return 0;
+    return bits >> 31 ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t order) {
+    return __uint_as_float(order >> 31 ? order & 0x7fffffffu : ~order);
+}
+__device__ __forceinline__ uint64_t key_of(float v, uint32_t token) {
+    return static_cast<uint64_t>(ordered(v)) << 32 | ~token;
+}
+__device__ __forceinline__ float logit_of(uint64_t key) { return unordered(static_cast<uint32_t>(key >> 32)); }
+__device__ __forceinline__ uint32_t token_of(uint64_t key) { return ~static_cast<uint32_t>(key); }
+
+// The keys that a block has collected.
+struct Keys {
+    uint64_t keys[kRoom];
+    uint64_t best[kMostTop];
+    uint64_t highest[kThreads];  // of each lane's batch
+    uint64_t least;              // of the batch's keys that are taken
+    int count;
+};
+
+// The `top` highest of the collected keys, in order, are what is left of them.
+__device__ void select(Keys& k, int count, int top) {
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+        const uint64_t key = k.keys[i];
+        int rank = 0;
+        for (int j = 0; j < count; j++) rank += k.keys[j] > key;
+        if (rank < top) k.best[rank] = key;
+    }
+    __syncthreads();
+    const int left = count < top ? count : top;
+    for (int i = threadIdx.x; i < left; i += kThreads) k.keys[i] = k.best[i];
+    if (threadIdx.x == 0) k.count = left;
+    __syncthreads();
+}
+
+// ---- a row's words -------------------------------------------------------------------
+
+// The row's words are those of memory: the first may begin before the row and
+// the last end behind it.
+template <typename S>
+struct Row {
+    static constexpr int E = kWordElements<S>;
+    const S* row;
+    uint64_t cols;
+    int lead;  // elements of the first word that are not the row's
+
+    __device__ __forceinline__ Row(const S* at, uint64_t n)
+        : row(at), cols(n), lead(static_cast<int>(reinterpret_cast<uintptr_t>(at) / sizeof(S) % E)) {}
+    __device__ __forceinline__ uint64_t words() const { return (cols + lead + E - 1) / E; }
+    // Column of the word's first element (of word 0, possibly before the row).
+    __device__ __forceinline__ int64_t column(uint64_t word) const {
+        return static_cast<int64_t>(word * E) - lead;
+    }
+    __device__ __forceinline__ bool whole(int64_t column) const {
+        return column >= 0 && column + E <= static_cast<int64_t>(cols);
+    }
+    __device__ __forceinline__ bool has(int64_t column) const {
+        return column >= 0 && column < static_cast<int64_t>(cols);
+    }
+    template <bool NT>
+    __device__ __forceinline__ void load(uint64_t word, Words<S, E>& out) const {
+        const int64_t at = column(word);
+        if (whole(at)) {
+            out.template load<NT>(row + at);
+        } else {
+            float v[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] = has(at + e) ? Elem<S>::widen(row[at + e]) : -INFINITY;
+            out.put(v);
+        }
+    }
+};
+
+// What a block leaves of its part of a row, where rows are split.
+struct Part {
+    State state;
+    uint32_t count;  // keys, best first
+};
+
+struct Results {
+    const uint32_t* tokens;
+    float* log_probabilities;
+    float* normalizers;
+    float* entropies;
+    uint32_t top;
+    float* top_log_probabilities;
+    uint32_t* top_tokens;
+
+    // Of the rows from `first` on.
+    Results from(uint64_t first) const {
+        const auto at = [&](auto* p, uint64_t each) { return p != nullptr ? p + first * each : nullptr; };
+        return {at(tokens, 1), at(log_probabilities, 1), at(normalizers, 1), at(entropies, 1), top,
+                at(top_log_probabilities, top), at(top_tokens, top)};
+    }
+};
+
+// log p of a logit from the row's state.
+__device__ __forceinline__ float log_probability(const State& s, float logit) {
+    if (s.most == -INFINITY && s.sum == 0.0f) return -INFINITY;  // nothing is possible
+    return (logit - s.most) - logf(s.sum);
+}
+
+// One lane writes the row's results.
+template <typename S>
+__device__ void finish(const State& s, const S* row, uint64_t cols, uint64_t at, const Results& out) {
+    const bool none = s.most == -INFINITY && s.sum == 0.0f;
+    if (out.normalizers != nullptr) out.normalizers[at] = none ? -INFINITY : s.most + logf(s.sum);
+    if (out.entropies != nullptr) out.entropies[at] = none ? 0.0f : logf(s.sum) - s.mean / s.sum;
+    if (out.log_probabilities != nullptr) {
+        const uint32_t token = out.tokens[at];
+        out.log_probabilities[at] = token < cols ? log_probability(s, Elem<S>::widen(row[token])) : 0.0f;
+    }
+}
+
+// A block takes part blockIdx % parts, of `part_words` words, of row
+// blockIdx / parts.  With one part the results are written here.
+template <typename S, bool TOP, bool NT>
+__global__ void __launch_bounds__(kThreads)
+    tokens_kernel(const S* logits, uint64_t step, uint64_t cols, uint32_t parts, uint64_t part_words,
+                  Results out, Part* left, uint64_t* left_keys) {
+    constexpr int E = kWordElements<S>;
+    __shared__ float shared[3][kThreads / 64];
+    __shared__ std::conditional_t<TOP, Keys, char> keys;
+    const uint64_t at = blockIdx.x / parts;
+    const uint32_t part = blockIdx.x % parts;
+    const Row<S> row(logits + at * step, cols);
+    const uint64_t first = part * part_words;
+    const uint64_t words = row.words();
+    const uint64_t end = first + part_words < words ? first + part_words : words;
+    const int top = TOP ? static_cast<int>(out.top) : 0;
+
+    State state;
+    uint32_t least = 0;   // a logit's order has to be above it to be among the best
+    bool enough = false;  // ... once there are `top` of them
+    int count = 0;
+    if constexpr (TOP) {
+        if (threadIdx.x == 0) keys.count = 0;
+    }
+
+    Words<S, E> next[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; u++) {
+        const uint64_t word = first + u * kThreads + threadIdx.x;
+        if (word < end) row.template load<NT>(word, next[u]);
+    }
+    for (uint64_t from = first; from < end; from += kBatch * kThreads) {
+        float value[kBatch][E];
+        float highest = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kBatch; u++) {
+            const uint64_t word = from + u * kThreads + threadIdx.x;
+            if (word < end) {
+                next[u].get(value[u]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; e++) value[u][e] = -INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < E; e++) highest = fmaxf(highest, value[u][e]);
+            const uint64_t later = word + kBatch * kThreads;
+            if (later < end) row.template load<NT>(later, next[u]);
+        }
+        if (highest > state.most) move(state, highest);
+        const float origin = state.most == -INFINITY ? 0.0f : state.most;
+#pragma unroll
+        for (int u = 0; u < kBatch; u++) {
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const float d = value[u][e] - origin;
+                const float p = power(d);
+                state.sum += p;
+                // -infinity, whose power is 0, would make a NaN.
+                state.mean = fmaf(fmaxf(d, -1000.0f), p, state.mean);
+            }
+        }
+        if constexpr (TOP) {
+            Keys& k = keys;
+            // Every element of the batch whose key is at least `lowest`, and
+            // (with `enough`) whose logit is above `least`: later tokens lose
+            // ties to the best so far.
+            const auto take = [&](uint64_t lowest) {
+#pragma unroll
+                for (int u = 0; u < kBatch; u++) {
+                    const int64_t column = row.column(from + u * kThreads + threadIdx.x);
+                    const bool inside = from + u * kThreads + threadIdx.x < end;
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        if (!inside || !row.has(column + e) || (enough && ordered(value[u][e]) <= least)) continue;
+                        const uint64_t key = key_of(value[u][e], static_cast<uint32_t>(column + e));
+                        if (key < lowest) continue;
+                        const int to = atomicAdd(&k.count, 1);
+                        if (to < kRoom) k.keys[to] = key;
+                    }
+                }
+            };
+            const int before = count;
+            if (enough) {
+                if (ordered(highest) > least) take(0);
+                __syncthreads();
+                count = k.count;
+                __syncthreads();
+            }
+            if (!enough || count > kRoom) {
+                // Too many, or nothing yet to hold them against.
+                uint64_t own = 0;
+#pragma unroll
+                for (int u = 0; u < kBatch; u++) {
+                    const int64_t column = row.column(from + u * kThreads + threadIdx.x);
+                    const bool inside = from + u * kThreads + threadIdx.x < end;
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        if (!inside || !row.has(column + e) || (enough && ordered(value[u][e]) <= least)) continue;
+                        const uint64_t key = key_of(value[u][e], static_cast<uint32_t>(column + e));
+                        own = key > own ? key : own;
+                    }
+                }
+                k.highest[threadIdx.x] = own;
+                if (threadIdx.x == 0) {
+                    k.count = before;
+                    k.least = 0;
+                }
+                __syncthreads();
+                int rank = 0;
+                for (int j = 0; j < kThreads; j++) rank += k.highest[j] > own;
+                if (own != 0 && rank == top - 1) k.least = own;  // one lane at most: keys differ
+                __syncthreads();
+                take(k.least);
+                __syncthreads();
+                count = k.count;
+                __syncthreads();
+            }
+            if (count > kFull || !enough) {
+                select(k, count, top);
+                count = count < top ? count : top;
+                enough = count == top;
+                if (enough) least = static_cast<uint32_t>(k.keys[top - 1] >> 32);
+            }
+        }
+    }
+    state = joined(state, shared);
+    if constexpr (TOP) {
+        Keys& k = keys;
+        select(k, count, top);
+        count = count < top ? count : top;
+        if (parts == 1) {
+            for (int i = threadIdx.x; i < top; i += kThreads) {
+                out.top_log_probabilities[at * top + i] = log_probability(state, logit_of(k.keys[i]));
+                out.top_tokens[at * top + i] = token_of(k.keys[i]);
+            }
+        } else {
+            for (int i = threadIdx.x; i < top; i += kThreads) {
+                left_keys[static_cast<uint64_t>(blockIdx.x) * top + i] = i < count ? k.keys[i] : 0;
+            }
+        }
+    }
+    if (threadIdx.x != 0) return;
+    if (parts == 1) {
+        finish(state, row.row, cols, at, out);
+    } else {
+        left[blockIdx.x] = Part{state, static_cast<uint32_t>(count)};
+    }
+}
+
+// A row's parts joined: a block a row.  Each part's keys are in order, so a
+// key's rank among all is what a search in each part says.
+template <typename S>
+__global__ void __launch_bounds__(kThreads)
+    join_tokens_kernel(const S* logits, uint64_t step, uint64_t cols, uint32_t parts, Results out, const Part* left,
+                       const uint64_t* left_keys) {
+    __shared__ float shared[3][kThreads / 64];
+    const uint64_t at = blockIdx.x;
+    const Part* mine = left + at * parts;
+    State state;
+    if (threadIdx.x < parts) state = mine[threadIdx.x].state;
+    state = joined(state, shared);
+    if (threadIdx.x == 0) finish(state, logits + at * step, cols, at, out);
+    const uint32_t top = out.top;
+    const uint64_t* keys = left_keys + at * parts * top;
+    for (uint32_t i = threadIdx.x; i < parts * top; i += kThreads) {
+        const uint64_t key = keys[i];
+        if (key == 0) continue;  // none
+        uint32_t rank = 0;
+        for (uint32_t p = 0; p < parts && rank < top; p++) {
+            uint32_t low = 0, high = mine[p].count;  // keys[p][low..high) may be higher or not
+            while (low < high) {
+                const uint32_t middle = (low + high) / 2;
+                if (keys[p * top + middle] > key) low = middle + 1;
+                else high = middle;
+            }
+            rank += low;
+        }
+        if (rank >= top) continue;
+        out.top_log_probabilities[at * top + rank] = log_probability(state, logit_of(key));
+        out.top_tokens[at * top + rank] = token_of(key);
+    }
+}
+
+// ---- the gradient ----------------------------------------------------------------------
+
+struct Gradients {
+    const uint32_t* tokens;
+    const float* normalizers;
+    const float* entropies;
+    const float* d_log_probabilities;
+    const float* d_entropies;
+
+    // Of the rows from `first` on.
+    Gradients from(uint64_t first) const {
+        const auto at = [&](auto* p) { return p != nullptr ? p + first : nullptr; };
+        return {at(tokens), at(normalizers), at(entropies), at(d_log_probabilities), at(d_entropies)};
+    }
+};
+
+// A block takes kBatch words a lane of a row.  Every element is read and
+// written by the same lane, so the gradient may take the logits' place.
+template <typename S, bool ENTROPY, bool NT>
+__global__ void __launch_bounds__(kThreads)
+    tokens_back_kernel(const S* logits, uint64_t step, uint64_t cols, uint32_t parts, Gradients in, S* d_logits,
+                       uint64_t d_step) {
+    constexpr int E = kWordElements<S>;
+    const uint64_t at = blockIdx.x / parts;
+    const uint64_t first = static_cast<uint64_t>(blockIdx.x % parts) * kBatch * kThreads + threadIdx.x;
+    const Row<S> row(logits + at * step, cols);
+    S* to = d_logits + at * d_step;
+    const uint64_t words = row.words();
+
+    const float normalizer = in.normalizers[at];
+    const uint32_t token = in.d_log_probabilities != nullptr ? in.tokens[at] : ~0u;
+    const float g = token < cols ? in.d_log_probabilities[at] : 0.0f;
+    const float h = ENTROPY ? in.d_entropies[at] : 0.0f;
+    // -p (g + h (log p + H)) = p (base + slope log p)
+    const float base = ENTROPY ? -(g + h * in.entropies[at]) : -g, slope = -h;
+    // A row that nothing asks of, or that has nothing possible, has no gradient.
+    const bool none = (g == 0.0f && h == 0.0f) || normalizer == -INFINITY;
+
+    Words<S, E> in_words[kBatch];
+    if (!none) {
+#pragma unroll
+        for (int u = 0; u < kBatch; u++) {
+            if (first + u * kThreads < words) row.template load<NT>(first + u * kThreads, in_words[u]);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; u++) {
+        const uint64_t word = first + u * kThreads;
+        if (word >= words) break;
+        const int64_t column = row.column(word);
+        float v[E];
+        if (none) {
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] = 0.0f;
+        } else {
+            in_words[u].get(v);
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const float log_p = v[e] - normalizer;
+                const float p = power(log_p);
+                v[e] = ENTROPY ? p * fmaf(slope, fmaxf(log_p, -1e30f), base) : p * base;
+            }
+            const int64_t place = static_cast<int64_t>(token) - column;
+            if (g != 0.0f && place >= 0 && place < E) {
+#pragma unroll
+                for (int e = 0; e < E; e++) v[e] += e == place ? g : 0.0f;
+            }
+        }
+        if (row.whole(column)) {
+            Words<S, E> result;
+            result.put(v);
+            result.template store<NT>(to + column);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                if (row.has(column + e)) to[column + e] = Elem<S>::narrow(v[e]);
+            }
+        }
+    }
+}
+
+// ---- launches ------------------------------------------------------------------------------
+
+// A dispatch holds fewer than 2^32 work-items: rows beyond that many blocks
+// take another launch.
+constexpr uint64_t kMostBlocks = 0xffffffffu / kThreads;
+
+// `call(first row, rows)` over all rows in turn, `parts` blocks a row.
+template <typename Call>
+int in_launches(uint64_t rows, uint64_t parts, Call&& call) {
+    const uint64_t most = kMostBlocks / parts;
+    for (uint64_t first = 0; first < rows; first += most) {
+        const int status = call(first, rows - first < most ? rows - first : most);
+        if (status != TC_OK) return status;
+    }
+    return TC_OK;
+}
+
+template <typename S>
+int tokens(const S* logits, uint64_t step, uint64_t rows, uint64_t cols, const Results& out) {
+    TC_STREAM(s);
+    const uint64_t words = (cols + 2 * kWordElements<S> - 2) / kWordElements<S>;  // at most, wherever a row starts
+    // As many parts as give every compute unit four blocks, of two words a
+    // lane at least.
+    const uint64_t wanted = (static_cast<uint64_t>(compute_units()) * 4 + rows - 1) / rows;
+    const uint64_t most = (words + 2 * kThreads - 1) / (2 * kThreads);
+    uint64_t parts = wanted < most ? wanted : most;
+    if (parts > kMostParts) parts = kMostParts;
+    const uint64_t part_words = ((words + parts - 1) / parts + kThreads - 1) / kThreads * kThreads;
+    parts = (words + part_words - 1) / part_words;
+    Scratch left(parts > 1 ? rows * parts * sizeof(Part) : 0);
+    Scratch left_keys(parts > 1 ? rows * parts * out.top * sizeof(uint64_t) : 0);
+    if (left.status != TC_OK) return left.status;
+    if (left_keys.status != TC_OK) return left_keys.status;
+    Part* states = static_cast<Part*>(left.ptr);
+    uint64_t* keys = static_cast<uint64_t*>(left_keys.ptr);
+    const bool streams = sizeof(S) * rows * cols >= kStreamBytes;
+    return in_launches(rows, parts, [&](uint64_t first, uint64_t count) {
+        const Results here = out.from(first);
+        const S* from = logits + first * step;
+        const auto launch = [&](auto kernel) {
+            kernel<<<static_cast<uint32_t>(count * parts), kThreads, 0, s>>>(
+                from, step, cols, static_cast<uint32_t>(parts), part_words, here, states, keys);
+        };
+        if (out.top > 0) {
+            if (streams) launch(tokens_kernel<S, true, true>);
+            else launch(tokens_kernel<S, true, false>);
+        } else {
+            if (streams) launch(tokens_kernel<S, false, true>);
+            else launch(tokens_kernel<S, false, false>);
+        }
+        const int status = check_launch("log probabilities");
+        if (status != TC_OK || parts == 1) return status;
+        join_tokens_kernel<S><<<static_cast<uint32_t>(count), kThreads, 0, s>>>(
+            from, step, cols, static_cast<uint32_t>(parts), here, states, keys);
+        return check_launch("log probabilities");
+    });
+}
+
+template <typename S>
+int tokens_back(const S* logits, uint64_t step, uint64_t rows, uint64_t cols, const Gradients& in, S* d_logits,
+                uint64_t d_step) {
+    TC_STREAM(s);
+    const uint64_t words = (cols + 2 * kWordElements<S> - 2) / kWordElements<S>;
+    const uint64_t parts = (words + kBatch * kThreads - 1) / (kBatch * kThreads);
+    const bool streams = 2 * sizeof(S) * rows * cols >= kStreamBytes;
+    return in_launches(rows, parts, [&](uint64_t first, uint64_t count) {
+        const Gradients here = in.from(first);
+        const auto launch = [&](auto kernel) {
+            kernel<<<static_cast<uint32_t>(count * parts), kThreads, 0, s>>>(
+                logits + first * step, step, cols, static_cast<uint32_t>(parts), here, d_logits + first * d_step,
+                d_step);
+        };
+        if (in.d_entropies != nullptr) {
+            if (streams) launch(tokens_back_kernel<S, true, true>);
+            else launch(tokens_back_kernel<S, true, false>);
+        } else {
+            if (streams) launch(tokens_back_kernel<S, false, true>);
+            else launch(tokens_back_kernel<S, false, false>);
+        }
+        return check_launch("log probabilities, backward");
+    });
+}
+
+int check_tokens(const std::string& what, uint32_t dtype, uint64_t rows, uint64_t cols,
+                 std::initializer_list<uint64_t> steps) {
+    if (dtype_size(dtype) == 0 || dtype == TC_F64) return fail(TC_UNSUPPORTED, what + ": no kernel for " + dtype_name(dtype));
+    if (cols >= 0xffffffffu) {
+        return fail(TC_UNSUPPORTED, what + ": a token of 32 bits does not reach " + std::to_string(cols) + " logits");
+    }
+    for (uint64_t step : steps) {
+        if (rows > 1 && step < cols) {
+            return fail(TC_INVALID, what + ": rows of " + std::to_string(cols) + " elements " + std::to_string(step) +
+                                        " apart overlap");
+        }
+        if (rows > 0 && step > UINT64_MAX / 8 / rows) {
+            return fail(TC_INVALID, what + ": " + std::to_string(rows) + " rows " + std::to_string(step) +
+                                        " apart reach past the address space");
+        }
+    }
+    return TC_OK;
+}
+
+}  // namespace
+}  // namespace tc
+
+using namespace tc;
+
+extern "C" {
+
+int tc_log_probabilities(uint32_t dtype, const void* logits, uint64_t step, uint64_t rows, uint64_t cols,
+                         const uint32_t* tokens, float* log_probabilities, float* normalizers, float* entropies,
+                         uint32_t top, float* top_log_probabilities, uint32_t* top_tokens) {
+    const char* what = "log probabilities";
+    const int status = check_tokens(what, dtype, rows, cols, {step});
+    if (status != TC_OK) return status;
+    if (top > kMostTop) {
+        return fail(TC_UNSUPPORTED, std::string(what) + ": the top " + std::to_string(top) + " of at most " +
+                                        std::to_string(kMostTop));
+    }
+    if (top > cols) {
+        return fail(TC_INVALID, std::string(what) + ": the top " + std::to_string(top) + " of " + std::to_string(cols) +
+                                    " logits");
+    }
+    if (rows == 0) return TC_OK;
+    if (cols == 0) return fail(TC_INVALID, std::string(what) + ": rows of no logits");
+    if (logits == nullptr || (tokens == nullptr) != (log_probabilities == nullptr) ||
+        (top > 0 && any_null({top_log_probabilities, top_tokens}))) {
+        return null_operand(what);
+    }
+    const Results out{tokens, log_probabilities, normalizers, entropies, top, top_log_probabilities, top_tokens};
+    TC_DISPATCH_FLOAT(dtype, what, S, return ::tc::tokens<S>(static_cast<const S*>(logits), step, rows, cols, out))
+    return TC_OK;
+}
+
+int tc_log_probabilities_backward(uint32_t dtype, const void* logits, uint64_t step, uint64_t rows, uint64_t cols,
+                                  const uint32_t* tokens, const float* normalizers, const float* entropies,
+                                  const float* d_log_probabilities, const float* d_entropies, void* d_logits,
+                                  uint64_t d_step) {
+    const char* what = "log probabilities, backward";
+    const int status = check_tokens(what, dtype, rows, cols, {step, d_step});
+    if (status != TC_OK) return status;
+    if (rows == 0) return TC_OK;
+    if (cols == 0) return fail(TC_INVALID, std::string(what) + ": rows of no logits");
+    if (any_null({logits, normalizers, d_logits}) || (d_log_probabilities != nullptr && tokens == nullptr) ||
+        (d_entropies != nullptr && entropies == nullptr)) {
+        return null_operand(what);
+    }
+    const Gradients in{tokens, normalizers, entropies, d_log_probabilities, d_entropies};
+    TC_DISPATCH_FLOAT(dtype, what, S, return tokens_back<S>(static_cast<const S*>(logits), step, rows, cols, in,
+                                                           static_cast<S*>(d_logits), d_step))
+    return TC_OK;
+}
+
+}  // extern "C"

@@ -82,3 +82,40 @@ def layer_norm_backward(dy, x, weight, mean, scale):
     g = dy * weight
     dx = scale[:, None] * (g - g.mean(1, keepdims=True) - u * (g * u).mean(1, keepdims=True))
     return dx, (dy * u).sum(0), dy.sum(0)
+
+
+# ---- log probabilities ------------------------------------------------------
+
+
+def log_probabilities(x, tokens, top):
+    """(log p of the tokens, normalizers, entropies, top log p, top tokens)."""
+    rows, cols = x.shape
+    with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
+        most = x.max(1, keepdims=True)
+        shift = np.where(most == -np.inf, 0.0, most)
+        total = np.exp(x - shift).sum(1, keepdims=True)
+        normalizers = (shift + np.log(total))[:, 0]
+        log_p = np.where(most == -np.inf, -np.inf, x - normalizers[:, None])
+        p = np.exp(log_p)
+        entropies = -np.where(p == 0, 0.0, p * log_p).sum(1) + 0.0
+    given = np.array([log_p[r, t] if t < cols else 0.0 for r, t in enumerate(tokens)])
+    # Highest first, a NaN last, equal logits by the lower token.
+    order = np.lexsort((np.arange(cols)[None].repeat(rows, 0), -np.where(np.isnan(x), -np.inf, x), np.isnan(x)))
+    picked = order[:, :top]
+    return given, normalizers, entropies, np.take_along_axis(log_p, picked, 1), picked
+
+
+def log_probabilities_backward(x, tokens, normalizers, entropies, d_given, d_entropies):
+    d = np.zeros_like(x)
+    for r, t in enumerate(tokens):
+        g = d_given[r] if t < x.shape[1] else 0.0
+        h = d_entropies[r]
+        if (g == 0 and h == 0) or normalizers[r] == -np.inf:
+            continue
+        log_p = x[r] - normalizers[r]
+        p = np.exp(log_p)
+        with np.errstate(invalid="ignore"):
+            d[r] = -np.where(p == 0, 0.0, p * (g + h * (log_p + entropies[r])))
+        if t < x.shape[1]:
+            d[r, t] += g
+    return d

@@ -35,3 +35,29 @@ def test_layer_norm():
         lib.INVALID, "layer norm, backward: rows of no elements")
     # Nothing wanted, or nothing there: nothing is done, and no device is needed.
     assert refused(back, F, F, 64, 8, 64, 8, 2, 8, None, 64, 64, None, 8, None, None)[0] == lib.OK
+
+
+def test_log_probabilities():
+    F = lib.F32
+    run, back = "tc_log_probabilities", "tc_log_probabilities_backward"
+    assert refused(run, lib.F64, 64, 8, 2, 8, None, None, 64, None, 0, None, None) == (
+        lib.UNSUPPORTED, "log probabilities: no kernel for f64")
+    assert refused(run, F, 64, 7, 2, 8, None, None, 64, None, 0, None, None) == (
+        lib.INVALID, "log probabilities: rows of 8 elements 7 apart overlap")
+    assert refused(run, F, 64, 800, 2, 800, None, None, 64, None, 65, 64, 64) == (
+        lib.UNSUPPORTED, "log probabilities: the top 65 of at most 64")
+    assert refused(run, F, 64, 8, 2, 8, None, None, 64, None, 9, 64, 64) == (
+        lib.INVALID, "log probabilities: the top 9 of 8 logits")
+    assert refused(run, F, 64, 0, 2, 0, None, None, 64, None, 0, None, None) == (
+        lib.INVALID, "log probabilities: rows of no logits")
+    null = (lib.INVALID, "log probabilities: a null operand")
+    assert refused(run, F, None, 8, 2, 8, None, None, 64, None, 0, None, None) == null
+    assert refused(run, F, 64, 8, 2, 8, 64, None, 64, None, 0, None, None) == null
+    assert refused(run, F, 64, 8, 2, 8, None, 64, 64, None, 0, None, None) == null
+    assert refused(run, F, 64, 8, 2, 8, None, None, 64, None, 2, 64, None) == null
+    assert refused(run, F, 64, 2**33, 1, 2**32, None, None, 64, None, 0, None, None)[0] == lib.UNSUPPORTED
+    null = (lib.INVALID, "log probabilities, backward: a null operand")
+    assert refused(back, F, 64, 8, 2, 8, 64, None, None, 64, None, 64, 8) == null
+    assert refused(back, F, 64, 8, 2, 8, None, 64, None, 64, None, 64, 8) == null
+    assert refused(back, F, 64, 8, 2, 8, 64, 64, None, 64, 64, 64, 8) == null
+    assert refused(back, F, 64, 8, 2, 8, 64, 64, 64, 64, 64, 64, 5)[0] == lib.INVALID

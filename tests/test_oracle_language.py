@@ -32,3 +32,26 @@ def test_layer_norm_gradients_are_the_differences():
     assert np.allclose(dx, differences(loss, x), atol=1e-7)
     assert np.allclose(dw, differences(loss, weight), atol=1e-7)
     assert np.allclose(db, differences(loss, bias), atol=1e-7)
+
+
+def test_log_probability_gradients_are_the_differences():
+    rng = np.random.default_rng(2)
+    x = rng.standard_normal((4, 6)) * 2
+    tokens, d_given, d_entropies = np.array([1, 5, 6, 0]), rng.standard_normal(4), rng.standard_normal(4)
+    given, normalizers, entropies, _, _ = language.log_probabilities(x, tokens, 0)
+    d = language.log_probabilities_backward(x, tokens, normalizers, entropies, d_given, d_entropies)
+
+    def loss():
+        given, _, entropies, _, _ = language.log_probabilities(x, tokens, 0)
+        return float((given * d_given).sum() + (entropies * d_entropies).sum())
+
+    # Third derivatives below 10 here: 2e-10 from the step, 1e-10 from rounding.
+    assert np.allclose(d, differences(loss, x), atol=1e-8)
+
+
+def test_log_probabilities_of_impossible_tokens():
+    x = np.array([[0.0, -np.inf, np.log(3.0)], [-np.inf] * 3])
+    given, normalizers, entropies, top, tokens = language.log_probabilities(x, np.array([1, 0]), 3)
+    assert np.array_equal(given, [-np.inf, -np.inf]) and np.allclose(normalizers[0], np.log(4.0))
+    assert np.allclose(entropies, [np.log(4.0) - 0.75 * np.log(3.0), 0.0]) and normalizers[1] == -np.inf
+    assert np.array_equal(tokens, [[2, 0, 1], [0, 1, 2]]) and np.allclose(top[0, :2], np.log([0.75, 0.25]))
