@@ -22,11 +22,15 @@
 //
 // The most probable tokens are kept by a 64-bit key, the logit's bits in
 // order above the token's complement, so that equal logits go to the lowest
-// token and no two keys are equal.  A block collects the keys that beat the
-// last of its best so far in LDS and selects from them when they are many and
-// at the end.  However the logits lie they fit: of a batch that would not,
-// only keys at least as high as the k-th highest of the lanes' highest are
-// taken, and those are in k lanes.
+// token and no two keys are equal.  A block collects in LDS the keys that may
+// be among its best: of the first batch those at or above a logit that enough
+// lanes reach, then those above the last of the best so far, from which it
+// selects after batches 1, 2, 4, 8 and every eighth, so that few keys pass
+// and no batch waits for another.  Where they do not fit (logits that rise
+// along the row, or thousands of equal ones) or are too few (fewer tokens
+// possible than wanted), the block reads its part again, batch by batch: of a
+// batch that would not fit, only keys at least as high as the k-th highest of
+// the lanes' highest are taken, and those are in k lanes.
 
 #include <type_traits>
 
@@ -104,12 +108,27 @@ __device__ __forceinline__ uint64_t key_of(float v, uint32_t token) {
 __device__ __forceinline__ float logit_of(uint64_t key) { return unordered(static_cast<uint32_t>(key >> 32)); }
 __device__ __forceinline__ uint32_t token_of(uint64_t key) { return ~static_cast<uint32_t>(key); }
 
+// The order of -infinity: of every logit that is no number above it.
+constexpr uint32_t kLowest = 0x007fffff;
+
+// The highest order that `lanes` lanes of the wave reach (0: fewer have any
+// logit), bit by bit.
+__device__ __forceinline__ uint32_t reached_by(int lanes, uint32_t order) {
+    uint32_t reached = 0;
+    for (int bit = 31; bit >= 0; bit--) {
+        const uint32_t next = reached | 1u << bit;
+        if (__popcll(__ballot(order >= next)) >= lanes) reached = next;
+    }
+    return reached;
+}
+
 // The keys that a block has collected.
 struct Keys {
     uint64_t keys[kRoom];
     uint64_t best[kMostTop];
     uint64_t highest[kThreads];  // of each lane's batch
-    uint64_t least;              // of the batch's keys that are taken
+    uint64_t lowest;             // of the batch's keys that are taken
+    uint32_t reached[kThreads / 64];
     int count;
 };
 
@@ -166,11 +185,73 @@ struct Row {
     }
 };
 
-// What a block leaves of its part of a row, where rows are split.
-struct Part {
-    State state;
-    uint32_t count;  // keys, best first
-};
+// The `top` best keys of words first .. end of a row (or all, if fewer), in
+// order, whatever the logits: every batch waits for the one before.
+template <typename S, bool NT>
+__device__ void collect_again(const Row<S>& row, uint64_t first, uint64_t end, int top, Keys& k) {
+    constexpr int E = Row<S>::E;
+    uint32_t least = 0;   // a logit's order has to be above it to be among the best
+    bool enough = false;  // ... once there are `top` of them: later tokens lose ties
+    int count = 0;
+    if (threadIdx.x == 0) k.count = 0;
+    __syncthreads();
+    for (uint64_t from = first; from < end; from += kBatch * kThreads) {
+        // `body(key)` of each element of the lane's batch that may be taken.
+        const auto each = [&](auto&& body) {
+            for (int u = 0; u < kBatch; u++) {
+                const uint64_t word = from + u * kThreads + threadIdx.x;
+                if (word >= end) break;
+                const int64_t column = row.column(word);
+                Words<S, E> words;
+                row.template load<false>(word, words);
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const float v = words.at(e);
+                    if (row.has(column + e) && !(enough && ordered(v) <= least)) {
+                        body(key_of(v, static_cast<uint32_t>(column + e)));
+                    }
+                }
+            }
+        };
+        const auto put = [&](uint64_t key) {
+            const int to = atomicAdd(&k.count, 1);
+            if (to < kRoom) k.keys[to] = key;
+        };
+        const int before = count;
+        if (enough) {
+            each(put);
+            __syncthreads();
+            count = k.count;
+            __syncthreads();
+        }
+        if (!enough || count > kRoom) {
+            // Too many, or nothing yet to hold them against.
+            uint64_t own = 0;
+            each([&](uint64_t key) { own = key > own ? key : own; });
+            k.highest[threadIdx.x] = own;
+            if (threadIdx.x == 0) k.count = before, k.lowest = 0;
+            __syncthreads();
+            int rank = 0;
+            for (int j = 0; j < kThreads; j++) rank += k.highest[j] > own;
+            if (own != 0 && rank == top - 1) k.lowest = own;  // one lane at most: keys differ
+            __syncthreads();
+            const uint64_t lowest = k.lowest;
+            each([&](uint64_t key) {
+                if (key >= lowest) put(key);
+            });
+            __syncthreads();
+            count = k.count;
+            __syncthreads();
+        }
+        if (count > kFull || !enough) {
+            select(k, count, top);
+            count = count < top ? count : top;
+            enough = count == top;
+            if (enough) least = static_cast<uint32_t>(k.keys[top - 1] >> 32);
+        }
+    }
+    select(k, count, top);
+}
 
 struct Results {
     const uint32_t* tokens;
@@ -212,10 +293,11 @@ __device__ void finish(const State& s, const S* row, uint64_t cols, uint64_t at,
 template <typename S, bool TOP, bool NT>
 __global__ void __launch_bounds__(kThreads)
     tokens_kernel(const S* logits, uint64_t step, uint64_t cols, uint32_t parts, uint64_t part_words,
-                  Results out, Part* left, uint64_t* left_keys) {
+                  Results out, State* left, uint64_t* left_keys) {
     constexpr int E = kWordElements<S>;
     __shared__ float shared[3][kThreads / 64];
     __shared__ std::conditional_t<TOP, Keys, char> keys;
+    (void)keys;
     const uint64_t at = blockIdx.x / parts;
     const uint32_t part = blockIdx.x % parts;
     const Row<S> row(logits + at * step, cols);
@@ -225,9 +307,8 @@ __global__ void __launch_bounds__(kThreads)
     const int top = TOP ? static_cast<int>(out.top) : 0;
 
     State state;
-    uint32_t least = 0;   // a logit's order has to be above it to be among the best
-    bool enough = false;  // ... once there are `top` of them
-    int count = 0;
+    uint32_t least = kLowest;  // a logit's order has to be above it to be collected
+    bool fits = true;          // what was collected
     if constexpr (TOP) {
         if (threadIdx.x == 0) keys.count = 0;
     }
@@ -238,9 +319,10 @@ __global__ void __launch_bounds__(kThreads)
         const uint64_t word = first + u * kThreads + threadIdx.x;
         if (word < end) row.template load<NT>(word, next[u]);
     }
+    uint32_t batch = 0;
     for (uint64_t from = first; from < end; from += kBatch * kThreads) {
         float value[kBatch][E];
-        float highest = -INFINITY;
+        float highest[kBatch], most = -INFINITY;
 #pragma unroll
         for (int u = 0; u < kBatch; u++) {
             const uint64_t word = from + u * kThreads + threadIdx.x;
@@ -250,12 +332,14 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
                 for (int e = 0; e < E; e++) value[u][e] = -INFINITY;
             }
+            highest[u] = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < E; e++) highest = fmaxf(highest, value[u][e]);
+            for (int e = 0; e < E; e++) highest[u] = fmaxf(highest[u], value[u][e]);
+            most = fmaxf(most, highest[u]);
             const uint64_t later = word + kBatch * kThreads;
             if (later < end) row.template load<NT>(later, next[u]);
         }
-        if (highest > state.most) move(state, highest);
+        if (most > state.most) move(state, most);
         const float origin = state.most == -INFINITY ? 0.0f : state.most;
 #pragma unroll
         for (int u = 0; u < kBatch; u++) {
@@ -269,82 +353,60 @@ __global__ void __launch_bounds__(kThreads)
             }
         }
         if constexpr (TOP) {
-            Keys& k = keys;
-            // Every element of the batch whose key is at least `lowest`, and
-            // (with `enough`) whose logit is above `least`: later tokens lose
-            // ties to the best so far.
-            const auto take = [&](uint64_t lowest) {
+            if (batch++ == 0) {
+                // The least of the waves' logits that a wave's share of the
+                // top is at or above: `top` lanes' highest are.
+                const uint32_t reached = reached_by((top + kThreads / 64 - 1) / (kThreads / 64), ordered(most));
+                if (threadIdx.x % 64 == 0) keys.reached[threadIdx.x / 64] = reached;
+                __syncthreads();
+                uint32_t all = keys.reached[0];
+                for (int w = 1; w < kThreads / 64; w++) all = keys.reached[w] < all ? keys.reached[w] : all;
+                if (all > kLowest) least = all - 1;
+            }
+            // (A row has fewer than 2^32 logits, and a NaN is never highest.)
+            if (fits && ordered(most) > least) {
 #pragma unroll
                 for (int u = 0; u < kBatch; u++) {
-                    const int64_t column = row.column(from + u * kThreads + threadIdx.x);
-                    const bool inside = from + u * kThreads + threadIdx.x < end;
+                    if (ordered(highest[u]) <= least) continue;
+                    const uint32_t column = static_cast<uint32_t>(row.column(from + u * kThreads + threadIdx.x));
 #pragma unroll
                     for (int e = 0; e < E; e++) {
-                        if (!inside || !row.has(column + e) || (enough && ordered(value[u][e]) <= least)) continue;
-                        const uint64_t key = key_of(value[u][e], static_cast<uint32_t>(column + e));
-                        if (key < lowest) continue;
-                        const int to = atomicAdd(&k.count, 1);
-                        if (to < kRoom) k.keys[to] = key;
+                        if (ordered(value[u][e]) <= least) continue;
+                        const int to = atomicAdd(&keys.count, 1);
+                        if (to < kRoom) keys.keys[to] = key_of(value[u][e], column + e);
                     }
                 }
-            };
-            const int before = count;
-            if (enough) {
-                if (ordered(highest) > least) take(0);
-                __syncthreads();
-                count = k.count;
-                __syncthreads();
             }
-            if (!enough || count > kRoom) {
-                // Too many, or nothing yet to hold them against.
-                uint64_t own = 0;
-#pragma unroll
-                for (int u = 0; u < kBatch; u++) {
-                    const int64_t column = row.column(from + u * kThreads + threadIdx.x);
-                    const bool inside = from + u * kThreads + threadIdx.x < end;
-#pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        if (!inside || !row.has(column + e) || (enough && ordered(value[u][e]) <= least)) continue;
-                        const uint64_t key = key_of(value[u][e], static_cast<uint32_t>(column + e));
-                        own = key > own ? key : own;
-                    }
+            if ((batch & (batch - 1)) == 0 || batch % 8 == 0) {
+                __syncthreads();
+                const int count = keys.count;
+                __syncthreads();
+                fits = count <= kRoom;
+                if (fits && count >= top) {
+                    select(keys, count, top);
+                    least = static_cast<uint32_t>(keys.keys[top - 1] >> 32);
                 }
-                k.highest[threadIdx.x] = own;
-                if (threadIdx.x == 0) {
-                    k.count = before;
-                    k.least = 0;
-                }
-                __syncthreads();
-                int rank = 0;
-                for (int j = 0; j < kThreads; j++) rank += k.highest[j] > own;
-                if (own != 0 && rank == top - 1) k.least = own;  // one lane at most: keys differ
-                __syncthreads();
-                take(k.least);
-                __syncthreads();
-                count = k.count;
-                __syncthreads();
-            }
-            if (count > kFull || !enough) {
-                select(k, count, top);
-                count = count < top ? count : top;
-                enough = count == top;
-                if (enough) least = static_cast<uint32_t>(k.keys[top - 1] >> 32);
             }
         }
     }
     state = joined(state, shared);
     if constexpr (TOP) {
-        Keys& k = keys;
-        select(k, count, top);
-        count = count < top ? count : top;
-        if (parts == 1) {
-            for (int i = threadIdx.x; i < top; i += kThreads) {
-                out.top_log_probabilities[at * top + i] = log_probability(state, logit_of(k.keys[i]));
-                out.top_tokens[at * top + i] = token_of(k.keys[i]);
-            }
+        __syncthreads();
+        int count = keys.count;
+        __syncthreads();
+        if (count < top || count > kRoom) {
+            collect_again<S, NT>(row, first, end, top, keys);
+            count = keys.count;
         } else {
-            for (int i = threadIdx.x; i < top; i += kThreads) {
-                left_keys[static_cast<uint64_t>(blockIdx.x) * top + i] = i < count ? k.keys[i] : 0;
+            select(keys, count, top);
+            count = top;
+        }
+        for (int i = threadIdx.x; i < top; i += kThreads) {
+            if (parts == 1) {
+                out.top_log_probabilities[at * top + i] = log_probability(state, logit_of(keys.keys[i]));
+                out.top_tokens[at * top + i] = token_of(keys.keys[i]);
+            } else {
+                left_keys[static_cast<uint64_t>(blockIdx.x) * top + i] = i < count ? keys.keys[i] : 0;
             }
         }
     }
@@ -352,38 +414,41 @@ __global__ void __launch_bounds__(kThreads)
     if (parts == 1) {
         finish(state, row.row, cols, at, out);
     } else {
-        left[blockIdx.x] = Part{state, static_cast<uint32_t>(count)};
+        left[blockIdx.x] = state;
     }
 }
 
-// A row's parts joined: a block a row.  Each part's keys are in order, so a
-// key's rank among all is what a search in each part says.
+// A row's parts joined: a block a row.  No key below the last of a part's
+// `top` is among the row's; what is left is few.
 template <typename S>
 __global__ void __launch_bounds__(kThreads)
-    join_tokens_kernel(const S* logits, uint64_t step, uint64_t cols, uint32_t parts, Results out, const Part* left,
+    join_tokens_kernel(const S* logits, uint64_t step, uint64_t cols, uint32_t parts, Results out, const State* left,
                        const uint64_t* left_keys) {
     __shared__ float shared[3][kThreads / 64];
+    __shared__ uint64_t keys[kMostParts * kMostTop];
+    __shared__ uint64_t lasts[kMostParts];
+    __shared__ int survivors;
     const uint64_t at = blockIdx.x;
-    const Part* mine = left + at * parts;
+    const uint32_t top = out.top;
     State state;
-    if (threadIdx.x < parts) state = mine[threadIdx.x].state;
+    if (threadIdx.x < parts) state = left[at * parts + threadIdx.x];
+    if (threadIdx.x < parts && top > 0) lasts[threadIdx.x] = left_keys[(at * parts + threadIdx.x) * top + top - 1];
+    if (threadIdx.x == 0) survivors = 0;
     state = joined(state, shared);
     if (threadIdx.x == 0) finish(state, logits + at * step, cols, at, out);
-    const uint32_t top = out.top;
-    const uint64_t* keys = left_keys + at * parts * top;
+    if (top == 0) return;
+    uint64_t lowest = 1;  // 0 is no key
+    for (uint32_t p = 0; p < parts; p++) lowest = lasts[p] > lowest ? lasts[p] : lowest;
     for (uint32_t i = threadIdx.x; i < parts * top; i += kThreads) {
+        const uint64_t key = left_keys[at * parts * top + i];
+        if (key >= lowest) keys[atomicAdd(&survivors, 1)] = key;
+    }
+    __syncthreads();
+    const int count = survivors;
+    for (int i = threadIdx.x; i < count; i += kThreads) {
         const uint64_t key = keys[i];
-        if (key == 0) continue;  // none
         uint32_t rank = 0;
-        for (uint32_t p = 0; p < parts && rank < top; p++) {
-            uint32_t low = 0, high = mine[p].count;  // keys[p][low..high) may be higher or not
-            while (low < high) {
-                const uint32_t middle = (low + high) / 2;
-                if (keys[p * top + middle] > key) low = middle + 1;
-                else high = middle;
-            }
-            rank += low;
-        }
+        for (int j = 0; j < count; j++) rank += keys[j] > key;
         if (rank >= top) continue;
         out.top_log_probabilities[at * top + rank] = log_probability(state, logit_of(key));
         out.top_tokens[at * top + rank] = token_of(key);
@@ -500,11 +565,11 @@ int tokens(const S* logits, uint64_t step, uint64_t rows, uint64_t cols, const R
     if (parts > kMostParts) parts = kMostParts;
     const uint64_t part_words = ((words + parts - 1) / parts + kThreads - 1) / kThreads * kThreads;
     parts = (words + part_words - 1) / part_words;
-    Scratch left(parts > 1 ? rows * parts * sizeof(Part) : 0);
+    Scratch left(parts > 1 ? rows * parts * sizeof(State) : 0);
     Scratch left_keys(parts > 1 ? rows * parts * out.top * sizeof(uint64_t) : 0);
     if (left.status != TC_OK) return left.status;
     if (left_keys.status != TC_OK) return left_keys.status;
-    Part* states = static_cast<Part*>(left.ptr);
+    State* states = static_cast<State*>(left.ptr);
     uint64_t* keys = static_cast<uint64_t*>(left_keys.ptr);
     const bool streams = sizeof(S) * rows * cols >= kStreamBytes;
     return in_launches(rows, parts, [&](uint64_t first, uint64_t count) {
