@@ -690,6 +690,24 @@ int tc_log_probabilities_backward(uint32_t dtype, const void* logits, uint64_t s
                                   const float* d_log_probabilities, const float* d_entropies, void* d_logits,
                                   uint64_t d_step);
 
+/* ---- the norm over all gradients ------------------------------------------ */
+
+/* The Euclidean norm over all elements of `count` tensors, tensor k holding
+ * `lens[k]` elements of `dtypes[k]` at `tensors[k]` (host arrays of device
+ * pointers), into the device f32 `norm`.  Squares are summed in f64 in an
+ * order that depends on the shapes alone. */
+int tc_global_norm(uint32_t count, const uint32_t* dtypes, const void* const* tensors, const uint64_t* lens,
+                   float* norm);
+
+/* The same, and every tensor into `outputs[k]` (which may be `tensors[k]`
+ * itself, and must not otherwise overlap any tensor) scaled by limit / norm
+ * where the norm is above `limit`, unscaled where it is not: gradients
+ * clipped before an optimizer's step.  A norm that is not finite scales
+ * nothing, so that the caller, who has it, can leave the step out.  A
+ * `limit` below zero or NaN is refused. */
+int tc_clip_global_norm(uint32_t count, const uint32_t* dtypes, const void* const* tensors, const uint64_t* lens,
+                        float limit, void* const* outputs, float* norm);
+
 #ifdef __cplusplus
 }
 #endif

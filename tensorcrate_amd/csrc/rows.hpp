@@ -196,4 +196,56 @@ struct Run {
 template <typename T>
 constexpr int kWordElements = 16 / static_cast<int>(sizeof(T));
 
+// A row in the words of memory, 16-byte aligned wherever it starts: the first
+// may begin before the row and the last end behind it, and of those only the
+// row's elements are read (`around` in place of the others) and written.
+template <typename S>
+struct Row {
+    static constexpr int E = kWordElements<S>;
+    const S* row;
+    uint64_t cols;
+    int lead;  // elements of the first word that are not the row's
+
+    __device__ __forceinline__ Row(const S* at, uint64_t n)
+        : row(at), cols(n), lead(static_cast<int>(reinterpret_cast<uintptr_t>(at) / sizeof(S) % E)) {}
+    __device__ __forceinline__ uint64_t words() const { return (cols + lead + E - 1) / E; }
+    // Column of the word's first element (of word 0, possibly before the row).
+    __device__ __forceinline__ int64_t column(uint64_t word) const {
+        return static_cast<int64_t>(word * E) - lead;
+    }
+    __device__ __forceinline__ bool whole(int64_t column) const {
+        return column >= 0 && column + E <= static_cast<int64_t>(cols);
+    }
+    __device__ __forceinline__ bool has(int64_t column) const {
+        return column >= 0 && column < static_cast<int64_t>(cols);
+    }
+    template <bool NT>
+    __device__ __forceinline__ void load(uint64_t word, Words<S, E>& out, float around = -INFINITY) const {
+        const int64_t at = column(word);
+        if (whole(at)) {
+            out.template load<NT>(row + at);
+        } else {
+            float v[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] = has(at + e) ? Elem<S>::widen(row[at + e]) : around;
+            out.put(v);
+        }
+    }
+    // The word's results, to the same columns of another row.
+    template <bool NT>
+    __device__ __forceinline__ void store(uint64_t word, S* to, const float (&v)[E]) const {
+        const int64_t at = column(word);
+        if (whole(at)) {
+            Words<S, E> out;
+            out.put(v);
+            out.template store<NT>(to + at);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                if (has(at + e)) to[at + e] = Elem<S>::narrow(v[e]);
+            }
+        }
+    }
+};
+
 }  // namespace tc

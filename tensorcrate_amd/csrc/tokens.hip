@@ -111,11 +111,11 @@ __device__ __forceinline__ uint32_t token_of(uint64_t key) { return ~static_cast
 // The order of -infinity: of every logit that is no number above it.
 constexpr uint32_t kLowest = 0x007fffff;
 
-// The highest order that `lanes` lanes of the wave reach (0: fewer have any
-// logit), bit by bit.
+// The highest order of 16 bits, zeros below them, that `lanes` lanes of the
+// wave reach (0: fewer have any logit), bit by bit.
 __device__ __forceinline__ uint32_t reached_by(int lanes, uint32_t order) {
     uint32_t reached = 0;
-    for (int bit = 31; bit >= 0; bit--) {
+    for (int bit = 31; bit >= 16; bit--) {
         const uint32_t next = reached | 1u << bit;
         if (__popcll(__ballot(order >= next)) >= lanes) reached = next;
     }
@@ -132,12 +132,26 @@ struct Keys {
     int count;
 };
 
+// How many of the keys are above `key`.  Eight are read at a time: one by one
+// the reads' latency, not their number, is what a rank would take.
+__device__ __forceinline__ int rank_among(const uint64_t* keys, int count, uint64_t key) {
+    int rank = 0, j = 0;
+    for (; j + 8 <= count; j += 8) {
+        uint64_t other[8];
+#pragma unroll
+        for (int q = 0; q < 8; q++) other[q] = keys[j + q];
+#pragma unroll
+        for (int q = 0; q < 8; q++) rank += other[q] > key;
+    }
+    for (; j < count; j++) rank += keys[j] > key;
+    return rank;
+}
+
 // The `top` highest of the collected keys, in order, are what is left of them.
 __device__ void select(Keys& k, int count, int top) {
     for (int i = threadIdx.x; i < count; i += kThreads) {
         const uint64_t key = k.keys[i];
-        int rank = 0;
-        for (int j = 0; j < count; j++) rank += k.keys[j] > key;
+        const int rank = rank_among(k.keys, count, key);
         if (rank < top) k.best[rank] = key;
     }
     __syncthreads();
@@ -146,44 +160,6 @@ __device__ void select(Keys& k, int count, int top) {
     if (threadIdx.x == 0) k.count = left;
     __syncthreads();
 }
-
-// ---- a row's words -------------------------------------------------------------------
-
-// The row's words are those of memory: the first may begin before the row and
-// the last end behind it.
-template <typename S>
-struct Row {
-    static constexpr int E = kWordElements<S>;
-    const S* row;
-    uint64_t cols;
-    int lead;  // elements of the first word that are not the row's
-
-    __device__ __forceinline__ Row(const S* at, uint64_t n)
-        : row(at), cols(n), lead(static_cast<int>(reinterpret_cast<uintptr_t>(at) / sizeof(S) % E)) {}
-    __device__ __forceinline__ uint64_t words() const { return (cols + lead + E - 1) / E; }
-    // Column of the word's first element (of word 0, possibly before the row).
-    __device__ __forceinline__ int64_t column(uint64_t word) const {
-        return static_cast<int64_t>(word * E) - lead;
-    }
-    __device__ __forceinline__ bool whole(int64_t column) const {
-        return column >= 0 && column + E <= static_cast<int64_t>(cols);
-    }
-    __device__ __forceinline__ bool has(int64_t column) const {
-        return column >= 0 && column < static_cast<int64_t>(cols);
-    }
-    template <bool NT>
-    __device__ __forceinline__ void load(uint64_t word, Words<S, E>& out) const {
-        const int64_t at = column(word);
-        if (whole(at)) {
-            out.template load<NT>(row + at);
-        } else {
-            float v[E];
-#pragma unroll
-            for (int e = 0; e < E; e++) v[e] = has(at + e) ? Elem<S>::widen(row[at + e]) : -INFINITY;
-            out.put(v);
-        }
-    }
-};
 
 // The `top` best keys of words first .. end of a row (or all, if fewer), in
 // order, whatever the logits: every batch waits for the one before.
@@ -231,8 +207,7 @@ __device__ void collect_again(const Row<S>& row, uint64_t first, uint64_t end, i
             k.highest[threadIdx.x] = own;
             if (threadIdx.x == 0) k.count = before, k.lowest = 0;
             __syncthreads();
-            int rank = 0;
-            for (int j = 0; j < kThreads; j++) rank += k.highest[j] > own;
+            const int rank = rank_among(k.highest, kThreads, own);
             if (own != 0 && rank == top - 1) k.lowest = own;  // one lane at most: keys differ
             __syncthreads();
             const uint64_t lowest = k.lowest;
@@ -276,22 +251,27 @@ __device__ __forceinline__ float log_probability(const State& s, float logit) {
     return (logit - s.most) - logf(s.sum);
 }
 
-// One lane writes the row's results.
+// The logit of the row's token, `*some` false where it has none; read before the row
+// is, so that the results do not wait for it.
 template <typename S>
-__device__ void finish(const State& s, const S* row, uint64_t cols, uint64_t at, const Results& out) {
+__device__ __forceinline__ float given_logit(const S* row, uint64_t cols, uint64_t at, const Results& out, bool* some) {
+    const uint32_t token = out.tokens != nullptr ? out.tokens[at] : ~0u;
+    *some = token < cols;
+    return *some ? Elem<S>::widen(row[token]) : 0.0f;
+}
+
+// One lane writes the row's results.
+__device__ void finish(const State& s, float logit, bool some, uint64_t at, const Results& out) {
     const bool none = s.most == -INFINITY && s.sum == 0.0f;
     if (out.normalizers != nullptr) out.normalizers[at] = none ? -INFINITY : s.most + logf(s.sum);
     if (out.entropies != nullptr) out.entropies[at] = none ? 0.0f : logf(s.sum) - s.mean / s.sum;
-    if (out.log_probabilities != nullptr) {
-        const uint32_t token = out.tokens[at];
-        out.log_probabilities[at] = token < cols ? log_probability(s, Elem<S>::widen(row[token])) : 0.0f;
-    }
+    if (out.log_probabilities != nullptr) out.log_probabilities[at] = some ? log_probability(s, logit) : 0.0f;
 }
 
 // A block takes part blockIdx % parts, of `part_words` words, of row
 // blockIdx / parts.  With one part the results are written here.
 template <typename S, bool TOP, bool NT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(TOP ? 5 : 6)))
     tokens_kernel(const S* logits, uint64_t step, uint64_t cols, uint32_t parts, uint64_t part_words,
                   Results out, State* left, uint64_t* left_keys) {
     constexpr int E = kWordElements<S>;
@@ -306,9 +286,11 @@ __global__ void __launch_bounds__(kThreads)
     const uint64_t end = first + part_words < words ? first + part_words : words;
     const int top = TOP ? static_cast<int>(out.top) : 0;
 
+    bool some;
+    const float logit = given_logit(row.row, cols, at, out, &some);
     State state;
-    uint32_t least = kLowest;  // a logit's order has to be above it to be collected
-    bool fits = true;          // what was collected
+    float least = -INFINITY;  // a logit has to be above it to be collected
+    bool fits = true;         // what was collected
     if constexpr (TOP) {
         if (threadIdx.x == 0) keys.count = 0;
     }
@@ -361,19 +343,22 @@ __global__ void __launch_bounds__(kThreads)
                 __syncthreads();
                 uint32_t all = keys.reached[0];
                 for (int w = 1; w < kThreads / 64; w++) all = keys.reached[w] < all ? keys.reached[w] : all;
-                if (all > kLowest) least = all - 1;
+                if (all > kLowest) least = unordered(all - 1);
             }
-            // (A row has fewer than 2^32 logits, and a NaN is never highest.)
-            if (fits && ordered(most) > least) {
+            if (fits && most > least) {
 #pragma unroll
                 for (int u = 0; u < kBatch; u++) {
-                    if (ordered(highest[u]) <= least) continue;
+                    if (!(highest[u] > least)) continue;
+                    int to = 0;
+#pragma unroll
+                    for (int e = 0; e < E; e++) to += value[u][e] > least;
+                    to = atomicAdd(&keys.count, to);
                     const uint32_t column = static_cast<uint32_t>(row.column(from + u * kThreads + threadIdx.x));
 #pragma unroll
                     for (int e = 0; e < E; e++) {
-                        if (ordered(value[u][e]) <= least) continue;
-                        const int to = atomicAdd(&keys.count, 1);
+                        if (!(value[u][e] > least)) continue;
                         if (to < kRoom) keys.keys[to] = key_of(value[u][e], column + e);
+                        to++;
                     }
                 }
             }
@@ -384,7 +369,7 @@ __global__ void __launch_bounds__(kThreads)
                 fits = count <= kRoom;
                 if (fits && count >= top) {
                     select(keys, count, top);
-                    least = static_cast<uint32_t>(keys.keys[top - 1] >> 32);
+                    least = logit_of(keys.keys[top - 1]);
                 }
             }
         }
@@ -412,43 +397,53 @@ __global__ void __launch_bounds__(kThreads)
     }
     if (threadIdx.x != 0) return;
     if (parts == 1) {
-        finish(state, row.row, cols, at, out);
+        finish(state, logit, some, at, out);
     } else {
         left[blockIdx.x] = state;
     }
 }
 
-// A row's parts joined: a block a row.  No key below the last of a part's
-// `top` is among the row's; what is left is few.
+// A row's parts joined: a block a row.  Each part's keys are in order, so if
+// the j-th of n parts is at or above a bound, j n keys are: with j n at least
+// `top`, no key below it is among the row's, and few are above it.
 template <typename S>
 __global__ void __launch_bounds__(kThreads)
     join_tokens_kernel(const S* logits, uint64_t step, uint64_t cols, uint32_t parts, Results out, const State* left,
                        const uint64_t* left_keys) {
     __shared__ float shared[3][kThreads / 64];
     __shared__ uint64_t keys[kMostParts * kMostTop];
-    __shared__ uint64_t lasts[kMostParts];
     __shared__ int survivors;
     const uint64_t at = blockIdx.x;
     const uint32_t top = out.top;
+    // Everything that is read is on its way before anything is worked on.
+    bool some;
+    const float logit = given_logit(logits + at * step, cols, at, out, &some);
     State state;
     if (threadIdx.x < parts) state = left[at * parts + threadIdx.x];
-    if (threadIdx.x < parts && top > 0) lasts[threadIdx.x] = left_keys[(at * parts + threadIdx.x) * top + top - 1];
+    uint64_t mine[kMostParts * kMostTop / kThreads];
+    const uint32_t depth = (top + parts - 1) / parts, part = threadIdx.x % 64;
+    const uint64_t jth = top > 0 && part < parts ? left_keys[(at * parts + part) * top + depth - 1] : 0;
+#pragma unroll
+    for (int k = 0; k < static_cast<int>(kMostParts * kMostTop) / kThreads; k++) {
+        const uint32_t i = threadIdx.x + k * kThreads;
+        mine[k] = i < parts * top ? left_keys[at * parts * top + i] : 0;
+    }
     if (threadIdx.x == 0) survivors = 0;
     state = joined(state, shared);
-    if (threadIdx.x == 0) finish(state, logits + at * step, cols, at, out);
+    if (threadIdx.x == 0) finish(state, logit, some, at, out);
     if (top == 0) return;
-    uint64_t lowest = 1;  // 0 is no key
-    for (uint32_t p = 0; p < parts; p++) lowest = lasts[p] > lowest ? lasts[p] : lowest;
-    for (uint32_t i = threadIdx.x; i < parts * top; i += kThreads) {
-        const uint64_t key = left_keys[at * parts * top + i];
+    const uint32_t reached =
+        reached_by(static_cast<int>((top + depth - 1) / depth), static_cast<uint32_t>(jth >> 32));
+    const uint64_t lowest = reached > 0 ? static_cast<uint64_t>(reached) << 32 : 1;  // 0 is no key
+#pragma unroll
+    for (const uint64_t key : mine) {
         if (key >= lowest) keys[atomicAdd(&survivors, 1)] = key;
     }
     __syncthreads();
     const int count = survivors;
     for (int i = threadIdx.x; i < count; i += kThreads) {
         const uint64_t key = keys[i];
-        uint32_t rank = 0;
-        for (int j = 0; j < count; j++) rank += keys[j] > key;
+        const uint32_t rank = static_cast<uint32_t>(rank_among(keys, count, key));
         if (rank >= top) continue;
         out.top_log_probabilities[at * top + rank] = log_probability(state, logit_of(key));
         out.top_tokens[at * top + rank] = token_of(key);
@@ -523,16 +518,7 @@ __global__ void __launch_bounds__(kThreads)
                 for (int e = 0; e < E; e++) v[e] += e == place ? g : 0.0f;
             }
         }
-        if (row.whole(column)) {
-            Words<S, E> result;
-            result.put(v);
-            result.template store<NT>(to + column);
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                if (row.has(column + e)) to[column + e] = Elem<S>::narrow(v[e]);
-            }
-        }
+        row.template store<NT>(word, to, v);
     }
 }
 

@@ -201,6 +201,9 @@ SIGNATURES = {
                            u32],
     "tc_layer_norm": [u32, u32, vp, u64, u64, u64, vp, vp, f32, vp, u64, vp, vp],
     "tc_layer_norm_backward": [u32, u32, vp, u64, vp, u64, u64, u64, vp, vp, vp, vp, u64, vp, vp],
+    "tc_global_norm": [u32, ctypes.POINTER(u32), ctypes.POINTER(vp), ctypes.POINTER(u64), vp],
+    "tc_clip_global_norm": [u32, ctypes.POINTER(u32), ctypes.POINTER(vp), ctypes.POINTER(u64), f32,
+                            ctypes.POINTER(vp), vp],
     "tc_log_probabilities": [u32, vp, u64, u64, u64, vp, vp, vp, vp, u32, vp, vp],
     "tc_log_probabilities_backward": [u32, vp, u64, u64, u64, vp, vp, vp, vp, vp, vp, u64],
 }

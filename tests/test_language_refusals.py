@@ -61,3 +61,30 @@ def test_log_probabilities():
     assert refused(back, F, 64, 8, 2, 8, None, 64, None, 64, None, 64, 8) == null
     assert refused(back, F, 64, 8, 2, 8, 64, 64, None, 64, 64, 64, 8) == null
     assert refused(back, F, 64, 8, 2, 8, 64, 64, 64, 64, 64, 64, 5)[0] == lib.INVALID
+
+
+def test_clip():
+    def arrays(*tensors):
+        n = max(len(tensors), 1)
+        kinds, pointers, lens = zip(*tensors)
+        return (lib.u32 * n)(*kinds), (lib.vp * n)(*pointers), (lib.u64 * n)(*lens)
+
+    kinds, tensors, lens = arrays((lib.F32, 64, 10), (lib.BF16, 64, 10))
+    run = "tc_clip_global_norm"
+    null = (lib.INVALID, "clip by global norm: a null operand")
+    assert refused(run, 2, kinds, tensors, lens, -1.0, tensors, 64) == (
+        lib.INVALID, "clip by global norm: a largest norm of -1.000000")
+    assert refused(run, 2, kinds, tensors, lens, float("nan"), tensors, 64)[0] == lib.INVALID
+    assert refused(run, 2, kinds, tensors, lens, 1.0, None, 64) == null
+    assert refused(run, 2, kinds, tensors, lens, 1.0, tensors, None) == null
+    assert refused(run, 2, None, tensors, lens, 1.0, tensors, 64) == null
+    assert refused(run, 2, kinds, None, lens, 1.0, tensors, 64) == null
+    assert refused(run, 2, kinds, tensors, None, 1.0, tensors, 64) == null
+    assert refused(run, 2, kinds, tensors, lens, 1.0, arrays((0, 64, 0), (0, None, 0))[1], 64) == null
+    some = arrays((lib.F32, 64, 10), (lib.BF16, None, 10))
+    assert refused(run, 2, *some, 1.0, tensors, 64) == null
+    assert refused("tc_global_norm", 2, *some, 64) == (lib.INVALID, "global norm: a null operand")
+    some = arrays((lib.F32, 64, 10), (lib.F64, 64, 10))
+    assert refused(run, 2, *some, 1.0, tensors, 64) == (lib.UNSUPPORTED, "clip by global norm: no kernel for f64")
+    some = arrays((lib.F32, 64, 10), (lib.F32, 64, 2**41))
+    assert refused("tc_global_norm", 2, *some, 64)[0] == lib.INVALID
