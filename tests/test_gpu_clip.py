@@ -65,7 +65,7 @@ def test_one_tensor(kind, size):
         check(tensors, limit, run(tensors, limit, in_place=True, shifts=[shift]))
 
 
-@pytest.mark.parametrize("count", [2, 95, 96, 97, 193, 400])
+@pytest.mark.parametrize("count", [2, 95, 96, 97, 139, 140, 141, 281, 400])
 def test_many_tensors_of_every_type(count):
     rng = np.random.default_rng(count)
     sizes = [int(s) for s in np.exp(rng.uniform(0, 10, count))]
