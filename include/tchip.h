@@ -708,6 +708,54 @@ int tc_global_norm(uint32_t count, const uint32_t* dtypes, const void* const* te
 int tc_clip_global_norm(uint32_t count, const uint32_t* dtypes, const void* const* tensors, const uint64_t* lens,
                         float limit, void* const* outputs, float* norm);
 
+/* ---- attention ------------------------------------------------------------- */
+
+/* Causal attention of `query_heads` heads of `head_size` (at most 128)
+ * elements over `tokens` tokens; key head i / (query_heads / key_heads)
+ * serves query head i.  Element e of head h of token t is at
+ * t * token_step + h * head_step + e of its tensor, for queries, keys, values
+ * and results each, so that they may be parts of one projection.
+ *   The tokens are `sequences` sequences one behind another, sequence s being
+ * tokens offsets[s] to offsets[s + 1] (`offsets`: sequences + 1 rising numbers
+ * on the device; sequences may be empty).  A token attends to those of its
+ * own sequence up to itself.  Tokens before the first or past the last offset
+ * are in none: their results and gradients are zeros and nothing reads their
+ * values.  With `sequences` 0 all tokens are one sequence, and `offsets` is
+ * not read.
+ *   Scores are scale * q . k (`scale` positive and finite). */
+typedef struct tc_attention_shape {
+    uint32_t dtype;
+    uint32_t query_heads;
+    uint32_t key_heads;
+    uint32_t head_size;
+    uint64_t tokens;
+    uint32_t sequences;
+    float scale;
+    const uint32_t* offsets;
+    uint64_t query_token_step, query_head_step;
+    uint64_t key_token_step, key_head_step;
+    uint64_t value_token_step, value_head_step;
+    uint64_t out_token_step, out_head_step;
+} tc_attention_shape;
+
+/* out = softmax of the scores times the values, and `normalizers`
+ * [query_heads][tokens] (f32; may be null), the log of each query's sum of
+ * exponentials (-infinity for a token in no sequence), for the backward pass.
+ * Sums and softmax are f32; the softmax's weights are rounded to `dtype` for
+ * their product with the values.  What a query does not attend to never
+ * reaches its result, not as an infinity or a NaN either. */
+int tc_attention(const tc_attention_shape* shape, const void* query, const void* key, const void* value, void* out,
+                 float* normalizers);
+
+/* The gradients of queries, keys and values (laid out as those) from `d_out`
+ * (laid out as `out`) and the forward pass's operands, `out` and
+ * `normalizers`.  Gradients of shared key heads are summed over their query
+ * heads in f32; every sum is taken in an order that depends on the shape and
+ * the offsets alone. */
+int tc_attention_backward(const tc_attention_shape* shape, const void* d_out, const void* query, const void* key,
+                          const void* value, const void* out, const float* normalizers, void* d_query, void* d_key,
+                          void* d_value);
+
 #ifdef __cplusplus
 }
 #endif

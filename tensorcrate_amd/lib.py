@@ -123,6 +123,14 @@ class Tcr1(ctypes.Structure):
                 ("data_offset", u64), ("end_offset", u64)]
 
 
+class AttentionShape(ctypes.Structure):
+    """``tc_attention_shape``: heads, tokens, sequences and layouts of an attention."""
+    _fields_ = [("dtype", u32), ("query_heads", u32), ("key_heads", u32), ("head_size", u32), ("tokens", u64),
+                ("sequences", u32), ("scale", f32), ("offsets", vp)] + [
+                    (f"{name}_{axis}_step", u64) for name in ("query", "key", "value", "out")
+                    for axis in ("token", "head")]
+
+
 # Every entry point of include/tchip.h with its argument types.
 SIGNATURES = {
     "tc_init": [i32],
@@ -201,6 +209,8 @@ SIGNATURES = {
                            u32],
     "tc_layer_norm": [u32, u32, vp, u64, u64, u64, vp, vp, f32, vp, u64, vp, vp],
     "tc_layer_norm_backward": [u32, u32, vp, u64, vp, u64, u64, u64, vp, vp, vp, vp, u64, vp, vp],
+    "tc_attention": [ctypes.POINTER(AttentionShape), vp, vp, vp, vp, vp],
+    "tc_attention_backward": [ctypes.POINTER(AttentionShape), vp, vp, vp, vp, vp, vp, vp, vp, vp],
     "tc_global_norm": [u32, ctypes.POINTER(u32), ctypes.POINTER(vp), ctypes.POINTER(u64), vp],
     "tc_clip_global_norm": [u32, ctypes.POINTER(u32), ctypes.POINTER(vp), ctypes.POINTER(u64), f32,
                             ctypes.POINTER(vp), vp],
@@ -402,6 +412,15 @@ def matmul_epilogue(dtype: int, code, places, a, b, m: int, k: int, n: int, inpu
     outs, out_lens = _buffers(outputs)
     call("tc_matmul_epilogue", dtype, enc, len(code), pl, len(places), m, k, n, a.ptr, b.ptr, ins, in_lens,
          len(inputs), outs, out_lens, len(outputs))
+
+
+def attention(dtype: int, tokens: int, query_heads: int, key_heads: int, head_size: int, scale: float, offsets,
+              sequences: int, query, key, value, out) -> AttentionShape:
+    """The shape that ``tc_attention`` and ``tc_attention_backward`` take:
+    ``offsets`` a device pointer or None, and the (token, head) steps of
+    queries, keys, values and results."""
+    return AttentionShape(dtype, query_heads, key_heads, head_size, tokens, sequences, scale, offsets, *query, *key,
+                          *value, *out)
 
 
 def region(source: Buffer | int, source_len: int, shape, src_offset, src_strides, dst_offset,

@@ -119,3 +119,56 @@ def log_probabilities_backward(x, tokens, normalizers, entropies, d_given, d_ent
         if t < x.shape[1]:
             d[r, t] += g
     return d
+
+
+# ---- attention --------------------------------------------------------------
+
+
+def attention(q, k, v, ends, scale):
+    """(out, normalizers, sum of p |v|) of queries [token, head, element] and
+    keys and values [token, key head, element], sequences ending at `ends`
+    (the first at ends[0] begins the first); what a query does not see is not
+    touched."""
+    tokens, heads, size = q.shape
+    group = heads // k.shape[1]
+    out, sizes = np.zeros_like(q), np.zeros_like(q)
+    normalizers = np.full((heads, tokens), -np.inf)
+    for begin, end in zip(ends, ends[1:]):
+        for head in range(heads):
+            h = head // group
+            for row in range(begin, end):
+                seen = slice(begin, row + 1)
+                with np.errstate(invalid="ignore", over="ignore"):
+                    scores = scale * (k[seen, h] @ q[row, head])
+                    most = scores.max()
+                    e = np.exp(scores - most)
+                    p = e / e.sum()
+                    out[row, head] = p @ v[seen, h]
+                    sizes[row, head] = p @ np.abs(v[seen, h])
+                    normalizers[head, row] = most + np.log(e.sum())
+    return out, normalizers, sizes
+
+
+def attention_backward(d, q, k, v, out, normalizers, ends, scale):
+    """((dq, dk, dv), the sums of magnitudes that their errors go by)."""
+    tokens, heads, size = q.shape
+    group = heads // k.shape[1]
+    grads = [np.zeros_like(t) for t in (q, k, v)]
+    sizes = [np.zeros_like(t) for t in (q, k, v)]
+    for begin, end in zip(ends, ends[1:]):
+        for head in range(heads):
+            h = head // group
+            for row in range(begin, end):
+                seen = slice(begin, row + 1)
+                with np.errstate(invalid="ignore", over="ignore"):
+                    p = np.exp(scale * (k[seen, h] @ q[row, head]) - normalizers[head, row])
+                    dot = d[row, head] @ out[row, head]
+                    ds = p * (v[seen, h] @ d[row, head] - dot)
+                    loose = p * (np.abs(v[seen, h]) @ np.abs(d[row, head]) + np.abs(d[row, head]) @ np.abs(out[row, head]))
+                    grads[0][row, head] = scale * (ds @ k[seen, h])
+                    grads[1][seen, h] += scale * np.outer(ds, q[row, head])
+                    grads[2][seen, h] += np.outer(p, d[row, head])
+                    sizes[0][row, head] = scale * (loose @ np.abs(k[seen, h]))
+                    sizes[1][seen, h] += scale * np.outer(loose, np.abs(q[row, head]))
+                    sizes[2][seen, h] += np.outer(p, np.abs(d[row, head]))
+    return grads, sizes

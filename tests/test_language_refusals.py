@@ -88,3 +88,39 @@ def test_clip():
     assert refused(run, 2, *some, 1.0, tensors, 64) == (lib.UNSUPPORTED, "clip by global norm: no kernel for f64")
     some = arrays((lib.F32, 64, 10), (lib.F32, 64, 2**41))
     assert refused("tc_global_norm", 2, *some, 64)[0] == lib.INVALID
+
+
+def test_attention():
+    def shape(dtype=lib.F32, tokens=10, heads=4, key_heads=2, size=16, scale=0.25, offsets=None, sequences=0,
+              query=(64, 16), key=(32, 16), value=(32, 16), out=(64, 16)):
+        return lib.attention(dtype, tokens, heads, key_heads, size, scale, offsets, sequences, query, key, value, out)
+
+    def forward(given, *operands):
+        return refused("tc_attention", given, *(operands or [64] * 5))
+
+    back = lambda given, *operands: refused("tc_attention_backward", given, *(operands or [64] * 9))
+    assert forward(None) == (lib.INVALID, "attention: no shape")
+    assert forward(shape(dtype=lib.F64)) == (lib.UNSUPPORTED, "attention: no kernel for f64")
+    for heads, key_heads in ((4, 3), (2, 4), (0, 1), (1, 0)):
+        assert forward(shape(heads=heads, key_heads=key_heads)) == (
+            lib.INVALID, f"attention: {heads} query heads do not share {key_heads} key heads evenly")
+    assert forward(shape(size=0))[0] == lib.INVALID
+    assert forward(shape(size=129, query=(516, 129), key=(258, 129), value=(258, 129), out=(516, 129))) == (
+        lib.UNSUPPORTED, "attention: heads of 129 elements, more than 128")
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        assert forward(shape(scale=scale))[0] == lib.INVALID
+    for name in ("query", "key", "value", "out"):
+        for steps in ((16, 16), (64, 15), (0, 16), (16, 0), (2**62, 16), (16, 2**62)):
+            assert forward(shape(**{name: steps}))[0] == lib.INVALID, (name, steps)
+            assert back(shape(**{name: steps}))[0] == lib.INVALID, (name, steps)
+    assert forward(shape(tokens=2**31, query=(64, 16))) [0] == lib.UNSUPPORTED
+    null = (lib.INVALID, "attention: a null operand")
+    assert forward(shape(sequences=2)) == null
+    for missing in range(4):
+        operands = [64] * 5
+        operands[missing] = None
+        assert forward(shape(), *operands) == null
+    for missing in range(9):
+        operands = [64] * 9
+        operands[missing] = None
+        assert back(shape(), *operands) == (lib.INVALID, "attention, backward: a null operand")

@@ -55,3 +55,18 @@ def test_log_probabilities_of_impossible_tokens():
     assert np.array_equal(given, [-np.inf, -np.inf]) and np.allclose(normalizers[0], np.log(4.0))
     assert np.allclose(entropies, [np.log(4.0) - 0.75 * np.log(3.0), 0.0]) and normalizers[1] == -np.inf
     assert np.array_equal(tokens, [[2, 0, 1], [0, 1, 2]]) and np.allclose(top[0, :2], np.log([0.75, 0.25]))
+
+
+def test_attention_gradients_are_the_differences():
+    rng = np.random.default_rng(3)
+    q, k, v, d = (rng.standard_normal((7, h, 3)) for h in (4, 2, 2, 4))
+    ends, scale = [1, 1, 4, 6], 0.7
+    out, normalizers, _ = language.attention(q, k, v, ends, scale)
+    grads, _ = language.attention_backward(d, q, k, v, out, normalizers, ends, scale)
+    loss = lambda: float((language.attention(q, k, v, ends, scale)[0] * d).sum())
+    # Third derivatives below 10 here: 2e-10 from the step, 1e-10 from rounding.
+    for name, grad, operand in zip("qkv", grads, (q, k, v)):
+        assert np.allclose(grad, differences(loss, operand), atol=1e-8), name
+    # What no sequence has, and the first token of each, whose softmax is of one.
+    assert not out[[0, 6]].any() and not grads[0][[0, 1, 4, 6]].any()
+    assert np.array_equal(out[1], np.repeat(v[1], 2, 0)) and np.isneginf(normalizers[:, [0, 6]]).all()
