@@ -39,6 +39,7 @@
 #pragma once
 
 #include <type_traits>
+#include <utility>
 
 #include "rows.hpp"
 
@@ -48,6 +49,9 @@ namespace attention {
 constexpr int kThreads = 256;
 constexpr uint32_t kOwned = 128;  // queries (or keys) of a block, 32 a wave
 constexpr uint32_t kNone = 0xffffffffu;
+constexpr int kBufferFlags = 0x00020000;       // raw 32-bit data
+constexpr uint32_t kOutside = 0x80000000u;    // an offset past any buffer resource here
+constexpr int kWaitForAll = 0x7 << 4;          // vmcnt(0), lgkmcnt(0)
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 struct Steps {
@@ -129,47 +133,70 @@ __device__ __forceinline__ uint4 operand(const f32x16& v, int n) {
 // ---- tiles in LDS -------------------------------------------------------------------
 
 // ROWS rows of SIZE elements (a multiple of 32, zeros behind a head's own) in
-// 16-byte words.  A row's words are permuted within groups by its number, so
-// that neither 16 rows' words of one column nor 4 rows' of a transposing read
-// meet in a bank (64 banks, 256 bytes).
+// 16-byte words.  Within groups of kGroup words a row's words are permuted by
+// an exclusive or with `mixed(row)`, so that neither 16 rows' words of one
+// column nor 4 rows' of a transposing read meet in a bank (64 banks, 256
+// bytes).  `mixed` only moves bits, so that the place of (row, word) is one
+// number of the lane, exclusive-ored and added to what is the same in all
+// lanes: the reads below take that number (`Lanes`), and few registers hold
+// all addresses.
+struct Lanes {
+    uint32_t row;     // of `by_row`
+    uint32_t column;  // of `by_column`
+};
+
 template <int SIZE, int ROWS>
 struct Tile {
     static constexpr int kWords = SIZE / E;  // of a row: 4, 8, 12, 16, 24 or 32
+    static constexpr int kGroup = kWords % 16 == 0 ? 16 : kWords % 8 == 0 ? 8 : 4;
     static constexpr int kBytes = ROWS * kWords * 16;
     char* at;
 
-    __device__ __forceinline__ static int permuted(int row, int word) {
-        if constexpr (kWords % 16 == 0) return word ^ ((row & 3) << 2 | (row >> 2 & 3));
-        if constexpr (kWords % 8 == 0) return word ^ ((row >> 1 & 1) << 2 | (row >> 2 & 3));
-        return word ^ (row >> 2 & 3);
+    __device__ __forceinline__ static constexpr int mixed(int row) {
+        return kGroup == 16  ? (row & 3) << 2 | (row >> 2 & 3)
+               : kGroup == 8 ? (row >> 1 & 1) << 2 | (row >> 2 & 3)
+                             : row >> 2 & 3;
     }
-    __device__ __forceinline__ char* word(int row, int word) const {
-        return at + (row * kWords + permuted(row, word)) * 16;
+    __device__ __forceinline__ static int permuted(int row, int word) { return word ^ mixed(row); }
+    __device__ __forceinline__ static uint32_t place(int row, int word) {
+        return (row * kWords + permuted(row, word)) * 16;
     }
-    // Operand word n of row `row`, which is this lane's own row.
-    __device__ __forceinline__ uint4 by_row(int row, int n, int half) const {
-        return *reinterpret_cast<const uint4*>(word(row, 2 * n + half));
+    // The place (row, word) away from a lane's, whose row and word have none of
+    // the bits of these.
+    __device__ __forceinline__ char* from(uint32_t lanes, int row, int word) const {
+        return at + (lanes ^ static_cast<uint32_t>((mixed(row) ^ word % kGroup) * 16)) +
+               (row * kWords + word / kGroup * kGroup) * 16;
     }
-    // Operand word of column `columns` + l % 32, summed over the kDeep rows from
-    // `rows` on in the order of `row_of`.
-    __device__ __forceinline__ uint4 by_column(int rows, int columns, int lane) const {
+    __device__ __forceinline__ static Lanes lanes_of(int lane) {
+        Lanes out;
+        out.row = place(lane % 32, lane / 32);
         if constexpr (kWide) {
-            float v[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int column = columns + lane % 32;
-                v[j] = reinterpret_cast<const float*>(word(rows + 4 * (lane / 32) + j, column / E))[column % E];
-            }
-            return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
-                              __float_as_uint(v[3]));
+            out.column = place(4 * (lane / 32), lane % 32 / 4) + lane % 4 * 4;
         } else {
             // Lane j of 16 addresses 4 columns of row j / 4 and receives the 4
             // rows of column j.
-            const int row = rows + 4 * (lane / 32) + lane % 16 / 4;
-            const int column = columns + 16 * (lane / 16 % 2) + 4 * (lane % 4);
-            const s16x4 low = transposed(word(row, column / E) + column % E * 2);
-            const s16x4 high = transposed(word(row + 8, column / E) + column % E * 2);
-            const u32x2 a = __builtin_bit_cast(u32x2, low), b = __builtin_bit_cast(u32x2, high);
+            out.column = place(4 * (lane / 32) + lane % 16 / 4, 2 * (lane / 16 % 2) + lane % 4 / 2) + lane % 2 * 8;
+        }
+        return out;
+    }
+    __device__ __forceinline__ char* word(int row, int word) const { return at + place(row, word); }
+    // Operand word n of row `rows` + l % 32, `rows` a multiple of 32.
+    __device__ __forceinline__ uint4 by_row(const Lanes& lanes, int rows, int n) const {
+        return *reinterpret_cast<const uint4*>(from(lanes.row, rows, 2 * n));
+    }
+    // Operand word of column `columns` + l % 32, summed over the kDeep rows from
+    // `rows` on in the order of `row_of`; multiples of 32 and kDeep.
+    __device__ __forceinline__ uint4 by_column(const Lanes& lanes, int rows, int columns) const {
+        if constexpr (kWide) {
+            uint32_t v[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                v[j] = *reinterpret_cast<const uint32_t*>(from(lanes.column, rows + j, columns / E));
+            }
+            return make_uint4(v[0], v[1], v[2], v[3]);
+        } else {
+            const u32x2 a = __builtin_bit_cast(u32x2, transposed(from(lanes.column, rows, columns / E)));
+            const u32x2 b = __builtin_bit_cast(u32x2, transposed(from(lanes.column, rows + 8, columns / E)));
             return make_uint4(a.x, a.y, b.x, b.y);
         }
     }
@@ -213,41 +240,87 @@ __device__ __forceinline__ uint32_t finite_bits(uint32_t bits) {
     return bits;
 }
 
-// A tile on its way from memory: each thread's words of it in registers.
-template <int SIZE, int ROWS>
-struct Flight {
+// How tiles get from memory to LDS.  DIRECT, for rows of whole 16-byte words:
+// loads that write LDS themselves, each lane fetching the word that belongs
+// where it writes, zeros past the rows and a head's size because those lie
+// past the buffer resource.  Otherwise through registers, word by word.
+template <int SIZE, int ROWS, bool DIRECT, int THREADS = kThreads>
+struct Stager {
     static constexpr int kWords = SIZE / E;
-    static constexpr int kEach = ROWS * kWords / kThreads;
-    static_assert(ROWS * kWords % kThreads == 0, "every thread has as many words");
-    uint4 words[kEach];
+    static constexpr int kEach = ROWS * kWords / THREADS;
+    static_assert(ROWS * kWords % THREADS == 0, "every thread has as many words");
+    using LdsTile = Tile<SIZE, ROWS>;
 
-    // Rows first .. first + ROWS of a head, zeros from token `limit` on.
-    __device__ __forceinline__ void load(const S* head, uint64_t step, uint32_t first, uint32_t limit, uint32_t size) {
+    uint64_t step;
+    uint32_t size;
+    uint32_t offsets[DIRECT ? kEach : 1];
+    uint4 words[DIRECT ? 1 : kEach];
+
+    __device__ __forceinline__ Stager(uint64_t token_step, uint32_t head_size) : step(token_step), size(head_size) {
+        if constexpr (DIRECT) {
 #pragma unroll
-        for (int k = 0; k < kEach; k++) {
-            const int i = threadIdx.x + k * kThreads;
-            const uint32_t token = first + i / kWords;
-            words[k] = token < limit ? head_word(head + token * step, i % kWords, size) : make_uint4(0, 0, 0, 0);
+            for (int k = 0; k < kEach; k++) {
+                const int i = threadIdx.x + k * THREADS;
+                const int row = i / kWords, word = LdsTile::permuted(row, i % kWords);
+                offsets[k] = word * E < static_cast<int>(size)
+                                 ? (row * static_cast<uint32_t>(step) + word * E) * sizeof(S)
+                                 : kOutside;
+            }
         }
     }
-    __device__ __forceinline__ void store(const Tile<SIZE, ROWS>& tile) const {
+    // Rows first .. first + ROWS of a head towards `tile`, zeros from token
+    // `limit` on; all arguments the same for the whole wave.
+    __device__ __forceinline__ void fetch(const LdsTile& tile, const S* head, uint32_t first, uint32_t limit) {
+        if constexpr (DIRECT) {
+            const uint32_t rows = first >= limit ? 0 : limit - first < ROWS ? limit - first : ROWS;
+            const uint32_t bytes = rows == 0 ? 0 : ((rows - 1) * static_cast<uint32_t>(step) + size) * sizeof(S);
+            const int wave = threadIdx.x / 64;
+#if defined(__HIP_DEVICE_COMPILE__)  // the host's pass drops kernels over these builtins
+            const auto resource =
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<S*>(head + first * step), 0, bytes, kBufferFlags);
 #pragma unroll
-        for (int k = 0; k < kEach; k++) {
-            const int i = threadIdx.x + k * kThreads;
-            *reinterpret_cast<uint4*>(tile.word(i / kWords, i % kWords)) = words[k];
+            for (int k = 0; k < kEach; k++) {
+                char* to = tile.at + 1024 * (wave + k * (THREADS / 64));
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(resource, (__attribute__((address_space(3))) void*)to, 16,
+                                                         offsets[k], 0, 0, 0);
+            }
+#else
+            (void)bytes, (void)wave;
+#endif
+        } else {
+#pragma unroll
+            for (int k = 0; k < kEach; k++) {
+                const int i = threadIdx.x + k * THREADS;
+                const uint32_t token = first + i / kWords;
+                words[k] = token < limit ? head_word(head + token * step, i % kWords, size) : make_uint4(0, 0, 0, 0);
+            }
         }
     }
-    // Whether any of this thread's elements is an infinity or a NaN.
-    __device__ __forceinline__ bool special() const {
-        bool any = false;
+    // The last rows fetched are in LDS, for this thread, when this returns.
+    __device__ __forceinline__ void land(const LdsTile& tile) const {
+        if constexpr (DIRECT) {
+            __builtin_amdgcn_s_waitcnt(kWaitForAll);
+        } else {
 #pragma unroll
-        for (int k = 0; k < kEach; k++) {
-            any |= special_bits(words[k].x) || special_bits(words[k].y) || special_bits(words[k].z) ||
-                   special_bits(words[k].w);
+            for (int k = 0; k < kEach; k++) {
+                const int i = threadIdx.x + k * THREADS;
+                *reinterpret_cast<uint4*>(tile.word(i / kWords, i % kWords)) = words[k];
+            }
         }
-        return any;
     }
 };
+
+// Whether any of this thread's share of a tile is an infinity or a NaN.
+template <int THREADS, int SIZE, int ROWS>
+__device__ __forceinline__ bool specials_in(const Tile<SIZE, ROWS>& tile) {
+    bool any = false;
+#pragma unroll
+    for (int k = 0; k < ROWS * Tile<SIZE, ROWS>::kWords / THREADS; k++) {
+        const uint4 w = reinterpret_cast<const uint4*>(tile.at)[threadIdx.x + k * THREADS];
+        any |= special_bits(w.x) || special_bits(w.y) || special_bits(w.z) || special_bits(w.w);
+    }
+    return any;
+}
 
 // ---- sequences ------------------------------------------------------------------------
 
@@ -273,7 +346,7 @@ __device__ __forceinline__ Span span_of(const Shape& shape, uint32_t token) {
 // The token behind the last sequence.
 __device__ __forceinline__ uint32_t limit_of(const Shape& shape) {
     if (shape.sequences == 0) return shape.tokens;
-    const uint32_t end = shape.offsets[shape.sequences];
+    const uint32_t end = __builtin_amdgcn_readfirstlane(shape.offsets[shape.sequences]);
     return end < shape.tokens ? end : shape.tokens;
 }
 
@@ -287,12 +360,15 @@ __device__ __forceinline__ uint32_t wave_least(uint32_t v) {
 __device__ __forceinline__ uint32_t wave_most(uint32_t v) { return ~wave_least(~v); }
 
 // The least of the waves' first values and the most of their second ones.
-__device__ __forceinline__ void over_waves(const uint32_t (&values)[2][kThreads / 64], uint32_t* least, uint32_t* most) {
+template <int WAVES>
+__device__ __forceinline__ void over_waves(const uint32_t (&values)[2][WAVES], uint32_t* least, uint32_t* most) {
     *least = values[0][0], *most = values[1][0];
-    for (int w = 1; w < kThreads / 64; w++) {
+    for (int w = 1; w < WAVES; w++) {
         *least = values[0][w] < *least ? values[0][w] : *least;
         *most = values[1][w] > *most ? values[1][w] : *most;
     }
+    *least = __builtin_amdgcn_readfirstlane(*least);
+    *most = __builtin_amdgcn_readfirstlane(*most);
 }
 
 // `v` of this lane and of the one that has the same column in the other half.
@@ -315,13 +391,13 @@ __device__ __forceinline__ float power2(float v) { return __builtin_amdgcn_exp2f
 // 32 x 32 weights; with FINITE, of the tile's finite elements.
 template <int SIZE, int ROWS, bool FINITE>
 __device__ __forceinline__ void weighted(f32x16 (&acc)[SIZE / 32], const Tile<SIZE, ROWS>& tile, int rows,
-                                         const f32x16& weights, int lane) {
+                                         const f32x16& weights, const Lanes& lanes) {
 #pragma unroll
     for (int n = 0; n < 32 / kDeep; n++) {
         const uint4 weight = operand(weights, n);
 #pragma unroll
         for (int t = 0; t < SIZE / 32; t++) {
-            uint4 column = tile.by_column(rows + n * kDeep, t * 32, lane);
+            uint4 column = tile.by_column(lanes, rows + n * kDeep, t * 32);
             if constexpr (FINITE) {
                 column = make_uint4(finite_bits(column.x), finite_bits(column.y), finite_bits(column.z),
                                     finite_bits(column.w));
@@ -351,6 +427,9 @@ __device__ __forceinline__ void weighted_specials(f32x16 (&acc)[SIZE / 32], cons
             for (int t = 0; t < SIZE / 32; t++) {
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
+                    // One read at a time: registers here would be missing in
+                    // the loop that this is the exception of.
+                    __builtin_amdgcn_sched_barrier(0);
                     float v[4];
                     tile.four(rows + 8 * g + r, t * 32 + 8 * q + 4 * half, v);
 #pragma unroll
@@ -363,15 +442,16 @@ __device__ __forceinline__ void weighted_specials(f32x16 (&acc)[SIZE / 32], cons
     }
 }
 
-// Both, where a tile is masked and `special`, or the plain product.
-template <int SIZE, int ROWS>
+// Both, where a tile is MASKED and `special`, or the plain product.
+template <int SIZE, int ROWS, bool MASKED>
 __device__ __forceinline__ void add_weighted(bool special, f32x16 (&acc)[SIZE / 32], const Tile<SIZE, ROWS>& tile,
-                                             int rows, const f32x16& weights, int lane, float* scratch) {
-    if (__builtin_expect(special, false)) {
-        weighted<SIZE, ROWS, true>(acc, tile, rows, weights, lane);
+                                             int rows, const f32x16& weights, const Lanes& lanes, int lane,
+                                             float* scratch) {
+    if (MASKED && __builtin_expect(special, false)) {
+        weighted<SIZE, ROWS, true>(acc, tile, rows, weights, lanes);
         weighted_specials<SIZE, ROWS>(acc, tile, rows, weights, lane, scratch);
     } else {
-        weighted<SIZE, ROWS, false>(acc, tile, rows, weights, lane);
+        weighted<SIZE, ROWS, false>(acc, tile, rows, weights, lanes);
     }
 }
 
@@ -404,17 +484,19 @@ __device__ __forceinline__ void store_column(T* row, const f32x16 (&acc)[SIZE / 
 
 // ---- forward ---------------------------------------------------------------------------
 
-template <int SIZE>
+template <int SIZE, bool DIRECT>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
     forward_kernel(const Shape shape, const S* __restrict__ q, const S* __restrict__ k, const S* __restrict__ v,
                    S* __restrict__ out, float* __restrict__ normalizers) {
     using KeyTile = Tile<SIZE, kSwept>;
-    __shared__ __attribute__((aligned(16))) char lds[4 * KeyTile::kBytes];
+    // A stage an array, so that reads of one do not wait for loads to the other.
+    __shared__ __attribute__((aligned(1024))) char stage_0[2 * KeyTile::kBytes], stage_1[2 * KeyTile::kBytes];
     __shared__ float scratch[kThreads / 64][8 * 32];
     __shared__ uint32_t seen[2][kThreads / 64];
     constexpr int kOperands = SIZE / kDeep;
 
     const int lane = threadIdx.x % 64, half = lane / 32, wave = threadIdx.x / 64;
+    const Lanes lanes = KeyTile::lanes_of(lane);
     // The latest tokens, which see the most keys, first.
     const uint32_t tiles = (shape.tokens + kOwned - 1) / kOwned;
     const uint32_t head = blockIdx.x % shape.heads;
@@ -442,39 +524,48 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     float most = -INFINITY, total = 0.0f;  // of this half's keys
 
     const uint32_t end = first + kOwned < limit ? first + kOwned : limit;
-    if (begin < end) {
-        Flight<SIZE, kSwept> key_words, value_words;
-        uint32_t at = begin / kSwept * kSwept;
-        key_words.load(keys, shape.k.token, at, limit, shape.size);
-        value_words.load(values, shape.v.token, at, limit, shape.size);
+    // One sweep over the keys.  Without SLOW it ends, true, at the first masked
+    // tile with a special value: what handles those is kept out of the sweep's
+    // registers.
+    const auto sweep = [&](auto is_slow) {
+        constexpr bool SLOW = decltype(is_slow)::value;
+        most = -INFINITY, total = 0.0f;
+#pragma unroll
+        for (int t = 0; t < SIZE / 32; t++) acc[t] = f32x16{};
         // Masked for some query of the block (and the same for all its waves):
         // before a sequence's first key or past the first query.
         const auto masked = [&](uint32_t tile) { return tile < block_all || tile + kSwept - 1 > first; };
-        int turn = 0;
-        key_words.store(KeyTile{lds});
-        value_words.store(KeyTile{lds + 2 * KeyTile::kBytes});
-        bool special = __syncthreads_or(value_words.special());
-        for (; at < end; at += kSwept, turn ^= 1) {
-            const KeyTile key_tile{lds + turn * KeyTile::kBytes};
-            const KeyTile value_tile{lds + (2 + turn) * KeyTile::kBytes};
+        Stager<SIZE, kSwept, DIRECT> key_stager(shape.k.token, shape.size), value_stager(shape.v.token, shape.size);
+        uint32_t at = begin / kSwept * kSwept;
+        bool special = false;
+        const auto fetch = [&](char* stage, uint32_t tile) {
+            key_stager.fetch(KeyTile{stage}, keys, tile, limit);
+            value_stager.fetch(KeyTile{stage + KeyTile::kBytes}, values, tile, limit);
+        };
+        const auto land = [&](char* stage, uint32_t tile) {
+            key_stager.land(KeyTile{stage});
+            value_stager.land(KeyTile{stage + KeyTile::kBytes});
+            __syncthreads();
+            special = masked(tile) && __syncthreads_or(specials_in<kThreads>(KeyTile{stage + KeyTile::kBytes}));
+        };
+        // The tile at `at` in stage `here`, while the next one is on its way.
+        const auto turn = [&](char* here, char* there) {
+            const KeyTile key_tile{here}, value_tile{here + KeyTile::kBytes};
             const uint32_t next = at + kSwept;
-            if (next < end) {
-                key_words.load(keys, shape.k.token, next, limit, shape.size);
-                value_words.load(values, shape.v.token, next, limit, shape.size);
-            }
-            if (at < wave_first + 32 && at + kSwept > some) {
+            if (next < end) fetch(there, next);
+            const auto tile = [&](auto is_whole) {
+                constexpr bool WHOLE = decltype(is_whole)::value;
                 f32x16 scores[kSwept / 32];
 #pragma unroll
                 for (int b = 0; b < static_cast<int>(kSwept) / 32; b++) {
                     f32x16 s = {};
 #pragma unroll
                     for (int n = 0; n < kOperands; n++) {
-                        s = product(key_tile.by_row(b * 32 + lane % 32, n, half), queries[n], s);
+                        s = product(key_tile.by_row(lanes, b * 32, n), queries[n], s);
                     }
                     scores[b] = s;
                 }
-                const bool whole = at >= all && at + kSwept - 1 <= wave_first;
-                if (!whole) {
+                if constexpr (!WHOLE) {
 #pragma unroll
                     for (int b = 0; b < static_cast<int>(kSwept) / 32; b++) {
 #pragma unroll
@@ -512,20 +603,30 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
                 }
 #pragma unroll
                 for (int b = 0; b < static_cast<int>(kSwept) / 32; b++) {
-                    add_weighted<SIZE, kSwept>(!whole && special, acc, value_tile, b * 32, scores[b], lane, scratch[wave]);
+                    add_weighted<SIZE, kSwept, SLOW && !WHOLE>(special, acc, value_tile, b * 32, scores[b], lanes, lane, scratch[wave]);
                 }
+            };
+            if (at >= all && at + kSwept - 1 <= wave_first) {
+                tile(std::true_type());
+            } else if (at < wave_first + 32 && at + kSwept > some) {
+                tile(std::false_type());
             }
-            if (next < end) {
-                key_words.store(KeyTile{lds + (turn ^ 1) * KeyTile::kBytes});
-                value_words.store(KeyTile{lds + (2 + (turn ^ 1)) * KeyTile::kBytes});
-                if (masked(next)) {
-                    special = __syncthreads_or(value_words.special());
-                } else {
-                    special = false;
-                    __syncthreads();
-                }
-            }
+            if (next < end) land(there, next);
+            at = next;
+        };
+        fetch(stage_0, at);
+        land(stage_0, at);
+        while (at < end) {
+            if (!SLOW && special) return true;
+            turn(stage_0, stage_1);
+            if (!SLOW && special) return true;
+            if (at < end) turn(stage_1, stage_0);
         }
+        return false;
+    };
+    if (begin < end && sweep(std::false_type())) {
+        __syncthreads();
+        sweep(std::true_type());
     }
     total = halves_sum(total);
     if (token >= shape.tokens) return;
@@ -539,11 +640,11 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
 
 // ---- backward ----------------------------------------------------------------------------
 
-// sums[head][token] = do . o, 16 lanes a row of a head; and in f16 the bits of
-// the largest finite |do|^2 and |v|^2 of any row into `largest`.
+// sums[head][token] = do . o, 16 lanes a row of a head; and in f16 each block's
+// largest finite |do|^2 and |v|^2 of a row, a pair behind the first of `largest`.
 __global__ void __launch_bounds__(kThreads)
     dots_kernel(const Shape shape, const S* __restrict__ d_out, const S* __restrict__ out, const S* __restrict__ v,
-                float* __restrict__ sums, uint32_t* __restrict__ largest) {
+                float* __restrict__ sums, float* __restrict__ largest) {
     const uint64_t first = uint64_t{blockIdx.x} * (kThreads / 16) + threadIdx.x / 16;
     const uint64_t apart = uint64_t{gridDim.x} * (kThreads / 16);
     const auto dot = [&](const S* a, const S* b) {
@@ -575,31 +676,46 @@ __global__ void __launch_bounds__(kThreads)
         __shared__ float shared[2][kMostWaves];
         for (int which = 0; which < 2; which++) {
             const float all = block_join<Largest>(most[which], shared[which]);
-            if (threadIdx.x == 0) atomicMax(largest + which, __float_as_uint(all));
+            if (threadIdx.x == 0) largest[2 + 2 * blockIdx.x + which] = all;
         }
     }
 }
 
+// The largest of the blocks' pairs behind the first two, into those.
+__global__ void __launch_bounds__(kThreads) largest_kernel(float* largest, uint32_t blocks) {
+    __shared__ float shared[2][kMostWaves];
+    float most[2] = {};
+    for (uint32_t n = threadIdx.x; n < blocks; n += kThreads) {
+        for (int which = 0; which < 2; which++) most[which] = fmaxf(most[which], largest[2 + 2 * n + which]);
+    }
+    for (int which = 0; which < 2; which++) {
+        const float all = block_join<Largest>(most[which], shared[which]);
+        if (threadIdx.x == 0) largest[which] = all;
+    }
+}
+
 // The power of two that ds is rounded times.
-__device__ __forceinline__ float ds_factor(const uint32_t* largest) {
+__device__ __forceinline__ float ds_factor(const float* largest) {
     if constexpr (!kHalf) return 1.0f;
-    const float bound = sqrtf(__uint_as_float(largest[0])) * sqrtf(__uint_as_float(largest[1]));
+    const float bound = sqrtf(largest[0]) * sqrtf(largest[1]);
     return bound == 0.0f ? 1.0f : ldexpf(1.0f, 13 - ilogbf(bound));
 }
 
 // dq: as forward, with the weights from the normalizers.
-template <int SIZE>
+template <int SIZE, bool DIRECT>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
     queries_kernel(const Shape shape, const S* __restrict__ d_out, const S* __restrict__ q, const S* __restrict__ k,
                    const S* __restrict__ v, const float* __restrict__ normalizers, const float* __restrict__ dots,
-                   const uint32_t* __restrict__ largest, S* __restrict__ dq) {
+                   const float* __restrict__ largest, S* __restrict__ dq) {
     using KeyTile = Tile<SIZE, kSwept>;
-    __shared__ __attribute__((aligned(16))) char lds[4 * KeyTile::kBytes];
+    // A stage an array, so that reads of one do not wait for loads to the other.
+    __shared__ __attribute__((aligned(1024))) char stage_0[2 * KeyTile::kBytes], stage_1[2 * KeyTile::kBytes];
     __shared__ float scratch[kThreads / 64][8 * 32];
     __shared__ uint32_t seen[2][kThreads / 64];
     constexpr int kOperands = SIZE / kDeep;
 
     const int lane = threadIdx.x % 64, half = lane / 32, wave = threadIdx.x / 64;
+    const Lanes lanes = KeyTile::lanes_of(lane);
     const uint32_t tiles = (shape.tokens + kOwned - 1) / kOwned;
     const uint32_t head = blockIdx.x % shape.heads;
     const uint32_t first = (tiles - 1 - blockIdx.x / shape.heads) * kOwned;
@@ -632,59 +748,75 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     f32x16 acc[SIZE / 32] = {};
 
     const uint32_t end = first + kOwned < limit ? first + kOwned : limit;
-    if (begin < end) {
-        Flight<SIZE, kSwept> key_words, value_words;
-        uint32_t at = begin / kSwept * kSwept;
-        key_words.load(keys, shape.k.token, at, limit, shape.size);
-        value_words.load(values, shape.v.token, at, limit, shape.size);
+    // One sweep over the keys.  Without SLOW it ends, true, at the first masked
+    // tile with a special value: what handles those is kept out of the sweep's
+    // registers.
+    const auto sweep = [&](auto is_slow) {
+        constexpr bool SLOW = decltype(is_slow)::value;
+#pragma unroll
+        for (int t = 0; t < SIZE / 32; t++) acc[t] = f32x16{};
+        // Masked for some query of the block (and the same for all its waves):
+        // before a sequence's first key or past the first query.
         const auto masked = [&](uint32_t tile) { return tile < block_all || tile + kSwept - 1 > first; };
-        int turn = 0;
-        key_words.store(KeyTile{lds});
-        value_words.store(KeyTile{lds + 2 * KeyTile::kBytes});
-        bool special = __syncthreads_or(key_words.special());
-        for (; at < end; at += kSwept, turn ^= 1) {
-            const KeyTile key_tile{lds + turn * KeyTile::kBytes};
-            const KeyTile value_tile{lds + (2 + turn) * KeyTile::kBytes};
+        Stager<SIZE, kSwept, DIRECT> key_stager(shape.k.token, shape.size), value_stager(shape.v.token, shape.size);
+        uint32_t at = begin / kSwept * kSwept;
+        bool special = false;
+        const auto fetch = [&](char* stage, uint32_t tile) {
+            key_stager.fetch(KeyTile{stage}, keys, tile, limit);
+            value_stager.fetch(KeyTile{stage + KeyTile::kBytes}, values, tile, limit);
+        };
+        const auto land = [&](char* stage, uint32_t tile) {
+            key_stager.land(KeyTile{stage});
+            value_stager.land(KeyTile{stage + KeyTile::kBytes});
+            __syncthreads();
+            special = masked(tile) && __syncthreads_or(specials_in<kThreads>(KeyTile{stage}));
+        };
+        // The tile at `at` in stage `here`, while the next one is on its way.
+        const auto turn = [&](char* here, char* there) {
+            const KeyTile key_tile{here}, value_tile{here + KeyTile::kBytes};
             const uint32_t next = at + kSwept;
-            if (next < end) {
-                key_words.load(keys, shape.k.token, next, limit, shape.size);
-                value_words.load(values, shape.v.token, next, limit, shape.size);
-            }
-            if (at < wave_first + 32 && at + kSwept > some) {
-                const bool whole = at >= all && at + kSwept - 1 <= wave_first;
+            if (next < end) fetch(there, next);
+            const auto keys_of_32 = [&](int b, auto is_whole) {
+                constexpr bool WHOLE = decltype(is_whole)::value;
+                f32x16 s = {}, d = {};
 #pragma unroll
-                for (int b = 0; b < static_cast<int>(kSwept) / 32; b++) {
-                    f32x16 s = {}, d = {};
-#pragma unroll
-                    for (int n = 0; n < kOperands; n++) {
-                        s = product(key_tile.by_row(b * 32 + lane % 32, n, half), queries[n], s);
-                        d = product(value_tile.by_row(b * 32 + lane % 32, n, half), d_rows[n], d);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        s[i] = power2(fmaf(s[i], c, -normalizer)) * fmaf(d[i], factor, -dot);
-                    }
-                    if (!whole) {
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const uint32_t key = at + b * 32 + row_of(i, half);
-                            if (key < span.first || key > token) s[i] = 0.0f;
-                        }
-                    }
-                    add_weighted<SIZE, kSwept>(!whole && special, acc, key_tile, b * 32, s, lane, scratch[wave]);
+                for (int n = 0; n < kOperands; n++) {
+                    s = product(key_tile.by_row(lanes, b * 32, n), queries[n], s);
+                    d = product(value_tile.by_row(lanes, b * 32, n), d_rows[n], d);
                 }
-            }
-            if (next < end) {
-                key_words.store(KeyTile{lds + (turn ^ 1) * KeyTile::kBytes});
-                value_words.store(KeyTile{lds + (2 + (turn ^ 1)) * KeyTile::kBytes});
-                if (masked(next)) {
-                    special = __syncthreads_or(key_words.special());
-                } else {
-                    special = false;
-                    __syncthreads();
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    s[i] = power2(fmaf(s[i], c, -normalizer)) * fmaf(d[i], factor, -dot);
+                    if constexpr (!WHOLE) {
+                        const uint32_t key = at + b * 32 + row_of(i, half);
+                        if (key < span.first || key > token) s[i] = 0.0f;
+                    }
                 }
+                add_weighted<SIZE, kSwept, SLOW && !WHOLE>(special, acc, key_tile, b * 32, s, lanes, lane, scratch[wave]);
+            };
+            if (at >= all && at + kSwept - 1 <= wave_first) {
+#pragma unroll
+                for (int b = 0; b < static_cast<int>(kSwept) / 32; b++) keys_of_32(b, std::true_type());
+            } else if (at < wave_first + 32 && at + kSwept > some) {
+#pragma unroll 1
+                for (int b = 0; b < static_cast<int>(kSwept) / 32; b++) keys_of_32(b, std::false_type());
             }
+            if (next < end) land(there, next);
+            at = next;
+        };
+        fetch(stage_0, at);
+        land(stage_0, at);
+        while (at < end) {
+            if (!SLOW && special) return true;
+            turn(stage_0, stage_1);
+            if (!SLOW && special) return true;
+            if (at < end) turn(stage_1, stage_0);
         }
+        return false;
+    };
+    if (begin < end && sweep(std::false_type())) {
+        __syncthreads();
+        sweep(std::true_type());
     }
     if (token >= shape.tokens) return;
     store_column<S, SIZE>(dq + token * shape.q.token + head * shape.q.head, acc, shape.scale / factor, shape.size, half);
@@ -693,27 +825,37 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
 // dk and dv of 128 keys from the queries of one of `splits` shares of the
 // heads that the key head serves.  With several shares they are left in f32
 // as `parts`[key head][share][dk, dv][token][size], to be added in their order.
-template <int SIZE>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1)))
+// Threads of a block: a wave of 32 keys each, all that a compute unit holds
+// where registers and LDS leave room for one block.
+constexpr int key_threads(int size) { return !kWide && size > 96 ? 512 : kThreads; }
+
+template <int SIZE, bool DIRECT>
+__global__ void __launch_bounds__(key_threads(SIZE)) __attribute__((amdgpu_waves_per_eu(kWide && SIZE > 96 ? 1 : 2)))
     keys_kernel(const Shape shape, uint32_t splits, const S* __restrict__ d_out, const S* __restrict__ q,
                 const S* __restrict__ k, const S* __restrict__ v, const float* __restrict__ normalizers,
-                const float* __restrict__ dots, const uint32_t* __restrict__ largest, S* __restrict__ dk, S* __restrict__ dv,
+                const float* __restrict__ dots, const float* __restrict__ largest, S* __restrict__ dk, S* __restrict__ dv,
                 float* __restrict__ parts) {
+    constexpr bool kValuesInLds = SIZE > 96;
+    constexpr int kWaves = key_threads(SIZE) / 64;
+    constexpr uint32_t kKeys = 32 * kWaves;
     using QueryTile = Tile<SIZE, kSwept>;
-    __shared__ __attribute__((aligned(16))) char lds[4 * QueryTile::kBytes];
-    __shared__ __attribute__((aligned(16))) float row_values[2][2][kSwept];
-    __shared__ float scratch[kThreads / 64][8 * 32];
-    __shared__ uint32_t seen[2][kThreads / 64];
+    using ValueTile = Tile<SIZE, kKeys>;
+    __shared__ __attribute__((aligned(1024))) char value_lds[kValuesInLds ? ValueTile::kBytes : 16];
+    __shared__ __attribute__((aligned(1024))) char stage_0[2 * QueryTile::kBytes], stage_1[2 * QueryTile::kBytes];
+    __shared__ __attribute__((aligned(16))) float values_0[2][kSwept], values_1[2][kSwept];
+    __shared__ float scratch[kWaves][8 * 32];
+    __shared__ uint32_t seen[2][kWaves];
     constexpr int kOperands = SIZE / kDeep;
 
     const int lane = threadIdx.x % 64, half = lane / 32, wave = threadIdx.x / 64;
+    const Lanes lanes = QueryTile::lanes_of(lane);
     // The first tokens, which are seen by the most queries, first.
     const uint32_t key_heads = shape.heads / shape.group;
     const uint32_t columns = key_heads * splits;
     const uint32_t key_head = blockIdx.x % columns / splits, share = blockIdx.x % splits;
     const uint32_t share_heads = shape.group / splits;
     const uint32_t first_head = key_head * shape.group + share * share_heads;
-    const uint32_t first = blockIdx.x / columns * kOwned;
+    const uint32_t first = blockIdx.x / columns * kKeys;
     const uint32_t wave_first = first + wave * 32;
     const uint32_t token = wave_first + lane % 32;
     const Span span = span_of(shape, token);
@@ -725,11 +867,17 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1
     const uint32_t inside = token < shape.tokens ? token : 0;
     const S* key = k + inside * shape.k.token + key_head * shape.k.head;
     const S* value = v + inside * shape.v.token + key_head * shape.v.head;
-    uint4 keys[kOperands], values[kOperands];
+    const ValueTile own_values{value_lds + wave * 32 * ValueTile::kWords * 16};  // each wave its own 32 rows
+    uint4 keys[kOperands], values[kValuesInLds ? 1 : kOperands];
 #pragma unroll
     for (int n = 0; n < kOperands; n++) {
         keys[n] = head_word(key, 2 * n + half, shape.size);
-        values[n] = head_word(value, 2 * n + half, shape.size);
+        const uint4 word = head_word(value, 2 * n + half, shape.size);
+        if constexpr (kValuesInLds) {
+            *reinterpret_cast<uint4*>(own_values.word(lane % 32, 2 * n + half)) = word;
+        } else {
+            values[n] = word;
+        }
     }
     __syncthreads();
     uint32_t block_all, end;
@@ -739,83 +887,104 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1
     // p is rounded times 2^kBackPower, ds times `factor`.
     const float factor = ds_factor(largest), ds_scale = factor * power2(-kBackPower);
     f32x16 acc_k[SIZE / 32] = {}, acc_v[SIZE / 32] = {};
-    if (first < end) {
-        Flight<SIZE, kSwept> query_words, d_words;
+    // One sweep over the queries, as over the keys in the kernels above.
+    const auto sweep = [&](auto is_slow) {
+        constexpr bool SLOW = decltype(is_slow)::value;
+#pragma unroll
+        for (int t = 0; t < SIZE / 32; t++) acc_k[t] = f32x16{}, acc_v[t] = f32x16{};
+        Stager<SIZE, kSwept, DIRECT, key_threads(SIZE)> query_stager(shape.q.token, shape.size), d_stager(shape.out.token, shape.size);
         float row_value = 0.0f;  // of one row: threads below kSwept the normalizer, the next ones the dot
         const uint32_t per_head = (end - first + kSwept - 1) / kSwept;
         const uint32_t turns = per_head * share_heads;
-        const auto load = [&](uint32_t n) {
-            const uint32_t head = first_head + n / per_head, at = first + n % per_head * kSwept;
-            query_words.load(q + head * shape.q.head, shape.q.token, at, limit, shape.size);
-            d_words.load(d_out + head * shape.out.head, shape.out.token, at, limit, shape.size);
+        bool special = false;
+        // Masked for some key of the block: before its last key, or past a
+        // sequence's end.
+        const auto masked = [&](uint32_t at) { return at < first + kKeys - 1 || at + kSwept > block_all; };
+        const auto tile_of = [&](uint32_t n) { return first + n % per_head * kSwept; };
+        const auto fetch = [&](char* stage, uint32_t n) {
+            const uint32_t head = first_head + n / per_head, at = tile_of(n);
+            query_stager.fetch(QueryTile{stage}, q + head * shape.q.head, at, limit);
+            d_stager.fetch(QueryTile{stage + QueryTile::kBytes}, d_out + head * shape.out.head, at, limit);
             if (threadIdx.x < 2 * kSwept) {
                 const uint32_t row = at + threadIdx.x % kSwept;
                 const float* from = threadIdx.x < kSwept ? normalizers : dots;
                 row_value = row < limit ? from[uint64_t{head} * shape.tokens + row] : 0.0f;
-                row_value = threadIdx.x < kSwept ? fmaf(row_value, kLog2e, -kBackPower) : row_value * ds_scale;
             }
         };
-        const auto store = [&](int turn) {
-            query_words.store(QueryTile{lds + turn * QueryTile::kBytes});
-            d_words.store(QueryTile{lds + (2 + turn) * QueryTile::kBytes});
-            if (threadIdx.x < 2 * kSwept) row_values[turn][threadIdx.x / kSwept][threadIdx.x % kSwept] = row_value;
+        const auto land = [&](char* stage, float (&values_here)[2][kSwept], uint32_t n) {
+            query_stager.land(QueryTile{stage});
+            d_stager.land(QueryTile{stage + QueryTile::kBytes});
+            if (threadIdx.x < 2 * kSwept) {
+                row_value = threadIdx.x < kSwept ? fmaf(row_value, kLog2e, -kBackPower) : row_value * ds_scale;
+                values_here[threadIdx.x / kSwept][threadIdx.x % kSwept] = row_value;
+            }
+            __syncthreads();
+            special = masked(tile_of(n)) && __syncthreads_or(specials_in<key_threads(SIZE)>(QueryTile{stage}) ||
+                                                             specials_in<key_threads(SIZE)>(QueryTile{stage + QueryTile::kBytes}));
         };
-        // Masked for some key of the block: before its last key, or past a
-        // sequence's end.
-        const auto masked = [&](uint32_t at) { return at < first + kOwned - 1 || at + kSwept > block_all; };
-        load(0);
-        store(0);
-        bool special = __syncthreads_or(query_words.special() || d_words.special());
-        for (uint32_t n = 0; n < turns; n++) {
-            const int turn = n % 2;
-            const uint32_t at = first + n % per_head * kSwept;
-            const QueryTile query_tile{lds + turn * QueryTile::kBytes};
-            const QueryTile d_tile{lds + (2 + turn) * QueryTile::kBytes};
-            if (n + 1 < turns) load(n + 1);
-            if (at + kSwept > wave_first && at < some) {
-                const bool whole = at >= wave_first + 31 && at + kSwept <= all;
+        uint32_t n = 0;
+        const auto turn = [&](char* here, const float (&row_values)[2][kSwept], char* there,
+                              float (&values_there)[2][kSwept]) {
+            const uint32_t at = tile_of(n);
+            const QueryTile query_tile{here}, d_tile{here + QueryTile::kBytes};
+            if (n + 1 < turns) fetch(there, n + 1);
+            const auto rows_of_32 = [&](int b, auto is_whole) {
+                constexpr bool WHOLE = decltype(is_whole)::value;
+                f32x16 s = {}, d = {};
 #pragma unroll
-                for (int b = 0; b < static_cast<int>(kSwept) / 32; b++) {
-                    f32x16 s = {}, d = {};
+                for (int o = 0; o < kOperands; o++) {
+                    s = product(query_tile.by_row(lanes, b * 32, o), keys[o], s);
+                    d = product(d_tile.by_row(lanes, b * 32, o), kValuesInLds ? own_values.by_row(lanes, 0, o) : values[kValuesInLds ? 0 : o], d);
+                }
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int n = 0; n < kOperands; n++) {
-                        s = product(query_tile.by_row(b * 32 + lane % 32, n, half), keys[n], s);
-                        d = product(d_tile.by_row(b * 32 + lane % 32, n, half), values[n], d);
-                    }
+                for (int g = 0; g < 4; g++) {
+                    const int row = b * 32 + 8 * g + 4 * half;
+                    const float4 normalizer = *reinterpret_cast<const float4*>(&row_values[0][row]);
+                    const float4 dot = *reinterpret_cast<const float4*>(&row_values[1][row]);
+                    const float l[4] = {normalizer.x, normalizer.y, normalizer.z, normalizer.w};
+                    const float o[4] = {dot.x, dot.y, dot.z, dot.w};
 #pragma unroll
-                    for (int g = 0; g < 4; g++) {
-                        const int row = b * 32 + 8 * g + 4 * half;
-                        const float4 normalizer = *reinterpret_cast<const float4*>(&row_values[turn][0][row]);
-                        const float4 dot = *reinterpret_cast<const float4*>(&row_values[turn][1][row]);
-                        const float l[4] = {normalizer.x, normalizer.y, normalizer.z, normalizer.w};
-                        const float o[4] = {dot.x, dot.y, dot.z, dot.w};
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            s[4 * g + j] = power2(fmaf(s[4 * g + j], c, -l[j]));
-                            d[4 * g + j] = s[4 * g + j] * fmaf(d[4 * g + j], ds_scale, -o[j]);
-                        }
-                    }
-                    if (!whole) {
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
+                    for (int j = 0; j < 4; j++) {
+                        const int i = 4 * g + j;
+                        s[i] = power2(fmaf(s[i], c, -l[j]));
+                        d[i] = s[i] * fmaf(d[i], ds_scale, -o[j]);
+                        if constexpr (!WHOLE) {
                             const uint32_t query = at + b * 32 + row_of(i, half);
                             if (query < token || query >= span.end) s[i] = 0.0f, d[i] = 0.0f;
                         }
                     }
-                    add_weighted<SIZE, kSwept>(!whole && special, acc_v, d_tile, b * 32, s, lane, scratch[wave]);
-                    add_weighted<SIZE, kSwept>(!whole && special, acc_k, query_tile, b * 32, d, lane, scratch[wave]);
                 }
+                __builtin_amdgcn_sched_barrier(0);
+                add_weighted<SIZE, kSwept, SLOW && !WHOLE>(special, acc_v, d_tile, b * 32, s, lanes, lane, scratch[wave]);
+                __builtin_amdgcn_sched_barrier(0);
+                add_weighted<SIZE, kSwept, SLOW && !WHOLE>(special, acc_k, query_tile, b * 32, d, lanes, lane, scratch[wave]);
+            };
+            // Whole tiles in one piece without a branch, so that one half's
+            // exponentials may run beside the other's products.
+            if (at >= wave_first + 31 && at + kSwept <= all) {
+#pragma unroll 1
+                for (int b = 0; b < static_cast<int>(kSwept) / 32; b++) rows_of_32(b, std::true_type());
+            } else if (at + kSwept > wave_first && at < some) {
+#pragma unroll 1
+                for (int b = 0; b < static_cast<int>(kSwept) / 32; b++) rows_of_32(b, std::false_type());
             }
-            if (n + 1 < turns) {
-                store(turn ^ 1);
-                if (masked(first + (n + 1) % per_head * kSwept)) {
-                    special = __syncthreads_or(query_words.special() || d_words.special());
-                } else {
-                    special = false;
-                    __syncthreads();
-                }
-            }
+            if (n + 1 < turns) land(there, values_there, n + 1);
+            n++;
+        };
+        fetch(stage_0, 0);
+        land(stage_0, values_0, 0);
+        while (n < turns) {
+            if (!SLOW && special) return true;
+            turn(stage_0, values_0, stage_1, values_1);
+            if (!SLOW && special) return true;
+            if (n < turns) turn(stage_1, values_1, stage_0, values_0);
         }
+        return false;
+    };
+    if (first < end && sweep(std::false_type())) {
+        __syncthreads();
+        sweep(std::true_type());
     }
     if (token >= shape.tokens) return;
     const float scale_k = shape.scale / factor, scale_v = power2(-kBackPower);
@@ -853,24 +1022,44 @@ __global__ void __launch_bounds__(kThreads)
 
 // ---- launches ------------------------------------------------------------------------------
 
-// `call` with the head size rounded up to 32.
-template <typename Call>
-int by_size(uint32_t size, Call&& call) {
-    if (size <= 32) return call(std::integral_constant<int, 32>());
-    if (size <= 64) return call(std::integral_constant<int, 64>());
-    if (size <= 96) return call(std::integral_constant<int, 96>());
-    return call(std::integral_constant<int, 128>());
+// Whether tiles of these rows may be loaded straight to LDS: whole aligned
+// words, and a tile within 31 bits of its first byte.
+bool direct(uint32_t size, std::initializer_list<std::pair<const void*, Steps>> operands) {
+    bool all = size % E == 0;
+    for (const auto& operand : operands) {
+        all = all && aligned16(operand.first) && operand.second.token % E == 0 && operand.second.head % E == 0 &&
+              operand.second.token < (uint64_t{1} << 31) / (kSwept * sizeof(S));
+    }
+    return all;
 }
+
+// The body with SIZE, the head size rounded up to 32, and DIRECT.
+#define TC_ATTENTION_SIZE(size, ...)                    \
+    if (size <= 32) {                                   \
+        constexpr int SIZE = 32; __VA_ARGS__;           \
+    } else if (size <= 64) {                            \
+        constexpr int SIZE = 64; __VA_ARGS__;           \
+    } else if (size <= 96) {                            \
+        constexpr int SIZE = 96; __VA_ARGS__;           \
+    } else {                                            \
+        constexpr int SIZE = 128; __VA_ARGS__;          \
+    }
+#define TC_ATTENTION_FORM(size, is_direct, ...)                                      \
+    if (is_direct) {                                                                 \
+        constexpr bool DIRECT = true; TC_ATTENTION_SIZE(size, __VA_ARGS__)           \
+    } else {                                                                         \
+        constexpr bool DIRECT = false; TC_ATTENTION_SIZE(size, __VA_ARGS__)          \
+    }
 
 int forward(const Shape& shape, const void* q, const void* k, const void* v, void* out, float* normalizers) {
     TC_STREAM(s);
     const uint32_t tiles = (shape.tokens + kOwned - 1) / kOwned;
-    return by_size(shape.size, [&](auto size) {
-        forward_kernel<decltype(size)::value><<<tiles * shape.heads, kThreads, 0, s>>>(
-            shape, static_cast<const S*>(q), static_cast<const S*>(k), static_cast<const S*>(v), static_cast<S*>(out),
-            normalizers);
-        return check_launch("attention");
-    });
+    const bool straight = direct(shape.size, {{k, shape.k}, {v, shape.v}});
+    TC_ATTENTION_FORM(shape.size, straight,
+                      forward_kernel<SIZE, DIRECT><<<tiles * shape.heads, kThreads, 0, s>>>(
+                          shape, static_cast<const S*>(q), static_cast<const S*>(k), static_cast<const S*>(v),
+                          static_cast<S*>(out), normalizers))
+    return check_launch("attention");
 }
 
 int backward(const Shape& shape, const void* d_out, const void* q, const void* k, const void* v, const void* out,
@@ -889,35 +1078,38 @@ int backward(const Shape& shape, const void* d_out, const void* q, const void* k
         }
     }
     const uint64_t rows = uint64_t{shape.tokens} * shape.heads;
-    Scratch dots((rows + 2) * sizeof(float));
+    const uint32_t dot_blocks = grid_for(rows, kThreads / 16, 8);
+    Scratch dots((rows + 2 + 2 * dot_blocks) * sizeof(float));
     Scratch parts(splits > 1 ? uint64_t{key_heads} * splits * 2 * shape.tokens * shape.size * sizeof(float) : 0);
     if (dots.status != TC_OK) return dots.status;
     if (parts.status != TC_OK) return parts.status;
-    float* sums = static_cast<float*>(dots.ptr) + 2;
-    uint32_t* largest = static_cast<uint32_t*>(dots.ptr);
-    int status = TC_OK;
+    float* sums = static_cast<float*>(dots.ptr);
+    float* largest = sums + rows;
+    const S* d = static_cast<const S*>(d_out);
+    const S* queries = static_cast<const S*>(q);
+    const S* keys = static_cast<const S*>(k);
+    const S* values = static_cast<const S*>(v);
+    dots_kernel<<<dot_blocks, kThreads, 0, s>>>(shape, d, static_cast<const S*>(out), values, sums, largest);
+    int status = check_launch(what);
+    if (status != TC_OK) return status;
     if constexpr (kHalf) {
-        const uint32_t none = 0;
-        status = tc_fill(largest, 2, sizeof(none), &none);
+        largest_kernel<<<1, kThreads, 0, s>>>(largest, dot_blocks);
+        status = check_launch(what);
         if (status != TC_OK) return status;
     }
-    dots_kernel<<<grid_for(rows, kThreads / 16, 8), kThreads, 0, s>>>(
-        shape, static_cast<const S*>(d_out), static_cast<const S*>(out), static_cast<const S*>(v), sums,
-        largest);
+    const bool rows_straight = direct(shape.size, {{q, shape.q}, {d_out, shape.out}});
+    TC_ATTENTION_FORM(shape.size, rows_straight,
+                      const uint32_t key_tiles = (shape.tokens + key_threads(SIZE) / 2 - 1) / (key_threads(SIZE) / 2);
+                      keys_kernel<SIZE, DIRECT><<<key_tiles * key_heads * splits, key_threads(SIZE), 0, s>>>(
+                          shape, splits, d, queries, keys, values, normalizers, sums, largest, static_cast<S*>(dk),
+                          static_cast<S*>(dv), static_cast<float*>(parts.ptr)))
     status = check_launch(what);
     if (status != TC_OK) return status;
-    status = by_size(shape.size, [&](auto size) {
-        keys_kernel<decltype(size)::value><<<tiles * key_heads * splits, kThreads, 0, s>>>(
-            shape, splits, static_cast<const S*>(d_out), static_cast<const S*>(q), static_cast<const S*>(k),
-            static_cast<const S*>(v), normalizers, sums, largest, static_cast<S*>(dk), static_cast<S*>(dv),
-            static_cast<float*>(parts.ptr));
-        const int launched = check_launch(what);
-        if (launched != TC_OK) return launched;
-        queries_kernel<decltype(size)::value><<<tiles * shape.heads, kThreads, 0, s>>>(
-            shape, static_cast<const S*>(d_out), static_cast<const S*>(q), static_cast<const S*>(k),
-            static_cast<const S*>(v), normalizers, sums, largest, static_cast<S*>(dq));
-        return check_launch(what);
-    });
+    const bool keys_straight = direct(shape.size, {{k, shape.k}, {v, shape.v}});
+    TC_ATTENTION_FORM(shape.size, keys_straight,
+                      queries_kernel<SIZE, DIRECT><<<tiles * shape.heads, kThreads, 0, s>>>(
+                          shape, d, queries, keys, values, normalizers, sums, largest, static_cast<S*>(dq)))
+    status = check_launch(what);
     if (status != TC_OK || splits == 1) return status;
     const uint64_t elements = uint64_t{shape.tokens} * shape.size * key_heads;
     shares_kernel<<<grid_for(elements, kThreads), kThreads, 0, s>>>(shape, splits, static_cast<float*>(parts.ptr),
