@@ -62,7 +62,8 @@ def near(got, want, bound, what: str) -> None:
     assert got.shape == want.shape, what
     special = ~np.isfinite(want)
     assert np.array_equal(got[special], want[special], equal_nan=True), what
-    off = np.abs(got - want)[~special]
+    with np.errstate(invalid="ignore"):
+        off = np.abs(got - want)[~special]
     most = np.broadcast_to(np.asarray(bound, np.float64), want.shape)[~special]
     bad = ~(off <= most)
     assert not bad.any(), f"{what}: {bad.sum()} of {bad.size} off, by up to {np.nanmax(off[bad] / np.maximum(most[bad], 1e-300)):.3g} bounds"
