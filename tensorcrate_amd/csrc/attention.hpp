@@ -63,6 +63,7 @@ struct Shape {
     uint32_t size;
     uint32_t tokens;
     uint32_t sequences;  // 0: all tokens are one
+    uint32_t by_sequence;  // blocks end where sequences do (`Owned`)
     const uint32_t* offsets;
     float scale;
     Steps q, k, v, out;
@@ -343,6 +344,65 @@ __device__ __forceinline__ Span span_of(const Shape& shape, uint32_t token) {
     return {first, end < shape.tokens ? end : shape.tokens};
 }
 
+// The tokens that a block owns: from `first` on, `end` not among them.
+//   By sequence, a block's tokens are of one sequence (or of none: those before
+// the first and past the last offset are taken like one), and what it sweeps
+// ends with it; otherwise tiles are every kOwned tokens, cheaper to find, and
+// each lane has its own token's span.
+struct Owned {
+    uint32_t first, end;
+    Span span;  // by sequence: of all its tokens
+};
+
+// Tile `tile` of `owned` tokens; kNone as `first` past the last one.  Its
+// sequence is the one whose tiles, counted over the sequences before it, have
+// it: a scan of THREADS sequences at a time.  `backwards` takes a sequence's
+// last tile first.
+template <int THREADS>
+__device__ __forceinline__ Owned owned_by(const Shape& shape, uint32_t owned, uint32_t tile, bool backwards) {
+    if (!shape.by_sequence) {
+        const uint32_t tiles = (shape.tokens + owned - 1) / owned;
+        const uint32_t first = (backwards ? tiles - 1 - tile : tile) * owned;
+        return {first, shape.tokens, {0, shape.tokens}};
+    }
+    __shared__ uint32_t sums[THREADS / 64];
+    __shared__ Owned found;
+    if (threadIdx.x == 0) found = {kNone, 0, {kNone, 0}};
+    uint32_t passed = 0;
+    for (uint32_t from = 0; from < shape.sequences + 2; from += THREADS) {
+        const uint32_t n = from + threadIdx.x;  // 0 and sequences + 1: of no sequence
+        uint32_t first = 0, end = 0;
+        if (n < shape.sequences + 2) {
+            first = n == 0 ? 0 : shape.offsets[n - 1];
+            end = n == shape.sequences + 1 ? shape.tokens : shape.offsets[n];
+            end = end < shape.tokens ? end : shape.tokens;
+        }
+        const uint32_t count = first < end ? (end - first + owned - 1) / owned : 0;
+        uint32_t upto = count;
+        for (int offset = 1; offset < 64; offset *= 2) {
+            const uint32_t other = __shfl_up(upto, offset);
+            if (static_cast<int>(threadIdx.x % 64) >= offset) upto += other;
+        }
+        if (threadIdx.x % 64 == 63) sums[threadIdx.x / 64] = upto;
+        __syncthreads();
+        uint32_t all = 0;
+        for (int w = 0; w < THREADS / 64; w++) {
+            if (w < static_cast<int>(threadIdx.x / 64)) upto += sums[w];
+            all += sums[w];
+        }
+        const uint32_t within = tile - (passed + upto - count);  // wraps where the tile is before these
+        if (tile >= passed + upto - count && within < count) {
+            const bool none = n == 0 || n == shape.sequences + 1;
+            found = {first + (backwards ? count - 1 - within : within) * owned, end,
+                     none ? Span{kNone, 0} : Span{first, end}};
+        }
+        passed += all;
+        __syncthreads();
+    }
+    const auto uniform = [](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(v)); };
+    return {uniform(found.first), uniform(found.end), {uniform(found.span.first), uniform(found.span.end)}};
+}
+
 // The token behind the last sequence.
 __device__ __forceinline__ uint32_t limit_of(const Shape& shape) {
     if (shape.sequences == 0) return shape.tokens;
@@ -492,22 +552,25 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     // A stage an array, so that reads of one do not wait for loads to the other.
     __shared__ __attribute__((aligned(1024))) char stage_0[2 * KeyTile::kBytes], stage_1[2 * KeyTile::kBytes];
     __shared__ float scratch[kThreads / 64][8 * 32];
-    __shared__ uint32_t seen[2][kThreads / 64];
+    __shared__ uint32_t seen[2][kThreads / 64], marks[2];
     constexpr int kOperands = SIZE / kDeep;
 
     const int lane = threadIdx.x % 64, half = lane / 32, wave = threadIdx.x / 64;
     const Lanes lanes = KeyTile::lanes_of(lane);
     // The latest tokens, which see the most keys, first.
-    const uint32_t tiles = (shape.tokens + kOwned - 1) / kOwned;
     const uint32_t head = blockIdx.x % shape.heads;
-    const uint32_t first = (tiles - 1 - blockIdx.x / shape.heads) * kOwned;
+    const Owned mine = owned_by<kThreads>(shape, kOwned, blockIdx.x / shape.heads, true);
+    const uint32_t first = mine.first;
+    if (first == kNone) return;
     const uint32_t wave_first = first + wave * 32;
     const uint32_t token = wave_first + lane % 32;
-    const Span span = span_of(shape, token);
-    const uint32_t limit = limit_of(shape);
+    // (Lanes past the block's tokens work as if they had one, for nothing.)
+    const Span span = shape.by_sequence ? mine.span : span_of(shape, token);
+    const uint32_t limit = shape.by_sequence ? mine.end : limit_of(shape);
     // Keys that some, and that all, of the wave's queries may see.
     const uint32_t some = wave_least(span.first), all = wave_most(span.first);
     if (lane == 0) seen[0][wave] = some, seen[1][wave] = all;
+    if (threadIdx.x < 2) marks[threadIdx.x] = 0;
 
     const S* query = q + (token < shape.tokens ? token : 0) * shape.q.token + head * shape.q.head;
     uint4 queries[kOperands];
@@ -536,7 +599,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
         // before a sequence's first key or past the first query.
         const auto masked = [&](uint32_t tile) { return tile < block_all || tile + kSwept - 1 > first; };
         Stager<SIZE, kSwept, DIRECT> key_stager(shape.k.token, shape.size), value_stager(shape.v.token, shape.size);
-        uint32_t at = begin / kSwept * kSwept;
+        uint32_t at = shape.by_sequence ? begin : begin / kSwept * kSwept;
         bool special = false;
         const auto fetch = [&](char* stage, uint32_t tile) {
             key_stager.fetch(KeyTile{stage}, keys, tile, limit);
@@ -545,8 +608,12 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
         const auto land = [&](char* stage, uint32_t tile) {
             key_stager.land(KeyTile{stage});
             value_stager.land(KeyTile{stage + KeyTile::kBytes});
+            // What this thread fetched it may look at before the others have
+            // theirs; a stage's mark names the tile, so that none is cleared.
+            uint32_t& mark = marks[stage == stage_1];
+            if (masked(tile) && specials_in<kThreads>(KeyTile{stage + KeyTile::kBytes})) mark = tile + 1;
             __syncthreads();
-            special = masked(tile) && __syncthreads_or(specials_in<kThreads>(KeyTile{stage + KeyTile::kBytes}));
+            special = masked(tile) && __builtin_amdgcn_readfirstlane(mark) == tile + 1;
         };
         // The tile at `at` in stage `here`, while the next one is on its way.
         const auto turn = [&](char* here, char* there) {
@@ -629,7 +696,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
         sweep(std::true_type());
     }
     total = halves_sum(total);
-    if (token >= shape.tokens) return;
+    if (token >= mine.end) return;
     store_column<S, SIZE>(out + token * shape.out.token + head * shape.out.head, acc, total == 0.0f ? 0.0f : 1.0f / total,
                           shape.size, half);
     if (normalizers != nullptr && half == 0) {
@@ -711,20 +778,23 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     // A stage an array, so that reads of one do not wait for loads to the other.
     __shared__ __attribute__((aligned(1024))) char stage_0[2 * KeyTile::kBytes], stage_1[2 * KeyTile::kBytes];
     __shared__ float scratch[kThreads / 64][8 * 32];
-    __shared__ uint32_t seen[2][kThreads / 64];
+    __shared__ uint32_t seen[2][kThreads / 64], marks[2];
     constexpr int kOperands = SIZE / kDeep;
 
     const int lane = threadIdx.x % 64, half = lane / 32, wave = threadIdx.x / 64;
     const Lanes lanes = KeyTile::lanes_of(lane);
-    const uint32_t tiles = (shape.tokens + kOwned - 1) / kOwned;
     const uint32_t head = blockIdx.x % shape.heads;
-    const uint32_t first = (tiles - 1 - blockIdx.x / shape.heads) * kOwned;
+    const Owned mine = owned_by<kThreads>(shape, kOwned, blockIdx.x / shape.heads, true);
+    const uint32_t first = mine.first;
+    if (first == kNone) return;
     const uint32_t wave_first = first + wave * 32;
     const uint32_t token = wave_first + lane % 32;
-    const Span span = span_of(shape, token);
-    const uint32_t limit = limit_of(shape);
+    // (Lanes past the block's tokens work as if they had one, for nothing.)
+    const Span span = shape.by_sequence ? mine.span : span_of(shape, token);
+    const uint32_t limit = shape.by_sequence ? mine.end : limit_of(shape);
     const uint32_t some = wave_least(span.first), all = wave_most(span.first);
     if (lane == 0) seen[0][wave] = some, seen[1][wave] = all;
+    if (threadIdx.x < 2) marks[threadIdx.x] = 0;
 
     const uint32_t inside = token < shape.tokens ? token : 0;
     const S* query = q + inside * shape.q.token + head * shape.q.head;
@@ -759,7 +829,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
         // before a sequence's first key or past the first query.
         const auto masked = [&](uint32_t tile) { return tile < block_all || tile + kSwept - 1 > first; };
         Stager<SIZE, kSwept, DIRECT> key_stager(shape.k.token, shape.size), value_stager(shape.v.token, shape.size);
-        uint32_t at = begin / kSwept * kSwept;
+        uint32_t at = shape.by_sequence ? begin : begin / kSwept * kSwept;
         bool special = false;
         const auto fetch = [&](char* stage, uint32_t tile) {
             key_stager.fetch(KeyTile{stage}, keys, tile, limit);
@@ -768,8 +838,12 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
         const auto land = [&](char* stage, uint32_t tile) {
             key_stager.land(KeyTile{stage});
             value_stager.land(KeyTile{stage + KeyTile::kBytes});
+            // What this thread fetched it may look at before the others have
+            // theirs; a stage's mark names the tile, so that none is cleared.
+            uint32_t& mark = marks[stage == stage_1];
+            if (masked(tile) && specials_in<kThreads>(KeyTile{stage})) mark = tile + 1;
             __syncthreads();
-            special = masked(tile) && __syncthreads_or(specials_in<kThreads>(KeyTile{stage}));
+            special = masked(tile) && __builtin_amdgcn_readfirstlane(mark) == tile + 1;
         };
         // The tile at `at` in stage `here`, while the next one is on its way.
         const auto turn = [&](char* here, char* there) {
@@ -818,7 +892,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
         __syncthreads();
         sweep(std::true_type());
     }
-    if (token >= shape.tokens) return;
+    if (token >= mine.end) return;
     store_column<S, SIZE>(dq + token * shape.q.token + head * shape.q.head, acc, shape.scale / factor, shape.size, half);
 }
 
@@ -844,7 +918,7 @@ __global__ void __launch_bounds__(key_threads(SIZE)) __attribute__((amdgpu_waves
     __shared__ __attribute__((aligned(1024))) char stage_0[2 * QueryTile::kBytes], stage_1[2 * QueryTile::kBytes];
     __shared__ __attribute__((aligned(16))) float values_0[2][kSwept], values_1[2][kSwept];
     __shared__ float scratch[kWaves][8 * 32];
-    __shared__ uint32_t seen[2][kWaves];
+    __shared__ uint32_t seen[2][kWaves], marks[2];
     constexpr int kOperands = SIZE / kDeep;
 
     const int lane = threadIdx.x % 64, half = lane / 32, wave = threadIdx.x / 64;
@@ -855,14 +929,18 @@ __global__ void __launch_bounds__(key_threads(SIZE)) __attribute__((amdgpu_waves
     const uint32_t key_head = blockIdx.x % columns / splits, share = blockIdx.x % splits;
     const uint32_t share_heads = shape.group / splits;
     const uint32_t first_head = key_head * shape.group + share * share_heads;
-    const uint32_t first = blockIdx.x / columns * kKeys;
+    const Owned mine = owned_by<key_threads(SIZE)>(shape, kKeys, blockIdx.x / columns, false);
+    const uint32_t first = mine.first;
+    if (first == kNone) return;
     const uint32_t wave_first = first + wave * 32;
     const uint32_t token = wave_first + lane % 32;
-    const Span span = span_of(shape, token);
-    const uint32_t limit = limit_of(shape);
+    // (Lanes past the block's tokens work as if they had one, for nothing.)
+    const Span span = shape.by_sequence ? mine.span : span_of(shape, token);
+    const uint32_t limit = shape.by_sequence ? mine.end : limit_of(shape);
     // Queries before which all, and some, of the wave's keys are seen.
     const uint32_t all = wave_least(span.end), some = wave_most(span.end);
     if (lane == 0) seen[0][wave] = all, seen[1][wave] = some;
+    if (threadIdx.x < 2) marks[threadIdx.x] = 0;
 
     const uint32_t inside = token < shape.tokens ? token : 0;
     const S* key = k + inside * shape.k.token + key_head * shape.k.head;
@@ -918,9 +996,13 @@ __global__ void __launch_bounds__(key_threads(SIZE)) __attribute__((amdgpu_waves
                 row_value = threadIdx.x < kSwept ? fmaf(row_value, kLog2e, -kBackPower) : row_value * ds_scale;
                 values_here[threadIdx.x / kSwept][threadIdx.x % kSwept] = row_value;
             }
+            uint32_t& mark = marks[stage == stage_1];
+            if (masked(tile_of(n)) && (specials_in<key_threads(SIZE)>(QueryTile{stage}) ||
+                                       specials_in<key_threads(SIZE)>(QueryTile{stage + QueryTile::kBytes}))) {
+                mark = n + 1;
+            }
             __syncthreads();
-            special = masked(tile_of(n)) && __syncthreads_or(specials_in<key_threads(SIZE)>(QueryTile{stage}) ||
-                                                             specials_in<key_threads(SIZE)>(QueryTile{stage + QueryTile::kBytes}));
+            special = masked(tile_of(n)) && __builtin_amdgcn_readfirstlane(mark) == n + 1;
         };
         uint32_t n = 0;
         const auto turn = [&](char* here, const float (&row_values)[2][kSwept], char* there,
@@ -986,7 +1068,7 @@ __global__ void __launch_bounds__(key_threads(SIZE)) __attribute__((amdgpu_waves
         __syncthreads();
         sweep(std::true_type());
     }
-    if (token >= shape.tokens) return;
+    if (token >= mine.end) return;
     const float scale_k = shape.scale / factor, scale_v = power2(-kBackPower);
     if (splits == 1) {
         store_column<S, SIZE>(dk + token * shape.k.token + key_head * shape.k.head, acc_k, scale_k, shape.size, half);
@@ -1051,9 +1133,15 @@ bool direct(uint32_t size, std::initializer_list<std::pair<const void*, Steps>> 
         constexpr bool DIRECT = false; TC_ATTENTION_SIZE(size, __VA_ARGS__)          \
     }
 
+// At most as many tiles of `owned` tokens as `owned_by` finds.
+uint32_t tiles_of(const Shape& shape, uint32_t owned) {
+    const uint32_t tiles = (shape.tokens + owned - 1) / owned;
+    return shape.by_sequence ? tiles + shape.sequences + 2 : tiles;
+}
+
 int forward(const Shape& shape, const void* q, const void* k, const void* v, void* out, float* normalizers) {
     TC_STREAM(s);
-    const uint32_t tiles = (shape.tokens + kOwned - 1) / kOwned;
+    const uint32_t tiles = tiles_of(shape, kOwned);
     const bool straight = direct(shape.size, {{k, shape.k}, {v, shape.v}});
     TC_ATTENTION_FORM(shape.size, straight,
                       forward_kernel<SIZE, DIRECT><<<tiles * shape.heads, kThreads, 0, s>>>(
@@ -1066,7 +1154,7 @@ int backward(const Shape& shape, const void* d_out, const void* q, const void* k
              const float* normalizers, void* dq, void* dk, void* dv) {
     TC_STREAM(s);
     const char* what = "attention, backward";
-    const uint32_t tiles = (shape.tokens + kOwned - 1) / kOwned;
+    const uint32_t tiles = tiles_of(shape, kOwned);
     const uint32_t key_heads = shape.heads / shape.group;
     // Shares of a key head's queries where the key heads alone would leave the
     // compute units idle: the most that divide its heads, up to four blocks
@@ -1099,7 +1187,7 @@ int backward(const Shape& shape, const void* d_out, const void* q, const void* k
     }
     const bool rows_straight = direct(shape.size, {{q, shape.q}, {d_out, shape.out}});
     TC_ATTENTION_FORM(shape.size, rows_straight,
-                      const uint32_t key_tiles = (shape.tokens + key_threads(SIZE) / 2 - 1) / (key_threads(SIZE) / 2);
+                      const uint32_t key_tiles = tiles_of(shape, key_threads(SIZE) / 2);
                       keys_kernel<SIZE, DIRECT><<<key_tiles * key_heads * splits, key_threads(SIZE), 0, s>>>(
                           shape, splits, d, queries, keys, values, normalizers, sums, largest, static_cast<S*>(dk),
                           static_cast<S*>(dv), static_cast<float*>(parts.ptr)))

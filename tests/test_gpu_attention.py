@@ -127,11 +127,15 @@ CASES = [
     (90, 2, 1, 24, [0, 1, 2, 3, 40, 40, 41, 90]), (190, 4, 2, 64, [3, 3, 70, 128, 129, 180]),
     (260, 2, 2, 128, [0, 64, 128, 192, 256]), (333, 6, 2, 72, [0, 32, 100, 333]), (140, 1, 1, 8, [0, 0, 0]),
     (400, 3, 3, 65, [100, 101, 231, 399]), (130, 2, 1, 48, list(range(131))),
+    # Long sequences, whose blocks end with them, and so many that blocks do not.
+    (1500, 2, 1, 64, [0, 1, 130, 700, 700, 1400]), (1100, 2, 2, 128, [50, 306, 562, 1090]),
+    (520, 16, 4, 16, [0, 129, 400, 520]), (600, 4, 2, 40, [5] + list(range(9, 599, 4))),
+    (300, 16, 4, 72, [0, 0, 0, 150, 151] + [290] * 40 + [291]), (700, 2, 1, 96, [0, 300] + [300] * 300 + [650]),
 ]
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=KIND_NAMES.get)
-@pytest.mark.parametrize("case", CASES, ids=str)
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c[:4])) + ("" if c[4] is None else f"-{len(c[4])}"))
 def test_attention(kind, case):
     tokens, heads, key_heads, size, ends = case
     operands = inputs(kind, tokens, heads, key_heads, size, seed=tokens + size)
@@ -162,11 +166,13 @@ def test_rising_scores(kind):
 @pytest.mark.parametrize("kind", KINDS, ids=KIND_NAMES.get)
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("size", [64, 100])
-def test_what_is_not_seen_does_not_matter(kind, value, size):
+@pytest.mark.parametrize("heads, empty", [(4, 0), (16, 40)])
+def test_what_is_not_seen_does_not_matter(kind, value, size, heads, empty):
     # Tokens of no sequence, of one sequence only, and a late token, hold no
     # number: nothing that does not see them changes.
-    ends = [2, 40, 90, 100, 230, 300]
-    q, k, v, d = inputs(kind, 310, 4, 2, size, 7)
+    # (Many sequences, most of them empty, have blocks across them.)
+    ends = [2, 40, 90, 100, 230] + [300] * (1 + empty)
+    q, k, v, d = inputs(kind, 310, heads, 2, size, 7)
     scale = float(np.float32(size ** -0.5))
     want = run(kind, q, k, v, d, ends, scale)
     for t in (q, k, v, d):
