@@ -772,7 +772,7 @@ __device__ __forceinline__ float ds_factor(const float* largest) {
 template <int SIZE, bool DIRECT>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
     queries_kernel(const Shape shape, const S* __restrict__ d_out, const S* __restrict__ q, const S* __restrict__ k,
-                   const S* __restrict__ v, const float* __restrict__ normalizers, const float* __restrict__ dots,
+                   const S* __restrict__ v, const float* __restrict__ normalizers, float* __restrict__ dots,
                    const float* __restrict__ largest, S* __restrict__ dq) {
     using KeyTile = Tile<SIZE, kSwept>;
     // A stage an array, so that reads of one do not wait for loads to the other.
@@ -807,7 +807,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     }
     const float normalizer = normalizers[uint64_t{head} * shape.tokens + inside] * kLog2e;
     const float factor = ds_factor(largest);
-    const float dot = dots[uint64_t{head} * shape.tokens + inside] * factor;
+    float dot = dots[uint64_t{head} * shape.tokens + inside] * factor;
     __syncthreads();
     uint32_t begin, block_all;
     over_waves(seen, &begin, &block_all);
@@ -818,6 +818,52 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     f32x16 acc[SIZE / 32] = {};
 
     const uint32_t end = first + kOwned < limit ? first + kOwned : limit;
+    // The first tokens of a sequence see few keys.  There o is as large as the
+    // v_j, and what it lost when it was rounded to 16 bits weighs as much in
+    // ds as ds's own rounding and more (2 tokens: dq off by 0.37%, where all
+    // other roundings come to 0.23%; it falls with the root of the number of
+    // keys).  So D of a sequence's first kOwned tokens is summed from the p_ij
+    // and do_i . v_j, and left for the kernel of dk and dv, which runs next.
+    if constexpr (!kWide) {
+        const bool early = span.first != kNone && token >= span.first && token - span.first < kOwned;
+        const uint32_t wave_early = wave_least(early ? span.first : kNone);
+        __syncthreads();
+        if (lane == 0) seen[0][wave] = wave_early;
+        __syncthreads();
+        uint32_t early_begin, unused;
+        over_waves(seen, &early_begin, &unused);
+        if (early_begin < end) {
+            Stager<SIZE, kSwept, DIRECT> key_stager(shape.k.token, shape.size), value_stager(shape.v.token, shape.size);
+            const KeyTile key_tile{stage_0}, value_tile{stage_0 + KeyTile::kBytes};
+            float sum = 0.0f;
+            for (uint32_t at = early_begin; at < end; at += kSwept) {
+                key_stager.fetch(key_tile, keys, at, limit);
+                value_stager.fetch(value_tile, values, at, limit);
+                key_stager.land(key_tile);
+                value_stager.land(value_tile);
+                __syncthreads();
+#pragma unroll 1
+                for (int b = 0; b < static_cast<int>(kSwept) / 32; b++) {
+                    f32x16 s = {}, d = {};
+#pragma unroll
+                    for (int n = 0; n < kOperands; n++) {
+                        s = product(key_tile.by_row(lanes, b * 32, n), queries[n], s);
+                        d = product(value_tile.by_row(lanes, b * 32, n), d_rows[n], d);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const uint32_t key = at + b * 32 + row_of(i, half);
+                        const float weighted_dot = power2(fmaf(s[i], c, -normalizer)) * d[i];
+                        if (key >= span.first && key <= token) sum += weighted_dot;
+                    }
+                }
+                __syncthreads();
+            }
+            sum = halves_sum(sum);
+            if (early) dot = sum * factor;
+            if (early && half == 0 && token < mine.end) dots[uint64_t{head} * shape.tokens + token] = sum;
+        }
+    }
     // One sweep over the keys.  Without SLOW it ends, true, at the first masked
     // tile with a special value: what handles those is kept out of the sweep's
     // registers.
@@ -1185,18 +1231,18 @@ int backward(const Shape& shape, const void* d_out, const void* q, const void* k
         status = check_launch(what);
         if (status != TC_OK) return status;
     }
+    const bool keys_straight = direct(shape.size, {{k, shape.k}, {v, shape.v}});
+    TC_ATTENTION_FORM(shape.size, keys_straight,
+                      queries_kernel<SIZE, DIRECT><<<tiles * shape.heads, kThreads, 0, s>>>(
+                          shape, d, queries, keys, values, normalizers, sums, largest, static_cast<S*>(dq)))
+    status = check_launch(what);
+    if (status != TC_OK) return status;
     const bool rows_straight = direct(shape.size, {{q, shape.q}, {d_out, shape.out}});
     TC_ATTENTION_FORM(shape.size, rows_straight,
                       const uint32_t key_tiles = tiles_of(shape, key_threads(SIZE) / 2);
                       keys_kernel<SIZE, DIRECT><<<key_tiles * key_heads * splits, key_threads(SIZE), 0, s>>>(
                           shape, splits, d, queries, keys, values, normalizers, sums, largest, static_cast<S*>(dk),
                           static_cast<S*>(dv), static_cast<float*>(parts.ptr)))
-    status = check_launch(what);
-    if (status != TC_OK) return status;
-    const bool keys_straight = direct(shape.size, {{k, shape.k}, {v, shape.v}});
-    TC_ATTENTION_FORM(shape.size, keys_straight,
-                      queries_kernel<SIZE, DIRECT><<<tiles * shape.heads, kThreads, 0, s>>>(
-                          shape, d, queries, keys, values, normalizers, sums, largest, static_cast<S*>(dq)))
     status = check_launch(what);
     if (status != TC_OK || splits == 1) return status;
     const uint64_t elements = uint64_t{shape.tokens} * shape.size * key_heads;

@@ -214,3 +214,21 @@ def test_no_tokens():
     shape = lib.attention(lib.F32, 0, 2, 1, 16, 1.0, None, 0, *[(32, 16)] * 4)
     lib.call("tc_attention", shape, None, None, None, None, None)
     lib.call("tc_attention_backward", shape, *[None] * 9)
+
+
+@pytest.mark.parametrize("kind", [lib.F16, lib.BF16], ids=KIND_NAMES.get)
+@pytest.mark.parametrize("heads", [2, 16])
+@pytest.mark.parametrize("length", [2, 5, 30, 200])
+def test_short_sequences_lose_nothing_to_the_rounding_of_the_result(kind, heads, length):
+    # Two roundings of independent values, of ds and of the result, are
+    # 0.42 roundings each in the root of the mean square; what o lost as it was
+    # rounded would be one more of up to a whole rounding.
+    tokens = 1200 if length > 2 else 600
+    ends = list(range(0, tokens + 1, length))
+    q, k, v, d = inputs(kind, tokens, heads, 1, 64, length, 1.2)
+    got = run(kind, q, k, v, d, ends, 0.125)
+    out, normalizers, _ = language.attention(q, k, v, ends, 0.125)
+    grads, _ = language.attention_backward(d, q, k, v, out, normalizers, ends, 0.125)
+    for name, have, want in zip(("dq", "dk", "dv"), got[2:], grads):
+        off = np.linalg.norm(have - want) / np.linalg.norm(want)
+        assert off < 0.75 * ROUNDING[kind], (name, off / ROUNDING[kind])
