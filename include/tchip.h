@@ -643,7 +643,8 @@ int tc_fused_resident(uint64_t limit, uint64_t* resident, uint64_t* current_limi
  * of `weight_dtype` (`dtype`, or TC_F32); either may be null (1, or 0).
  * `means` and `scales` receive each row's f32 statistics for the backward
  * pass, and may be null.  y may be x itself (with the same step), not
- * otherwise overlap it.  Rows of no elements are refused. */
+ * otherwise overlap it.  Rows of no elements, and of more than 2^24, are
+ * refused. */
 int tc_layer_norm(uint32_t dtype, uint32_t weight_dtype, const void* x, uint64_t x_step, uint64_t rows, uint64_t cols,
                   const void* weight, const void* bias, float epsilon, void* y, uint64_t y_step, float* means,
                   float* scales);
@@ -722,7 +723,9 @@ int tc_clip_global_norm(uint32_t count, const uint32_t* dtypes, const void* cons
  * are in none: their results and gradients are zeros and nothing reads their
  * values.  With `sequences` 0 all tokens are one sequence, and `offsets` is
  * not read.
- *   Scores are scale * q . k (`scale` positive and finite). */
+ *   Scores are scale * q . k (`scale` positive and finite).  Fewer than 2^24
+ * blocks of 128 tokens of a head, counting a part of one for each sequence,
+ * are taken. */
 typedef struct tc_attention_shape {
     uint32_t dtype;
     uint32_t query_heads;

@@ -40,9 +40,11 @@ int check(const std::string& what, const tc_attention_shape* given, Shape* shape
     if (!(a.scale > 0.0f && a.scale < INFINITY)) {
         return fail(TC_INVALID, what + ": a scale of " + std::to_string(a.scale));
     }
-    // A dispatch holds fewer than 2^32 work-items, and tokens are counted in
-    // 32 bits with room for a tile behind them.
-    if (a.tokens > 0x7fffff00u || a.tokens * a.query_heads > 0x0fffffffu * uint64_t{8}) {
+    // Tokens are counted in 32 bits with room for a tile behind them, and a
+    // dispatch holds fewer than 2^32 work-items, 256 for every 128 tokens.
+    const bool apart = by_sequence(a);
+    const uint64_t tiles = a.tokens / attention::kOwned + 1 + (apart ? uint64_t{a.sequences} + 2 : 0);
+    if (a.tokens > 0x7fffff00u || tiles > 0xffffffu / a.query_heads) {
         return fail(TC_UNSUPPORTED, what + ": " + std::to_string(a.tokens) + " tokens of " +
                                         std::to_string(a.query_heads) + " heads");
     }
@@ -78,7 +80,7 @@ int check(const std::string& what, const tc_attention_shape* given, Shape* shape
                    a.head_size,
                    static_cast<uint32_t>(a.tokens),
                    a.sequences,
-                   by_sequence(a),
+                   apart,
                    a.offsets,
                    a.scale,
                    {a.query_token_step, a.query_head_step},

@@ -30,12 +30,22 @@
 // |do| times the largest |v|, times the power of two that brings that below
 // 2^15.
 //
-// Sequences lie one behind another, and tiles of tokens do not stop at their
-// ends: a tile that some row of a wave sees only in part is masked element by
-// element.  A masked weight is 0, and 0 times an infinity or a NaN would be a
-// NaN, so a tile that is masked and holds such a value takes a slow path: the
-// product with zeros in their place, then theirs alone where the weight is not
-// 0.
+// Measured (a large bf16 product reaches 1372 TFLOP/s): 8192 tokens, 16 heads
+// of 128 on 4 key heads, bf16: forward 305 us (900 TFLOP/s, the matrix cores
+// busy 55% of the time), dq 400 (1030), dk and dv 610 to 670 (850; both with
+// the two products that the other computes too); 16384 tokens, 8 heads of 64 on
+// one, forward 315 us (870); 7001 f16 tokens of 19 sequences, 12 heads of 80,
+// forward and backward 155 us, the longest sequence's 18 tiles one after
+// another.  What carried it: loads straight to LDS (forward 397 -> 330 us), one
+// number a lane for all LDS addresses and a path without masks (330 -> 305),
+// 256 keys a block for dk and dv (816 -> 675), blocks by sequence (7001 tokens,
+// 237 -> 154).
+//
+// Sequences lie one behind another.  A tile that some row of a wave sees only
+// in part is masked element by element.  A masked weight is 0, and 0 times an
+// infinity or a NaN would be a NaN, so a tile that is masked and holds such a
+// value takes a slow path: the product with zeros in their place, then theirs
+// alone where the weight is not 0.
 #pragma once
 
 #include <type_traits>
@@ -946,7 +956,10 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
 // heads that the key head serves.  With several shares they are left in f32
 // as `parts`[key head][share][dk, dv][token][size], to be added in their order.
 // Threads of a block: a wave of 32 keys each, all that a compute unit holds
-// where registers and LDS leave room for one block.
+// where LDS leaves room for one block.  In the largest 16-bit heads it holds the
+// values, so that registers let two waves share a matrix core: 8192 bf16 tokens,
+// 16 heads of 128, 816 us with the values in registers and one wave, 776 with
+// blocks of 128 keys and tiles of 32 queries, 675 so.
 constexpr int key_threads(int size) { return !kWide && size > 96 ? 512 : kThreads; }
 
 template <int SIZE, bool DIRECT>
@@ -1062,7 +1075,11 @@ __global__ void __launch_bounds__(key_threads(SIZE)) __attribute__((amdgpu_waves
 #pragma unroll
                 for (int o = 0; o < kOperands; o++) {
                     s = product(query_tile.by_row(lanes, b * 32, o), keys[o], s);
-                    d = product(d_tile.by_row(lanes, b * 32, o), kValuesInLds ? own_values.by_row(lanes, 0, o) : values[kValuesInLds ? 0 : o], d);
+                    if constexpr (kValuesInLds) {
+                        d = product(d_tile.by_row(lanes, b * 32, o), own_values.by_row(lanes, 0, o), d);
+                    } else {
+                        d = product(d_tile.by_row(lanes, b * 32, o), values[o], d);
+                    }
                 }
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll

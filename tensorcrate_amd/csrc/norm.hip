@@ -12,6 +12,13 @@
 // a sum of squares would cancel).  A group of lanes walks rows a grid apart
 // with the next row's words already in flight, and keeps its columns' weights.
 //
+// Measured (a large copy moves 6.5 TB/s): 16384 bf16 rows of 4096 forward
+// 50 us, 5.4 TB/s; 10007 f16 rows of 2050, views that start at any element,
+// backward 40 us, 3.1 TB/s, of which 7 are the sums of dw and db and about 8
+// the blocks' first and last rows; 64 f32 rows of 1024 the 4.5 us of a launch.
+// One word a lane instead of two and grids that fill the chip without walking
+// rows took 68 and 52 us forward; one row a block backward 47.
+//
 // dw and db are sums over all rows: a lane sums its columns over the rows of
 // its walk in registers, each block writes those sums once, and a second
 // kernel adds the blocks' in block order, so the result does not depend on
@@ -659,7 +666,7 @@ int check_norm(const char* what, uint32_t dtype, uint32_t weight_dtype, uint64_t
         return fail(TC_INVALID, std::string(what) + ": shape [" + std::to_string(rows) + ", " + std::to_string(cols) +
                                     "] has more elements than fit in a usize");
     }
-    if (cols > (uint64_t{1} << 31)) {
+    if (cols > (uint64_t{1} << 24)) {  // 128 work-items a column are to stay below 2^32
         return fail(TC_UNSUPPORTED, std::string(what) + ": rows of " + std::to_string(cols) + " elements");
     }
     return TC_OK;

@@ -1,6 +1,8 @@
 """What the language-model operators refuse, on the host and before any device
 work (no test here touches a device)."""
 
+import ctypes
+
 from tensorcrate_amd import lib
 
 
@@ -22,6 +24,7 @@ def test_layer_norm():
     assert refused("tc_layer_norm", F, F, 64, 8, 2, 8, None, None, E, 64, 5, None, None)[0] == lib.INVALID
     assert refused("tc_layer_norm", F, F, 64, 0, 2, 0, None, None, E, 64, 0, None, None) == (
         lib.INVALID, "layer norm: rows of no elements")
+    assert refused("tc_layer_norm", F, F, 64, 2**25, 1, 2**25, None, None, E, 64, 2**25, None, None)[0] == lib.UNSUPPORTED
     assert refused("tc_layer_norm", F, F, None, 8, 2, 8, None, None, E, 64, 8, None, None) == (
         lib.INVALID, "layer norm: a null operand")
     assert refused("tc_layer_norm", F, F, 64, 8, 2, 8, None, None, E, None, 8, None, None)[0] == lib.INVALID
@@ -90,6 +93,12 @@ def test_clip():
     assert refused("tc_global_norm", 2, *some, 64)[0] == lib.INVALID
 
 
+def test_the_attention_shape_is_the_headers():
+    # Natural C alignment of `tc_attention_shape`.
+    assert ctypes.sizeof(lib.AttentionShape) == 4 * 4 + 8 + 4 + 4 + 8 + 8 * 8
+    assert lib.AttentionShape.tokens.offset == 16 and lib.AttentionShape.offsets.offset == 32
+
+
 def test_attention():
     def shape(dtype=lib.F32, tokens=10, heads=4, key_heads=2, size=16, scale=0.25, offsets=None, sequences=0,
               query=(64, 16), key=(32, 16), value=(32, 16), out=(64, 16)):
@@ -113,7 +122,11 @@ def test_attention():
         for steps in ((16, 16), (64, 15), (0, 16), (16, 0), (2**62, 16), (16, 2**62)):
             assert forward(shape(**{name: steps}))[0] == lib.INVALID, (name, steps)
             assert back(shape(**{name: steps}))[0] == lib.INVALID, (name, steps)
-    assert forward(shape(tokens=2**31, query=(64, 16))) [0] == lib.UNSUPPORTED
+    assert forward(shape(tokens=2**31))[0] == lib.UNSUPPORTED
+    # 2^24 blocks and more are no dispatch: of tokens, of heads, of sequences.
+    many = dict(heads=2**24, key_heads=2**24, size=1, query=(2**24, 1), key=(2**24, 1), value=(2**24, 1), out=(2**24, 1))
+    assert forward(shape(tokens=1, **many))[0] == lib.UNSUPPORTED
+    assert forward(shape(tokens=2**30, heads=4, key_heads=2))[0] == lib.UNSUPPORTED
     null = (lib.INVALID, "attention: a null operand")
     assert forward(shape(sequences=2)) == null
     for missing in range(4):
