@@ -32,7 +32,7 @@
 //
 // Measured (a large bf16 product reaches 1372 TFLOP/s): 8192 tokens, 16 heads
 // of 128 on 4 key heads, bf16: forward 305 us (900 TFLOP/s, the matrix cores
-// busy 55% of the time), dq 400 (1030), dk and dv 610 to 670 (850; both with
+// busy 54% of the time), dq 392 (1050, 60%), dk and dv 609 (900, 47%; both with
 // the two products that the other computes too); 16384 tokens, 8 heads of 64 on
 // one, forward 315 us (870); 7001 f16 tokens of 19 sequences, 12 heads of 80,
 // forward and backward 155 us, the longest sequence's 18 tiles one after

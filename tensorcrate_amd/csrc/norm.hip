@@ -14,7 +14,7 @@
 //
 // Measured (a large copy moves 6.5 TB/s): 16384 bf16 rows of 4096 forward
 // 50 us, 5.4 TB/s; 10007 f16 rows of 2050, views that start at any element,
-// backward 40 us, 3.1 TB/s, of which 7 are the sums of dw and db and about 8
+// backward 40 us, 3.1 TB/s, of which 4 to 5 are the launch that adds dw and db and about 8
 // the blocks' first and last rows; 64 f32 rows of 1024 the 4.5 us of a launch.
 // One word a lane instead of two and grids that fill the chip without walking
 // rows took 68 and 52 us forward; one row a block backward 47.
