@@ -63,11 +63,17 @@ struct State {
 
 __device__ __forceinline__ float power(float v) { return __builtin_amdgcn_exp2f(v * kLog2e); }
 
+// Differences of logits below which a power is 0 in 32 bits, by far: larger
+// ones are taken for this one where they are multiplied by such a power, which
+// is 0 times infinity where the difference or its product with a sum overflows
+// (logits masked with the type's lowest number, or with -infinity).
+constexpr float kVanished = -1000.0f;
+
 // The state with another m, not less than its own.
 // A state of nothing but -infinity holds zeros (or the NaN of a NaN logit),
 // which stay.
 __device__ __forceinline__ void move(State& s, float to) {
-    const float shift = s.most == -INFINITY ? 0.0f : s.most - to;
+    const float shift = s.most == -INFINITY ? 0.0f : fmaxf(s.most - to, kVanished);
     const float factor = power(shift);
     s.mean = fmaf(s.sum, shift, s.mean) * factor;
     s.sum *= factor;
@@ -334,8 +340,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(T
                 const float d = value[u][e] - origin;
                 const float p = power(d);
                 state.sum += p;
-                // -infinity, whose power is 0, would make a NaN.
-                state.mean = fmaf(fmaxf(d, -1000.0f), p, state.mean);
+                state.mean = fmaf(fmaxf(d, kVanished), p, state.mean);
             }
         }
         if constexpr (TOP) {

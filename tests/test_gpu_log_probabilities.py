@@ -195,3 +195,37 @@ def test_backward_of_rows_with_nothing():
 def test_no_rows():
     lib.call("tc_log_probabilities", lib.F32, None, 9, 0, 9, None, None, None, None, 0, None, None)
     lib.call("tc_log_probabilities_backward", lib.F32, None, 9, 0, 9, None, None, None, None, None, None, 9)
+
+
+# The lowest finite numbers of the types, and others that masks are made with.
+FINITE_MASKS = [(lib.F32, -np.finfo(np.float32).max), (lib.F32, -1e38), (lib.F32, -1e37), (lib.F32, -1e9),
+                (lib.F16, -65504.0), (lib.BF16, -3.3895313892515355e38), (lib.BF16, -1e38)]
+
+
+@pytest.mark.parametrize("shape", [(3, 40), (3, 1000), (1, 33000), (2, 131072), (1100, 2050)], ids=str)
+@pytest.mark.parametrize("kind, mask", FINITE_MASKS)
+def test_logits_masked_with_a_number(kind, mask, shape):
+    # Their probability is 0 in 64 bits and in 32, as that of -infinity is.
+    rows, cols = shape
+    column = np.arange(cols)
+    x, tokens = inputs(kind, rows, cols, seed=11)
+    for masked in (column >= cols - 40 // 2, column < cols // 2, column // 8 % 2 == 0, column != cols // 3):
+        here = np.where(masked, stored(mask, kind), x)
+        removed = np.where(masked, -np.inf, x)
+        kept = np.flatnonzero(~masked).astype(np.uint32)
+        given = np.where(tokens == NONE, NONE, kept[tokens.astype(np.int64) % len(kept)]).astype(np.uint32)
+        top = min(5, len(kept))
+        check(removed, given, 0, run(kind, here, given, 0))
+        check(removed, given, top, run(kind, here, given, top))
+
+
+@pytest.mark.parametrize("kind, mask", FINITE_MASKS)
+@pytest.mark.parametrize("cols", [40, 33000])
+def test_rows_of_nothing_but_a_masks_number(kind, mask, cols):
+    # All alike, whatever the number: every token has the probability 1 / cols.
+    x = stored(np.full((2, cols), mask), kind)
+    got = run(kind, x, np.zeros(2, np.uint32), 3)
+    sums = (cols / 256 + 64) * EPSILON_32
+    near(got["entropies"], np.full(2, np.log(cols)), 2 * sums * (1 + np.log(cols)), "entropies")
+    near(got["given"], np.full(2, -np.log(cols)), sums + 4 * EPSILON_32 * np.log(cols), "log probabilities")
+    assert np.array_equal(got["tokens"], [[0, 1, 2]] * 2)
