@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(kThreads)
             for (int e = 0; e < E; e++) {
                 const float log_p = v[e] - normalizer;
                 const float p = power(log_p);
-                v[e] = ENTROPY ? p * fmaf(slope, fmaxf(log_p, -1e30f), base) : p * base;
+                v[e] = ENTROPY ? p * fmaf(slope, fmaxf(log_p, kVanished), base) : p * base;
             }
             const int64_t place = static_cast<int64_t>(token) - column;
             if (g != 0.0f && place >= 0 && place < E) {

@@ -229,3 +229,24 @@ def test_rows_of_nothing_but_a_masks_number(kind, mask, cols):
     near(got["entropies"], np.full(2, np.log(cols)), 2 * sums * (1 + np.log(cols)), "entropies")
     near(got["given"], np.full(2, -np.log(cols)), sums + 4 * EPSILON_32 * np.log(cols), "log probabilities")
     assert np.array_equal(got["tokens"], [[0, 1, 2]] * 2)
+
+
+@pytest.mark.parametrize("kind, mask", [*FINITE_MASKS, (lib.F32, -np.inf), (lib.BF16, -np.inf)])
+@pytest.mark.parametrize("slope", [1.0, 1e9])
+def test_backward_of_masked_logits(kind, mask, slope):
+    # An impossible token's gradient is 0, however large the entropy's is.
+    if kind == lib.F16 and slope > 1:
+        pytest.skip("the results themselves are past f16")
+    rows, cols = 3, 9001
+    x, tokens = inputs(kind, rows, cols, seed=12)
+    masked = np.arange(cols) % 9 < 3
+    here, removed = np.where(masked, stored(mask, kind), x), np.where(masked, -np.inf, x)
+    tokens[:] = [3, NONE, 8]
+    got = run(kind, here, tokens, 0)
+    _, normalizers, entropies, _, _ = language.log_probabilities(removed, tokens, 0)
+    normalizers, entropies = (v.astype(np.float32).astype(np.float64) for v in (normalizers, entropies))
+    h = np.array([-slope, slope, slope])
+    have = backward(kind, here, tokens, normalizers, entropies, np.ones(rows), h)
+    check_backward(kind, removed, tokens, normalizers, entropies, np.ones(rows), h, have)
+    assert not have[:, masked].any()
+    assert np.isfinite(backward(kind, here, tokens, got["normalizers"], got["entropies"], np.ones(rows), h)).all()
