@@ -26,9 +26,8 @@
 // element for f32.  p and ds are rounded to the operands' type for it, once;
 // sums, maxima and all else are f32.  The least normal f16 is 2^-14, which p
 // of a long sequence and ds fall below: in f16 p is rounded times 2^14 (or 2^6
-// forward, where it may reach 2^8), and ds, which is at most twice the largest
-// |do| times the largest |v|, times the power of two that brings that below
-// 2^15.
+// forward, where it may reach 2^8), and ds, which is at most 2 |do| |v|, times
+// the power of two that brings the largest of that in its own sum below 2^15.
 //
 // Measured (a large bf16 product reaches 1372 TFLOP/s): 8192 tokens, 16 heads
 // of 128 on 4 key heads, bf16: forward 305 us (900 TFLOP/s, the matrix cores
@@ -717,19 +716,20 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
 
 // ---- backward ----------------------------------------------------------------------------
 
-// sums[head][token] = do . o, 16 lanes a row of a head; and in f16 each block's
-// largest finite |do|^2 and |v|^2 of a row, a pair behind the first of `largest`.
+// sums[head][token] = do . o, 16 lanes a row of a head; and in f16 behind them
+// |do|^2, as much room for the largest of it from each token on
+// (`queries_kernel`), and |v|^2, [key head][token]; 0 where a square is no
+// finite number.
 // Bound by memory; 7001 f16 tokens of 12 heads of 80, 40 MB, 10.7 us (12.6 with
 // do read for each of its two sums and places divided in 64 bits).
 __global__ void __launch_bounds__(kThreads)
     dots_kernel(const Shape shape, const S* __restrict__ d_out, const S* __restrict__ out, const S* __restrict__ v,
-                float* __restrict__ sums, float* __restrict__ largest) {
+                float* __restrict__ sums) {
     const uint64_t first = uint64_t{blockIdx.x} * (kThreads / 16) + threadIdx.x / 16;
     const uint64_t apart = uint64_t{gridDim.x} * (kThreads / 16);
-    float most[2] = {};
-    const auto note = [&](int which, float square) {
-        if (square < INFINITY) most[which] = fmaxf(most[which], square);
-    };
+    const uint64_t rows = uint64_t{shape.tokens} * shape.heads;
+    const bool writes = threadIdx.x % 16 == 0;
+    const auto finite = [](float square) { return square < INFINITY ? square : 0.0f; };
     // A row's place: 64 bits only divide where rows are that many.
     const auto place = [&](uint64_t row, uint32_t heads, Steps steps, uint32_t* token, uint32_t* head) {
         if (row >> 32 == 0) {
@@ -740,7 +740,7 @@ __global__ void __launch_bounds__(kThreads)
         return *token * steps.token + *head * steps.head;
     };
     uint32_t token, head;
-    for (uint64_t row = first; row < uint64_t{shape.tokens} * shape.heads; row += apart) {
+    for (uint64_t row = first; row < rows; row += apart) {
         const uint64_t at = place(row, shape.heads, shape.out, &token, &head);
         float sum = 0.0f, square = 0.0f;
         for (uint32_t word = threadIdx.x % 16; word * E < shape.size; word += 16) {
@@ -752,8 +752,12 @@ __global__ void __launch_bounds__(kThreads)
             }
         }
         sum = row16<Added>(sum);
-        if (threadIdx.x % 16 == 0) sums[uint64_t{head} * shape.tokens + token] = sum;
-        if constexpr (kHalf) note(0, row16<Added>(square));
+        const uint64_t to = uint64_t{head} * shape.tokens + token;
+        if (writes) sums[to] = sum;
+        if constexpr (kHalf) {
+            square = row16<Added>(square);
+            if (writes) sums[rows + to] = finite(square);
+        }
     }
     if constexpr (kHalf) {
         const uint32_t heads = shape.heads / shape.group;
@@ -765,33 +769,55 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
                 for (int e = 0; e < E; e++) square = fmaf(x.at(e), x.at(e), square);
             }
-            note(1, row16<Added>(square));
-        }
-        __shared__ float shared[2][kMostWaves];
-        for (int which = 0; which < 2; which++) {
-            const float all = block_join<Largest>(most[which], shared[which]);
-            if (threadIdx.x == 0) largest[2 + 2 * blockIdx.x + which] = all;
+            square = row16<Added>(square);
+            if (writes) sums[3 * rows + uint64_t{head} * shape.tokens + token] = finite(square);
         }
     }
 }
 
-// The largest of the blocks' pairs behind the first two, into those.
-__global__ void __launch_bounds__(kThreads) largest_kernel(float* largest, uint32_t blocks) {
-    __shared__ float shared[2][kMostWaves];
-    float most[2] = {};
-    for (uint32_t n = threadIdx.x; n < blocks; n += kThreads) {
-        for (int which = 0; which < 2; which++) most[which] = fmaxf(most[which], largest[2 + 2 * n + which]);
+// The largest of `values`, by token: among the tokens of a sequence up to each
+// lane's own, or with BEHIND from it on.  The block has the 32 tokens of each
+// wave from `first` on, and one sequence at most reaches past them there.
+template <bool BEHIND>
+__device__ __forceinline__ float most_of_sum(const Shape& shape, const float* __restrict__ values, uint32_t first,
+                                             uint32_t token, const Span& span, float (*scratch)[8 * 32]) {
+    const uint32_t wave = threadIdx.x / 64, column = threadIdx.x % 32;
+    __shared__ uint32_t edge;
+    if (threadIdx.x == (BEHIND ? kThreads - 1 : 0)) edge = BEHIND ? span.end : span.first;
+    __syncthreads();
+    const uint32_t from = BEHIND ? first + kOwned : edge, to = BEHIND ? edge : first;
+    float past = 0.0f;
+    if (from < to) {
+#pragma unroll 8
+        for (uint32_t i = from + threadIdx.x; i < to; i += kThreads) past = fmaxf(past, values[i]);
     }
-    for (int which = 0; which < 2; which++) {
-        const float all = block_join<Largest>(most[which], shared[which]);
-        if (threadIdx.x == 0) largest[which] = all;
+    past = wave64<Largest>(past);
+    float most = token < shape.tokens ? values[token] : 0.0f;
+    for (uint32_t offset = 1; offset < 32; offset *= 2) {
+        const float other = BEHIND ? __shfl_down(most, offset, 32) : __shfl_up(most, offset, 32);
+        const bool seen = BEHIND ? column + offset < 32 && token + offset < span.end
+                                 : column >= offset && token - offset >= span.first;
+        if (seen) most = fmaxf(most, other);
     }
+    float(&held)[8 * 32] = scratch[wave];
+    if (threadIdx.x % 64 < 32) held[column] = most;
+    if (threadIdx.x % 64 == 0) held[32] = past;
+    __syncthreads();
+    for (uint32_t w = 0; w < kThreads / 64; w++) {
+        past = fmaxf(past, scratch[w][32]);
+        if (BEHIND ? w > wave && first + w * 32 < span.end : w < wave && first + w * 32 + 31 >= span.first) {
+            most = fmaxf(most, scratch[w][BEHIND ? 0 : 31]);
+        }
+    }
+    __syncthreads();  // `scratch` is free
+    return (BEHIND ? span.end > first + kOwned : span.first < first) ? fmaxf(most, past) : most;
 }
 
-// The power of two that ds is rounded times.
-__device__ __forceinline__ float ds_factor(const float* largest) {
-    if constexpr (!kHalf) return 1.0f;
-    const float bound = sqrtf(largest[0]) * sqrtf(largest[1]);
+// The power of two that ds of a sum are rounded times in f16, from the largest
+// |do|^2 and |v|^2 among them: those of rows that are no part of the sum would
+// take its bits.
+__device__ __forceinline__ float ds_factor(float d_square, float v_square) {
+    const float bound = sqrtf(d_square) * sqrtf(v_square);
     return bound == 0.0f ? 1.0f : ldexpf(1.0f, 13 - ilogbf(bound));
 }
 
@@ -800,7 +826,7 @@ template <int SIZE, bool DIRECT>
 __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
     queries_kernel(const Shape shape, const S* __restrict__ d_out, const S* __restrict__ q, const S* __restrict__ k,
                    const S* __restrict__ v, const float* __restrict__ normalizers, float* __restrict__ dots,
-                   const float* __restrict__ largest, S* __restrict__ dq) {
+                   S* __restrict__ dq) {
     using KeyTile = Tile<SIZE, kSwept>;
     // A stage an array, so that reads of one do not wait for loads to the other.
     __shared__ __attribute__((aligned(1024))) char stage_0[2 * KeyTile::kBytes], stage_1[2 * KeyTile::kBytes];
@@ -833,11 +859,21 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
         d_rows[n] = head_word(d_row, 2 * n + half, shape.size);
     }
     const float normalizer = normalizers[uint64_t{head} * shape.tokens + inside] * kLog2e;
-    const float factor = ds_factor(largest);
-    float dot = dots[uint64_t{head} * shape.tokens + inside] * factor;
+    float dot = dots[uint64_t{head} * shape.tokens + inside];
     __syncthreads();
     uint32_t begin, block_all;
     over_waves(seen, &begin, &block_all);
+    float factor = 1.0f;
+    if constexpr (kHalf) {
+        const uint64_t rows = uint64_t{shape.tokens} * shape.heads;
+        const float* d_squares = dots + rows + uint64_t{head} * shape.tokens;
+        const float* v_squares = dots + 3 * rows + uint64_t{head / shape.group} * shape.tokens;
+        factor = ds_factor(d_squares[inside], most_of_sum<false>(shape, v_squares, first, token, span, scratch));
+        dot *= factor;
+        // For the kernel of dk and dv, which runs next.
+        const float later = most_of_sum<true>(shape, d_squares, first, token, span, scratch);
+        if (half == 0 && token < mine.end) dots[2 * rows + uint64_t{head} * shape.tokens + token] = later;
+    }
 
     const S* keys = k + head / shape.group * shape.k.head;
     const S* values = v + head / shape.group * shape.v.head;
@@ -983,8 +1019,7 @@ template <int SIZE, bool DIRECT>
 __global__ void __launch_bounds__(key_threads(SIZE)) __attribute__((amdgpu_waves_per_eu(kWide && SIZE > 96 ? 1 : 2)))
     keys_kernel(const Shape shape, uint32_t splits, const S* __restrict__ d_out, const S* __restrict__ q,
                 const S* __restrict__ k, const S* __restrict__ v, const float* __restrict__ normalizers,
-                const float* __restrict__ dots, const float* __restrict__ largest, S* __restrict__ dk, S* __restrict__ dv,
-                float* __restrict__ parts) {
+                const float* __restrict__ dots, S* __restrict__ dk, S* __restrict__ dv, float* __restrict__ parts) {
     constexpr bool kValuesInLds = SIZE > 96;
     constexpr int kWaves = key_threads(SIZE) / 64;
     constexpr uint32_t kKeys = 32 * kWaves;
@@ -1039,7 +1074,16 @@ __global__ void __launch_bounds__(key_threads(SIZE)) __attribute__((amdgpu_waves
 
     const float c = shape.scale * kLog2e;
     // p is rounded times 2^kBackPower, ds times `factor`.
-    const float factor = ds_factor(largest), ds_scale = factor * power2(-kBackPower);
+    float factor = 1.0f;
+    if constexpr (kHalf) {
+        const uint64_t rows = uint64_t{shape.tokens} * shape.heads;
+        float d_square = 0.0f;
+        for (uint32_t h = first_head; h < first_head + share_heads; h++) {
+            d_square = fmaxf(d_square, dots[2 * rows + uint64_t{h} * shape.tokens + inside]);
+        }
+        factor = ds_factor(d_square, dots[3 * rows + uint64_t{key_head} * shape.tokens + inside]);
+    }
+    const float ds_scale = factor * power2(-kBackPower);
     f32x16 acc_k[SIZE / 32] = {}, acc_v[SIZE / 32] = {};
     // One sweep over the queries, as over the keys in the kernels above.
     const auto sweep = [&](auto is_slow) {
@@ -1069,7 +1113,7 @@ __global__ void __launch_bounds__(key_threads(SIZE)) __attribute__((amdgpu_waves
             query_stager.land(QueryTile{stage});
             d_stager.land(QueryTile{stage + QueryTile::kBytes});
             if (threadIdx.x < 2 * kSwept) {
-                row_value = threadIdx.x < kSwept ? fmaf(row_value, kLog2e, -kBackPower) : row_value * ds_scale;
+                if (threadIdx.x < kSwept) row_value = fmaf(row_value, kLog2e, -kBackPower);
                 values_here[threadIdx.x / kSwept][threadIdx.x % kSwept] = row_value;
             }
             uint32_t& mark = marks[stage == stage_1];
@@ -1110,7 +1154,8 @@ __global__ void __launch_bounds__(key_threads(SIZE)) __attribute__((amdgpu_waves
                     for (int j = 0; j < 4; j++) {
                         const int i = 4 * g + j;
                         s[i] = power2(fmaf(s[i], c, -l[j]));
-                        d[i] = s[i] * fmaf(d[i], ds_scale, -o[j]);
+                        d[i] = s[i] * (d[i] - o[j]);
+                        if constexpr (kHalf) d[i] *= ds_scale;
                         if constexpr (!WHOLE) {
                             const uint32_t query = at + b * 32 + row_of(i, half);
                             if (query < token || query >= span.end) s[i] = 0.0f, d[i] = 0.0f;
@@ -1246,36 +1291,30 @@ int backward(const Shape& shape, const void* d_out, const void* q, const void* k
         }
     }
     const uint64_t rows = uint64_t{shape.tokens} * shape.heads;
-    const uint32_t dot_blocks = grid_for(rows, kThreads / 16, 8);
-    Scratch dots((rows + 2 + 2 * dot_blocks) * sizeof(float));
+    Scratch dots((kHalf ? 3 * rows + uint64_t{shape.tokens} * key_heads : rows) * sizeof(float));
     Scratch parts(splits > 1 ? uint64_t{key_heads} * splits * 2 * shape.tokens * shape.size * sizeof(float) : 0);
     if (dots.status != TC_OK) return dots.status;
     if (parts.status != TC_OK) return parts.status;
     float* sums = static_cast<float*>(dots.ptr);
-    float* largest = sums + rows;
     const S* d = static_cast<const S*>(d_out);
     const S* queries = static_cast<const S*>(q);
     const S* keys = static_cast<const S*>(k);
     const S* values = static_cast<const S*>(v);
-    dots_kernel<<<dot_blocks, kThreads, 0, s>>>(shape, d, static_cast<const S*>(out), values, sums, largest);
+    dots_kernel<<<grid_for(rows, kThreads / 16, 8), kThreads, 0, s>>>(shape, d, static_cast<const S*>(out), values,
+                                                                      sums);
     int status = check_launch(what);
     if (status != TC_OK) return status;
-    if constexpr (kHalf) {
-        largest_kernel<<<1, kThreads, 0, s>>>(largest, dot_blocks);
-        status = check_launch(what);
-        if (status != TC_OK) return status;
-    }
     const bool keys_straight = direct(shape.size, {{k, shape.k}, {v, shape.v}});
     TC_ATTENTION_FORM(shape.size, keys_straight,
                       queries_kernel<SIZE, DIRECT><<<tiles * shape.heads, kThreads, 0, s>>>(
-                          shape, d, queries, keys, values, normalizers, sums, largest, static_cast<S*>(dq)))
+                          shape, d, queries, keys, values, normalizers, sums, static_cast<S*>(dq)))
     status = check_launch(what);
     if (status != TC_OK) return status;
     const bool rows_straight = direct(shape.size, {{q, shape.q}, {d_out, shape.out}});
     TC_ATTENTION_FORM(shape.size, rows_straight,
                       const uint32_t key_tiles = tiles_of(shape, key_threads(SIZE) / 2);
                       keys_kernel<SIZE, DIRECT><<<key_tiles * key_heads * splits, key_threads(SIZE), 0, s>>>(
-                          shape, splits, d, queries, keys, values, normalizers, sums, largest, static_cast<S*>(dk),
+                          shape, splits, d, queries, keys, values, normalizers, sums, static_cast<S*>(dk),
                           static_cast<S*>(dv), static_cast<float*>(parts.ptr)))
     status = check_launch(what);
     if (status != TC_OK || splits == 1) return status;

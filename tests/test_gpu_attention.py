@@ -232,3 +232,65 @@ def test_short_sequences_lose_nothing_to_the_rounding_of_the_result(kind, heads,
     for name, have, want in zip(("dq", "dk", "dv"), got[2:], grads):
         off = np.linalg.norm(have - want) / np.linalg.norm(want)
         assert off < 0.75 * ROUNDING[kind], (name, off / ROUNDING[kind])
+
+
+LARGEST = {lib.F32: float(np.finfo(np.float32).max), lib.F16: 65504.0, lib.BF16: 3.3895313892515355e38}
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=KIND_NAMES.get)
+@pytest.mark.parametrize("size", [64, 100])
+@pytest.mark.parametrize("heads, empty", [(4, 0), (16, 40)])
+def test_numbers_that_are_not_seen_do_not_matter(kind, size, heads, empty):
+    # The largest numbers in tokens of no sequence, and 2^13 times the usual
+    # ones in another sequence, change no bit of what does not see them.
+    ends = [2, 40, 90, 100, 230] + [300] * (1 + empty)
+    operands = inputs(kind, 310, heads, 2, size, 13)
+    scale = float(np.float32(size ** -0.5))
+    want = run(kind, *operands, ends, scale)
+    for sign in (1.0, -1.0):
+        for t in operands:
+            t[:2] = t[300:] = sign * LARGEST[kind]
+        got = run(kind, *operands, ends, scale)
+        for n, (have, kept) in enumerate(zip(got, want)):
+            assert np.array_equal(have, kept), n
+    for t in operands[2:]:  # values and the results' gradients
+        t[100:230] *= 2.0**13
+    got = run(kind, *operands, ends, scale)
+    other = np.ones(310, bool)
+    other[100:230] = False
+    for n, (have, kept) in enumerate(zip(got, want)):
+        if n == 1:
+            have, kept = have.T, kept.T
+        assert np.array_equal(have[other], kept[other]), n
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=KIND_NAMES.get)
+@pytest.mark.parametrize("heads", [2, 16])
+def test_gradients_depend_on_what_they_sum_over_alone(kind, heads):
+    # A query's gradient on the keys up to it, a key's on the queries from it on.
+    tokens, at, size = 400, 150, 64
+    q, k, v, d = inputs(kind, tokens, heads, 2, size, 17)
+    want = run(kind, q, k, v, d, None, 0.125)
+    for t in (k, v):
+        t[at + 1:] *= 2.0**10
+    got = run(kind, q, k, v, d, None, 0.125)
+    assert np.array_equal(got[2][:at + 1], want[2][:at + 1])
+    q, k, v, d = inputs(kind, tokens, heads, 2, size, 17)
+    d[:at] *= 2.0**13
+    got = run(kind, q, k, v, d, None, 0.125)
+    for n in (3, 4):
+        assert np.array_equal(got[n][at:], want[n][at:])
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=KIND_NAMES.get)
+@pytest.mark.parametrize("heads", [2, 16])
+@pytest.mark.parametrize("where", ["first", "last", "rising", "falling"])
+def test_gradients_of_rows_of_very_different_magnitudes(kind, heads, where):
+    tokens, size = 300, 64
+    q, k, v, d = inputs(kind, tokens, heads, 2, size, 19)
+    at = np.arange(tokens)
+    power = {"first": np.where(at == 0, 11, -8), "last": np.where(at == tokens - 1, 11, -8), "rising": at // 16 - 8,
+             "falling": 10 - at // 16}[where]
+    d *= 2.0 ** power.astype(float)[:, None, None]
+    for ends in (None, [0, 150, 300]):
+        check(kind, q, k, v, d, ends, 0.125, run(kind, q, k, v, d, ends, 0.125))
