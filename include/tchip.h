@@ -746,7 +746,9 @@ typedef struct tc_attention_shape {
  * exponentials (-infinity for a token in no sequence), for the backward pass.
  * Sums and softmax are f32; the softmax's weights are rounded to `dtype` for
  * their product with the values.  What a query does not attend to never
- * reaches its result, not as an infinity or a NaN either. */
+ * reaches its result, not as an infinity or a NaN either.  A query in a
+ * sequence all of whose scores are -infinity has the normalizer -infinity and,
+ * as 0 / 0, a NaN result. */
 int tc_attention(const tc_attention_shape* shape, const void* query, const void* key, const void* value, void* out,
                  float* normalizers);
 

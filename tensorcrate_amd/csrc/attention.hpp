@@ -706,8 +706,9 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
     }
     total = halves_sum(total);
     if (token >= mine.end) return;
-    store_column<S, SIZE>(out + token * shape.out.token + head * shape.out.head, acc, total == 0.0f ? 0.0f : 1.0f / total,
-                          shape.size, half);
+    // (A total of 0 within a sequence is of scores of -infinity alone: 0 / 0.)
+    store_column<S, SIZE>(out + token * shape.out.token + head * shape.out.head, acc,
+                          span.first == kNone ? 0.0f : 1.0f / total, shape.size, half);
     if (normalizers != nullptr && half == 0) {
         normalizers[uint64_t{head} * shape.tokens + token] =
             total == 0.0f ? -INFINITY : (most + log2f(total) - kForwardPower) * kLn2;

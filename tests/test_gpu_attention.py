@@ -294,3 +294,19 @@ def test_gradients_of_rows_of_very_different_magnitudes(kind, heads, where):
     d *= 2.0 ** power.astype(float)[:, None, None]
     for ends in (None, [0, 150, 300]):
         check(kind, q, k, v, d, ends, 0.125, run(kind, q, k, v, d, ends, 0.125))
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=KIND_NAMES.get)
+@pytest.mark.parametrize("heads", [1, 8])
+def test_a_query_whose_scores_are_all_minus_infinity(kind, heads):
+    # 0 / 0 of the definition, not the zeros of a token in no sequence; and a
+    # key of that score beside others has the weight 0.
+    q, k, v, d = inputs(kind, 200, heads, 1, 64, 21)
+    q[:] = np.abs(q) + 0.5
+    k[50] = -np.inf
+    for ends in ([10, 50, 190], [10, 50] + [190] * 120):
+        got = run(kind, q, k, v, d, ends, 0.125)
+        assert np.isnan(got[0][50]).all() and np.isneginf(got[1][:, 50]).all()
+        assert np.isfinite(got[0][:50]).all() and np.isfinite(got[0][51:]).all()
+        assert not got[0][:10].any() and not got[0][190:].any()
+        assert np.isfinite(got[1][:, 51:190]).all() and np.isneginf(got[1][:, 190:]).all()
