@@ -70,13 +70,22 @@ __device__ __forceinline__ double block_sum(double v, double* shared) {
 template <typename S>
 __device__ __forceinline__ double squares(const Entry& entry, uint64_t first) {
     constexpr int E = kWordElements<S>;
-    const Row<S> row(static_cast<const S*>(entry.from), entry.length);
-    const uint64_t words = row.words();
+    // Words from the tensor's start on, wherever it is, so that its address
+    // has no part in which squares are added first.
+    const S* from = static_cast<const S*>(entry.from);
+    const uint64_t length = entry.length, words = (length + E - 1) / E;
     Words<S, E> in[kInFlight];
 #pragma unroll
     for (int u = 0; u < kInFlight; u++) {
-        const uint64_t word = first + u * kThreads + threadIdx.x;
-        if (word < words) row.template load<false>(word, in[u], 0.0f);
+        const uint64_t word = first + u * kThreads + threadIdx.x, at = word * E;
+        if (at + E <= length) {
+            in[u].template load<false>(from + at);
+        } else if (word < words) {
+            float v[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] = at + e < length ? Elem<S>::widen(from[at + e]) : 0.0f;
+            in[u].put(v);
+        }
     }
     double sum = 0.0;
 #pragma unroll

@@ -108,3 +108,17 @@ def test_the_same_bits_again():
     tensors = tensors_of([3000001, 77, 1000000], [lib.F32, lib.BF16, lib.F16], seed=3)
     (first, norm), (again, norm_again) = (run(tensors, 1.0) for _ in range(2))
     assert norm == norm_again and all(np.array_equal(a, b) for a, b in zip(first, again))
+
+
+def test_the_norm_does_not_depend_on_where_a_tensor_starts():
+    # 64 runs of one 2^-3 and seven 2^-30 behind it, whose squares vanish one
+    # by one beside the first and together would be two units of the sum's last
+    # place, and 2^-23 + 2^-48 more: all but those seven come to the square of
+    # a number halfway between two of 32 bits, so that every unit of the sum's
+    # last place shows in the norm's.
+    values = np.full((64, 8), 2.0**-30)
+    values[:, 0] = 2.0**-3
+    values = np.concatenate([values.reshape(-1), [2.0**-12, 2.0**-12, 2.0**-24]])
+    for kind in (lib.BF16, lib.F32):
+        norms = {run([(kind, stored(values, kind))], 1e9, shifts=[shift])[1] for shift in range(9)}
+        assert len(norms) == 1, (KIND_NAMES[kind], norms)
