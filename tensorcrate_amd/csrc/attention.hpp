@@ -344,7 +344,7 @@ __device__ __forceinline__ Span span_of(const Shape& shape, uint32_t token) {
     if (shape.sequences == 0) return {0, shape.tokens};
     uint32_t low = 0, high = shape.sequences;
     while (high - low > 1) {
-        const uint32_t middle = (low + high) / 2;
+        const uint32_t middle = low + (high - low) / 2;  // their sum may pass 32 bits
         if (shape.offsets[middle] <= token) low = middle;
         else high = middle;
     }

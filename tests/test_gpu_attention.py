@@ -310,3 +310,25 @@ def test_a_query_whose_scores_are_all_minus_infinity(kind, heads):
         assert np.isfinite(got[0][:50]).all() and np.isfinite(got[0][51:]).all()
         assert not got[0][:10].any() and not got[0][190:].any()
         assert np.isfinite(got[1][:, 51:190]).all() and np.isneginf(got[1][:, 190:]).all()
+
+
+def test_more_than_2_31_sequences():
+    # All but the last few of them empty.
+    count, ends = 2**31 + 1000, [0, 30, 30, 101, 190]
+    q, k, v, d = inputs(lib.F32, 200, 1, 1, 16, 23)
+    want = run(lib.F32, q, k, v, d, ends, 0.25)
+    zero, last = np.zeros(1, np.uint32), np.array(ends, np.uint32)
+    offsets = lib.Buffer(4 * (count + 1))
+    lib.call("tc_fill", offsets.ptr, count + 1, 4, zero.ctypes.data)
+    lib.call("tc_upload", offsets.ptr + 4 * (count + 1 - last.size), last.ctypes.data, last.nbytes)
+    parts = [Heads([t], lib.F32) for t in (q, k, v, d)]
+    out, *grads = [Heads.like(p) for p in (parts[3], *parts[:3])]
+    at = [p.ptr() for p in parts]
+    shape = lib.attention(lib.F32, 200, 1, 1, 16, 0.25, offsets.ptr, count, *[p.steps for p in parts])
+    normalizers = lib.Buffer(4 * 200)
+    lib.call("tc_attention", shape, *at[:3], out.ptr(), normalizers.ptr)
+    lib.call("tc_attention_backward", shape, at[3], *at[:3], out.ptr(), normalizers.ptr, *[g.ptr() for g in grads])
+    have = [out.read()[0], normalizers.download(np.float32, 200)[None].astype(np.float64)] + [g.read()[0] for g in grads]
+    ends = [0, 30, 101, 190]
+    check(lib.F32, q, k, v, d, ends, 0.25, have)
+    check(lib.F32, q, k, v, d, ends, 0.25, want)
