@@ -756,7 +756,9 @@ int tc_attention(const tc_attention_shape* shape, const void* query, const void*
  * (laid out as `out`) and the forward pass's operands, `out` and
  * `normalizers`.  Gradients of shared key heads are summed over their query
  * heads in f32; every sum is taken in an order that depends on the shape and
- * the offsets alone. */
+ * the offsets alone.  For their products the softmax's weights and the scores'
+ * gradients are rounded to `dtype`: in f16 times powers of two, the latter's
+ * from the largest rows of `d_out` and of the values in the same sum. */
 int tc_attention_backward(const tc_attention_shape* shape, const void* d_out, const void* query, const void* key,
                           const void* value, const void* out, const float* normalizers, void* d_query, void* d_key,
                           void* d_value);

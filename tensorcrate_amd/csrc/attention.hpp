@@ -30,15 +30,22 @@
 // the power of two that brings the largest of that in its own sum below 2^15.
 //
 // Measured (a large bf16 product reaches 1372 TFLOP/s): 8192 tokens, 16 heads
-// of 128 on 4 key heads, bf16: forward 305 us (900 TFLOP/s, the matrix cores
-// busy 54% of the time), dq 392 (1050, 60%), dk and dv 609 (900, 47%; both with
-// the two products that the other computes too); 16384 tokens, 8 heads of 64 on
-// one, forward 315 us (870); 7001 f16 tokens of 19 sequences, 12 heads of 80,
-// forward and backward 155 us, the longest sequence's 18 tiles one after
-// another.  What carried it: loads straight to LDS (forward 397 -> 330 us), one
-// number a lane for all LDS addresses and a path without masks (330 -> 305),
-// 256 keys a block for dk and dv (816 -> 675), blocks by sequence (7001 tokens,
-// 237 -> 154).
+// of 128 on 4 key heads, bf16, 1252 us in all, of which forward 306 (900
+// TFLOP/s, the matrix cores busy 54% of the time), dq 395 (1040, 60%), dk and dv
+// 616 (890, 47%; both with the two products that the other computes too); 16384
+// tokens, 8 heads of 64 on one, forward 323 us (850); 7001 f16 tokens of 19
+// sequences, 12 heads of 80, forward and backward 154 us, in which the matrix
+// cores are busy 19 to 23% of the time and waves wait for 42 to 46% of theirs:
+// a tile's loads are issued one tile before all of them are waited for.  What
+// carried it: loads straight to LDS (forward 397 -> 330 us), one number a lane
+// for all LDS addresses and a path without masks (330 -> 305), 256 keys a block
+// for dk and dv (816 -> 675 then), blocks by sequence (7001 tokens, 237 -> 154).
+//   Rows that are no whole 16-byte words go through registers to LDS, several
+// times slower: those 8192 tokens with heads of 127 4280 us, the 16384 with
+// heads of 63 1464.  f32, 4096 tokens, 8 heads on 2: of 64 1251 us forward and
+// backward (48 TFLOP/s of the 143 of a large product), of 128 2555; the
+// gradients' kernels of f32 heads past 64 keep up to 22 registers a tile in
+// memory.
 //
 // Sequences lie one behind another.  A tile that some row of a wave sees only
 // in part is masked element by element.  A masked weight is 0, and 0 times an
@@ -721,7 +728,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
 // |do|^2, as much room for the largest of it from each token on
 // (`queries_kernel`), and |v|^2, [key head][token]; 0 where a square is no
 // finite number.
-// Bound by memory; 7001 f16 tokens of 12 heads of 80, 40 MB, 10.7 us (12.6 with
+// Bound by memory; 7001 f16 tokens of 12 heads of 80, 40 MB, 10.2 us (12.6 with
 // do read for each of its two sums and places divided in 64 bits).
 __global__ void __launch_bounds__(kThreads)
     dots_kernel(const Shape shape, const S* __restrict__ d_out, const S* __restrict__ out, const S* __restrict__ v,
@@ -816,7 +823,9 @@ __device__ __forceinline__ float most_of_sum(const Shape& shape, const float* __
 
 // The power of two that ds of a sum are rounded times in f16, from the largest
 // |do|^2 and |v|^2 among them: those of rows that are no part of the sum would
-// take its bits.
+// take its bits.  7001 tokens, 12 heads of 80: 154 us, as with one power for all
+// sums from a kernel of its own; 165 where the power followed each tile's ds
+// (and 1773 against 1348 for 8192 tokens, 16 heads of 128, out of registers).
 __device__ __forceinline__ float ds_factor(float d_square, float v_square) {
     const float bound = sqrtf(d_square) * sqrtf(v_square);
     return bound == 0.0f ? 1.0f : ldexpf(1.0f, 13 - ilogbf(bound));
@@ -1013,7 +1022,8 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2
 // where LDS leaves room for one block.  In the largest 16-bit heads it holds the
 // values, so that registers let two waves share a matrix core: 8192 bf16 tokens,
 // 16 heads of 128, 816 us with the values in registers and one wave, 776 with
-// blocks of 128 keys and tiles of 32 queries, 675 so.
+// blocks of 128 keys and tiles of 32 queries, 675 so, all three timed as it was
+// chosen (616 now).
 constexpr int key_threads(int size) { return !kWide && size > 96 ? 512 : kThreads; }
 
 template <int SIZE, bool DIRECT>
@@ -1168,8 +1178,8 @@ __global__ void __launch_bounds__(key_threads(SIZE)) __attribute__((amdgpu_waves
                 __builtin_amdgcn_sched_barrier(0);
                 add_weighted<SIZE, kSwept, SLOW && !WHOLE>(special, acc_k, query_tile, b * 32, d, lanes, lane, scratch[wave]);
             };
-            // Whole tiles in one piece without a branch, so that one half's
-            // exponentials may run beside the other's products.
+            // 32 rows at a time, whole or masked: the scores and do . v of 64
+            // would take 32 registers more.
             if (at >= wave_first + 31 && at + kSwept <= all) {
 #pragma unroll 1
                 for (int b = 0; b < static_cast<int>(kSwept) / 32; b++) rows_of_32(b, std::true_type());

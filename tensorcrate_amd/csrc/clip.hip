@@ -9,8 +9,9 @@
 // read and written once each: 61 us with plain stores, 53 so).
 //
 // Measured: those gradients now 51 us, 19 for the norm (5.2 TB/s) and 31 to
-// scale (6.4); 300 tensors of 300 M elements, 1.83 GB moved, 335 us, 5.5 TB/s.
-// Eight words a lane at a time instead of four took 403.
+// scale (6.4); 300 tensors of 300 M elements, 1.83 GB moved, 339 us, 5.4 TB/s
+// (336 where the norm read words of memory whose lanes hold other elements for
+// every alignment).  Eight words a lane at a time instead of four took 403.
 //
 // The tensors' pointers and lengths travel in the kernels' arguments, up to
 // kTable of them a launch, so that no table is uploaded; blocks take chunks

@@ -13,9 +13,13 @@
 // with the next row's words already in flight, and keeps its columns' weights.
 //
 // Measured (a large copy moves 6.5 TB/s): 16384 bf16 rows of 4096 forward
-// 50 us, 5.4 TB/s; 10007 f16 rows of 2050, views that start at any element,
-// backward 40 us, 3.1 TB/s, of which 4 to 5 are the launch that adds dw and db and about 8
-// the blocks' first and last rows; 64 f32 rows of 1024 the 4.5 us of a launch.
+// 47 us, 5.7 TB/s, and backward 89, 4.5 TB/s; 10007 f16 rows of 2050, views that
+// start at any element, with an f32 weight, backward 40 us, 3.1 TB/s: 33.5 at
+// 2048 columns (3.7), 4 more for the fifth word of a lane that two columns more
+// take, 3 for the odd starts.  4 to 5 of each are the launch that adds dw and
+// db.  With an f16 weight those rows take 55 us, since that form keeps some 25
+// of a lane's words in memory.  8192 f32 rows of 4096 backward 79 us, 5.1 TB/s;
+// 64 of 1024 forward the 4 us of a launch.
 // One word a lane instead of two and grids that fill the chip without walking
 // rows took 68 and 52 us forward; one row a block backward 47.
 //
@@ -150,7 +154,8 @@ __global__ void __launch_bounds__(LANES ? 256 : kMostLanes)
 
 // Rows longer than a block's registers: a block a row, which it reads three
 // times (from the caches, mostly).  Elements are read and written one by one
-// at a row's ragged end, so that y may be x.
+// at a row's ragged end, so that y may be x.  2000 bf16 rows of 40000: 225 us,
+// 1.4 TB/s, and 418 backward, 1.1 TB/s.
 template <typename S, typename W>
 __global__ void __launch_bounds__(kMostLanes)
     norm_long_kernel(const S* x, uint64_t x_step, uint64_t rows, uint64_t cols, const W* weight, const W* bias,
@@ -500,7 +505,11 @@ struct Layout {
 
 // Rows of up to 64 x `wave` words take a wave, several rows to a block of
 // `block` threads; longer ones a block of at most `most` threads, two words a
-// lane at least and `held` elements at most.
+// lane at least and `held` elements at most.  With `wave` 5, past 256 words, as
+// waves and as blocks: 10007 f16 rows of 2050 forward 17.2 and 22.6 us, of 2560
+// (320 words) 21.8 and 24.5, 16384 f32 rows of 1025 26.6 and 34.9; backward with
+// an f32 weight 40.5 and 48.7, 42.3 and 49.0, 45.7 and 52.1, but with an f16 one,
+// whose waves keep words in memory, 55 and 50, 69 and 49.
 Layout layout_of(uint64_t cols, int run, uint32_t block, int wave, uint32_t most, int held) {
     const uint64_t words = (cols + run - 1) / run;
     Layout out;

@@ -17,12 +17,12 @@
 // Both are bound by memory, the forward pass at one read of the logits, the
 // backward pass at one read and one write; forward the exponentials come to
 // nearly as much.  Measured (a large copy moves 6.5 TB/s): 4096 bf16 rows of
-// 100000, 819 MB, 149 us, with the top 8 192 and the top 64 269; the gradient
-// of 4096 bf16 rows of 50001, odd rows, 142 us, 5.8 TB/s; 16 f32 rows of 50001
-// with the top 20, split over 25 blocks each and joined, 12.5 us.  Rows are read in words that are
-// 16-byte aligned wherever the row starts, its first and last elements one by
-// one.  A block takes a row; few rows are split over several blocks each, and
-// a second kernel joins them.
+// 100000, 819 MB, 151 us, with the top 8 192 to 197 and the top 64 270 (f16 159,
+// 206 and 274); the gradient of 4096 bf16 rows of 50001, odd rows, 142 us,
+// 5.8 TB/s; 16 f32 rows of 50001 with the top 20, split over 25 blocks each and
+// joined, 12.7 us.  Rows are read in words that are 16-byte aligned wherever the
+// row starts, its first and last elements one by one.  A block takes a row; few
+// rows are split over several blocks each, and a second kernel joins them.
 //
 // The most probable tokens are kept by a 64-bit key, the logit's bits in
 // order above the token's complement, so that equal logits go to the lowest
