@@ -763,6 +763,62 @@ int tc_attention_backward(const tc_attention_shape* shape, const void* d_out, co
                           const void* value, const void* out, const float* normalizers, void* d_query, void* d_key,
                           void* d_value);
 
+/* ---- rotary positions ------------------------------------------------------- */
+
+/* The pairs of a head's first `rotary_size` elements that are rotated: element
+ * i with element i + rotary_size / 2, or element 2 i with element 2 i + 1. */
+typedef enum tc_rotary_pairs { TC_ROTARY_HALVES = 0, TC_ROTARY_NEIGHBOURS = 1 } tc_rotary_pairs;
+
+/* `query_heads` and `key_heads` heads (either may be 0) of `head_size` (at
+ * most 128) elements of `tokens` tokens.  Element e of head h of token t is at
+ * t * token_step + h * head_step + e of its tensor, for queries, keys and the
+ * rotated ones each, so that they may be parts of one projection.
+ *   Token t is at `positions[t]` (on the device; null: at t).  Pair i turns by
+ * the position times `frequencies[i]` (rotary_size / 2 numbers on the device),
+ * an angle held in 64 bits.  `rotary_size` is even and may be 0.
+ *   With `normalize` (0 or not) every head is first divided by its root mean
+ * square and multiplied with a weight of `weight_dtype` (`dtype`, or TC_F32). */
+typedef struct tc_rotary_shape {
+    uint32_t dtype;
+    uint32_t weight_dtype;
+    uint32_t query_heads;
+    uint32_t key_heads;
+    uint32_t head_size;
+    uint32_t rotary_size;
+    uint32_t pairs;
+    uint32_t normalize;
+    float epsilon;
+    uint64_t tokens;
+    const uint32_t* positions;
+    const float* frequencies;
+    uint64_t query_token_step, query_head_step;
+    uint64_t key_token_step, key_head_step;
+    uint64_t query_out_token_step, query_out_head_step;
+    uint64_t key_out_token_step, key_out_head_step;
+} tc_rotary_shape;
+
+/* Of each head x of the queries and keys
+ *   y = x / sqrt(mean of x^2 + epsilon) * weight
+ * (or x itself without `normalize`), its pairs (a, b) turned to
+ * (a cos - b sin, b cos + a sin), in f32 and rounded to `dtype` once.  The
+ * weights, `head_size` elements for all heads of the queries and of the keys,
+ * may each be null (1), and are refused without `normalize`.  The results may
+ * take the operands' place (the same pointer with the same steps), and must
+ * not otherwise overlap them. */
+int tc_rotary_norm(const tc_rotary_shape* shape, const void* query, const void* key, const void* query_weight,
+                   const void* key_weight, void* query_out, void* key_out);
+
+/* The gradients of queries and keys (laid out as those) from the results'
+ * (laid out as those) and the operands, which are not read, and may be null,
+ * without `normalize`.  The gradients of the weights, summed over tokens and
+ * heads in f32 in an order that depends on the shape alone, may each be null
+ * and are then left out; with no tokens or no heads they are zeros.  A
+ * gradient may take the place of the result's (with the same steps) or of the
+ * operand. */
+int tc_rotary_norm_backward(const tc_rotary_shape* shape, const void* d_query_out, const void* d_key_out,
+                            const void* query, const void* key, const void* query_weight, const void* key_weight,
+                            void* d_query, void* d_key, void* d_query_weight, void* d_key_weight);
+
 #ifdef __cplusplus
 }
 #endif

@@ -50,29 +50,15 @@ int check(const std::string& what, const tc_attention_shape* given, Shape* shape
     }
     const struct {
         const char* name;
-        uint64_t token, head;
+        Steps steps;
         uint32_t heads;
-    } operands[] = {{"queries", a.query_token_step, a.query_head_step, a.query_heads},
-                    {"keys", a.key_token_step, a.key_head_step, a.key_heads},
-                    {"values", a.value_token_step, a.value_head_step, a.key_heads},
-                    {"results", a.out_token_step, a.out_head_step, a.query_heads}};
+    } operands[] = {{"queries", {a.query_token_step, a.query_head_step}, a.query_heads},
+                    {"keys", {a.key_token_step, a.key_head_step}, a.key_heads},
+                    {"values", {a.value_token_step, a.value_head_step}, a.key_heads},
+                    {"results", {a.out_token_step, a.out_head_step}, a.query_heads}};
     for (const auto& o : operands) {
-        // Rows of a head may not overlap: whichever of the two axes steps
-        // further has to step past the other.
-        const bool by_token = o.token >= o.head;
-        const uint64_t inner = by_token ? o.head : o.token, outer = by_token ? o.token : o.head;
-        const uint64_t inner_count = by_token ? o.heads : a.tokens, outer_count = by_token ? a.tokens : o.heads;
-        uint64_t within = 0, whole = 0;
-        const bool fits = !__builtin_mul_overflow(inner, inner_count - (inner_count > 0), &within) &&
-                          !__builtin_add_overflow(within, uint64_t{a.head_size}, &within) &&
-                          !__builtin_mul_overflow(outer, outer_count, &whole) && whole < (uint64_t{1} << 60) &&
-                          within < (uint64_t{1} << 60);
-        if (!fits) return fail(TC_INVALID, what + ": the " + o.name + " reach past the address space");
-        if ((inner_count > 1 && inner < a.head_size) || (outer_count > 1 && outer < within)) {
-            return fail(TC_INVALID, what + ": the " + o.name + " of heads of " + std::to_string(a.head_size) +
-                                        " elements, tokens " + std::to_string(o.token) + " and heads " +
-                                        std::to_string(o.head) + " apart, overlap");
-        }
+        const int status = check_heads(what, o.name, o.steps, o.heads, a.tokens, a.head_size);
+        if (status != TC_OK) return status;
     }
     if (a.sequences > 0 && a.tokens > 0 && a.offsets == nullptr) return null_operand(what.c_str());
     *shape = Shape{a.query_heads,

@@ -57,7 +57,7 @@
 #include <type_traits>
 #include <utility>
 
-#include "rows.hpp"
+#include "heads.hpp"
 
 namespace tc {
 namespace attention {
@@ -69,10 +69,6 @@ constexpr int kBufferFlags = 0x00020000;       // raw 32-bit data
 constexpr uint32_t kOutside = 0x80000000u;    // an offset past any buffer resource here
 constexpr int kWaitForAll = 0x7 << 4;          // vmcnt(0), lgkmcnt(0)
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-
-struct Steps {
-    uint64_t token, head;
-};
 
 struct Shape {
     uint32_t heads, group;  // query heads, and of them to a key head

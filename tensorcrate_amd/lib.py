@@ -35,6 +35,8 @@ ARITHMETIC, COMPARE, POWER = range(3)
 FOLD, MEAN, VARIANCE = range(3)
 # Transposed (kernels.rs:462-467), plus PLAIN.
 PLAIN, LEFT, RIGHT = range(3)
+# Pairs of a rotation (tc_rotary_pairs).
+HALVES, NEIGHBOURS = range(2)
 
 DTYPE_SIZE = {F32: 4, F16: 2, BF16: 2}
 # How each element type is held on the host: bf16 as its raw bits.
@@ -131,6 +133,15 @@ class AttentionShape(ctypes.Structure):
                     for axis in ("token", "head")]
 
 
+class RotaryShape(ctypes.Structure):
+    """``tc_rotary_shape``: heads, tokens, positions and layouts of a rotation."""
+    _fields_ = [(name, u32) for name in ("dtype", "weight_dtype", "query_heads", "key_heads", "head_size",
+                                         "rotary_size", "pairs", "normalize")] + [
+        ("epsilon", f32), ("tokens", u64), ("positions", vp), ("frequencies", vp)] + [
+            (f"{name}_{axis}_step", u64) for name in ("query", "key", "query_out", "key_out")
+            for axis in ("token", "head")]
+
+
 # Every entry point of include/tchip.h with its argument types.
 SIGNATURES = {
     "tc_init": [i32],
@@ -211,6 +222,8 @@ SIGNATURES = {
     "tc_layer_norm_backward": [u32, u32, vp, u64, vp, u64, u64, u64, vp, vp, vp, vp, u64, vp, vp],
     "tc_attention": [ctypes.POINTER(AttentionShape), vp, vp, vp, vp, vp],
     "tc_attention_backward": [ctypes.POINTER(AttentionShape), vp, vp, vp, vp, vp, vp, vp, vp, vp],
+    "tc_rotary_norm": [ctypes.POINTER(RotaryShape), vp, vp, vp, vp, vp, vp],
+    "tc_rotary_norm_backward": [ctypes.POINTER(RotaryShape), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp],
     "tc_global_norm": [u32, ctypes.POINTER(u32), ctypes.POINTER(vp), ctypes.POINTER(u64), vp],
     "tc_clip_global_norm": [u32, ctypes.POINTER(u32), ctypes.POINTER(vp), ctypes.POINTER(u64), f32,
                             ctypes.POINTER(vp), vp],
@@ -421,6 +434,16 @@ def attention(dtype: int, tokens: int, query_heads: int, key_heads: int, head_si
     queries, keys, values and results."""
     return AttentionShape(dtype, query_heads, key_heads, head_size, tokens, sequences, scale, offsets, *query, *key,
                           *value, *out)
+
+
+def rotary(dtype: int, weight_dtype: int, tokens: int, query_heads: int, key_heads: int, head_size: int,
+           rotary_size: int, pairs: int, normalize: bool, epsilon: float, positions, frequencies, query, key, query_out,
+           key_out) -> RotaryShape:
+    """The shape that ``tc_rotary_norm`` and ``tc_rotary_norm_backward`` take:
+    ``positions`` and ``frequencies`` device pointers (or None), and the
+    (token, head) steps of queries, keys and the rotated ones."""
+    return RotaryShape(dtype, weight_dtype, query_heads, key_heads, head_size, rotary_size, pairs, int(normalize),
+                       epsilon, tokens, positions, frequencies, *query, *key, *query_out, *key_out)
 
 
 def region(source: Buffer | int, source_len: int, shape, src_offset, src_strides, dst_offset,
