@@ -819,6 +819,96 @@ int tc_rotary_norm_backward(const tc_rotary_shape* shape, const void* d_query_ou
                             const void* query, const void* key, const void* query_weight, const void* key_weight,
                             void* d_query, void* d_key, void* d_query_weight, void* d_key_weight);
 
+/* ---- a cache of keys and values ---------------------------------------------- */
+
+/* How a cache holds its entries: as they are, or in 8 bits: a row (a head of
+ * one token) as whole numbers of -127 to 127 times the row's own f32 scale,
+ * the largest magnitude of the row divided by 127. */
+typedef enum tc_cache_format { TC_CACHE_PLAIN = 0, TC_CACHE_INT8 = 1 } tc_cache_format;
+
+/* A pool of `page_count` pages, each of `page_size` tokens of `key_heads` heads
+ * of `head_size` (at most 128) elements.  Element e of head h of slot i of page
+ * p is at ((p * key_heads + h) * page_size + i) * row + e of `keys` and of
+ * `values`, `row` being `head_size` rounded up to whole 16-byte words (elements
+ * behind a head's own are written as zeros), and its scale, in 8 bits, at
+ * (p * key_heads + h) * page_size + i of `key_scales` and `value_scales` (else
+ * null).  `keys` and `values` are 16-byte aligned.  `dtype` is that of the rows
+ * that are written, read and attended with.  Fewer than 2^32 rows are taken. */
+typedef struct tc_cache {
+    uint32_t dtype;
+    uint32_t format;
+    uint32_t key_heads;
+    uint32_t head_size;
+    uint32_t page_size;
+    uint32_t page_count;
+    void* keys;
+    void* values;
+    float* key_scales;
+    float* value_scales;
+} tc_cache;
+
+/* The sequences that a call works on (all pointers on the device).  Sequence s
+ * has `lengths[s]` tokens, the n = offsets[s + 1] - offsets[s] last of which
+ * are the call's tokens offsets[s] to offsets[s + 1] (`offsets`: sequences + 1
+ * rising numbers; null: every sequence has one token, `tokens` of them).  The
+ * sequence's token j is at slot j % page_size of page
+ * pages[s * most_pages + j / page_size].  Tokens before the first or past the
+ * last offset are in no sequence.
+ *   A page number of `page_count` or more is no page, and neither is one past
+ * `most_pages`.
+ *   Where `prefix_length` is not 0, every sequence begins with that many tokens
+ * more, the same for all and kept once, on the pages `prefix_pages`;
+ * `lengths` and `pages` are those of the tokens behind it. */
+typedef struct tc_cache_batch {
+    uint64_t tokens;
+    uint32_t sequences;
+    uint32_t most_pages;
+    uint32_t prefix_length;
+    const uint32_t* offsets;
+    const uint32_t* lengths;
+    const uint32_t* pages;
+    const uint32_t* prefix_pages;
+} tc_cache_batch;
+
+/* The bytes of `keys` (and of `values`), and of `key_scales` (and of
+ * `value_scales`; 0 where the entries are plain).  Needs no device. */
+int tc_cache_bytes(const tc_cache* cache, uint64_t* entries, uint64_t* scales);
+
+/* Keys and values of the batch's tokens into their places.  Element e of head h
+ * of token t is at t * token_step + h * head_step + e.  Tokens in no sequence,
+ * on no page, or (where a sequence's length is less than its tokens here)
+ * before the sequence's first are not written.  In 8 bits each element is
+ * divided by its row's scale and rounded to the nearest whole number, ties to
+ * even; a row with an infinity or a NaN gets the scale NaN and zeros.  No two
+ * of the tokens may have the same place. */
+int tc_cache_write(const tc_cache* cache, const tc_cache_batch* batch, const void* key, uint64_t key_token_step,
+                   uint64_t key_head_step, const void* value, uint64_t value_token_step, uint64_t value_head_step);
+
+/* The same tokens' keys and values back from their places, times their scales
+ * and rounded to `dtype` once; zeros for tokens that have no place. */
+int tc_cache_read(const tc_cache* cache, const tc_cache_batch* batch, void* key, uint64_t key_token_step,
+                  uint64_t key_head_step, void* value, uint64_t value_token_step, uint64_t value_head_step);
+
+/* Attention of the batch's tokens over their sequences' keys and values, which
+ * have been written before.  Each token attends to the prefix and to the tokens
+ * of its own sequence up to itself, with scores scale * q . k (`scale` positive
+ * and finite); key head i / (query_heads / key_heads) serves query head i.
+ * Element e of head h of token t is at t * token_step + h * head_step + e of
+ * queries and results.  `normalizers` [query_heads][tokens] (f32; may be null)
+ * receives the log of each query's sum of exponentials.
+ *   Sums and softmax are f32; the weights are rounded to `dtype` in f16 and to
+ * 16 bits in two parts in bf16 and over 8-bit entries.  A query that attends to
+ * nothing (a token in no sequence, or before its first) gets zeros and the
+ * normalizer -infinity.  Keys and values of no page are zeros; no other row
+ * than those a query attends to reaches its result (of those, an infinite value
+ * makes a NaN where its weight is 0).  A query all of whose
+ * scores are -infinity has the normalizer -infinity and, as 0 / 0, a NaN
+ * result.  The order of every sum depends on the batch's counts and lengths
+ * alone. */
+int tc_cache_attention(const tc_cache* cache, const tc_cache_batch* batch, uint32_t query_heads, float scale,
+                       const void* query, uint64_t query_token_step, uint64_t query_head_step, void* out,
+                       uint64_t out_token_step, uint64_t out_head_step, float* normalizers);
+
 #ifdef __cplusplus
 }
 #endif

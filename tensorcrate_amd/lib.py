@@ -37,6 +37,8 @@ FOLD, MEAN, VARIANCE = range(3)
 PLAIN, LEFT, RIGHT = range(3)
 # Pairs of a rotation (tc_rotary_pairs).
 HALVES, NEIGHBOURS = range(2)
+# How a cache holds its entries (tc_cache_format).
+CACHE_PLAIN, CACHE_INT8 = range(2)
 
 DTYPE_SIZE = {F32: 4, F16: 2, BF16: 2}
 # How each element type is held on the host: bf16 as its raw bits.
@@ -142,6 +144,18 @@ class RotaryShape(ctypes.Structure):
             for axis in ("token", "head")]
 
 
+class Cache(ctypes.Structure):
+    """``tc_cache``: a pool of pages of keys and values."""
+    _fields_ = [(name, u32) for name in ("dtype", "format", "key_heads", "head_size", "page_size", "page_count")] + [
+        (name, vp) for name in ("keys", "values", "key_scales", "value_scales")]
+
+
+class CacheBatch(ctypes.Structure):
+    """``tc_cache_batch``: the sequences and tokens that a call works on."""
+    _fields_ = [("tokens", u64), ("sequences", u32), ("most_pages", u32), ("prefix_length", u32)] + [
+        (name, vp) for name in ("offsets", "lengths", "pages", "prefix_pages")]
+
+
 # Every entry point of include/tchip.h with its argument types.
 SIGNATURES = {
     "tc_init": [i32],
@@ -224,6 +238,10 @@ SIGNATURES = {
     "tc_attention_backward": [ctypes.POINTER(AttentionShape), vp, vp, vp, vp, vp, vp, vp, vp, vp],
     "tc_rotary_norm": [ctypes.POINTER(RotaryShape), vp, vp, vp, vp, vp, vp],
     "tc_rotary_norm_backward": [ctypes.POINTER(RotaryShape), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp],
+    "tc_cache_bytes": [ctypes.POINTER(Cache), ctypes.POINTER(u64), ctypes.POINTER(u64)],
+    "tc_cache_write": [ctypes.POINTER(Cache), ctypes.POINTER(CacheBatch), vp, u64, u64, vp, u64, u64],
+    "tc_cache_read": [ctypes.POINTER(Cache), ctypes.POINTER(CacheBatch), vp, u64, u64, vp, u64, u64],
+    "tc_cache_attention": [ctypes.POINTER(Cache), ctypes.POINTER(CacheBatch), u32, f32, vp, u64, u64, vp, u64, u64, vp],
     "tc_global_norm": [u32, ctypes.POINTER(u32), ctypes.POINTER(vp), ctypes.POINTER(u64), vp],
     "tc_clip_global_norm": [u32, ctypes.POINTER(u32), ctypes.POINTER(vp), ctypes.POINTER(u64), f32,
                             ctypes.POINTER(vp), vp],
@@ -444,6 +462,28 @@ def rotary(dtype: int, weight_dtype: int, tokens: int, query_heads: int, key_hea
     (token, head) steps of queries, keys and the rotated ones."""
     return RotaryShape(dtype, weight_dtype, query_heads, key_heads, head_size, rotary_size, pairs, int(normalize),
                        epsilon, tokens, positions, frequencies, *query, *key, *query_out, *key_out)
+
+
+def cache(dtype: int, format: int, key_heads: int, head_size: int, page_size: int, page_count: int, keys, values,
+          key_scales=None, value_scales=None) -> Cache:
+    """The pool that the ``tc_cache_*`` calls take: device pointers of as many
+    bytes as ``cache_bytes`` says."""
+    return Cache(dtype, format, key_heads, head_size, page_size, page_count, keys, values, key_scales, value_scales)
+
+
+def cache_bytes(pool: Cache) -> tuple[int, int]:
+    """Bytes of the keys (and of the values) and of the keys' scales (and the
+    values') of a pool, whose pointers need not be set."""
+    entries, scales = u64(), u64()
+    call("tc_cache_bytes", pool, ctypes.byref(entries), ctypes.byref(scales))
+    return entries.value, scales.value
+
+
+def cache_batch(tokens: int, sequences: int, offsets, lengths, pages, most_pages: int, prefix_length: int = 0,
+                prefix_pages=None) -> CacheBatch:
+    """The sequences that a ``tc_cache_*`` call works on: device pointers to
+    their offsets (or None: a token each), lengths and tables of pages."""
+    return CacheBatch(tokens, sequences, most_pages, prefix_length, offsets, lengths, pages, prefix_pages)
 
 
 def region(source: Buffer | int, source_len: int, shape, src_offset, src_strides, dst_offset,
