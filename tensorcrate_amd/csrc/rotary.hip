@@ -18,6 +18,8 @@
 // An angle is a product in 64 bits, reduced to a part of a turn there, so that
 // far positions lose nothing; the functions of that part are taken in 32.
 
+#include <type_traits>
+
 #include "heads.hpp"
 
 namespace tc {
@@ -68,7 +70,6 @@ struct Lane {
     }
     __device__ __forceinline__ static constexpr int a(int i) { return HALVES ? i : 2 * i; }
     __device__ __forceinline__ static constexpr int b(int i) { return HALVES ? i + 4 : 2 * i + 1; }
-    __device__ __forceinline__ bool turns(int i) const { return pair + i < half; }
     // Column of a slot, `size` or more if it has none.
     __device__ __forceinline__ uint32_t column(int slot) const {
         if (whole) return slot < 4 ? first + slot : second + slot - 4;
@@ -76,12 +77,14 @@ struct Lane {
         const uint32_t other = HALVES ? slot / 4 : slot % 2;
         return HALVES && p < half ? p + other * half : 2 * p + other;
     }
-    template <typename S>
+    template <bool NT, typename S>
     __device__ __forceinline__ void load(const S* row, Words<S, 8>& out) const {
         typedef uint32_t piece __attribute__((ext_vector_type(sizeof(S)), aligned(sizeof(S))));
         if (whole) {
-            const piece low = *reinterpret_cast<const piece*>(row + first);
-            const piece high = *reinterpret_cast<const piece*>(row + second);
+            const piece* const from[2] = {reinterpret_cast<const piece*>(row + first),
+                                          reinterpret_cast<const piece*>(row + second)};
+            const piece low = NT ? __builtin_nontemporal_load(from[0]) : *from[0];
+            const piece high = NT ? __builtin_nontemporal_load(from[1]) : *from[1];
             __builtin_memcpy(out.w, &low, sizeof(low));
             __builtin_memcpy(reinterpret_cast<char*>(out.w) + sizeof(low), &high, sizeof(high));
         } else {
@@ -94,7 +97,7 @@ struct Lane {
             out.put(v);
         }
     }
-    template <typename S>
+    template <bool NT, typename S>
     __device__ __forceinline__ void store(S* row, const float (&v)[8]) const {
         typedef uint32_t piece __attribute__((ext_vector_type(sizeof(S)), aligned(sizeof(S))));
         if (whole) {
@@ -103,8 +106,13 @@ struct Lane {
             piece low, high;
             __builtin_memcpy(&low, words.w, sizeof(low));
             __builtin_memcpy(&high, reinterpret_cast<const char*>(words.w) + sizeof(low), sizeof(high));
-            *reinterpret_cast<piece*>(row + first) = low;
-            *reinterpret_cast<piece*>(row + second) = high;
+            if constexpr (NT) {
+                __builtin_nontemporal_store(low, reinterpret_cast<piece*>(row + first));
+                __builtin_nontemporal_store(high, reinterpret_cast<piece*>(row + second));
+            } else {
+                *reinterpret_cast<piece*>(row + first) = low;
+                *reinterpret_cast<piece*>(row + second) = high;
+            }
         } else {
 #pragma unroll
             for (int k = 0; k < 8; k++) {
@@ -113,17 +121,66 @@ struct Lane {
             }
         }
     }
+    // The pairs' turns, back with SIGN -1.
+    template <int SIGN>
+    __device__ __forceinline__ void turn(float (&v)[8], const float2* turns) const {
+        if (pair >= half) return;
+        const bool all = pair + 4 <= half;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 t = turns[pair + i];
+            const float x = v[a(i)], y = v[b(i)], s = SIGN < 0 ? -t.y : t.y;
+            const bool turned = all || pair + i < half;
+            v[a(i)] = turned ? fmaf(x, t.x, -(y * s)) : x;
+            v[b(i)] = turned ? fmaf(y, t.x, x * s) : y;
+        }
+    }
 };
+
+// The rows of one of the two tensors that a group of 16 lanes takes in a
+// block's turn, every kGroups-th: token and head, and the row's place in each
+// of up to three layouts, moved on by sums that are the same for the block.
+template <int LAYOUTS>
+struct RowWalk {
+    uint32_t heads, tokens_on, heads_on;
+    uint64_t on[LAYOUTS], wrap[LAYOUTS];
+    uint32_t token, head;
+    uint64_t at[LAYOUTS];
+
+    __device__ __forceinline__ RowWalk(uint32_t count, const Steps (&steps)[LAYOUTS], uint32_t group, uint64_t first)
+        : heads(count), tokens_on(kGroups / count), heads_on(kGroups % count), token(group / count), head(group % count) {
+#pragma unroll
+        for (int n = 0; n < LAYOUTS; n++) {
+            on[n] = tokens_on * steps[n].token + heads_on * steps[n].head;
+            wrap[n] = steps[n].token - heads * steps[n].head;
+            at[n] = (first + token) * steps[n].token + head * steps[n].head;
+        }
+    }
+    __device__ __forceinline__ void move() {
+        token += tokens_on, head += heads_on;
+        const bool over = head >= heads;
+        token += over;
+        head -= over ? heads : 0;
+#pragma unroll
+        for (int n = 0; n < LAYOUTS; n++) at[n] += on[n] + (over ? wrap[n] : 0);
+    }
+};
+
+// 1 / sqrt(v), by the instruction, which takes no subnormal number.
+__device__ __forceinline__ float reciprocal_root(float v) {
+    const bool small = v < 0x1p-100f;
+    const float root = __builtin_amdgcn_rsqf(small ? v * 0x1p64f : v);
+    return small ? root * 0x1p32f : root;
+}
 
 // `sums` (BACK; null if no weight's gradient is wanted): of each block, for
 // queries and then keys, 8 slots of 16 lanes.
-template <typename S, typename W, bool HALVES, bool BACK>
+template <typename S, typename W, bool HALVES, bool BACK, bool NT>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary<S, W> r, float* __restrict__ sums) {
-    __shared__ float2 turns[kMostTokens][kMostPairs];
+    __shared__ __attribute__((aligned(16))) float2 turns[2][kMostTokens][kMostPairs];
     const uint32_t lane = threadIdx.x % 16, group = threadIdx.x / 16;
-    const uint32_t heads = r.heads[0] + r.heads[1];
     const Lane<HALVES> at(lane, r.size, r.half);
-    const float count = static_cast<float>(r.size);
+    const float part = 1.0f / static_cast<float>(r.size);
 
     float weight[2][8];
 #pragma unroll
@@ -136,10 +193,11 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary<S, W> r, 
     }
     float along[BACK ? 2 : 1][8] = {};
 
-    for (uint64_t first = uint64_t{blockIdx.x} * r.chunk; first < r.tokens; first += uint64_t{gridDim.x} * r.chunk) {
-        const uint32_t here = r.tokens - first < r.chunk ? static_cast<uint32_t>(r.tokens - first) : r.chunk;
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < here * r.half; i += kThreads) {
+    const auto tokens_at = [&](uint64_t first) {
+        return r.tokens <= first ? 0 : r.tokens - first < r.chunk ? static_cast<uint32_t>(r.tokens - first) : r.chunk;
+    };
+    const auto find_turns = [&](int stage, uint64_t first) {
+        for (uint32_t i = threadIdx.x; i < tokens_at(first) * r.half; i += kThreads) {
             const uint32_t token = i / r.half, pair = i % r.half;
             const uint32_t position =
                 r.positions != nullptr ? r.positions[first + token] : static_cast<uint32_t>(first + token);
@@ -148,63 +206,77 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary<S, W> r, 
                                  0.15915494309189533577;
             float2 turn;
             sincospif(2.0f * static_cast<float>(angle - rint(angle)), &turn.y, &turn.x);
-            turns[token][pair] = turn;
+            turns[stage][token][pair] = turn;
         }
-        __syncthreads();
-        for (uint32_t row = group; row < here * heads; row += kGroups) {
-            const uint32_t token = row / heads, number = row % heads;
-            const int n = number < r.heads[0] ? 0 : 1;
-            const uint32_t head = n == 0 ? number : number - r.heads[0];
-            const auto place = [&](Steps steps) { return (first + token) * steps.token + head * steps.head; };
-            Words<S, 8> words, words_x;
-            at.load(r.from[n] + place(r.from_steps[n]), words);
-            if (BACK && r.normalize) at.load(r.x[n] + place(r.x_steps[n]), words_x);
+    };
+    // The rows of queries or keys of the tokens from `first` on, each with the
+    // next one's words in flight.
+    const auto rows_of = [&](auto which, int stage, uint64_t first, uint32_t here) {
+        constexpr int n = decltype(which)::value;
+        if (r.heads[n] == 0) return;
+        constexpr int LAYOUTS = BACK ? 3 : 2;
+        const Steps steps[3] = {r.from_steps[n], r.to_steps[n], r.x_steps[n]};
+        RowWalk<LAYOUTS> walk(r.heads[n], reinterpret_cast<const Steps(&)[LAYOUTS]>(steps), group, first);
+        Words<S, 8> next, next_x;
+        const auto fetch = [&]() {
+            at.template load<NT>(r.from[n] + walk.at[0], next);
+            if constexpr (BACK) {
+                if (r.normalize) at.template load<NT>(r.x[n] + walk.at[2], next_x);
+            }
+        };
+        if (walk.token < here) fetch();
+        while (walk.token < here) {
+            const uint32_t token = walk.token;
+            S* const to = r.to[n] + walk.at[1];
             float v[8], x[8];
-            words.get(v);
-            // The scale of the row, from x.
+            next.get(v);
+            if constexpr (BACK) next_x.get(x);
+            walk.move();
+            if (walk.token < here) fetch();
             float scale = 1.0f;
             if (r.normalize) {
-                if constexpr (BACK) words_x.get(x);
-                else words.get(x);
                 float squares = 0.0f;
 #pragma unroll
-                for (int k = 0; k < 8; k++) squares = fmaf(x[k], x[k], squares);
-                scale = 1.0f / sqrtf(row16<Added>(squares) / count + r.epsilon);
+                for (int k = 0; k < 8; k++) squares = fmaf(BACK ? x[k] : v[k], BACK ? x[k] : v[k], squares);
+                scale = reciprocal_root(fmaf(row16<Added>(squares), part, r.epsilon));
             }
             if constexpr (!BACK) {
                 if (r.normalize) {
 #pragma unroll
-                    for (int k = 0; k < 8; k++) v[k] = v[k] * scale * (n == 0 ? weight[0][k] : weight[1][k]);
+                    for (int k = 0; k < 8; k++) v[k] = v[k] * scale * weight[n][k];
                 }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (!at.turns(i)) continue;
-                const float2 turn = turns[token][at.pair + i];
-                const float a = v[at.a(i)], b = v[at.b(i)];
-                const float s = BACK ? -turn.y : turn.y;
-                v[at.a(i)] = a * turn.x - b * s;
-                v[at.b(i)] = b * turn.x + a * s;
-            }
-            if constexpr (BACK) {
+                at.template turn<1>(v, turns[stage][token]);
+            } else {
+                at.template turn<-1>(v, turns[stage][token]);
                 if (r.normalize) {
                     float dot = 0.0f;
 #pragma unroll
                     for (int k = 0; k < 8; k++) {
                         x[k] *= scale;
-                        const float product = v[k] * x[k];
-                        if (n == 0) along[0][k] += product;
-                        else along[1][k] += product;
-                        v[k] *= n == 0 ? weight[0][k] : weight[1][k];
+                        along[n][k] = fmaf(v[k], x[k], along[n][k]);
+                        v[k] *= weight[n][k];
                         dot = fmaf(v[k], x[k], dot);
                     }
-                    dot = row16<Added>(dot) / count;
+                    dot = row16<Added>(dot) * part;
 #pragma unroll
-                    for (int k = 0; k < 8; k++) v[k] = scale * (v[k] - x[k] * dot);
+                    for (int k = 0; k < 8; k++) v[k] = scale * fmaf(-x[k], dot, v[k]);
                 }
             }
-            at.store(r.to[n] + place(r.to_steps[n]), v);
+            at.template store<NT>(to, v);
         }
+    };
+
+    const uint64_t apart = uint64_t{gridDim.x} * r.chunk;
+    uint64_t first = uint64_t{blockIdx.x} * r.chunk;
+    find_turns(0, first);
+    int stage = 0;
+    for (; first < r.tokens; first += apart, stage ^= 1) {
+        // (The stage that is written was read before the last barrier.)
+        __syncthreads();
+        find_turns(stage ^ 1, first + apart);
+        const uint32_t here = tokens_at(first);
+        rows_of(std::integral_constant<int, 0>(), stage, first, here);
+        rows_of(std::integral_constant<int, 1>(), stage, first, here);
     }
     if constexpr (BACK) {
         if (sums == nullptr) return;
@@ -258,18 +330,19 @@ int rotary(const tc_rotary_shape& a, Rotary<S, W> r, W* d_query_weight, W* d_key
     r.chunk = a.tokens >= units * 8 * kMostTokens ? kMostTokens : 1;
     const bool weights = BACK && (d_query_weight != nullptr || d_key_weight != nullptr);
     const bool rows = a.tokens > 0 && a.query_heads + uint64_t{a.key_heads} > 0;
-    const uint32_t blocks = rows ? grid_for(a.tokens, r.chunk, weights ? 4 : 32) : 0;
+    const uint32_t blocks = rows ? grid_for(a.tokens, r.chunk, weights ? 4 : 8) : 0;
     Scratch scratch(weights ? uint64_t{blocks} * 256 * sizeof(float) : 0);
     if (scratch.status != TC_OK) return scratch.status;
     float* sums = weights ? static_cast<float*>(scratch.ptr) : nullptr;
     const bool halves = a.pairs == TC_ROTARY_HALVES;
     int status = TC_OK;
     if (rows) {
-        if (halves) {
-            rotary_kernel<S, W, true, BACK><<<blocks, kThreads, 0, s>>>(r, sums);
-        } else {
-            rotary_kernel<S, W, false, BACK><<<blocks, kThreads, 0, s>>>(r, sums);
-        }
+        const uint64_t moved = (BACK ? 3 : 2) * sizeof(S) * a.tokens * r.size * (uint64_t{r.heads[0]} + r.heads[1]);
+        const bool streams = moved >= kStreamBytes;
+        if (halves && streams) rotary_kernel<S, W, true, BACK, true><<<blocks, kThreads, 0, s>>>(r, sums);
+        if (halves && !streams) rotary_kernel<S, W, true, BACK, false><<<blocks, kThreads, 0, s>>>(r, sums);
+        if (!halves && streams) rotary_kernel<S, W, false, BACK, true><<<blocks, kThreads, 0, s>>>(r, sums);
+        if (!halves && !streams) rotary_kernel<S, W, false, BACK, false><<<blocks, kThreads, 0, s>>>(r, sums);
         status = check_launch(what);
     }
     if (status != TC_OK || !weights) return status;
