@@ -28,6 +28,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kGroups = kThreads / 16;  // rows that a block holds at a time
 constexpr uint32_t kMostPairs = 64;     // of a head
+constexpr uint32_t kForwardPerUnit = 6, kBackPerUnit = 4;  // blocks of a compute unit
 constexpr uint32_t kMostTokens = 4;     // whose cosines and sines a block holds
 
 template <typename S, typename W>
@@ -73,9 +74,19 @@ struct Lane {
     // Column of a slot, `size` or more if it has none.
     __device__ __forceinline__ uint32_t column(int slot) const {
         if (whole) return slot < 4 ? first + slot : second + slot - 4;
-        const uint32_t p = pair + (HALVES ? slot % 4 : slot / 2);
+        return scattered(pair, slot);
+    }
+    __device__ __forceinline__ uint32_t scattered(uint32_t from, int slot) const {
+        const uint32_t p = from + (HALVES ? slot % 4 : slot / 2);
         const uint32_t other = HALVES ? slot / 4 : slot % 2;
         return HALVES && p < half ? p + other * half : 2 * p + other;
+    }
+    // `pair`, so that columns are found where they are used: kept through the
+    // loop over rows they would take registers of all lanes.
+    __device__ __forceinline__ uint32_t here() const {
+        uint32_t from = pair;
+        asm volatile("" : "+v"(from));
+        return from;
     }
     template <bool NT, typename S>
     __device__ __forceinline__ void load(const S* row, Words<S, 8>& out) const {
@@ -88,10 +99,11 @@ struct Lane {
             __builtin_memcpy(out.w, &low, sizeof(low));
             __builtin_memcpy(reinterpret_cast<char*>(out.w) + sizeof(low), &high, sizeof(high));
         } else {
+            const uint32_t from = here();
             float v[8];
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const uint32_t c = column(k);
+                const uint32_t c = scattered(from, k);
                 v[k] = c < size ? Elem<S>::widen(row[c]) : 0.0f;
             }
             out.put(v);
@@ -114,9 +126,10 @@ struct Lane {
                 *reinterpret_cast<piece*>(row + second) = high;
             }
         } else {
+            const uint32_t from = here();
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const uint32_t c = column(k);
+                const uint32_t c = scattered(from, k);
                 if (c < size) row[c] = Elem<S>::narrow(v[k]);
             }
         }
@@ -176,20 +189,19 @@ __device__ __forceinline__ float reciprocal_root(float v) {
 // `sums` (BACK; null if no weight's gradient is wanted): of each block, for
 // queries and then keys, 8 slots of 16 lanes.
 template <typename S, typename W, bool HALVES, bool BACK, bool NT>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary<S, W> r, float* __restrict__ sums) {
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(BACK ? kBackPerUnit : kForwardPerUnit))) rotary_kernel(const Rotary<S, W> r, float* __restrict__ sums) {
     __shared__ __attribute__((aligned(16))) float2 turns[2][kMostTokens][kMostPairs];
     const uint32_t lane = threadIdx.x % 16, group = threadIdx.x / 16;
     const Lane<HALVES> at(lane, r.size, r.half);
     const float part = 1.0f / static_cast<float>(r.size);
 
-    float weight[2][8];
-#pragma unroll
-    for (int n = 0; n < 2; n++) {
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const uint32_t c = at.column(k);
-            weight[n][k] = r.weight[n] != nullptr && c < r.size ? Elem<W>::widen(r.weight[n][c]) : 1.0f;
-        }
+    // Each lane's weights, the same for the block's groups.
+    __shared__ __attribute__((aligned(16))) float weights[2][16][8];
+    if (threadIdx.x < 2 * 16 * 8) {
+        const uint32_t n = threadIdx.x / 128, k = threadIdx.x % 8, of = threadIdx.x / 8 % 16;
+        const uint32_t c = Lane<HALVES>(of, r.size, r.half).column(k);
+        const W* const from = n == 0 ? r.weight[0] : r.weight[1];
+        weights[n][of][k] = from != nullptr && c < r.size ? Elem<W>::widen(from[c]) : 1.0f;
     }
     float along[BACK ? 2 : 1][8] = {};
 
@@ -243,7 +255,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary<S, W> r, 
             if constexpr (!BACK) {
                 if (r.normalize) {
 #pragma unroll
-                    for (int k = 0; k < 8; k++) v[k] = v[k] * scale * weight[n][k];
+                    for (int k = 0; k < 8; k++) v[k] = v[k] * scale * weights[n][lane][k];
                 }
                 at.template turn<1>(v, turns[stage][token]);
             } else {
@@ -254,7 +266,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Rotary<S, W> r, 
                     for (int k = 0; k < 8; k++) {
                         x[k] *= scale;
                         along[n][k] = fmaf(v[k], x[k], along[n][k]);
-                        v[k] *= weight[n][k];
+                        v[k] *= weights[n][lane][k];
                         dot = fmaf(v[k], x[k], dot);
                     }
                     dot = row16<Added>(dot) * part;
@@ -326,11 +338,13 @@ int rotary(const tc_rotary_shape& a, Rotary<S, W> r, W* d_query_weight, W* d_key
     r.epsilon = a.epsilon;
     r.tokens = a.tokens;
     r.positions = a.positions, r.frequencies = a.frequencies;
+    // As many blocks as run at once, walking the tokens together.
+    const uint32_t per_unit = BACK ? kBackPerUnit : kForwardPerUnit;
     const uint64_t units = static_cast<uint64_t>(compute_units());
-    r.chunk = a.tokens >= units * 8 * kMostTokens ? kMostTokens : 1;
+    r.chunk = a.tokens >= units * per_unit * 2 ? kMostTokens : 1;
     const bool weights = BACK && (d_query_weight != nullptr || d_key_weight != nullptr);
     const bool rows = a.tokens > 0 && a.query_heads + uint64_t{a.key_heads} > 0;
-    const uint32_t blocks = rows ? grid_for(a.tokens, r.chunk, weights ? 4 : 8) : 0;
+    const uint32_t blocks = rows ? grid_for(a.tokens, r.chunk, per_unit) : 0;
     Scratch scratch(weights ? uint64_t{blocks} * 256 * sizeof(float) : 0);
     if (scratch.status != TC_OK) return scratch.status;
     float* sums = weights ? static_cast<float*>(scratch.ptr) : nullptr;
