@@ -60,7 +60,10 @@ template <bool HALVES>
 struct Lane {
     uint32_t pair, size, half;
     uint32_t first, second;  // columns of slots 0 and 4, of whole runs
-    bool whole;
+    // Whole runs, and whether the lane has elements at all: one that has none
+    // reads the head's first ones, since a branch that zeroes its registers
+    // would wait for the other lanes' loads, and adds nothing to any sum.
+    bool whole, has;
 
     __device__ __forceinline__ Lane(uint32_t lane, uint32_t n, uint32_t turned)
         : pair(4 * lane), size(n), half(turned) {
@@ -68,11 +71,14 @@ struct Lane {
         first = halves ? pair : 2 * pair;
         second = halves ? pair + half : 2 * pair + 4;
         whole = halves || ((!HALVES || pair >= half) && 2 * pair + 8 <= size);
+        has = pair < half || 2 * pair < size;
+        if (!has && size >= 8) whole = true, first = 0, second = 4;
     }
     __device__ __forceinline__ static constexpr int a(int i) { return HALVES ? i : 2 * i; }
     __device__ __forceinline__ static constexpr int b(int i) { return HALVES ? i + 4 : 2 * i + 1; }
     // Column of a slot, `size` or more if it has none.
     __device__ __forceinline__ uint32_t column(int slot) const {
+        if (!has) return size;
         if (whole) return slot < 4 ? first + slot : second + slot - 4;
         return scattered(pair, slot);
     }
@@ -112,6 +118,7 @@ struct Lane {
     template <bool NT, typename S>
     __device__ __forceinline__ void store(S* row, const float (&v)[8]) const {
         typedef uint32_t piece __attribute__((ext_vector_type(sizeof(S)), aligned(sizeof(S))));
+        if (!has) return;
         if (whole) {
             Words<S, 8> words;
             words.put(v);
@@ -221,36 +228,41 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(B
             turns[stage][token][pair] = turn;
         }
     };
-    // The rows of queries or keys of the tokens from `first` on, each with the
-    // next one's words in flight.
-    const auto rows_of = [&](auto which, int stage, uint64_t first, uint32_t here) {
+    // A row's words on their way: of x forward, of dz and x backward.
+    struct Fetched {
+        Words<S, 8> row, x;
+    };
+    constexpr int LAYOUTS = BACK ? 3 : 2;
+    const auto walk_of = [&](auto which, uint64_t first) {
         constexpr int n = decltype(which)::value;
-        if (r.heads[n] == 0) return;
-        constexpr int LAYOUTS = BACK ? 3 : 2;
         const Steps steps[3] = {r.from_steps[n], r.to_steps[n], r.x_steps[n]};
-        RowWalk<LAYOUTS> walk(r.heads[n], reinterpret_cast<const Steps(&)[LAYOUTS]>(steps), group, first);
-        Words<S, 8> next, next_x;
-        const auto fetch = [&]() {
-            at.template load<NT>(r.from[n] + walk.at[0], next);
-            if constexpr (BACK) {
-                if (r.normalize) at.template load<NT>(r.x[n] + walk.at[2], next_x);
-            }
-        };
-        if (walk.token < here) fetch();
+        return RowWalk<LAYOUTS>(r.heads[n], reinterpret_cast<const Steps(&)[LAYOUTS]>(steps), group, first);
+    };
+    const auto fetch = [&](auto which, const RowWalk<LAYOUTS>& walk, Fetched& out) {
+        constexpr int n = decltype(which)::value;
+        at.template load<NT>(r.from[n] + walk.at[0], out.row);
+        if constexpr (BACK) {
+            if (r.normalize) at.template load<NT>(r.x[n] + walk.at[2], out.x);
+        }
+    };
+    // The rows of queries or keys of `here` tokens, the first of them in `next`
+    // and each one's successor in flight.
+    const auto rows_of = [&](auto which, int stage, RowWalk<LAYOUTS>& walk, uint32_t here, Fetched& next) {
+        constexpr int n = decltype(which)::value;
         while (walk.token < here) {
             const uint32_t token = walk.token;
             S* const to = r.to[n] + walk.at[1];
             float v[8], x[8];
-            next.get(v);
-            if constexpr (BACK) next_x.get(x);
+            next.row.get(v);
+            if constexpr (BACK) next.x.get(x);
             walk.move();
-            if (walk.token < here) fetch();
+            if (walk.token < here) fetch(which, walk, next);
             float scale = 1.0f;
             if (r.normalize) {
                 float squares = 0.0f;
 #pragma unroll
                 for (int k = 0; k < 8; k++) squares = fmaf(BACK ? x[k] : v[k], BACK ? x[k] : v[k], squares);
-                scale = reciprocal_root(fmaf(row16<Added>(squares), part, r.epsilon));
+                scale = reciprocal_root(fmaf(row16<Added>(at.has ? squares : 0.0f), part, r.epsilon));
             }
             if constexpr (!BACK) {
                 if (r.normalize) {
@@ -269,7 +281,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(B
                         v[k] *= weights[n][lane][k];
                         dot = fmaf(v[k], x[k], dot);
                     }
-                    dot = row16<Added>(dot) * part;
+                    dot = row16<Added>(at.has ? dot : 0.0f) * part;
 #pragma unroll
                     for (int k = 0; k < 8; k++) v[k] = scale * fmaf(-x[k], dot, v[k]);
                 }
@@ -280,15 +292,35 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(B
 
     const uint64_t apart = uint64_t{gridDim.x} * r.chunk;
     uint64_t first = uint64_t{blockIdx.x} * r.chunk;
+    const std::integral_constant<int, 0> queries;
+    const std::integral_constant<int, 1> keys;
+    Fetched next_query, next_key;
+    // The first query row of a turn is on its way before the last turn's keys
+    // are done, the first key row before the turn's queries are.
+    const auto begin = [&](auto which, uint64_t from, Fetched& out) {
+        constexpr int n = decltype(which)::value;
+        if (r.heads[n] == 0) return;
+        const RowWalk<LAYOUTS> walk = walk_of(which, from);
+        if (walk.token < tokens_at(from)) fetch(which, walk, out);
+    };
+    begin(queries, first, next_query);
     find_turns(0, first);
     int stage = 0;
     for (; first < r.tokens; first += apart, stage ^= 1) {
         // (The stage that is written was read before the last barrier.)
         __syncthreads();
-        find_turns(stage ^ 1, first + apart);
         const uint32_t here = tokens_at(first);
-        rows_of(std::integral_constant<int, 0>(), stage, first, here);
-        rows_of(std::integral_constant<int, 1>(), stage, first, here);
+        begin(keys, first, next_key);
+        find_turns(stage ^ 1, first + apart);
+        if (r.heads[0] > 0) {
+            RowWalk<LAYOUTS> walk = walk_of(queries, first);
+            rows_of(queries, stage, walk, here, next_query);
+        }
+        begin(queries, first + apart, next_query);
+        if (r.heads[1] > 0) {
+            RowWalk<LAYOUTS> walk = walk_of(keys, first);
+            rows_of(keys, stage, walk, here, next_key);
+        }
     }
     if constexpr (BACK) {
         if (sums == nullptr) return;
