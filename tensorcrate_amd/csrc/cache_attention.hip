@@ -6,9 +6,8 @@ namespace tc {
 namespace cache {
 namespace {
 
-// Blocks of 16 query rows that a wave holds, where `rows` query rows share
-// keys.
-int row_blocks_of(uint64_t rows) { return rows > 16 ? 2 : 1; }
+// The form for `rows` query rows that share keys.
+int form_of(uint64_t rows) { return rows <= 16 ? kRows16 : rows <= 32 ? kRows32 : kRows128; }
 
 // The storage of one line's parts.
 struct Storage {
@@ -37,19 +36,19 @@ int run(const AttentionLaunches& launches, const Attention& a, bool quant) {
     const uint64_t size = (a.pool.size + 31) / 32 * 32, tokens = a.batch.tokens, rows = tokens * a.query_heads;
     const bool prefix = a.batch.prefix > 0;
     const uint64_t sequences = a.batch.sequences;
-    const int own_rb = row_blocks_of(tokens * a.group / (sequences > 0 ? sequences : 1));
-    const int prefix_rb = row_blocks_of(tokens * a.group);
-    const uint64_t own_rows = 16 * own_rb, prefix_rows = 16 * prefix_rb;
-    const Storage own(2 * uint64_t{blocks} * own_rows, prefix ? rows : 0,
+    const int own_form = form_of(tokens * a.group / (sequences > 0 ? sequences : 1));
+    const int prefix_form = form_of(tokens * a.group);
+    const uint64_t own_rows = rows_of_form(own_form), prefix_rows = rows_of_form(prefix_form);
+    const Storage own(2 * uint64_t{workers_of(own_form, blocks)} * own_rows, prefix ? rows : 0,
                       (tokens * a.group / own_rows + sequences) * a.pool.heads, size);
-    const Storage shared(prefix ? 2 * uint64_t{blocks} * prefix_rows : 0, prefix ? rows : 0,
+    const Storage shared(prefix ? 2 * uint64_t{workers_of(prefix_form, blocks)} * prefix_rows : 0, prefix ? rows : 0,
                          prefix ? (tokens * a.group / prefix_rows + 1) * a.pool.heads : 0, size);
     if (own.status() != TC_OK) return own.status();
     if (shared.status() != TC_OK) return shared.status();
-    int status = launches.attend(a, own.parts(), quant, false, !prefix, own_rb, blocks);
-    if (status == TC_OK && prefix) status = launches.attend(a, shared.parts(), quant, true, false, prefix_rb, blocks);
+    int status = launches.attend(a, own.parts(), quant, false, !prefix, own_form, blocks);
+    if (status == TC_OK && prefix) status = launches.attend(a, shared.parts(), quant, true, false, prefix_form, blocks);
     if (status != TC_OK) return status;
-    return launches.join(a, own.parts(), shared.parts(), quant, own_rb, prefix_rb, blocks);
+    return launches.join(a, own.parts(), shared.parts(), quant, own_form, prefix_form, blocks);
 }
 
 }  // namespace

@@ -8,23 +8,30 @@
 // with the larger maximum and both sums scaled down to it, in any grouping, so
 // the keys of a sequence may be split over waves and blocks.
 //   Bound by memory: a new token's keys and values are read once and used for
-// the few query heads that share a key head.  So the keys of all sequences and
-// key heads are one line of units, cut evenly over as many blocks as the chip
-// holds, whatever the lengths are (`Line`); a block's waves take tiles of their
-// unit each and join at the end of a sequence's part, and parts of a sequence
-// that lie in several blocks are joined by a second kernel.
+// the few query heads that share a key head.  So the tiles of all sequences and
+// key heads are one line, cut evenly over as many waves as the chip holds,
+// whatever the lengths are (`Line`); parts of a sequence that lie in several
+// waves are joined by a second kernel.
 //   A prefix that all sequences share is a line of its own, of as many blocks
 // of query rows as all tokens' heads fill: its keys are read once for each of
 // those and not for each sequence.
 //
-// A wave holds 16 query rows (token and head of a key head's group; RB times
-// as many where there are more) as the columns of 16 x 16 products.  s
-// transposed is k . q^T, so that a lane has 4 keys of a row in each product's
-// result, and those registers are the operand of o^T = v^T . p^T.  Keys and
-// values go through registers to the wave's own tile in LDS, since rows on
-// pages have no step between them and 8-bit entries are widened on the way:
-// whole numbers up to 127 are exact in every type, and their scales go into
-// the scores and the weights.  The next tile's rows are in flight meanwhile.
+// A wave holds 16 query rows (token and head of a key head's group) or 32 as
+// the columns of 16 x 16 products.  s transposed is k . q^T, so that a lane has
+// 4 keys of a row in each product's result, and those registers are the operand
+// of o^T = v^T . p^T.  Keys and values go through registers to the wave's own
+// tile in LDS, since rows on pages have no step between them and 8-bit entries
+// are widened on the way; the next tile's rows are in flight meanwhile.  Where
+// more rows than 32 share keys, a block's four waves hold 128 of them and share
+// each tile (SHARED): the widening is done once for all of them.
+//
+// The weights are multiplied with the values in two parts of 16 bits, their
+// rounding and the rounding of what that leaves, so that they keep 16 bits of
+// bf16 or 22 of f16: twice the products of a kernel that waits for memory.
+// 8-bit entries under 16-bit queries are multiplied as f16, where whole numbers
+// to 127 are exact: their scales go into the scores and, against a power of two
+// that no scale so far has reached, into the weights, and queries in bf16 are
+// brought into range by a power of two a row.
 #pragma once
 
 #include "attention_tiles.hpp"
@@ -35,6 +42,11 @@ namespace cache {
 
 constexpr int kAttendThreads = 256;
 constexpr int kAttendWaves = kAttendThreads / 64;
+// The forms of the first kernel: 16 or 32 query rows a wave, or 128 a block.
+enum Form { kRows16 = 0, kRows32 = 1, kRows128 = 2 };
+constexpr uint32_t rows_of_form(int form) { return form == kRows16 ? 16 : form == kRows32 ? 32 : 128; }
+// Whose parts are one behind another on the line: waves, or blocks.
+constexpr uint32_t workers_of(int form, uint32_t blocks) { return form == kRows128 ? blocks : blocks * kAttendWaves; }
 
 // One launch's operands.
 struct Attention {
@@ -51,16 +63,16 @@ struct Attention {
 };
 
 // Where an item (a key head's block of query rows of a sequence) has its
-// results: whole in the rows' own place, or in the blocks first to last, the
+// results: whole in the rows' own place, or with the workers first to last, the
 // first one's in `slot`, the others' in their first slot.
 struct Plan {
     uint32_t first, last, slot, whole;
 };
 
-// Partial results.  A block has two slots, for parts at its two ends.
+// Partial results.  A worker has two slots, for parts at its two ends.
 struct Parts {
-    float* slots;         // [2 blocks][rows][size]
-    float2* slot_stats;   // [2 blocks][rows] (maximum, in powers of two; sum)
+    float* slots;         // [2 workers][rows][size]
+    float2* slot_stats;   // [2 workers][rows] (maximum, in powers of two; sum)
     float* rows;          // [token][query head][size], of whole items
     float2* row_stats;
     Plan* plans;
@@ -70,9 +82,9 @@ struct Parts {
 struct AttentionLaunches {
     // Items' parts over the sequences' own keys, or with `prefix` over the
     // prefix; `final`: whole items are results.
-    int (*attend)(const Attention&, const Parts&, bool quant, bool prefix, bool final, int row_blocks, uint32_t blocks);
-    int (*join)(const Attention&, const Parts& own, const Parts& prefix, bool quant, int own_row_blocks,
-                int prefix_row_blocks, uint32_t blocks);
+    int (*attend)(const Attention&, const Parts&, bool quant, bool prefix, bool final, int form, uint32_t blocks);
+    int (*join)(const Attention&, const Parts& own, const Parts& prefix, bool quant, int own_form, int prefix_form,
+                uint32_t blocks);
 };
 const AttentionLaunches& attend_f32();
 const AttentionLaunches& attend_f16();
@@ -110,8 +122,7 @@ using attention::u32x2;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kKeys = kWide ? 16 : 32;  // rows of a wave's tile
-constexpr uint32_t kUnit = kKeys * kAttendWaves;
+constexpr int kKeys = kWide ? 16 : 32;  // rows of a tile
 constexpr int kBlocks16 = kKeys / 16;
 // Elements of the summed axis that one operand word of all quarters covers.
 constexpr int kDeep16 = 4 * E;
@@ -183,10 +194,26 @@ struct KeyTile : attention::Tile<SIZE, kKeys> {
 template <typename T>
 __device__ __forceinline__ void widened(uint4 bytes, Words<T, 16>& out) {
     const uint32_t four[4] = {bytes.x, bytes.y, bytes.z, bytes.w};
-    float v[16];
+    if constexpr (sizeof(T) == 2) {
+        // Behind the upper byte of 1024 in f16, whose step is 1: 1024 + 128 + q.
+        static_assert(Elem<T>::dtype == TC_F16, "8 bits are widened to f16 or f32");
+        typedef _Float16 pair __attribute__((ext_vector_type(2)));
+        uint32_t* const to = reinterpret_cast<uint32_t*>(out.w);
 #pragma unroll
-    for (int e = 0; e < 16; e++) v[e] = static_cast<float>(static_cast<int8_t>(four[e / 4] >> (8 * (e % 4))));
-    out.put(v);
+        for (int n = 0; n < 4; n++) {
+            const uint32_t shifted = four[n] ^ 0x80808080u;
+            const pair low = __builtin_bit_cast(pair, __builtin_amdgcn_perm(0x64646464u, shifted, 0x04010400u));
+            const pair high = __builtin_bit_cast(pair, __builtin_amdgcn_perm(0x64646464u, shifted, 0x04030402u));
+            const pair origin = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+            to[2 * n] = __builtin_bit_cast(uint32_t, low - origin);
+            to[2 * n + 1] = __builtin_bit_cast(uint32_t, high - origin);
+        }
+    } else {
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++) v[e] = static_cast<float>(static_cast<int8_t>(four[e / 4] >> (8 * (e % 4))));
+        out.put(v);
+    }
 }
 
 // Which values a sweep takes: the finite ones as they are, or as ones the
@@ -239,67 +266,100 @@ __device__ __forceinline__ Sequence sequence_at(const Attention& a, uint32_t seq
     }
 }
 
-// The units of all items one behind another: sequences, of each the key heads,
-// of each the blocks of ROWS query rows, of each the units of kUnit keys.
+// The tiles of all items one behind another: sequences, of each the key heads,
+// of each the blocks of ROWS query rows, of each the tiles of kKeys keys.
 template <int ROWS>
 struct Line {
-    __device__ __forceinline__ static uint32_t units(const Sequence& s) { return (s.keys + kUnit - 1) / kUnit; }
+    __device__ __forceinline__ static uint32_t tiles(const Sequence& s) { return (s.keys + kKeys - 1) / kKeys; }
     __device__ __forceinline__ static uint32_t blocks(const Attention& a, const Sequence& s) {
         return static_cast<uint32_t>((uint64_t{s.tokens} * a.group + ROWS - 1) / ROWS);
     }
     __device__ __forceinline__ static uint64_t count(const Attention& a, const Sequence& s) {
-        return uint64_t{units(s)} * blocks(a, s) * a.pool.heads;
+        return uint64_t{tiles(s)} * blocks(a, s) * a.pool.heads;
     }
 };
 
-template <int SIZE, int RB, bool QUANT, bool PREFIX>
+// Four elements from `first` on to a row of `size`.
+__device__ __forceinline__ void store_four(S* row, uint32_t first, uint32_t size, f32x4 v) {
+    typedef uint32_t piece __attribute__((ext_vector_type(sizeof(S)), aligned(sizeof(S))));
+    S out[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) out[j] = Elem<S>::narrow(v[j]);
+    if (first + 4 <= size) {
+        piece bits;
+        __builtin_memcpy(&bits, out, sizeof(bits));
+        *reinterpret_cast<piece*>(row + first) = bits;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (first + j < size) row[first + j] = out[j];
+        }
+    }
+}
+
+// Power of two that weights are rounded times in f16, whose least normal is
+// 2^-14: the largest, which may reach 2^8, stay below 2^15.
+constexpr float kHalfPower = 6.0f;
+
+template <int SIZE, int FORM, bool QUANT, bool PREFIX>
 __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_per_eu(2)))
     attend_kernel(const Attention a, const Parts parts, bool final) {
-    constexpr int ROWS = 16 * RB;
+    constexpr bool SHARED = FORM == kRows128;
+    constexpr int RB = FORM == kRows16 ? 1 : 2;  // blocks of 16 rows of a wave
+    constexpr int ROWS = rows_of_form(FORM);
+    constexpr int kWorkers = SHARED ? 1 : kAttendWaves;  // of a block
+    constexpr int kMovers = SHARED ? kAttendThreads : 64;  // threads that move a tile
     using LineOf = Line<ROWS>;
     using TileOf = KeyTile<SIZE>;
-    // Weights and values are multiplied in S, but 8-bit entries with bf16
-    // weights where S is f16, whose range scales may leave.
-    using V = std::conditional_t<QUANT && kHalf, bf16_t, S>;
-    constexpr bool kTwoParts = sizeof(V) == 2 && Elem<V>::dtype == TC_BF16;
-    constexpr float kPower = sizeof(V) == 2 && Elem<V>::dtype == TC_F16 ? 6.0f : 0.0f;
+    // The type that is multiplied in.
+    constexpr bool kScaled = QUANT && sizeof(S) == 2;
+    using M = std::conditional_t<kScaled, _Float16, S>;
+    constexpr bool kTwoParts = sizeof(M) == 2;
+    constexpr float kPower = sizeof(M) == 2 && Elem<M>::dtype == TC_F16 ? kHalfPower : 0.0f;
     constexpr int kOperands = SIZE / kDeep16;
     constexpr int kEntry = QUANT ? 1 : static_cast<int>(sizeof(S));
     constexpr int kRowWords = SIZE * kEntry / 16;
-    constexpr int kEach = (kKeys * kRowWords + 63) / 64;
-    constexpr int kStride = SIZE + 4;  // of a row where waves join
+    constexpr int kEach = (kKeys * kRowWords + kMovers - 1) / kMovers;
+    constexpr int kStages = SHARED ? 2 : kAttendWaves;
 
-    __shared__ __attribute__((aligned(1024))) char tiles[kAttendWaves][2 * TileOf::kBytes];
-    __shared__ float scales[QUANT ? kAttendWaves : 1][64];
-    __shared__ float2 stats[kAttendWaves][ROWS];
-    __shared__ uint64_t sums[kAttendWaves], found[2];
-    static_assert(sizeof(tiles) >= kAttendWaves * 16 * kStride * sizeof(float), "waves join in the tiles' place");
+    __shared__ __attribute__((aligned(1024))) char tiles[kStages][2 * TileOf::kBytes];
+    __shared__ __attribute__((aligned(16))) float scales[QUANT ? kStages : 1][64];
+    __shared__ uint64_t sums[kAttendWaves], found[kWorkers][2];
 
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, quarter = lane / 16;
 
-    // ---- this block's units ----------------------------------------------------
+    // ---- this worker's tiles -----------------------------------------------------
     const uint32_t sequences = PREFIX ? 1 : a.batch.sequences;
-    uint64_t total_units = 0;
+    uint64_t total_tiles = 0;
     if constexpr (PREFIX) {
-        total_units = LineOf::count(a, sequence_at<true>(a, 0));
+        total_tiles = LineOf::count(a, sequence_at<true>(a, 0));
     } else {
         uint64_t mine = 0;
         for (uint32_t n = threadIdx.x; n < sequences; n += kAttendThreads) mine += LineOf::count(a, sequence_at<false>(a, n));
         for (int offset = 32; offset > 0; offset >>= 1) mine += __shfl_xor(static_cast<unsigned long long>(mine), offset);
         if (lane == 0) sums[wave] = mine;
         __syncthreads();
-        for (int w = 0; w < kAttendWaves; w++) total_units += sums[w];
+        for (int w = 0; w < kAttendWaves; w++) total_tiles += sums[w];
         __syncthreads();
     }
-    // No block has nothing, so that every block between two parts of an item
-    // has a part of it.
-    const uint64_t blocks = total_units < gridDim.x ? total_units : gridDim.x;
-    if (blockIdx.x >= blocks) return;
-    const uint64_t begin = blockIdx.x * total_units / blocks, end = (blockIdx.x + 1) * total_units / blocks;
+    // No worker has nothing, so that every one between two parts of an item has
+    // a part of it.
+    const uint64_t most_workers = uint64_t{gridDim.x} * kWorkers;
+    const uint64_t workers = total_tiles < most_workers ? total_tiles : most_workers;
+    const uint32_t first_worker = blockIdx.x * kWorkers;
+    if (first_worker >= workers) return;
+    const auto begin_of = [&](uint64_t worker) { return worker * total_tiles / workers; };
 
+    const uint32_t worker = __builtin_amdgcn_readfirstlane(first_worker + (SHARED ? 0 : wave));
     uint32_t sequence = 0;
-    uint64_t before = 0;  // units of the sequences before
+    uint64_t before = 0;  // tiles of the sequences before
     if constexpr (!PREFIX) {
+        uint64_t begins[kWorkers];
+#pragma unroll
+        for (int w = 0; w < kWorkers; w++) {
+            // (Of a worker past the last one: the last one's.)
+            begins[w] = begin_of(first_worker + w < workers ? first_worker + w : workers - 1);
+        }
         for (uint32_t from = 0; from < sequences; from += kAttendThreads) {
             const uint32_t n = from + threadIdx.x;
             const uint64_t count = n < sequences ? LineOf::count(a, sequence_at<false>(a, n)) : 0;
@@ -316,78 +376,111 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                 all += sums[w];
             }
             const uint64_t start = before + upto - count;
-            if (begin >= start && begin - start < count) found[0] = n, found[1] = start;
+#pragma unroll
+            for (int w = 0; w < kWorkers; w++) {
+                if (begins[w] >= start && begins[w] - start < count) found[w][0] = n, found[w][1] = start;
+            }
             __syncthreads();
-            if (begin - before < all) break;  // the same for the whole block
+            if (begins[kWorkers - 1] - before < all) break;  // the same for the whole block
             before += all;
         }
-        sequence = static_cast<uint32_t>(found[0]);
-        before = found[1];
-        sequence = __builtin_amdgcn_readfirstlane(sequence);
+        sequence = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(found[SHARED ? 0 : wave][0]));
+        before = found[SHARED ? 0 : wave][1];
     }
+    if (worker >= workers) return;  // (a wave by itself: no barrier follows)
+    const uint64_t begin = begin_of(worker), end = begin_of(worker + uint64_t{1});
 
-    const TileOf key_tile{tiles[wave]};
-    const TileOf value_tile{tiles[wave] + TileOf::kBytes};
     const uint32_t row_place = TileOf::row_place(lane), column_place = TileOf::column_place(lane);
     const float c = a.scale * attention::kLog2e;
+    int stage = SHARED ? 0 : wave;
 
-    for (uint64_t unit = begin; unit < end;) {
+    for (uint64_t at = begin; at < end;) {
         const Sequence s = sequence_at<PREFIX>(a, sequence);
-        const uint32_t units = LineOf::units(s), row_blocks = LineOf::blocks(a, s);
-        const uint64_t count = uint64_t{units} * row_blocks * a.pool.heads;
-        if (unit - before >= count) {
+        const uint32_t tile_count = LineOf::tiles(s), row_blocks = LineOf::blocks(a, s);
+        const uint64_t count = uint64_t{tile_count} * row_blocks * a.pool.heads;
+        if (at - before >= count) {
             before += count;
             sequence++;
             continue;
         }
-        const uint32_t item = static_cast<uint32_t>((unit - before) / units);
-        const uint32_t unit_0 = static_cast<uint32_t>((unit - before) % units);
-        const uint32_t unit_1 = end - unit < units - unit_0 ? unit_0 + static_cast<uint32_t>(end - unit) : units;
+        const uint32_t item = static_cast<uint32_t>((at - before) / tile_count);
+        const uint32_t tile_0 = static_cast<uint32_t>((at - before) % tile_count);
+        const uint32_t tile_1 = end - at < tile_count - tile_0 ? tile_0 + static_cast<uint32_t>(end - at) : tile_count;
         const uint32_t key_head = item / row_blocks, row_block = item % row_blocks;
-        const bool whole = unit_0 == 0 && unit_1 == units;
-        // (An item's first part is the block's first if both begin together.)
-        const uint32_t slot = 2 * blockIdx.x + (unit > begin);
-        if (unit_0 == 0 && threadIdx.x == 0) {
-            const uint64_t last_unit = unit + units - 1;
-            const uint64_t last = ((last_unit + 1) * blocks - 1) / total_units;
-            const uint64_t at = (PREFIX ? 0 : first_item(a, ROWS, sequence, s.first)) + item;
-            parts.plans[at] = {blockIdx.x, static_cast<uint32_t>(last), slot, whole};
+        const bool whole = tile_0 == 0 && tile_1 == tile_count;
+        // (An item's first part is the worker's first if both begin together.)
+        const uint32_t slot = 2 * worker + (at > begin);
+        if (tile_0 == 0 && (SHARED ? threadIdx.x : lane) == 0) {
+            const uint64_t last = ((at + tile_count) * workers - 1) / total_tiles;
+            const uint64_t place = (PREFIX ? 0 : first_item(a, ROWS, sequence, s.first)) + item;
+            parts.plans[place] = {worker, static_cast<uint32_t>(last), slot, whole};
         }
 
         // ---- the item's query rows -------------------------------------------------
-        const uint32_t rows = s.tokens * a.group - row_block * ROWS < ROWS ? s.tokens * a.group - row_block * ROWS : ROWS;
+        const uint32_t first_row = row_block * ROWS, left_rows = s.tokens * a.group - first_row;
+        const uint32_t rows = left_rows < ROWS ? left_rows : ROWS;
+        const auto row_of_lane = [&](int r) { return static_cast<uint32_t>((SHARED ? wave * 16 * RB : 0) + r * 16 + lane % 16); };
         uint4 queries[RB][kOperands];
+        [[maybe_unused]] float shrunk[RB];  // what a row of queries was multiplied with, undone
         uint32_t seen[RB];
-        uint32_t least = s.keys, most_seen = 0;
+        bool all_see = true;
 #pragma unroll
         for (int r = 0; r < RB; r++) {
-            const uint32_t row = r * 16 + lane % 16, number = row_block * ROWS + row;
+            const uint32_t row = row_of_lane(r), number = first_row + row;
             const bool real = row < rows;
             const uint32_t place = a.group_of.div(real ? number : 0);
             const uint32_t token = s.first + place;
             const uint32_t head = key_head * a.group + (real ? number : 0) - place * a.group;
-            if constexpr (PREFIX) {
-                Span span;
-                const uint32_t own = sequence_of(a.batch, token, &span);
-                seen[r] = own == kNowhere ? s.keys : seen_of(a.batch.lengths[own], span.end - token, s.keys, s.keys);
-            } else {
-                seen[r] = seen_of(s.length, s.tokens - place, 0, s.keys);
-            }
-            if (!real) seen[r] = s.keys;
+            seen[r] = s.keys;
             if (real) {
-                least = seen[r] < least ? seen[r] : least;
-                most_seen = seen[r] > most_seen ? seen[r] : most_seen;
+                if constexpr (PREFIX) {
+                    Span span;
+                    const uint32_t own = sequence_of(a.batch, token, &span);
+                    if (own != kNowhere) seen[r] = seen_of(a.batch.lengths[own], span.end - token, s.keys, s.keys);
+                } else {
+                    seen[r] = seen_of(s.length, s.tokens - place, 0, s.keys);
+                }
             }
+            all_see = all_see && seen[r] == s.keys;
             const S* from = static_cast<const S*>(a.query) + token * a.query_steps.token + head * a.query_steps.head;
 #pragma unroll
             for (int n = 0; n < kOperands; n++) {
                 queries[r][n] = real ? head_word(from, 4 * n + quarter, a.pool.size) : make_uint4(0, 0, 0, 0);
             }
+            if constexpr (kScaled && !std::is_same_v<S, M>) {
+                // The largest of the row to 2^14 and above, an infinity or a
+                // NaN as it is.
+                float most = 0.0f;
+#pragma unroll
+                for (int n = 0; n < kOperands; n++) {
+                    const Words<S, E> words{{queries[r][n]}};
+#pragma unroll
+                    for (int e = 0; e < E; e++) most = fmaxf(most, fabsf(words.at(e)));
+                }
+                most = quarters<Largest>(most);
+                int power = most > 0.0f && most < INFINITY ? 14 - ilogbf(most) : 0;
+                power = power > 126 ? 126 : power;
+                shrunk[r] = ldexpf(1.0f, -power);
+                const float factor = ldexpf(1.0f, power);
+#pragma unroll
+                for (int n = 0; n < kOperands; n++) {
+                    const Words<S, E> words{{queries[r][n]}};
+                    Words<M, E> to;
+                    float v[E];
+#pragma unroll
+                    for (int e = 0; e < E; e++) v[e] = words.at(e) * factor;
+                    to.put(v);
+                    queries[r][n] = to.w[0];
+                }
+            }
         }
-        for (int offset = 8; offset > 0; offset >>= 1) {
-            const uint32_t other = __shfl_xor(least, offset), more = __shfl_xor(most_seen, offset);
-            least = other < least ? other : least;
-            most_seen = more > most_seen ? more : most_seen;
+        // Keys that every, and that any, row of the block sees.
+        uint32_t least, most_seen = s.keys;
+        if constexpr (PREFIX) {
+            least = (SHARED ? __syncthreads_and(all_see) : __ballot(!all_see) == 0) ? s.keys : 0;
+        } else {
+            least = seen_of(s.length, s.tokens - a.group_of.div(first_row), 0, s.keys);
+            most_seen = seen_of(s.length, s.tokens - a.group_of.div(first_row + rows - 1), 0, s.keys);
         }
         least = __builtin_amdgcn_readfirstlane(least);
         most_seen = __builtin_amdgcn_readfirstlane(most_seen);
@@ -395,27 +488,28 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
         // ---- a sweep over the part's tiles -----------------------------------------
         f32x4 acc[RB][SIZE / 16];
         float most[RB], total[RB];
+        [[maybe_unused]] float unit = 0x1p-126f;  // above every value's scale so far, and a power of two
 
-        const uint32_t key_end = uint64_t{unit_1} * kUnit < most_seen ? unit_1 * kUnit : most_seen;
+        const uint32_t key_end = uint64_t{tile_1} * kKeys < most_seen ? tile_1 * kKeys : most_seen;
         uint32_t tile = 0;
         uint4 key_words[kEach], value_words[kEach];
         float entry_scale = 0.0f;
-        // The page of key l % 32 of the tile at `at`, and its row there.
-        const auto page_at = [&](uint32_t at) {
-            const uint32_t key = at + lane % 32;
+        // The page of key l % 32 of the tile at `first`, and its row there.
+        const auto page_at = [&](uint32_t first) {
+            const uint32_t key = first + lane % 32;
             const uint32_t n = a.pool.pages_of.div(key);
             return lane % 32 < kKeys && key < key_end && n < s.page_count ? s.pages[n] : kNowhere;
         };
-        const auto row_at = [&](uint32_t at, uint32_t page) {
-            const uint32_t key = at + lane % 32;
-            const uint32_t slot_in = key - a.pool.pages_of.div(key) * a.pool.page_size;
-            return page < a.pool.page_count ? (page * a.pool.heads + key_head) * a.pool.page_size + slot_in : kNowhere;
+        const auto row_at = [&](uint32_t first, uint32_t page) {
+            const uint32_t key = first + lane % 32;
+            const uint32_t within = key - a.pool.pages_of.div(key) * a.pool.page_size;
+            return page < a.pool.page_count ? (page * a.pool.heads + key_head) * a.pool.page_size + within : kNowhere;
         };
         const auto fetch = [&](uint32_t row) {
             const uint32_t row_bytes = a.pool.row * kEntry;
 #pragma unroll
             for (int k = 0; k < kEach; k++) {
-                const int i = k * 64 + lane;
+                const int i = k * kMovers + (SHARED ? threadIdx.x : lane);
                 const uint32_t from = __shfl(row, i / kRowWords < kKeys ? i / kRowWords : 0);
                 const uint32_t byte = i % kRowWords * 16;
                 key_words[k] = value_words[k] = make_uint4(0, 0, 0, 0);
@@ -429,15 +523,14 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                 entry_scale = row == kNowhere ? 0.0f : (lane < 32 ? a.pool.key_scales : a.pool.value_scales)[row];
             }
         };
-        const auto land = [&]() {
+        const auto land = [&](const TileOf& key_tile, const TileOf& value_tile) {
 #pragma unroll
             for (int k = 0; k < kEach; k++) {
-                const int i = k * 64 + lane;
-                if (kKeys * kRowWords % 64 != 0 && i >= kKeys * kRowWords) continue;
+                const int i = k * kMovers + (SHARED ? threadIdx.x : lane);
+                if (kKeys * kRowWords % kMovers != 0 && i >= kKeys * kRowWords) continue;
                 const int row = i / kRowWords, word = i % kRowWords;
                 if constexpr (QUANT) {
-                    Words<S, 16> keys;
-                    Words<V, 16> values;
+                    Words<M, 16> keys, values;
                     widened(key_words[k], keys);
                     widened(value_words[k], values);
 #pragma unroll
@@ -450,19 +543,39 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                     *reinterpret_cast<uint4*>(value_tile.word(row, word)) = value_words[k];
                 }
             }
-            if constexpr (QUANT) scales[wave][lane] = entry_scale;
+            if constexpr (QUANT) {
+                if (!SHARED || wave == 0) scales[stage][lane] = entry_scale;
+            }
         };
         uint32_t next_page = kNowhere;
         [[maybe_unused]] int pick = kFinite;
         const auto turn = [&](auto is_masked, auto is_slow) {
             constexpr bool MASKED = decltype(is_masked)::value, SLOW = decltype(is_slow)::value;
-            wave_order();
-            land();
-            wave_order();
-            const uint32_t next = tile + kUnit;
+            const TileOf key_tile{tiles[stage]};
+            const TileOf value_tile{tiles[stage] + TileOf::kBytes};
+            if constexpr (kScaled) {
+                const float high = wave64<Largest>(lane < 32 ? 0.0f : entry_scale);
+                if (high >= unit && high < INFINITY) {
+                    const float grown = ldexpf(1.0f, ilogbf(high) + 3);
+                    const float factor = unit / grown;
+                    unit = grown;
+#pragma unroll
+                    for (int r = 0; r < RB; r++) {
+#pragma unroll
+                        for (int t = 0; t < SIZE / 16; t++) acc[r][t] *= factor;
+                    }
+                }
+            }
+            // A stage that a block shares was read before the last barrier; a
+            // wave's own is in the order of the program.
+            if constexpr (!SHARED) wave_order();
+            land(key_tile, value_tile);
+            if constexpr (SHARED) __syncthreads();
+            else wave_order();
+            const uint32_t next = tile + kKeys;
             if (next < key_end) {
                 fetch(row_at(next, next_page));
-                next_page = page_at(next + kUnit);
+                next_page = page_at(next + kKeys);
             }
             // Scores, and their maximum over the tile.
             f32x4 scores[RB][kBlocks16];
@@ -474,14 +587,17 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                 for (int n = 0; n < kOperands; n++) {
                     const uint4 keys = key_tile.by_row(row_place, b, n);
 #pragma unroll
-                    for (int r = 0; r < RB; r++) scores[r][b] = product16<S>(keys, queries[r][n], scores[r][b]);
+                    for (int r = 0; r < RB; r++) scores[r][b] = product16<M>(keys, queries[r][n], scores[r][b]);
                 }
                 if constexpr (QUANT) {
-                    const f32x4 scale = *reinterpret_cast<const f32x4*>(&scales[wave][16 * b + 4 * quarter]);
+                    const f32x4 scale = *reinterpret_cast<const f32x4*>(&scales[stage][16 * b + 4 * quarter]);
 #pragma unroll
                     for (int r = 0; r < RB; r++) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) scores[r][b][i] *= scale[i];
+                        for (int i = 0; i < 4; i++) {
+                            if constexpr (kScaled && !std::is_same_v<S, M>) scores[r][b][i] *= shrunk[r];
+                            scores[r][b][i] *= scale[i];
+                        }
                     }
                 }
             }
@@ -522,17 +638,17 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                         total[r] += scores[r][b][i];
                     }
                     if constexpr (QUANT) {
-                        const f32x4 scale = *reinterpret_cast<const f32x4*>(&scales[wave][32 + 16 * b + 4 * quarter]);
+                        const f32x4 scale = *reinterpret_cast<const f32x4*>(&scales[stage][32 + 16 * b + 4 * quarter]);
+                        const float against = kScaled ? 1.0f / unit : 1.0f;
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const bool out_of = MASKED && tile + 16 * b + 4 * quarter + i >= seen[r];
-                            scores[r][b][i] = out_of ? 0.0f : scores[r][b][i] * scale[i];
+                            scores[r][b][i] = out_of ? 0.0f : scores[r][b][i] * (scale[i] * against);
                         }
                     }
                 }
             }
-            // The weights as operands: their rounding to V, and where that
-            // keeps 8 bits, the rounding of what it leaves.
+            // The weights as operands.
             uint4 high_part[RB], low_part[RB];
 #pragma unroll
             for (int r = 0; r < RB; r++) {
@@ -545,7 +661,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                         v[e] = (pick == kNaN ? sees : pick == kZero ? sees && v[e] == 0.0f : v[e] != 0.0f) ? 1.0f : 0.0f;
                     }
                 }
-                Words<V, E> high, low;
+                Words<M, E> high, low;
                 high.put(v);
                 high_part[r] = high.w[0];
                 if constexpr (kTwoParts) {
@@ -564,11 +680,12 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                 }
 #pragma unroll
                 for (int r = 0; r < RB; r++) {
-                    acc[r][t] = product16<V>(values, high_part[r], acc[r][t]);
-                    if constexpr (kTwoParts) acc[r][t] = product16<V>(values, low_part[r], acc[r][t]);
+                    acc[r][t] = product16<M>(values, high_part[r], acc[r][t]);
+                    if constexpr (kTwoParts) acc[r][t] = product16<M>(values, low_part[r], acc[r][t]);
                 }
             }
             tile = next;
+            if constexpr (SHARED) stage ^= 1;
         };
         const auto sweep = [&](auto is_slow) {
 #pragma unroll
@@ -577,11 +694,11 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
 #pragma unroll
                 for (int t = 0; t < SIZE / 16; t++) acc[r][t] = f32x4{};
             }
-            tile = unit_0 * kUnit + wave * kKeys;
+            tile = tile_0 * kKeys;
             if (tile >= key_end) return;
             fetch(row_at(tile, page_at(tile)));
-            next_page = page_at(tile + kUnit);
-            // (Rows past `key_end` are masked too.)
+            next_page = page_at(tile + kKeys);
+            // (Keys past `key_end` are seen by no row, or by none that is real.)
             const uint32_t plain_end = least < key_end ? least : key_end;
             if constexpr (!decltype(is_slow)::value) {
                 while (tile < plain_end && plain_end - tile >= kKeys) turn(std::false_type(), is_slow);
@@ -603,7 +720,8 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                     for (int i = 0; i < 4; i++) spoiled |= !(fabsf(acc[r][t][i]) < INFINITY);
                 }
             }
-            if (__builtin_expect(__ballot(spoiled) != 0, false)) {
+            const bool any = SHARED ? __syncthreads_or(spoiled) != 0 : __ballot(spoiled) != 0;
+            if (__builtin_expect(any, false)) {
                 uint32_t up[RB] = {}, down[RB] = {};  // a bit an element, both for a NaN
 #pragma unroll 1
                 for (pick = kZero; pick >= kFinite; pick--) {
@@ -635,173 +753,127 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             }
         }
 
-        // ---- the waves' sums joined, and stored --------------------------------------
+        // ---- the part's sums stored ----------------------------------------------------
 #pragma unroll
         for (int r = 0; r < RB; r++) {
-            total[r] = quarters<Added>(total[r]);
-            if (lane < 16) stats[wave][r * 16 + lane] = make_float2(most[r], total[r]);
-        }
-        __syncthreads();
-        float* const shared = reinterpret_cast<float*>(&tiles[0][0]);
+            const float all = quarters<Added>(total[r]);
+            const uint32_t row = row_of_lane(r);
+            if (row >= rows) continue;
+            const uint32_t number = first_row + row, place = a.group_of.div(number);
+            const uint32_t token = s.first + place, head = key_head * a.group + number - place * a.group;
+            const float back = kScaled ? unit : 1.0f;
+            if (whole && final) {
+                // (A sum of 0 over keys that are seen is of scores of -infinity
+                // alone: 0 / 0.)
+                const float scale = back / all;
+                S* const to = static_cast<S*>(a.out) + token * a.out_steps.token + head * a.out_steps.head;
 #pragma unroll
-        for (int r = 0; r < RB; r++) {
-            const auto over_waves = [&](uint32_t row, float* top, float* all) {
-                *top = -INFINITY, *all = 0.0f;
-                for (int w = 0; w < kAttendWaves; w++) *top = fmaxf(*top, stats[w][row].x);
-                const float origin = *top == -INFINITY ? 0.0f : *top;
-                for (int w = 0; w < kAttendWaves; w++) *all += power2(stats[w][row].x - origin) * stats[w][row].y;
-            };
-            float top, all;
-            over_waves(r * 16 + lane % 16, &top, &all);
-            const float factor = power2(most[r] - (top == -INFINITY ? 0.0f : top));
-#pragma unroll
-            for (int t = 0; t < SIZE / 16; t++) {
-                *reinterpret_cast<f32x4*>(shared + (wave * 16 + lane % 16) * kStride + 16 * t + 4 * quarter) =
-                    acc[r][t] * factor;
-            }
-            __syncthreads();
-            for (uint32_t i = threadIdx.x; i < 16 * SIZE / 4; i += kAttendThreads) {
-                const uint32_t row = i / (SIZE / 4), column = i % (SIZE / 4) * 4;
-                if (r * 16 + row >= rows) continue;
-                f32x4 v = *reinterpret_cast<const f32x4*>(shared + row * kStride + column);
-                for (int w = 1; w < kAttendWaves; w++) {
-                    v += *reinterpret_cast<const f32x4*>(shared + (w * 16 + row) * kStride + column);
+                for (int t = 0; t < SIZE / 16; t++) {
+                    store_four(to, 16 * t + 4 * quarter, a.pool.size, seen[r] > 0 ? acc[r][t] * scale : f32x4{});
                 }
-                over_waves(r * 16 + row, &top, &all);
-                const uint32_t number = row_block * ROWS + r * 16 + row;
-                const uint32_t place = a.group_of.div(number);
-                const uint32_t token = s.first + place, head = key_head * a.group + number - place * a.group;
-                if (whole && final) {
-                    // (A sum of 0 over keys that are seen is of scores of
-                    // -infinity alone: 0 / 0.)
-                    const bool sees = seen_of(s.length, s.tokens - place, 0, s.keys) > 0;
-                    S* const to = static_cast<S*>(a.out) + token * a.out_steps.token + head * a.out_steps.head;
-                    const float scale = sees ? 1.0f / all : 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        if (column + j < a.pool.size) to[column + j] = Elem<S>::narrow(sees ? v[j] * scale : 0.0f);
-                    }
-                    if (column == 0 && a.normalizers != nullptr) {
-                        a.normalizers[uint64_t{head} * a.batch.tokens + token] =
-                            all == 0.0f ? -INFINITY : (top + log2f(all) - kPower) * attention::kLn2;
-                    }
-                } else {
-                    const uint64_t at = whole ? uint64_t{token} * a.query_heads + head
-                                              : uint64_t{slot} * ROWS + r * 16 + row;
-                    float* const to = (whole ? parts.rows : parts.slots) + at * SIZE + column;
-                    *reinterpret_cast<f32x4*>(to) = v;
-                    if (column == 0) (whole ? parts.row_stats : parts.slot_stats)[at] = make_float2(top, all);
+                if (quarter == 0 && a.normalizers != nullptr) {
+                    a.normalizers[uint64_t{head} * a.batch.tokens + token] =
+                        all == 0.0f ? -INFINITY : (most[r] + log2f(all) - kPower) * attention::kLn2;
                 }
+            } else {
+                const uint64_t to = whole ? uint64_t{token} * a.query_heads + head : uint64_t{slot} * ROWS + row;
+                float* const values = (whole ? parts.rows : parts.slots) + to * SIZE + 4 * quarter;
+#pragma unroll
+                for (int t = 0; t < SIZE / 16; t++) *reinterpret_cast<f32x4*>(values + 16 * t) = acc[r][t] * back;
+                if (quarter == 0) (whole ? parts.row_stats : parts.slot_stats)[to] = make_float2(most[r], all);
             }
-            __syncthreads();
         }
-        unit += unit_1 - unit_0;
+        at += tile_1 - tile_0;
     }
 }
 
-// Each row's parts joined, a block a row: the row's own sequence's and the
-// prefix's, in the order of their blocks, 8 of them at a time.
+// Each row's parts joined, a wave a row: the row's own sequence's and the
+// prefix's, in the order of their workers, two at a time.
 template <int SIZE>
 __global__ void __launch_bounds__(kAttendThreads)
     join_kernel(const Attention a, const Parts own, const Parts prefix, uint32_t own_rows, uint32_t prefix_rows,
-                uint32_t blocks, bool half_power) {
-    constexpr int kGroups = kAttendThreads / 32;
-    __shared__ f32x4 sums[kGroups][32];
-    __shared__ float totals[kGroups];
-    for (uint64_t row = blockIdx.x; row < uint64_t{a.batch.tokens} * a.query_heads; row += gridDim.x) {
-        const uint32_t token = static_cast<uint32_t>(row / a.query_heads);
-        const uint32_t head = static_cast<uint32_t>(row % a.query_heads);
-        const uint32_t key_head = head / a.group, within = head % a.group;
+                uint32_t own_workers, uint32_t prefix_workers, float power) {
+    const uint64_t apart = uint64_t{gridDim.x} * kAttendWaves, all_rows = uint64_t{a.batch.tokens} * a.query_heads;
+    for (uint64_t at = uint64_t{blockIdx.x} * kAttendWaves + threadIdx.x / 64; at < all_rows; at += apart) {
+        const uint32_t row = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at));
+        const uint32_t token = row / a.query_heads, head = row % a.query_heads;
+        const uint32_t key_head = a.group_of.div(head), within = head - key_head * a.group;
         Span span{0, 0};
         const uint32_t sequence = wave_sequence_of(a.batch, token, &span);
 
-        // A line's parts of the row: n of them, the first at `first` of its
-        // slots, or the one of a whole item.
+        // A line's parts of the row: n of them, the first in `first_slot`, or
+        // the one of a whole item.
         struct Found {
-            uint32_t n = 0, first_block = 0, first_slot = 0, line = 0;
-            uint64_t within = 0;
+            uint32_t n = 0, first_worker = 0, first_slot = 0, line = 0, within = 0;
             bool whole = false;
         } mine, shared;
         bool sees = false;
         if (sequence != kNowhere) {
             const Sequence s = sequence_at<false>(a, sequence);
             const uint32_t place = token - s.first, left = s.tokens - place;
-            const auto find = [&](const Parts& parts, uint32_t rows, uint64_t first, uint64_t number,
-                                  uint32_t row_blocks) {
+            const auto find = [&](const Parts& parts, uint32_t rows, uint32_t workers, uint64_t first, uint32_t number,
+                                  uint32_t tokens) {
                 Found f;
-                const uint32_t block = static_cast<uint32_t>(number / rows);
-                const Plan plan = parts.plans[first + uint64_t{key_head} * row_blocks + block];
+                const uint32_t row_blocks = static_cast<uint32_t>((uint64_t{tokens} * a.group + rows - 1) / rows);
+                const Plan plan = parts.plans[first + uint64_t{key_head} * row_blocks + number / rows];
                 f.whole = plan.whole != 0;
-                f.n = f.whole ? 1 : plan.first <= plan.last && plan.last < blocks ? plan.last - plan.first + 1 : 0;
-                f.first_block = plan.first, f.first_slot = plan.slot;
-                f.line = rows;
-                f.within = number % rows;
+                f.n = f.whole ? 1 : plan.first <= plan.last && plan.last < workers ? plan.last - plan.first + 1 : 0;
+                f.first_worker = plan.first, f.first_slot = plan.slot;
+                f.line = rows, f.within = number % rows;
                 return f;
             };
             if (s.keys > 0) {
-                const uint32_t row_blocks = static_cast<uint32_t>((uint64_t{s.tokens} * a.group + own_rows - 1) / own_rows);
-                mine = find(own, own_rows, first_item(a, own_rows, sequence, s.first),
-                            uint64_t{place} * a.group + within, row_blocks);
+                mine = find(own, own_rows, own_workers, first_item(a, own_rows, sequence, s.first),
+                            place * a.group + within, s.tokens);
                 sees = seen_of(s.length, left, 0, s.keys) > 0;
             }
             if (a.batch.prefix > 0) {
-                const uint32_t row_blocks =
-                    static_cast<uint32_t>((uint64_t{a.batch.tokens} * a.group + prefix_rows - 1) / prefix_rows);
-                shared = find(prefix, prefix_rows, 0, uint64_t{token} * a.group + within, row_blocks);
+                shared = find(prefix, prefix_rows, prefix_workers, 0, token * a.group + within, a.batch.tokens);
                 sees = sees || seen_of(s.length, left, a.batch.prefix, a.batch.prefix) > 0;
             }
         }
         const uint32_t count = mine.n + shared.n;
         // A whole item without a prefix is a result already.
-        if (count == 1 && mine.n == 1 && mine.whole && a.batch.prefix == 0) continue;
+        if (count == 1 && mine.whole && a.batch.prefix == 0) continue;
 
-        const auto place_of = [&](uint32_t n, const float** values, const float2** stats) {
-            const bool is_mine = n < mine.n;
+        const uint32_t half = threadIdx.x % 64 / 32, column = threadIdx.x % 32 * 4;
+        float top = -INFINITY, total = 0.0f;
+        f32x4 sum = {};
+#pragma unroll 4
+        for (uint32_t i = half; i < count; i += 2) {
+            const bool is_mine = i < mine.n;
             const Found& f = is_mine ? mine : shared;
             const Parts& parts = is_mine ? own : prefix;
-            n = is_mine ? n : n - mine.n;
-            const uint64_t at = f.whole ? row : (n == 0 ? f.first_slot : uint64_t{2} * (f.first_block + n)) * f.line + f.within;
-            *values = (f.whole ? parts.rows : parts.slots) + at * SIZE;
-            *stats = (f.whole ? parts.row_stats : parts.slot_stats) + at;
-        };
-        const float* values;
-        const float2* stats;
-        float top = -INFINITY;
-        for (uint32_t n = threadIdx.x % 64; n < count; n += 64) {
-            place_of(n, &values, &stats);
-            top = fmaxf(top, stats->x);
+            const uint32_t n = is_mine ? i : i - mine.n;
+            const uint64_t slot = n == 0 ? f.first_slot : uint64_t{2} * (f.first_worker + n);
+            const uint64_t place = f.whole ? row : slot * f.line + f.within;
+            const float2 stats = (f.whole ? parts.row_stats : parts.slot_stats)[place];
+            f32x4 values = {};
+            if (column < SIZE) values = *reinterpret_cast<const f32x4*>((f.whole ? parts.rows : parts.slots) + place * SIZE + column);
+            const float higher = fmaxf(top, stats.x), origin = higher == -INFINITY ? 0.0f : higher;
+            const float kept = power2(top - origin), added = power2(stats.x - origin);
+            total = fmaf(total, kept, stats.y * added);
+            sum = sum * kept + values * added;
+            top = higher;
         }
-        top = wave64<Largest>(top);
-        const float origin = top == -INFINITY ? 0.0f : top;
-        const uint32_t group = threadIdx.x / 32, column = threadIdx.x % 32 * 4;
-        f32x4 sum = {};
-        float total = 0.0f;
-        for (uint32_t n = group; n < count; n += kGroups) {
-            place_of(n, &values, &stats);
-            const float factor = power2(stats->x - origin);
-            total += factor * stats->y;
-            if (column < SIZE) sum += factor * *reinterpret_cast<const f32x4*>(values + column);
-        }
-        sums[group][threadIdx.x % 32] = sum;
-        if (threadIdx.x % 32 == 0) totals[group] = total;
-        __syncthreads();
-        if (threadIdx.x < 32) {
-            for (int g = 1; g < kGroups; g++) {
-                sum += sums[g][threadIdx.x];
-                total += totals[g];
-            }
-            S* const to = static_cast<S*>(a.out) + token * a.out_steps.token + head * a.out_steps.head;
-            const float scale = sees ? 1.0f / total : 0.0f;
+        const float higher = fmaxf(top, __shfl_xor(top, 32)), origin = higher == -INFINITY ? 0.0f : higher;
+        const float kept = power2(top - origin);
+        total *= kept;
+        total += __shfl_xor(total, 32);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (column + j < a.pool.size) to[column + j] = Elem<S>::narrow(sees ? sum[j] * scale : 0.0f);
-            }
-            if (threadIdx.x == 0 && a.normalizers != nullptr) {
+        for (int j = 0; j < 4; j++) {
+            sum[j] *= kept;
+            sum[j] += __shfl_xor(sum[j], 32);
+        }
+        if (half == 0) {
+            S* const to = static_cast<S*>(a.out) + token * a.out_steps.token + head * a.out_steps.head;
+            const float scale = 1.0f / total;
+            store_four(to, column, a.pool.size, sees ? sum * scale : f32x4{});
+            if (threadIdx.x % 32 == 0 && a.normalizers != nullptr) {
                 a.normalizers[uint64_t{head} * a.batch.tokens + token] =
-                    total == 0.0f ? -INFINITY : (top + log2f(total) - (half_power ? 6.0f : 0.0f)) * attention::kLn2;
+                    total == 0.0f ? -INFINITY : (higher + log2f(total) - power) * attention::kLn2;
             }
         }
-        __syncthreads();
     }
 }
 
@@ -816,38 +888,50 @@ __global__ void __launch_bounds__(kAttendThreads)
         constexpr int SIZE = 128; __VA_ARGS__;          \
     }
 
-template <int SIZE, int RB, bool QUANT>
-void attend_rows(const Attention& a, const Parts& parts, bool prefix, bool final, uint32_t blocks, hipStream_t s) {
+template <int SIZE, int FORM, bool QUANT>
+void attend_form(const Attention& a, const Parts& parts, bool prefix, bool final, uint32_t blocks, hipStream_t s) {
     if (prefix) {
-        attend_kernel<SIZE, RB, QUANT, true><<<blocks, kAttendThreads, 0, s>>>(a, parts, false);
+        attend_kernel<SIZE, FORM, QUANT, true><<<blocks, kAttendThreads, 0, s>>>(a, parts, false);
     } else {
-        attend_kernel<SIZE, RB, QUANT, false><<<blocks, kAttendThreads, 0, s>>>(a, parts, final);
+        attend_kernel<SIZE, FORM, QUANT, false><<<blocks, kAttendThreads, 0, s>>>(a, parts, final);
     }
 }
 
-int attend(const Attention& a, const Parts& parts, bool quant, bool prefix, bool final, int row_blocks,
-           uint32_t blocks) {
+template <int SIZE, bool QUANT>
+void attend_size(const Attention& a, const Parts& parts, bool prefix, bool final, int form, uint32_t blocks,
+                 hipStream_t s) {
+    if (form == kRows16) {
+        attend_form<SIZE, kRows16, QUANT>(a, parts, prefix, final, blocks, s);
+    } else if (form == kRows32) {
+        attend_form<SIZE, kRows32, QUANT>(a, parts, prefix, final, blocks, s);
+    } else {
+        attend_form<SIZE, kRows128, QUANT>(a, parts, prefix, final, blocks, s);
+    }
+}
+
+int attend(const Attention& a, const Parts& parts, bool quant, bool prefix, bool final, int form, uint32_t blocks) {
     TC_STREAM(s);
     TC_CACHE_SIZE(a.pool.size, {
         if (quant) {
-            if (row_blocks == 1) attend_rows<SIZE, 1, true>(a, parts, prefix, final, blocks, s);
-            else attend_rows<SIZE, 2, true>(a, parts, prefix, final, blocks, s);
+            attend_size<SIZE, true>(a, parts, prefix, final, form, blocks, s);
         } else {
-            if (row_blocks == 1) attend_rows<SIZE, 1, false>(a, parts, prefix, final, blocks, s);
-            else attend_rows<SIZE, 2, false>(a, parts, prefix, final, blocks, s);
+            attend_size<SIZE, false>(a, parts, prefix, final, form, blocks, s);
         }
     })
     return check_launch("cache attention");
 }
 
-int join(const Attention& a, const Parts& own, const Parts& prefix, bool quant, int own_row_blocks,
-         int prefix_row_blocks, uint32_t blocks) {
+int join(const Attention& a, const Parts& own, const Parts& prefix, bool quant, int own_form, int prefix_form,
+         uint32_t blocks) {
     TC_STREAM(s);
     const uint64_t rows = uint64_t{a.batch.tokens} * a.query_heads;
-    const uint32_t grid = rows < (1u << 20) ? static_cast<uint32_t>(rows) : 1u << 20;
+    const uint64_t turns = (rows + kAttendWaves - 1) / kAttendWaves;
+    const uint32_t grid = turns < (1u << 20) ? static_cast<uint32_t>(turns) : 1u << 20;
+    const float power = sizeof(S) == 2 && (quant || kHalf) ? kHalfPower : 0.0f;
     TC_CACHE_SIZE(a.pool.size, {
-        join_kernel<SIZE><<<grid, kAttendThreads, 0, s>>>(a, own, prefix, 16 * own_row_blocks, 16 * prefix_row_blocks,
-                                                          blocks, kHalf && !quant);
+        join_kernel<SIZE><<<grid, kAttendThreads, 0, s>>>(a, own, prefix, rows_of_form(own_form),
+                                                          rows_of_form(prefix_form), workers_of(own_form, blocks),
+                                                          workers_of(prefix_form, blocks), power);
     })
     return check_launch("cache attention");
 }
