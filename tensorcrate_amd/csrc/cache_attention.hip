@@ -11,23 +11,24 @@ int form_of(uint64_t rows) { return rows <= 16 ? kRows16 : rows <= 32 ? kRows32 
 
 // The storage of one line's parts.
 struct Storage {
-    Scratch slots, slot_stats, rows, row_stats, plans;
+    Scratch slots, slot_stats, rows, row_stats, plans, cut;
 
     Storage(uint64_t slot_rows, uint64_t whole_rows, uint64_t items, uint64_t size)
         : slots(slot_rows * size * sizeof(float)),
           slot_stats(slot_rows * sizeof(float2)),
           rows(whole_rows * size * sizeof(float)),
           row_stats(whole_rows * sizeof(float2)),
-          plans(items * sizeof(Plan)) {}
+          plans(items * sizeof(Plan)),
+          cut(sizeof(uint32_t)) {}
     int status() const {
-        for (int s : {slots.status, slot_stats.status, rows.status, row_stats.status, plans.status}) {
+        for (int s : {slots.status, slot_stats.status, rows.status, row_stats.status, plans.status, cut.status}) {
             if (s != TC_OK) return s;
         }
         return TC_OK;
     }
     Parts parts() const {
         return {static_cast<float*>(slots.ptr), static_cast<float2*>(slot_stats.ptr), static_cast<float*>(rows.ptr),
-                static_cast<float2*>(row_stats.ptr), static_cast<Plan*>(plans.ptr)};
+                static_cast<float2*>(row_stats.ptr), static_cast<Plan*>(plans.ptr), static_cast<uint32_t*>(cut.ptr)};
     }
 };
 
@@ -45,8 +46,12 @@ int run(const AttentionLaunches& launches, const Attention& a, bool quant) {
                          prefix ? (tokens * a.group / prefix_rows + 1) * a.pool.heads : 0, size);
     if (own.status() != TC_OK) return own.status();
     if (shared.status() != TC_OK) return shared.status();
+    // (The first launch tells the second whether any token does not see the
+    // whole prefix.)
+    Parts prefix_parts = shared.parts();
+    prefix_parts.cut = own.parts().cut;
     int status = launches.attend(a, own.parts(), quant, false, !prefix, own_form, blocks);
-    if (status == TC_OK && prefix) status = launches.attend(a, shared.parts(), quant, true, false, prefix_form, blocks);
+    if (status == TC_OK && prefix) status = launches.attend(a, prefix_parts, quant, true, false, prefix_form, blocks);
     if (status != TC_OK) return status;
     return launches.join(a, own.parts(), shared.parts(), quant, own_form, prefix_form, blocks);
 }

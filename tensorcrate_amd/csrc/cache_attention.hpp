@@ -76,6 +76,7 @@ struct Parts {
     float* rows;          // [token][query head][size], of whole items
     float2* row_stats;
     Plan* plans;
+    uint32_t* cut;  // whether any token comes before its sequence's first
 };
 
 // The launches of one element type; `blocks` of the first kernel.
@@ -235,6 +236,15 @@ __device__ __forceinline__ uint32_t picked(uint32_t bits, int pick) {
     return taken(bits & 0xffffu) | taken(bits >> 16) << 16;
 }
 
+// body(0), body(1), ... body(N - 1), each a constant.
+template <int N, typename F>
+__device__ __forceinline__ void each(F&& body) {
+    if constexpr (N > 0) {
+        each<N - 1>(body);
+        body(std::integral_constant<int, N - 1>());
+    }
+}
+
 // Order within a wave's own LDS is the program's; the compiler is told here.
 __device__ __forceinline__ void wave_order() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -321,6 +331,8 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
     constexpr int kRowWords = SIZE * kEntry / 16;
     constexpr int kEach = (kKeys * kRowWords + kMovers - 1) / kMovers;
     constexpr int kStages = SHARED ? 2 : kAttendWaves;
+    // Tiles in flight, of 8 kEach registers each.
+    constexpr int kAhead = (SHARED ? 4 : 8) / kEach < 1 ? 1 : (SHARED ? 4 : 8) / kEach > 4 ? 4 : (SHARED ? 4 : 8) / kEach;
 
     __shared__ __attribute__((aligned(1024))) char tiles[kStages][2 * TileOf::kBytes];
     __shared__ __attribute__((aligned(16))) float scales[QUANT ? kStages : 1][64];
@@ -331,16 +343,31 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
     // ---- this worker's tiles -----------------------------------------------------
     const uint32_t sequences = PREFIX ? 1 : a.batch.sequences;
     uint64_t total_tiles = 0;
+    [[maybe_unused]] uint64_t count_here = 0, upto_here = 0;  // of this thread's sequence, and with those before
     if constexpr (PREFIX) {
         total_tiles = LineOf::count(a, sequence_at<true>(a, 0));
     } else {
+        // (With up to kAttendThreads sequences each thread keeps its one's.)
         uint64_t mine = 0;
-        for (uint32_t n = threadIdx.x; n < sequences; n += kAttendThreads) mine += LineOf::count(a, sequence_at<false>(a, n));
-        for (int offset = 32; offset > 0; offset >>= 1) mine += __shfl_xor(static_cast<unsigned long long>(mine), offset);
-        if (lane == 0) sums[wave] = mine;
-        __syncthreads();
-        for (int w = 0; w < kAttendWaves; w++) total_tiles += sums[w];
-        __syncthreads();
+        bool cut = false;
+        for (uint32_t n = threadIdx.x; n < sequences; n += kAttendThreads) {
+            const Sequence s = sequence_at<false>(a, n);
+            count_here = LineOf::count(a, s);
+            cut = cut || s.length < s.tokens;
+            mine += count_here;
+        }
+        upto_here = mine;
+        for (int offset = 1; offset < 64; offset *= 2) {
+            const uint64_t other = __shfl_up(static_cast<unsigned long long>(upto_here), offset);
+            if (lane >= offset) upto_here += other;
+        }
+        if (lane == 63) sums[wave] = upto_here;
+        cut = __syncthreads_or(cut);
+        for (int w = 0; w < kAttendWaves; w++) {
+            if (w < wave) upto_here += sums[w];
+            total_tiles += sums[w];
+        }
+        if (blockIdx.x == 0 && threadIdx.x == 0) *parts.cut = cut;
     }
     // No worker has nothing, so that every one between two parts of an item has
     // a part of it.
@@ -360,7 +387,15 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             // (Of a worker past the last one: the last one's.)
             begins[w] = begin_of(first_worker + w < workers ? first_worker + w : workers - 1);
         }
-        for (uint32_t from = 0; from < sequences; from += kAttendThreads) {
+        const auto find = [&](uint32_t n, uint64_t start, uint64_t count) {
+#pragma unroll
+            for (int w = 0; w < kWorkers; w++) {
+                if (begins[w] >= start && begins[w] - start < count) found[w][0] = n, found[w][1] = start;
+            }
+        };
+        if (sequences <= kAttendThreads) find(threadIdx.x, upto_here - count_here, count_here);
+        __syncthreads();
+        for (uint32_t from = 0; sequences > kAttendThreads && from < sequences; from += kAttendThreads) {
             const uint32_t n = from + threadIdx.x;
             const uint64_t count = n < sequences ? LineOf::count(a, sequence_at<false>(a, n)) : 0;
             uint64_t upto = count;
@@ -375,11 +410,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                 if (w < wave) upto += sums[w];
                 all += sums[w];
             }
-            const uint64_t start = before + upto - count;
-#pragma unroll
-            for (int w = 0; w < kWorkers; w++) {
-                if (begins[w] >= start && begins[w] - start < count) found[w][0] = n, found[w][1] = start;
-            }
+            find(n, before + upto - count, count);
             __syncthreads();
             if (begins[kWorkers - 1] - before < all) break;  // the same for the whole block
             before += all;
@@ -387,6 +418,8 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
         sequence = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(found[SHARED ? 0 : wave][0]));
         before = found[SHARED ? 0 : wave][1];
     }
+    [[maybe_unused]] bool cut = false;
+    if constexpr (PREFIX) cut = __builtin_amdgcn_readfirstlane(*parts.cut) != 0;
     if (worker >= workers) return;  // (a wave by itself: no barrier follows)
     const uint64_t begin = begin_of(worker), end = begin_of(worker + uint64_t{1});
 
@@ -435,7 +468,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             if (real) {
                 if constexpr (PREFIX) {
                     Span span;
-                    const uint32_t own = sequence_of(a.batch, token, &span);
+                    const uint32_t own = cut ? sequence_of(a.batch, token, &span) : kNowhere;
                     if (own != kNowhere) seen[r] = seen_of(a.batch.lengths[own], span.end - token, s.keys, s.keys);
                 } else {
                     seen[r] = seen_of(s.length, s.tokens - place, 0, s.keys);
@@ -492,8 +525,8 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
 
         const uint32_t key_end = uint64_t{tile_1} * kKeys < most_seen ? tile_1 * kKeys : most_seen;
         uint32_t tile = 0;
-        uint4 key_words[kEach], value_words[kEach];
-        float entry_scale = 0.0f;
+        uint4 key_words[kAhead][kEach], value_words[kAhead][kEach];
+        float entry_scale[kAhead];
         // The page of key l % 32 of the tile at `first`, and its row there.
         const auto page_at = [&](uint32_t first) {
             const uint32_t key = first + lane % 32;
@@ -505,25 +538,27 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             const uint32_t within = key - a.pool.pages_of.div(key) * a.pool.page_size;
             return page < a.pool.page_count ? (page * a.pool.heads + key_head) * a.pool.page_size + within : kNowhere;
         };
-        const auto fetch = [&](uint32_t row) {
+        const auto fetch = [&](auto set, uint32_t row) {
+            constexpr int d = decltype(set)::value;
             const uint32_t row_bytes = a.pool.row * kEntry;
 #pragma unroll
             for (int k = 0; k < kEach; k++) {
                 const int i = k * kMovers + (SHARED ? threadIdx.x : lane);
                 const uint32_t from = __shfl(row, i / kRowWords < kKeys ? i / kRowWords : 0);
                 const uint32_t byte = i % kRowWords * 16;
-                key_words[k] = value_words[k] = make_uint4(0, 0, 0, 0);
+                key_words[d][k] = value_words[d][k] = make_uint4(0, 0, 0, 0);
                 if (i < kKeys * kRowWords && from != kNowhere && byte < row_bytes) {
                     const uint64_t place = uint64_t{from} * row_bytes + byte;
-                    key_words[k] = load_word<false>(static_cast<const char*>(a.pool.keys) + place);
-                    value_words[k] = load_word<false>(static_cast<const char*>(a.pool.values) + place);
+                    key_words[d][k] = load_word<false>(static_cast<const char*>(a.pool.keys) + place);
+                    value_words[d][k] = load_word<false>(static_cast<const char*>(a.pool.values) + place);
                 }
             }
             if constexpr (QUANT) {
-                entry_scale = row == kNowhere ? 0.0f : (lane < 32 ? a.pool.key_scales : a.pool.value_scales)[row];
+                entry_scale[d] = row == kNowhere ? 0.0f : (lane < 32 ? a.pool.key_scales : a.pool.value_scales)[row];
             }
         };
-        const auto land = [&](const TileOf& key_tile, const TileOf& value_tile) {
+        const auto land = [&](auto set, const TileOf& key_tile, const TileOf& value_tile) {
+            constexpr int d = decltype(set)::value;
 #pragma unroll
             for (int k = 0; k < kEach; k++) {
                 const int i = k * kMovers + (SHARED ? threadIdx.x : lane);
@@ -531,30 +566,32 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                 const int row = i / kRowWords, word = i % kRowWords;
                 if constexpr (QUANT) {
                     Words<M, 16> keys, values;
-                    widened(key_words[k], keys);
-                    widened(value_words[k], values);
+                    widened(key_words[d][k], keys);
+                    widened(value_words[d][k], values);
 #pragma unroll
                     for (int w = 0; w < 16 / E; w++) {
                         *reinterpret_cast<uint4*>(key_tile.word(row, word * (16 / E) + w)) = keys.w[w];
                         *reinterpret_cast<uint4*>(value_tile.word(row, word * (16 / E) + w)) = values.w[w];
                     }
                 } else {
-                    *reinterpret_cast<uint4*>(key_tile.word(row, word)) = key_words[k];
-                    *reinterpret_cast<uint4*>(value_tile.word(row, word)) = value_words[k];
+                    *reinterpret_cast<uint4*>(key_tile.word(row, word)) = key_words[d][k];
+                    *reinterpret_cast<uint4*>(value_tile.word(row, word)) = value_words[d][k];
                 }
             }
             if constexpr (QUANT) {
-                if (!SHARED || wave == 0) scales[stage][lane] = entry_scale;
+                if (!SHARED || wave == 0) scales[stage][lane] = entry_scale[d];
             }
         };
-        uint32_t next_page = kNowhere;
+        uint32_t next_page[2];  // of the next tiles to fetch
         [[maybe_unused]] int pick = kFinite;
-        const auto turn = [&](auto is_masked, auto is_slow) {
-            constexpr bool MASKED = decltype(is_masked)::value, SLOW = decltype(is_slow)::value;
+        // The tile that is in `set`; of every `parity`-th page of the two.
+        const auto turn = [&](auto set, auto parity, auto is_slow) {
+            constexpr bool SLOW = decltype(is_slow)::value;
+            const bool masked = tile + kKeys > least || tile + kKeys > key_end;
             const TileOf key_tile{tiles[stage]};
             const TileOf value_tile{tiles[stage] + TileOf::kBytes};
             if constexpr (kScaled) {
-                const float high = wave64<Largest>(lane < 32 ? 0.0f : entry_scale);
+                const float high = wave64<Largest>(lane < 32 ? 0.0f : entry_scale[decltype(set)::value]);
                 if (high >= unit && high < INFINITY) {
                     const float grown = ldexpf(1.0f, ilogbf(high) + 3);
                     const float factor = unit / grown;
@@ -569,13 +606,13 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             // A stage that a block shares was read before the last barrier; a
             // wave's own is in the order of the program.
             if constexpr (!SHARED) wave_order();
-            land(key_tile, value_tile);
+            land(set, key_tile, value_tile);
             if constexpr (SHARED) __syncthreads();
             else wave_order();
-            const uint32_t next = tile + kKeys;
+            const uint32_t next = tile + kAhead * kKeys;
             if (next < key_end) {
-                fetch(row_at(next, next_page));
-                next_page = page_at(next + kKeys);
+                fetch(set, row_at(next, next_page[decltype(parity)::value]));
+                next_page[decltype(parity)::value] = page_at(next + 2 * kKeys);
             }
             // Scores, and their maximum over the tile.
             f32x4 scores[RB][kBlocks16];
@@ -603,7 +640,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             }
 #pragma unroll
             for (int r = 0; r < RB; r++) {
-                if constexpr (MASKED) {
+                if (masked) {
 #pragma unroll
                     for (int b = 0; b < kBlocks16; b++) {
 #pragma unroll
@@ -641,9 +678,13 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                         const f32x4 scale = *reinterpret_cast<const f32x4*>(&scales[stage][32 + 16 * b + 4 * quarter]);
                         const float against = kScaled ? 1.0f / unit : 1.0f;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const bool out_of = MASKED && tile + 16 * b + 4 * quarter + i >= seen[r];
-                            scores[r][b][i] = out_of ? 0.0f : scores[r][b][i] * (scale[i] * against);
+                        for (int i = 0; i < 4; i++) scores[r][b][i] *= scale[i] * against;
+                        if (masked) {
+                            // (A scale may be a NaN.)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                if (tile + 16 * b + 4 * quarter + i >= seen[r]) scores[r][b][i] = 0.0f;
+                            }
                         }
                     }
                 }
@@ -684,7 +725,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                     if constexpr (kTwoParts) acc[r][t] = product16<M>(values, low_part[r], acc[r][t]);
                 }
             }
-            tile = next;
+            tile += kKeys;
             if constexpr (SHARED) stage ^= 1;
         };
         const auto sweep = [&](auto is_slow) {
@@ -695,15 +736,20 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                 for (int t = 0; t < SIZE / 16; t++) acc[r][t] = f32x4{};
             }
             tile = tile_0 * kKeys;
-            if (tile >= key_end) return;
-            fetch(row_at(tile, page_at(tile)));
-            next_page = page_at(tile + kKeys);
             // (Keys past `key_end` are seen by no row, or by none that is real.)
-            const uint32_t plain_end = least < key_end ? least : key_end;
-            if constexpr (!decltype(is_slow)::value) {
-                while (tile < plain_end && plain_end - tile >= kKeys) turn(std::false_type(), is_slow);
+            uint32_t pages[kAhead];
+            each<kAhead>([&](auto n) { pages[n.value] = page_at(tile + n.value * kKeys); });
+            next_page[0] = page_at(tile + kAhead * kKeys);
+            next_page[1] = page_at(tile + (kAhead + 1) * kKeys);
+            each<kAhead>([&](auto n) { fetch(n, row_at(tile + n.value * kKeys, pages[n.value])); });
+            while (tile < key_end) {
+                each<(kAhead > 2 ? kAhead : 2)>([&](auto n) {
+                    constexpr int set = n.value % kAhead, parity = n.value % 2;
+                    if (n.value == 0 || tile < key_end) {
+                        turn(std::integral_constant<int, set>(), std::integral_constant<int, parity>(), is_slow);
+                    }
+                });
             }
-            while (tile < key_end) turn(std::true_type(), is_slow);
         };
         sweep(std::false_type());
         if constexpr (!QUANT) {
@@ -787,14 +833,18 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
     }
 }
 
-// Each row's parts joined, a wave a row: the row's own sequence's and the
-// prefix's, in the order of their workers, two at a time.
-template <int SIZE>
+// Each row's parts joined, by WAVES waves: the row's own sequence's and the
+// prefix's, in the order of their workers, two a wave at a time.
+template <int SIZE, int WAVES>
 __global__ void __launch_bounds__(kAttendThreads)
     join_kernel(const Attention a, const Parts own, const Parts prefix, uint32_t own_rows, uint32_t prefix_rows,
                 uint32_t own_workers, uint32_t prefix_workers, float power) {
-    const uint64_t apart = uint64_t{gridDim.x} * kAttendWaves, all_rows = uint64_t{a.batch.tokens} * a.query_heads;
-    for (uint64_t at = uint64_t{blockIdx.x} * kAttendWaves + threadIdx.x / 64; at < all_rows; at += apart) {
+    constexpr int kRows = kAttendWaves / WAVES;  // of a block
+    __shared__ f32x4 sums[WAVES > 1 ? WAVES : 1][32];
+    __shared__ float2 stats_of[WAVES > 1 ? WAVES : 1];
+    const int wave = threadIdx.x / 64 % WAVES;
+    const uint64_t apart = uint64_t{gridDim.x} * kRows, all_rows = uint64_t{a.batch.tokens} * a.query_heads;
+    for (uint64_t at = uint64_t{blockIdx.x} * kRows + threadIdx.x / 64 / WAVES; at < all_rows; at += apart) {
         const uint32_t row = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at));
         const uint32_t token = row / a.query_heads, head = row % a.query_heads;
         const uint32_t key_head = a.group_of.div(head), within = head - key_head * a.group;
@@ -839,25 +889,40 @@ __global__ void __launch_bounds__(kAttendThreads)
         const uint32_t half = threadIdx.x % 64 / 32, column = threadIdx.x % 32 * 4;
         float top = -INFINITY, total = 0.0f;
         f32x4 sum = {};
-#pragma unroll 4
-        for (uint32_t i = half; i < count; i += 2) {
-            const bool is_mine = i < mine.n;
-            const Found& f = is_mine ? mine : shared;
-            const Parts& parts = is_mine ? own : prefix;
-            const uint32_t n = is_mine ? i : i - mine.n;
-            const uint64_t slot = n == 0 ? f.first_slot : uint64_t{2} * (f.first_worker + n);
-            const uint64_t place = f.whole ? row : slot * f.line + f.within;
-            const float2 stats = (f.whole ? parts.row_stats : parts.slot_stats)[place];
-            f32x4 values = {};
-            if (column < SIZE) values = *reinterpret_cast<const f32x4*>((f.whole ? parts.rows : parts.slots) + place * SIZE + column);
-            const float higher = fmaxf(top, stats.x), origin = higher == -INFINITY ? 0.0f : higher;
-            const float kept = power2(top - origin), added = power2(stats.x - origin);
-            total = fmaf(total, kept, stats.y * added);
-            sum = sum * kept + values * added;
-            top = higher;
+        // Four parts in flight: their loads, then their sums.
+        constexpr int kParts = 4;
+        for (uint32_t first = 2 * wave + half; first < count; first += kParts * 2 * WAVES) {
+            float2 stats[kParts];
+            f32x4 values[kParts];
+#pragma unroll
+            for (int k = 0; k < kParts; k++) {
+                const uint32_t i = first + k * 2 * WAVES;
+                stats[k] = make_float2(-INFINITY, 0.0f);
+                values[k] = f32x4{};
+                if (i >= count) continue;
+                const bool is_mine = i < mine.n;
+                const Found& f = is_mine ? mine : shared;
+                const Parts& parts = is_mine ? own : prefix;
+                const uint32_t n = is_mine ? i : i - mine.n;
+                const uint64_t slot = n == 0 ? f.first_slot : uint64_t{2} * (f.first_worker + n);
+                const uint64_t place = f.whole ? row : slot * f.line + f.within;
+                stats[k] = (f.whole ? parts.row_stats : parts.slot_stats)[place];
+                if (column < SIZE) {
+                    values[k] =
+                        *reinterpret_cast<const f32x4*>((f.whole ? parts.rows : parts.slots) + place * SIZE + column);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kParts; k++) {
+                const float higher = fmaxf(top, stats[k].x), origin = higher == -INFINITY ? 0.0f : higher;
+                const float kept = power2(top - origin), added = power2(stats[k].x - origin);
+                total = fmaf(total, kept, stats[k].y * added);
+                sum = sum * kept + values[k] * added;
+                top = higher;
+            }
         }
-        const float higher = fmaxf(top, __shfl_xor(top, 32)), origin = higher == -INFINITY ? 0.0f : higher;
-        const float kept = power2(top - origin);
+        float higher = fmaxf(top, __shfl_xor(top, 32));
+        const float kept = power2(top - (higher == -INFINITY ? 0.0f : higher));
         total *= kept;
         total += __shfl_xor(total, 32);
 #pragma unroll
@@ -865,7 +930,20 @@ __global__ void __launch_bounds__(kAttendThreads)
             sum[j] *= kept;
             sum[j] += __shfl_xor(sum[j], 32);
         }
-        if (half == 0) {
+        if constexpr (WAVES > 1) {
+            if (half == 0) sums[wave][threadIdx.x % 32] = sum;
+            if (threadIdx.x % 64 == 0) stats_of[wave] = make_float2(higher, total);
+            __syncthreads();
+            higher = -INFINITY, total = 0.0f, sum = f32x4{};
+            for (int w = 0; w < WAVES; w++) higher = fmaxf(higher, stats_of[w].x);
+            for (int w = 0; w < WAVES; w++) {
+                const float factor = power2(stats_of[w].x - (higher == -INFINITY ? 0.0f : higher));
+                total += stats_of[w].y * factor;
+                sum += sums[w][threadIdx.x % 32] * factor;
+            }
+            __syncthreads();
+        }
+        if (half == 0 && wave == 0) {
             S* const to = static_cast<S*>(a.out) + token * a.out_steps.token + head * a.out_steps.head;
             const float scale = 1.0f / total;
             store_four(to, column, a.pool.size, sees ? sum * scale : f32x4{});
@@ -925,13 +1003,15 @@ int join(const Attention& a, const Parts& own, const Parts& prefix, bool quant, 
          uint32_t blocks) {
     TC_STREAM(s);
     const uint64_t rows = uint64_t{a.batch.tokens} * a.query_heads;
-    const uint64_t turns = (rows + kAttendWaves - 1) / kAttendWaves;
+    // A block a row where rows are few and their parts, therefore, many.
+    const bool few = rows <= static_cast<uint64_t>(compute_units()) * 4;
+    const uint64_t turns = few ? rows : (rows + kAttendWaves - 1) / kAttendWaves;
     const uint32_t grid = turns < (1u << 20) ? static_cast<uint32_t>(turns) : 1u << 20;
     const float power = sizeof(S) == 2 && (quant || kHalf) ? kHalfPower : 0.0f;
     TC_CACHE_SIZE(a.pool.size, {
-        join_kernel<SIZE><<<grid, kAttendThreads, 0, s>>>(a, own, prefix, rows_of_form(own_form),
-                                                          rows_of_form(prefix_form), workers_of(own_form, blocks),
-                                                          workers_of(prefix_form, blocks), power);
+        const auto kernel = few ? join_kernel<SIZE, kAttendWaves> : join_kernel<SIZE, 1>;
+        kernel<<<grid, kAttendThreads, 0, s>>>(a, own, prefix, rows_of_form(own_form), rows_of_form(prefix_form),
+                                               workers_of(own_form, blocks), workers_of(prefix_form, blocks), power);
     })
     return check_launch("cache attention");
 }
