@@ -123,8 +123,10 @@ using attention::u32x2;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kKeys = kWide ? 16 : 32;  // rows of a tile
-constexpr int kBlocks16 = kKeys / 16;
+// Rows of a tile: what one product of weights with values sums over, or twice
+// that where a block shares it.
+constexpr int kDeepKeys = kWide ? 16 : 32;
+constexpr int keys_of_form(int form) { return form == kRows128 ? 2 * kDeepKeys : kDeepKeys; }
 // Elements of the summed axis that one operand word of all quarters covers.
 constexpr int kDeep16 = 4 * E;
 
@@ -159,10 +161,10 @@ __device__ __forceinline__ float quarters(float v) {
     return Op::join(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
 }
 
-// A tile of kKeys rows, read 16 rows at a time.
-template <int SIZE>
-struct KeyTile : attention::Tile<SIZE, kKeys> {
-    using Base = attention::Tile<SIZE, kKeys>;
+// A tile of KEYS rows, read 16 rows at a time.
+template <int SIZE, int KEYS>
+struct KeyTile : attention::Tile<SIZE, KEYS> {
+    using Base = attention::Tile<SIZE, KEYS>;
     // A lane's places for `by_row` and `by_column`.
     __device__ __forceinline__ static uint32_t row_place(int lane) { return Base::place(lane % 16, lane / 16); }
     __device__ __forceinline__ static uint32_t column_place(int lane) {
@@ -175,17 +177,17 @@ struct KeyTile : attention::Tile<SIZE, kKeys> {
     __device__ __forceinline__ uint4 by_row(uint32_t place, int b, int n) const {
         return *reinterpret_cast<const uint4*>(this->from(place, 16 * b, 4 * n));
     }
-    // Operand word of column 16 t + l % 16, summed over the rows in the order
-    // of products' results.
-    __device__ __forceinline__ uint4 by_column(uint32_t place, int t) const {
+    // Operand word of column 16 t + l % 16, summed over the kDeepKeys rows from
+    // `rows` on in the order of products' results.
+    __device__ __forceinline__ uint4 by_column(uint32_t place, int rows, int t) const {
         if constexpr (kWide) {
             uint32_t v[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = *reinterpret_cast<const uint32_t*>(this->from(place, j, 4 * t));
+            for (int j = 0; j < 4; j++) v[j] = *reinterpret_cast<const uint32_t*>(this->from(place, rows + j, 4 * t));
             return make_uint4(v[0], v[1], v[2], v[3]);
         } else {
-            const u32x2 a = __builtin_bit_cast(u32x2, Base::transposed(this->from(place, 0, 2 * t)));
-            const u32x2 b = __builtin_bit_cast(u32x2, Base::transposed(this->from(place, 16, 2 * t)));
+            const u32x2 a = __builtin_bit_cast(u32x2, Base::transposed(this->from(place, rows, 2 * t)));
+            const u32x2 b = __builtin_bit_cast(u32x2, Base::transposed(this->from(place, rows + 16, 2 * t)));
             return make_uint4(a.x, a.y, b.x, b.y);
         }
     }
@@ -277,10 +279,10 @@ __device__ __forceinline__ Sequence sequence_at(const Attention& a, uint32_t seq
 }
 
 // The tiles of all items one behind another: sequences, of each the key heads,
-// of each the blocks of ROWS query rows, of each the tiles of kKeys keys.
-template <int ROWS>
+// of each the blocks of ROWS query rows, of each the tiles of KEYS keys.
+template <int ROWS, int KEYS>
 struct Line {
-    __device__ __forceinline__ static uint32_t tiles(const Sequence& s) { return (s.keys + kKeys - 1) / kKeys; }
+    __device__ __forceinline__ static uint32_t tiles(const Sequence& s) { return (s.keys + KEYS - 1) / KEYS; }
     __device__ __forceinline__ static uint32_t blocks(const Attention& a, const Sequence& s) {
         return static_cast<uint32_t>((uint64_t{s.tokens} * a.group + ROWS - 1) / ROWS);
     }
@@ -319,23 +321,32 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
     constexpr int ROWS = rows_of_form(FORM);
     constexpr int kWorkers = SHARED ? 1 : kAttendWaves;  // of a block
     constexpr int kMovers = SHARED ? kAttendThreads : 64;  // threads that move a tile
-    using LineOf = Line<ROWS>;
-    using TileOf = KeyTile<SIZE>;
+    constexpr int kKeys = keys_of_form(FORM), kBlocks16 = kKeys / 16, kDeeps = kKeys / kDeepKeys;
+    using LineOf = Line<ROWS, kKeys>;
+    using TileOf = KeyTile<SIZE, kKeys>;
     // The type that is multiplied in.
     constexpr bool kScaled = QUANT && sizeof(S) == 2;
     using M = std::conditional_t<kScaled, _Float16, S>;
-    constexpr bool kTwoParts = sizeof(M) == 2;
+    constexpr bool kTwoParts = sizeof(M) == 2 && Elem<M>::dtype == TC_BF16;
     constexpr float kPower = sizeof(M) == 2 && Elem<M>::dtype == TC_F16 ? kHalfPower : 0.0f;
     constexpr int kOperands = SIZE / kDeep16;
     constexpr int kEntry = QUANT ? 1 : static_cast<int>(sizeof(S));
     constexpr int kRowWords = SIZE * kEntry / 16;
     constexpr int kEach = (kKeys * kRowWords + kMovers - 1) / kMovers;
+    // Words of a tile's row.  Of the two (or four) that a word of 8-bit entries
+    // becomes, each goes to its own part of the row: neighbouring lanes then
+    // write neighbouring words.
+    constexpr int kSpread = QUANT ? 16 / E : 1;
+    const auto element_of = [](int column) {  // that is at this column of a tile, for runs of E
+        const int word = column / E;
+        return (word % kRowWords * kSpread + word / kRowWords) * E + column % E;
+    };
     constexpr int kStages = SHARED ? 2 : kAttendWaves;
     // Tiles in flight, of 8 kEach registers each.
     constexpr int kAhead = (SHARED ? 4 : 8) / kEach < 1 ? 1 : (SHARED ? 4 : 8) / kEach > 4 ? 4 : (SHARED ? 4 : 8) / kEach;
 
     __shared__ __attribute__((aligned(1024))) char tiles[kStages][2 * TileOf::kBytes];
-    __shared__ __attribute__((aligned(16))) float scales[QUANT ? kStages : 1][64];
+    __shared__ __attribute__((aligned(16))) float scales[QUANT ? kStages : 1][kKeys == 64 ? 128 : 64];
     __shared__ uint64_t sums[kAttendWaves], found[kWorkers][2];
 
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, quarter = lane / 16;
@@ -454,7 +465,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
         const uint32_t rows = left_rows < ROWS ? left_rows : ROWS;
         const auto row_of_lane = [&](int r) { return static_cast<uint32_t>((SHARED ? wave * 16 * RB : 0) + r * 16 + lane % 16); };
         uint4 queries[RB][kOperands];
-        [[maybe_unused]] float shrunk[RB];  // what a row of queries was multiplied with, undone
+        float factors[RB];  // of the scores: `c`, and what a row of queries was multiplied with undone
         uint32_t seen[RB];
         bool all_see = true;
 #pragma unroll
@@ -475,14 +486,15 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                 }
             }
             all_see = all_see && seen[r] == s.keys;
+            factors[r] = c;
             const S* from = static_cast<const S*>(a.query) + token * a.query_steps.token + head * a.query_steps.head;
 #pragma unroll
             for (int n = 0; n < kOperands; n++) {
-                queries[r][n] = real ? head_word(from, 4 * n + quarter, a.pool.size) : make_uint4(0, 0, 0, 0);
+                queries[r][n] = real ? head_word(from, element_of((4 * n + quarter) * E) / E, a.pool.size) : make_uint4(0, 0, 0, 0);
             }
             if constexpr (kScaled && !std::is_same_v<S, M>) {
-                // The largest of the row to 2^14 and above, an infinity or a
-                // NaN as it is.
+                // The largest of the row to 2^8 and above, an infinity or a NaN
+                // as it is: what f16 then loses is below 2^-32 of the largest.
                 float most = 0.0f;
 #pragma unroll
                 for (int n = 0; n < kOperands; n++) {
@@ -491,9 +503,9 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                     for (int e = 0; e < E; e++) most = fmaxf(most, fabsf(words.at(e)));
                 }
                 most = quarters<Largest>(most);
-                int power = most > 0.0f && most < INFINITY ? 14 - ilogbf(most) : 0;
+                int power = most > 0.0f && most < INFINITY ? 8 - ilogbf(most) : 0;
                 power = power > 126 ? 126 : power;
-                shrunk[r] = ldexpf(1.0f, -power);
+                factors[r] = ldexpf(c, -power);
                 const float factor = ldexpf(1.0f, power);
 #pragma unroll
                 for (int n = 0; n < kOperands; n++) {
@@ -526,35 +538,68 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
         const uint32_t key_end = uint64_t{tile_1} * kKeys < most_seen ? tile_1 * kKeys : most_seen;
         uint32_t tile = 0;
         uint4 key_words[kAhead][kEach], value_words[kAhead][kEach];
-        float entry_scale[kAhead];
-        // The page of key l % 32 of the tile at `first`, and its row there.
+        // The scales of keys in the lower half of a wave and of values in the
+        // upper, or of 64 keys and of their values.
+        constexpr int kScaleWords = kKeys == 64 ? 2 : 1;
+        float entry_scale[kAhead][kScaleWords];
+        // The page of key l (% 32 where a tile has no more) of the tile at
+        // `first`, and its row there.
+        const uint32_t key_lane = kKeys == 64 ? lane : lane % 32;
         const auto page_at = [&](uint32_t first) {
-            const uint32_t key = first + lane % 32;
+            const uint32_t key = first + key_lane;
             const uint32_t n = a.pool.pages_of.div(key);
-            return lane % 32 < kKeys && key < key_end && n < s.page_count ? s.pages[n] : kNowhere;
+            return key_lane < kKeys && key < key_end && n < s.page_count ? s.pages[n] : kNowhere;
         };
         const auto row_at = [&](uint32_t first, uint32_t page) {
-            const uint32_t key = first + lane % 32;
+            const uint32_t key = first + key_lane;
             const uint32_t within = key - a.pool.pages_of.div(key) * a.pool.page_size;
             return page < a.pool.page_count ? (page * a.pool.heads + key_head) * a.pool.page_size + within : kNowhere;
         };
+        const uint32_t row_bytes = a.pool.row * kEntry;
         const auto fetch = [&](auto set, uint32_t row) {
             constexpr int d = decltype(set)::value;
-            const uint32_t row_bytes = a.pool.row * kEntry;
+            // Where pages hold whole runs of 16 tokens and the tile is full, a
+            // run's first row tells the others': one address of the wave's, and
+            // one number of the lane's.
+            const bool runs = a.pool.page_size % 16 == 0 && row_bytes == kRowWords * 16 && __ballot(row == kNowhere && key_lane < kKeys) == 0;
+            if (runs) {
+                uint64_t at_run[kKeys / 16];
 #pragma unroll
-            for (int k = 0; k < kEach; k++) {
-                const int i = k * kMovers + (SHARED ? threadIdx.x : lane);
-                const uint32_t from = __shfl(row, i / kRowWords < kKeys ? i / kRowWords : 0);
-                const uint32_t byte = i % kRowWords * 16;
-                key_words[d][k] = value_words[d][k] = make_uint4(0, 0, 0, 0);
-                if (i < kKeys * kRowWords && from != kNowhere && byte < row_bytes) {
-                    const uint64_t place = uint64_t{from} * row_bytes + byte;
-                    key_words[d][k] = load_word<false>(static_cast<const char*>(a.pool.keys) + place);
-                    value_words[d][k] = load_word<false>(static_cast<const char*>(a.pool.values) + place);
+                for (int n = 0; n < kKeys / 16; n++) {
+                    at_run[n] = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(row, 16 * n))) * row_bytes;
+                }
+#pragma unroll
+                for (int k = 0; k < kEach; k++) {
+                    const int i = k * kMovers + (SHARED ? threadIdx.x : lane);
+                    if (kKeys * kRowWords % kMovers != 0 && i >= kKeys * kRowWords) continue;
+                    uint64_t from = at_run[0];
+#pragma unroll
+                    for (int n = 1; n < kKeys / 16; n++) from = i / kRowWords / 16 == n ? at_run[n] : from;
+                    const uint32_t within = i % (16 * kRowWords) * 16;
+                    key_words[d][k] = load_word<false>(static_cast<const char*>(a.pool.keys) + from + within);
+                    value_words[d][k] = load_word<false>(static_cast<const char*>(a.pool.values) + from + within);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < kEach; k++) {
+                    const int i = k * kMovers + (SHARED ? threadIdx.x : lane);
+                    const uint32_t from = __shfl(row, i / kRowWords < kKeys ? i / kRowWords : 0);
+                    const uint32_t byte = i % kRowWords * 16;
+                    key_words[d][k] = value_words[d][k] = make_uint4(0, 0, 0, 0);
+                    if (i < kKeys * kRowWords && from != kNowhere && byte < row_bytes) {
+                        const uint64_t place = uint64_t{from} * row_bytes + byte;
+                        key_words[d][k] = load_word<false>(static_cast<const char*>(a.pool.keys) + place);
+                        value_words[d][k] = load_word<false>(static_cast<const char*>(a.pool.values) + place);
+                    }
                 }
             }
             if constexpr (QUANT) {
-                entry_scale[d] = row == kNowhere ? 0.0f : (lane < 32 ? a.pool.key_scales : a.pool.value_scales)[row];
+                if constexpr (kKeys == 64) {
+                    entry_scale[d][0] = row == kNowhere ? 0.0f : a.pool.key_scales[row];
+                    entry_scale[d][1] = row == kNowhere ? 0.0f : a.pool.value_scales[row];
+                } else {
+                    entry_scale[d][0] = row == kNowhere ? 0.0f : (lane < 32 ? a.pool.key_scales : a.pool.value_scales)[row];
+                }
             }
         };
         const auto land = [&](auto set, const TileOf& key_tile, const TileOf& value_tile) {
@@ -570,8 +615,8 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                     widened(value_words[d][k], values);
 #pragma unroll
                     for (int w = 0; w < 16 / E; w++) {
-                        *reinterpret_cast<uint4*>(key_tile.word(row, word * (16 / E) + w)) = keys.w[w];
-                        *reinterpret_cast<uint4*>(value_tile.word(row, word * (16 / E) + w)) = values.w[w];
+                        *reinterpret_cast<uint4*>(key_tile.word(row, word + w * kRowWords)) = keys.w[w];
+                        *reinterpret_cast<uint4*>(value_tile.word(row, word + w * kRowWords)) = values.w[w];
                     }
                 } else {
                     *reinterpret_cast<uint4*>(key_tile.word(row, word)) = key_words[d][k];
@@ -579,7 +624,10 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                 }
             }
             if constexpr (QUANT) {
-                if (!SHARED || wave == 0) scales[stage][lane] = entry_scale[d];
+                if (!SHARED || wave == 0) {
+#pragma unroll
+                    for (int n = 0; n < kScaleWords; n++) scales[stage][64 * n + lane] = entry_scale[d][n];
+                }
             }
         };
         uint32_t next_page[2];  // of the next tiles to fetch
@@ -591,7 +639,8 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             const TileOf key_tile{tiles[stage]};
             const TileOf value_tile{tiles[stage] + TileOf::kBytes};
             if constexpr (kScaled) {
-                const float high = wave64<Largest>(lane < 32 ? 0.0f : entry_scale[decltype(set)::value]);
+                const auto& entry = entry_scale[decltype(set)::value];
+                const float high = wave64<Largest>(kKeys == 64 ? entry[kScaleWords - 1] : lane < 32 ? 0.0f : entry[0]);
                 if (high >= unit && high < INFINITY) {
                     const float grown = ldexpf(1.0f, ilogbf(high) + 3);
                     const float factor = unit / grown;
@@ -631,10 +680,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
 #pragma unroll
                     for (int r = 0; r < RB; r++) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            if constexpr (kScaled && !std::is_same_v<S, M>) scores[r][b][i] *= shrunk[r];
-                            scores[r][b][i] *= scale[i];
-                        }
+                        for (int i = 0; i < 4; i++) scores[r][b][i] *= scale[i];
                     }
                 }
             }
@@ -655,7 +701,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
 #pragma unroll
                     for (int i = 0; i < 4; i++) high = fmaxf(high, scores[r][b][i]);
                 }
-                high = quarters<Largest>(high) * c;
+                high = quarters<Largest>(high) * factors[r];
                 // The maximum only moves when it grows past 2^8: the weights
                 // stay that small, and the sums are rarely rescaled.
                 const bool grows = high > most[r] + 8.0f;
@@ -671,11 +717,11 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                 for (int b = 0; b < kBlocks16; b++) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        scores[r][b][i] = power2(fmaf(scores[r][b][i], c, -origin));
+                        scores[r][b][i] = power2(fmaf(scores[r][b][i], factors[r], -origin));
                         total[r] += scores[r][b][i];
                     }
                     if constexpr (QUANT) {
-                        const f32x4 scale = *reinterpret_cast<const f32x4*>(&scales[stage][32 + 16 * b + 4 * quarter]);
+                        const f32x4 scale = *reinterpret_cast<const f32x4*>(&scales[stage][(kKeys == 64 ? 64 : 32) + 16 * b + 4 * quarter]);
                         const float against = kScaled ? 1.0f / unit : 1.0f;
 #pragma unroll
                         for (int i = 0; i < 4; i++) scores[r][b][i] *= scale[i] * against;
@@ -689,40 +735,44 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                     }
                 }
             }
-            // The weights as operands.
-            uint4 high_part[RB], low_part[RB];
+            // The weights as operands, and their products with the values.
 #pragma unroll
-            for (int r = 0; r < RB; r++) {
-                float v[E];
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    v[e] = scores[r][e / 4][e % 4];
-                    if (SLOW && pick != kFinite) {
-                        const bool sees = tile + 16 * (e / 4) + 4 * quarter + e % 4 < seen[r];
-                        v[e] = (pick == kNaN ? sees : pick == kZero ? sees && v[e] == 0.0f : v[e] != 0.0f) ? 1.0f : 0.0f;
-                    }
-                }
-                Words<M, E> high, low;
-                high.put(v);
-                high_part[r] = high.w[0];
-                if constexpr (kTwoParts) {
-#pragma unroll
-                    for (int e = 0; e < E; e++) v[e] -= high.at(e);
-                    low.put(v);
-                    low_part[r] = low.w[0];
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < SIZE / 16; t++) {
-                uint4 values = value_tile.by_column(column_place, t);
-                if constexpr (SLOW) {
-                    values = make_uint4(picked(values.x, pick), picked(values.y, pick), picked(values.z, pick),
-                                        picked(values.w, pick));
-                }
+            for (int deep = 0; deep < kDeeps; deep++) {
+                uint4 high_part[RB], low_part[RB];
 #pragma unroll
                 for (int r = 0; r < RB; r++) {
-                    acc[r][t] = product16<M>(values, high_part[r], acc[r][t]);
-                    if constexpr (kTwoParts) acc[r][t] = product16<M>(values, low_part[r], acc[r][t]);
+                    float v[E];
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        const int b = deep * (kDeepKeys / 16) + e / 4;
+                        v[e] = scores[r][b][e % 4];
+                        if (SLOW && pick != kFinite) {
+                            const bool sees = tile + 16 * b + 4 * quarter + e % 4 < seen[r];
+                            v[e] = (pick == kNaN ? sees : pick == kZero ? sees && v[e] == 0.0f : v[e] != 0.0f) ? 1.0f : 0.0f;
+                        }
+                    }
+                    Words<M, E> high, low;
+                    high.put(v);
+                    high_part[r] = high.w[0];
+                    if constexpr (kTwoParts) {
+#pragma unroll
+                        for (int e = 0; e < E; e++) v[e] -= high.at(e);
+                        low.put(v);
+                        low_part[r] = low.w[0];
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < SIZE / 16; t++) {
+                    uint4 values = value_tile.by_column(column_place, deep * kDeepKeys, t);
+                    if constexpr (SLOW) {
+                        values = make_uint4(picked(values.x, pick), picked(values.y, pick), picked(values.z, pick),
+                                            picked(values.w, pick));
+                    }
+#pragma unroll
+                    for (int r = 0; r < RB; r++) {
+                        acc[r][t] = product16<M>(values, high_part[r], acc[r][t]);
+                        if constexpr (kTwoParts) acc[r][t] = product16<M>(values, low_part[r], acc[r][t]);
+                    }
                 }
             }
             tile += kKeys;
@@ -815,7 +865,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                 S* const to = static_cast<S*>(a.out) + token * a.out_steps.token + head * a.out_steps.head;
 #pragma unroll
                 for (int t = 0; t < SIZE / 16; t++) {
-                    store_four(to, 16 * t + 4 * quarter, a.pool.size, seen[r] > 0 ? acc[r][t] * scale : f32x4{});
+                    store_four(to, element_of(16 * t + 4 * quarter), a.pool.size, seen[r] > 0 ? acc[r][t] * scale : f32x4{});
                 }
                 if (quarter == 0 && a.normalizers != nullptr) {
                     a.normalizers[uint64_t{head} * a.batch.tokens + token] =
@@ -823,9 +873,11 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                 }
             } else {
                 const uint64_t to = whole ? uint64_t{token} * a.query_heads + head : uint64_t{slot} * ROWS + row;
-                float* const values = (whole ? parts.rows : parts.slots) + to * SIZE + 4 * quarter;
+                float* const values = (whole ? parts.rows : parts.slots) + to * SIZE;
 #pragma unroll
-                for (int t = 0; t < SIZE / 16; t++) *reinterpret_cast<f32x4*>(values + 16 * t) = acc[r][t] * back;
+                for (int t = 0; t < SIZE / 16; t++) {
+                    *reinterpret_cast<f32x4*>(values + element_of(16 * t + 4 * quarter)) = acc[r][t] * back;
+                }
                 if (quarter == 0) (whole ? parts.row_stats : parts.slot_stats)[to] = make_float2(most[r], all);
             }
         }

@@ -2,9 +2,11 @@
 
 Bounds: a weight is off relatively by its score's error and a few roundings of
 32 bits (`loose`), and by its rounding before the product with the values: none
-in f32, one of f16, of bf16 and over 8 bits one of 16 bits (two parts of bf16's
-8).  In f16 weights are rounded times 2^6 where the largest is at least 1, so
-that one is off by at most 2^-31 besides, of a sum of 1 or more."""
+in f32, one of f16 in f16 and over 8 bits, in bf16 one of 16 bits (two parts of
+bf16's 8).  As f16 weights are rounded times 2^6 where the largest is at least 1,
+so that one is off by at most 2^-31 besides, of a sum of 1 or more; over 8 bits
+they are weights times a scale, against a power of two at most 16 times the
+largest scale: 2^-27 of that."""
 
 import numpy as np
 import pytest
@@ -37,9 +39,13 @@ def check(world, q, scale, got):
     score = scale * longest(rows[:len(rows) // 2]) * np.sqrt((finite(q) ** 2).sum(2)).max(initial=0)
     keys = max((len(r) for r in rows), default=0)
     loose = EPSILON_32 * (64 + keys / 8 + 2 * (world.size + 6) * score)
-    f16 = world.kind == lib.F16 and world.fmt == lib.CACHE_PLAIN
+    quant = world.fmt == lib.CACHE_INT8
+    f16 = world.kind == lib.F16 or (quant and world.kind == lib.BF16)
     weight = 2.0**-11 if f16 else 0.0 if world.kind == lib.F32 else 2.0**-16
-    far = 2.0**-31 * sum(np.abs(finite(r)).sum(0).max(initial=0) for r in rows[len(rows) // 2:]) if f16 else 0.0
+    # Over 8 bits every value counts as the largest one of all.
+    far = 0.0
+    for r in rows[len(rows) // 2:] if f16 else []:
+        far += 2.0**-27 * len(r) * np.abs(finite(r)).max(initial=0) if quant else 2.0**-31 * np.abs(finite(r)).sum(0).max(initial=0)
     near(got[0], out, (weight + loose) * sizes + far + ROUNDING[world.kind] * np.abs(out) + TINY[world.kind], "out")
     near(got[1], normalizers, loose + 4 * EPSILON_32 * np.abs(finite(normalizers)), "normalizers")
 
