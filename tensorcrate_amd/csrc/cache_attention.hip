@@ -6,54 +6,52 @@ namespace tc {
 namespace cache {
 namespace {
 
-// The form for `rows` query rows that share keys.
-int form_of(uint64_t rows) { return rows <= 16 ? kRows16 : rows <= 32 ? kRows32 : kRows128; }
+// Whether blocks share tiles, where `rows` query rows share keys.
+bool shares(uint64_t rows) { return rows > 16; }
 
 // The storage of one line's parts.
 struct Storage {
-    Scratch slots, slot_stats, rows, row_stats, plans, cut;
+    Scratch slots, slot_stats, rows, row_stats, found, cut;
 
-    Storage(uint64_t slot_rows, uint64_t whole_rows, uint64_t items, uint64_t size)
+    Storage(uint64_t slot_rows, uint64_t whole_rows, uint64_t all_rows, uint64_t size)
         : slots(slot_rows * size * sizeof(float)),
           slot_stats(slot_rows * sizeof(float2)),
           rows(whole_rows * size * sizeof(float)),
           row_stats(whole_rows * sizeof(float2)),
-          plans(items * sizeof(Plan)),
+          found(all_rows * sizeof(Found)),
           cut(sizeof(uint32_t)) {}
     int status() const {
-        for (int s : {slots.status, slot_stats.status, rows.status, row_stats.status, plans.status, cut.status}) {
+        for (int s : {slots.status, slot_stats.status, rows.status, row_stats.status, found.status, cut.status}) {
             if (s != TC_OK) return s;
         }
         return TC_OK;
     }
     Parts parts() const {
         return {static_cast<float*>(slots.ptr), static_cast<float2*>(slot_stats.ptr), static_cast<float*>(rows.ptr),
-                static_cast<float2*>(row_stats.ptr), static_cast<Plan*>(plans.ptr), static_cast<uint32_t*>(cut.ptr)};
+                static_cast<float2*>(row_stats.ptr), static_cast<Found*>(found.ptr), static_cast<uint32_t*>(cut.ptr)};
     }
 };
 
 int run(const AttentionLaunches& launches, const Attention& a, bool quant) {
-    const uint32_t blocks = static_cast<uint32_t>(compute_units()) * 2;
+    const uint64_t units = static_cast<uint64_t>(compute_units());
     const uint64_t size = (a.pool.size + 31) / 32 * 32, tokens = a.batch.tokens, rows = tokens * a.query_heads;
     const bool prefix = a.batch.prefix > 0;
     const uint64_t sequences = a.batch.sequences;
-    const int own_form = form_of(tokens * a.group / (sequences > 0 ? sequences : 1));
-    const int prefix_form = form_of(tokens * a.group);
-    const uint64_t own_rows = rows_of_form(own_form), prefix_rows = rows_of_form(prefix_form);
-    const Storage own(2 * uint64_t{workers_of(own_form, blocks)} * own_rows, prefix ? rows : 0,
-                      (tokens * a.group / own_rows + sequences) * a.pool.heads, size);
-    const Storage shared(prefix ? 2 * uint64_t{workers_of(prefix_form, blocks)} * prefix_rows : 0, prefix ? rows : 0,
-                         prefix ? (tokens * a.group / prefix_rows + 1) * a.pool.heads : 0, size);
+    const bool own_shared = shares(tokens * a.group / (sequences > 0 ? sequences : 1));
+    const bool prefix_shared = shares(tokens * a.group);
+    const auto slot_rows = [&](bool form) { return 2 * units * workers_of_form(form) * rows_of_form(form); };
+    const Storage own(slot_rows(own_shared), prefix ? rows : 0, rows, size);
+    const Storage shared(prefix ? slot_rows(prefix_shared) : 0, prefix ? rows : 0, prefix ? rows : 0, size);
     if (own.status() != TC_OK) return own.status();
     if (shared.status() != TC_OK) return shared.status();
     // (The first launch tells the second whether any token does not see the
     // whole prefix.)
     Parts prefix_parts = shared.parts();
     prefix_parts.cut = own.parts().cut;
-    int status = launches.attend(a, own.parts(), quant, false, !prefix, own_form, blocks);
-    if (status == TC_OK && prefix) status = launches.attend(a, prefix_parts, quant, true, false, prefix_form, blocks);
+    int status = launches.attend(a, own.parts(), quant, false, !prefix, own_shared);
+    if (status == TC_OK && prefix) status = launches.attend(a, prefix_parts, quant, true, false, prefix_shared);
     if (status != TC_OK) return status;
-    return launches.join(a, own.parts(), shared.parts(), quant, own_form, prefix_form, blocks);
+    return launches.join(a, own.parts(), shared.parts(), quant, own_shared, prefix_shared);
 }
 
 }  // namespace

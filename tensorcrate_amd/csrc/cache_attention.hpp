@@ -42,11 +42,13 @@ namespace cache {
 
 constexpr int kAttendThreads = 256;
 constexpr int kAttendWaves = kAttendThreads / 64;
-// The forms of the first kernel: 16 or 32 query rows a wave, or 128 a block.
-enum Form { kRows16 = 0, kRows32 = 1, kRows128 = 2 };
-constexpr uint32_t rows_of_form(int form) { return form == kRows16 ? 16 : form == kRows32 ? 32 : 128; }
-// Whose parts are one behind another on the line: waves, or blocks.
-constexpr uint32_t workers_of(int form, uint32_t blocks) { return form == kRows128 ? blocks : blocks * kAttendWaves; }
+// The first kernel's two forms: waves by themselves of 16 query rows each, or
+// blocks of 64 rows that share their tiles (SHARED).
+constexpr uint32_t rows_of_form(bool shared) { return shared ? 64 : 16; }
+// Blocks of a compute unit at a time, as registers allow, and whose parts are
+// one behind another on the line: waves, or blocks.
+constexpr uint32_t blocks_of_form(bool shared) { return shared ? 3 : 2; }
+constexpr uint32_t workers_of_form(bool shared) { return blocks_of_form(shared) * (shared ? 1 : kAttendWaves); }
 
 // One launch's operands.
 struct Attention {
@@ -62,30 +64,30 @@ struct Attention {
     float* normalizers;
 };
 
-// Where an item (a key head's block of query rows of a sequence) has its
-// results: whole in the rows' own place, or with the workers first to last, the
-// first one's in `slot`, the others' in their first slot.
-struct Plan {
-    uint32_t first, last, slot, whole;
+// Where a query row's parts over a line are: whole in the row's own place, or
+// with the workers first to last, the first one's at `place` of the slots, the
+// others' in their first slot.
+struct Found {
+    uint32_t first, last, place, whole;
 };
 
 // Partial results.  A worker has two slots, for parts at its two ends.
 struct Parts {
-    float* slots;         // [2 workers][rows][size]
-    float2* slot_stats;   // [2 workers][rows] (maximum, in powers of two; sum)
-    float* rows;          // [token][query head][size], of whole items
+    float* slots;        // [2 workers][rows][size]
+    float2* slot_stats;  // [2 workers][rows] (maximum, in powers of two; sum)
+    float* rows;         // [token][query head][size], of whole items
     float2* row_stats;
-    Plan* plans;
+    Found* found;   // [token][query head]
     uint32_t* cut;  // whether any token comes before its sequence's first
 };
 
-// The launches of one element type; `blocks` of the first kernel.
+// The launches of one element type.
 struct AttentionLaunches {
     // Items' parts over the sequences' own keys, or with `prefix` over the
     // prefix; `final`: whole items are results.
-    int (*attend)(const Attention&, const Parts&, bool quant, bool prefix, bool final, int form, uint32_t blocks);
-    int (*join)(const Attention&, const Parts& own, const Parts& prefix, bool quant, int own_form, int prefix_form,
-                uint32_t blocks);
+    int (*attend)(const Attention&, const Parts&, bool quant, bool prefix, bool final, bool shared);
+    int (*join)(const Attention&, const Parts& own, const Parts& prefix, bool quant, bool own_shared,
+                bool prefix_shared);
 };
 const AttentionLaunches& attend_f32();
 const AttentionLaunches& attend_f16();
@@ -98,12 +100,6 @@ __host__ __device__ inline uint32_t seen_of(uint64_t length, uint32_t left, uint
     const uint64_t upto = before + length + 1;  // past the query's own place, plus `left`
     const uint64_t seen = upto > left ? upto - left : 0;
     return static_cast<uint32_t>(seen < count ? seen : count);
-}
-
-// Index of a sequence's first item among the plans: no two sequences' overlap,
-// without a sum over the ones before.
-__device__ __forceinline__ uint64_t first_item(const Attention& a, uint32_t rows, uint32_t sequence, uint32_t token) {
-    return (uint64_t{token} * a.group / rows + sequence) * a.pool.heads;
 }
 
 #if defined(TC_ATTENTION_TYPE)
@@ -123,10 +119,14 @@ using attention::u32x2;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// Rows of a tile: what one product of weights with values sums over, or twice
-// that where a block shares it.
-constexpr int kDeepKeys = kWide ? 16 : 32;
-constexpr int keys_of_form(int form) { return form == kRows128 ? 2 * kDeepKeys : kDeepKeys; }
+constexpr int kKeys = kWide ? 16 : 32;  // rows of a tile: what a product of weights with values sums over
+constexpr int kBlocks16 = kKeys / 16;
+
+// A value that is the same in the whole wave, kept as one.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint64_t uniform(uint64_t v) {
+    return uniform(static_cast<uint32_t>(v)) | uint64_t{uniform(static_cast<uint32_t>(v >> 32))} << 32;
+}
 // Elements of the summed axis that one operand word of all quarters covers.
 constexpr int kDeep16 = 4 * E;
 
@@ -161,10 +161,10 @@ __device__ __forceinline__ float quarters(float v) {
     return Op::join(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
 }
 
-// A tile of KEYS rows, read 16 rows at a time.
-template <int SIZE, int KEYS>
-struct KeyTile : attention::Tile<SIZE, KEYS> {
-    using Base = attention::Tile<SIZE, KEYS>;
+// A tile of kKeys rows, read 16 rows at a time.
+template <int SIZE>
+struct KeyTile : attention::Tile<SIZE, kKeys> {
+    using Base = attention::Tile<SIZE, kKeys>;
     // A lane's places for `by_row` and `by_column`.
     __device__ __forceinline__ static uint32_t row_place(int lane) { return Base::place(lane % 16, lane / 16); }
     __device__ __forceinline__ static uint32_t column_place(int lane) {
@@ -177,17 +177,17 @@ struct KeyTile : attention::Tile<SIZE, KEYS> {
     __device__ __forceinline__ uint4 by_row(uint32_t place, int b, int n) const {
         return *reinterpret_cast<const uint4*>(this->from(place, 16 * b, 4 * n));
     }
-    // Operand word of column 16 t + l % 16, summed over the kDeepKeys rows from
-    // `rows` on in the order of products' results.
-    __device__ __forceinline__ uint4 by_column(uint32_t place, int rows, int t) const {
+    // Operand word of column 16 t + l % 16, summed over the rows in the order of
+    // products' results.
+    __device__ __forceinline__ uint4 by_column(uint32_t place, int t) const {
         if constexpr (kWide) {
             uint32_t v[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = *reinterpret_cast<const uint32_t*>(this->from(place, rows + j, 4 * t));
+            for (int j = 0; j < 4; j++) v[j] = *reinterpret_cast<const uint32_t*>(this->from(place, j, 4 * t));
             return make_uint4(v[0], v[1], v[2], v[3]);
         } else {
-            const u32x2 a = __builtin_bit_cast(u32x2, Base::transposed(this->from(place, rows, 2 * t)));
-            const u32x2 b = __builtin_bit_cast(u32x2, Base::transposed(this->from(place, rows + 16, 2 * t)));
+            const u32x2 a = __builtin_bit_cast(u32x2, Base::transposed(this->from(place, 0, 2 * t)));
+            const u32x2 b = __builtin_bit_cast(u32x2, Base::transposed(this->from(place, 16, 2 * t)));
             return make_uint4(a.x, a.y, b.x, b.y);
         }
     }
@@ -279,10 +279,10 @@ __device__ __forceinline__ Sequence sequence_at(const Attention& a, uint32_t seq
 }
 
 // The tiles of all items one behind another: sequences, of each the key heads,
-// of each the blocks of ROWS query rows, of each the tiles of KEYS keys.
-template <int ROWS, int KEYS>
+// of each the blocks of ROWS query rows, of each the tiles of kKeys keys.
+template <int ROWS>
 struct Line {
-    __device__ __forceinline__ static uint32_t tiles(const Sequence& s) { return (s.keys + KEYS - 1) / KEYS; }
+    __device__ __forceinline__ static uint32_t tiles(const Sequence& s) { return (s.keys + kKeys - 1) / kKeys; }
     __device__ __forceinline__ static uint32_t blocks(const Attention& a, const Sequence& s) {
         return static_cast<uint32_t>((uint64_t{s.tokens} * a.group + ROWS - 1) / ROWS);
     }
@@ -313,17 +313,14 @@ __device__ __forceinline__ void store_four(S* row, uint32_t first, uint32_t size
 // 2^-14: the largest, which may reach 2^8, stay below 2^15.
 constexpr float kHalfPower = 6.0f;
 
-template <int SIZE, int FORM, bool QUANT, bool PREFIX>
-__global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_per_eu(2)))
+template <int SIZE, bool SHARED, bool QUANT, bool PREFIX>
+__global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_per_eu(blocks_of_form(SHARED))))
     attend_kernel(const Attention a, const Parts parts, bool final) {
-    constexpr bool SHARED = FORM == kRows128;
-    constexpr int RB = FORM == kRows16 ? 1 : 2;  // blocks of 16 rows of a wave
-    constexpr int ROWS = rows_of_form(FORM);
+    constexpr int ROWS = rows_of_form(SHARED);
     constexpr int kWorkers = SHARED ? 1 : kAttendWaves;  // of a block
     constexpr int kMovers = SHARED ? kAttendThreads : 64;  // threads that move a tile
-    constexpr int kKeys = keys_of_form(FORM), kBlocks16 = kKeys / 16, kDeeps = kKeys / kDeepKeys;
-    using LineOf = Line<ROWS, kKeys>;
-    using TileOf = KeyTile<SIZE, kKeys>;
+    using LineOf = Line<ROWS>;
+    using TileOf = KeyTile<SIZE>;
     // The type that is multiplied in.
     constexpr bool kScaled = QUANT && sizeof(S) == 2;
     using M = std::conditional_t<kScaled, _Float16, S>;
@@ -343,10 +340,11 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
     };
     constexpr int kStages = SHARED ? 2 : kAttendWaves;
     // Tiles in flight, of 8 kEach registers each.
-    constexpr int kAhead = (SHARED ? 4 : 8) / kEach < 1 ? 1 : (SHARED ? 4 : 8) / kEach > 4 ? 4 : (SHARED ? 4 : 8) / kEach;
+    constexpr int kMostAhead = SHARED ? 2 : 4;
+    constexpr int kAhead = 8 / kEach < 1 ? 1 : 8 / kEach > kMostAhead ? kMostAhead : 8 / kEach;
 
     __shared__ __attribute__((aligned(1024))) char tiles[kStages][2 * TileOf::kBytes];
-    __shared__ __attribute__((aligned(16))) float scales[QUANT ? kStages : 1][kKeys == 64 ? 128 : 64];
+    __shared__ __attribute__((aligned(16))) float scales[QUANT ? kStages : 1][64];
     __shared__ uint64_t sums[kAttendWaves], found[kWorkers][2];
 
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, quarter = lane / 16;
@@ -378,6 +376,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             if (w < wave) upto_here += sums[w];
             total_tiles += sums[w];
         }
+        total_tiles = uniform(total_tiles);
         if (blockIdx.x == 0 && threadIdx.x == 0) *parts.cut = cut;
     }
     // No worker has nothing, so that every one between two parts of an item has
@@ -388,7 +387,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
     if (first_worker >= workers) return;
     const auto begin_of = [&](uint64_t worker) { return worker * total_tiles / workers; };
 
-    const uint32_t worker = __builtin_amdgcn_readfirstlane(first_worker + (SHARED ? 0 : wave));
+    const uint32_t worker = uniform(first_worker + (SHARED ? 0 : wave));
     uint32_t sequence = 0;
     uint64_t before = 0;  // tiles of the sequences before
     if constexpr (!PREFIX) {
@@ -426,8 +425,8 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             if (begins[kWorkers - 1] - before < all) break;  // the same for the whole block
             before += all;
         }
-        sequence = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(found[SHARED ? 0 : wave][0]));
-        before = found[SHARED ? 0 : wave][1];
+        sequence = uniform(static_cast<uint32_t>(found[SHARED ? 0 : wave][0]));
+        before = uniform(found[SHARED ? 0 : wave][1]);
     }
     [[maybe_unused]] bool cut = false;
     if constexpr (PREFIX) cut = __builtin_amdgcn_readfirstlane(*parts.cut) != 0;
@@ -435,11 +434,13 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
     const uint64_t begin = begin_of(worker), end = begin_of(worker + uint64_t{1});
 
     const uint32_t row_place = TileOf::row_place(lane), column_place = TileOf::column_place(lane);
-    const float c = a.scale * attention::kLog2e;
     int stage = SHARED ? 0 : wave;
 
     for (uint64_t at = begin; at < end;) {
-        const Sequence s = sequence_at<PREFIX>(a, sequence);
+        Sequence s = sequence_at<PREFIX>(a, sequence);
+        if constexpr (!PREFIX) {
+            s.first = uniform(s.first), s.tokens = uniform(s.tokens), s.keys = uniform(s.keys), s.length = uniform(s.length);
+        }
         const uint32_t tile_count = LineOf::tiles(s), row_blocks = LineOf::blocks(a, s);
         const uint64_t count = uint64_t{tile_count} * row_blocks * a.pool.heads;
         if (at - before >= count) {
@@ -454,202 +455,207 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
         const bool whole = tile_0 == 0 && tile_1 == tile_count;
         // (An item's first part is the worker's first if both begin together.)
         const uint32_t slot = 2 * worker + (at > begin);
-        if (tile_0 == 0 && (SHARED ? threadIdx.x : lane) == 0) {
-            const uint64_t last = ((at + tile_count) * workers - 1) / total_tiles;
-            const uint64_t place = (PREFIX ? 0 : first_item(a, ROWS, sequence, s.first)) + item;
-            parts.plans[place] = {worker, static_cast<uint32_t>(last), slot, whole};
-        }
 
-        // ---- the item's query rows -------------------------------------------------
+        // ---- this lane's query row ---------------------------------------------------
         const uint32_t first_row = row_block * ROWS, left_rows = s.tokens * a.group - first_row;
         const uint32_t rows = left_rows < ROWS ? left_rows : ROWS;
-        const auto row_of_lane = [&](int r) { return static_cast<uint32_t>((SHARED ? wave * 16 * RB : 0) + r * 16 + lane % 16); };
-        uint4 queries[RB][kOperands];
-        float factors[RB];  // of the scores: `c`, and what a row of queries was multiplied with undone
-        uint32_t seen[RB];
-        bool all_see = true;
-#pragma unroll
-        for (int r = 0; r < RB; r++) {
-            const uint32_t row = row_of_lane(r), number = first_row + row;
-            const bool real = row < rows;
-            const uint32_t place = a.group_of.div(real ? number : 0);
-            const uint32_t token = s.first + place;
-            const uint32_t head = key_head * a.group + (real ? number : 0) - place * a.group;
-            seen[r] = s.keys;
-            if (real) {
-                if constexpr (PREFIX) {
-                    Span span;
-                    const uint32_t own = cut ? sequence_of(a.batch, token, &span) : kNowhere;
-                    if (own != kNowhere) seen[r] = seen_of(a.batch.lengths[own], span.end - token, s.keys, s.keys);
-                } else {
-                    seen[r] = seen_of(s.length, s.tokens - place, 0, s.keys);
-                }
+        const uint32_t row = (SHARED ? wave * 16 : 0) + lane % 16;
+        const bool real = row < rows;
+        const uint32_t place = a.group_of.div(real ? first_row + row : 0);
+        const uint32_t token = s.first + place;
+        const uint32_t head = key_head * a.group + (real ? first_row + row : 0) - place * a.group;
+        uint32_t seen = s.keys;
+        if (real) {
+            if constexpr (PREFIX) {
+                Span span;
+                const uint32_t own = cut ? sequence_of(a.batch, token, &span) : kNowhere;
+                if (own != kNowhere) seen = seen_of(a.batch.lengths[own], span.end - token, s.keys, s.keys);
+            } else {
+                seen = seen_of(s.length, s.tokens - place, 0, s.keys);
             }
-            all_see = all_see && seen[r] == s.keys;
-            factors[r] = c;
-            const S* from = static_cast<const S*>(a.query) + token * a.query_steps.token + head * a.query_steps.head;
-#pragma unroll
-            for (int n = 0; n < kOperands; n++) {
-                queries[r][n] = real ? head_word(from, element_of((4 * n + quarter) * E) / E, a.pool.size) : make_uint4(0, 0, 0, 0);
-            }
-            if constexpr (kScaled && !std::is_same_v<S, M>) {
-                // The largest of the row to 2^8 and above, an infinity or a NaN
-                // as it is: what f16 then loses is below 2^-32 of the largest.
-                float most = 0.0f;
-#pragma unroll
-                for (int n = 0; n < kOperands; n++) {
-                    const Words<S, E> words{{queries[r][n]}};
-#pragma unroll
-                    for (int e = 0; e < E; e++) most = fmaxf(most, fabsf(words.at(e)));
-                }
-                most = quarters<Largest>(most);
-                int power = most > 0.0f && most < INFINITY ? 8 - ilogbf(most) : 0;
-                power = power > 126 ? 126 : power;
-                factors[r] = ldexpf(c, -power);
-                const float factor = ldexpf(1.0f, power);
-#pragma unroll
-                for (int n = 0; n < kOperands; n++) {
-                    const Words<S, E> words{{queries[r][n]}};
-                    Words<M, E> to;
-                    float v[E];
-#pragma unroll
-                    for (int e = 0; e < E; e++) v[e] = words.at(e) * factor;
-                    to.put(v);
-                    queries[r][n] = to.w[0];
-                }
+            if (tile_0 == 0 && quarter == 0) {
+                const uint64_t last = ((at + tile_count) * workers - 1) / total_tiles;
+                parts.found[uint64_t{token} * a.query_heads + head] = {worker, static_cast<uint32_t>(last),
+                                                                       slot * ROWS + row, whole};
             }
         }
         // Keys that every, and that any, row of the block sees.
         uint32_t least, most_seen = s.keys;
         if constexpr (PREFIX) {
+            const bool all_see = seen == s.keys;
             least = (SHARED ? __syncthreads_and(all_see) : __ballot(!all_see) == 0) ? s.keys : 0;
         } else {
             least = seen_of(s.length, s.tokens - a.group_of.div(first_row), 0, s.keys);
             most_seen = seen_of(s.length, s.tokens - a.group_of.div(first_row + rows - 1), 0, s.keys);
         }
-        least = __builtin_amdgcn_readfirstlane(least);
-        most_seen = __builtin_amdgcn_readfirstlane(most_seen);
-
-        // ---- a sweep over the part's tiles -----------------------------------------
-        f32x4 acc[RB][SIZE / 16];
-        float most[RB], total[RB];
-        [[maybe_unused]] float unit = 0x1p-126f;  // above every value's scale so far, and a power of two
-
+        least = uniform(least), most_seen = uniform(most_seen);
         const uint32_t key_end = uint64_t{tile_1} * kKeys < most_seen ? tile_1 * kKeys : most_seen;
-        uint32_t tile = 0;
+
+        // ---- tiles on their way --------------------------------------------------------
         uint4 key_words[kAhead][kEach], value_words[kAhead][kEach];
-        // The scales of keys in the lower half of a wave and of values in the
-        // upper, or of 64 keys and of their values.
-        constexpr int kScaleWords = kKeys == 64 ? 2 : 1;
-        float entry_scale[kAhead][kScaleWords];
-        // The page of key l (% 32 where a tile has no more) of the tile at
-        // `first`, and its row there.
-        const uint32_t key_lane = kKeys == 64 ? lane : lane % 32;
+        float entry_scale[kAhead];  // of keys in the lower half of a wave, of values in the upper
+        // The page of key l % 32 of the tile at `first`, and its row there.
         const auto page_at = [&](uint32_t first) {
-            const uint32_t key = first + key_lane;
+            const uint32_t key = first + lane % 32;
             const uint32_t n = a.pool.pages_of.div(key);
-            return key_lane < kKeys && key < key_end && n < s.page_count ? s.pages[n] : kNowhere;
+            return lane % 32 < kKeys && key < key_end && n < s.page_count ? s.pages[n] : kNowhere;
         };
         const auto row_at = [&](uint32_t first, uint32_t page) {
-            const uint32_t key = first + key_lane;
+            const uint32_t key = first + lane % 32;
             const uint32_t within = key - a.pool.pages_of.div(key) * a.pool.page_size;
             return page < a.pool.page_count ? (page * a.pool.heads + key_head) * a.pool.page_size + within : kNowhere;
         };
         const uint32_t row_bytes = a.pool.row * kEntry;
-        const auto fetch = [&](auto set, uint32_t row) {
+        const uint32_t mover = SHARED ? threadIdx.x : lane;
+        const auto fetch = [&](auto set, uint32_t from_row) {
             constexpr int d = decltype(set)::value;
             // Where pages hold whole runs of 16 tokens and the tile is full, a
             // run's first row tells the others': one address of the wave's, and
             // one number of the lane's.
-            const bool runs = a.pool.page_size % 16 == 0 && row_bytes == kRowWords * 16 && __ballot(row == kNowhere && key_lane < kKeys) == 0;
+            const bool runs = a.pool.page_size % 16 == 0 && row_bytes == kRowWords * 16 &&
+                              __ballot(from_row == kNowhere && lane % 32 < kKeys) == 0;
             if (runs) {
-                uint64_t at_run[kKeys / 16];
+                uint64_t run[kBlocks16];
 #pragma unroll
-                for (int n = 0; n < kKeys / 16; n++) {
-                    at_run[n] = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(row, 16 * n))) * row_bytes;
+                for (int n = 0; n < kBlocks16; n++) {
+                    run[n] = uint64_t{static_cast<uint32_t>(__builtin_amdgcn_readlane(from_row, 16 * n))} * row_bytes;
                 }
 #pragma unroll
                 for (int k = 0; k < kEach; k++) {
-                    const int i = k * kMovers + (SHARED ? threadIdx.x : lane);
+                    const int i = k * kMovers + mover;
                     if (kKeys * kRowWords % kMovers != 0 && i >= kKeys * kRowWords) continue;
-                    uint64_t from = at_run[0];
-#pragma unroll
-                    for (int n = 1; n < kKeys / 16; n++) from = i / kRowWords / 16 == n ? at_run[n] : from;
-                    const uint32_t within = i % (16 * kRowWords) * 16;
-                    key_words[d][k] = load_word<false>(static_cast<const char*>(a.pool.keys) + from + within);
-                    value_words[d][k] = load_word<false>(static_cast<const char*>(a.pool.values) + from + within);
+                    const uint64_t from = run[kBlocks16 > 1 && i / kRowWords >= 16 ? 1 : 0] + i % (16 * kRowWords) * 16;
+                    key_words[d][k] = load_word<false>(static_cast<const char*>(a.pool.keys) + from);
+                    value_words[d][k] = load_word<false>(static_cast<const char*>(a.pool.values) + from);
                 }
             } else {
+                // (The lane's numbers are found here: kept through the loop they
+                // would take registers of the path above.)
+                uint32_t here = mover;
+                asm volatile("" : "+v"(here));
 #pragma unroll
                 for (int k = 0; k < kEach; k++) {
-                    const int i = k * kMovers + (SHARED ? threadIdx.x : lane);
-                    const uint32_t from = __shfl(row, i / kRowWords < kKeys ? i / kRowWords : 0);
+                    const int i = k * kMovers + here;
+                    const uint32_t from = __shfl(from_row, i / kRowWords < kKeys ? i / kRowWords : 0);
                     const uint32_t byte = i % kRowWords * 16;
                     key_words[d][k] = value_words[d][k] = make_uint4(0, 0, 0, 0);
                     if (i < kKeys * kRowWords && from != kNowhere && byte < row_bytes) {
-                        const uint64_t place = uint64_t{from} * row_bytes + byte;
-                        key_words[d][k] = load_word<false>(static_cast<const char*>(a.pool.keys) + place);
-                        value_words[d][k] = load_word<false>(static_cast<const char*>(a.pool.values) + place);
+                        const uint64_t at_byte = uint64_t{from} * row_bytes + byte;
+                        key_words[d][k] = load_word<false>(static_cast<const char*>(a.pool.keys) + at_byte);
+                        value_words[d][k] = load_word<false>(static_cast<const char*>(a.pool.values) + at_byte);
                     }
                 }
             }
             if constexpr (QUANT) {
-                if constexpr (kKeys == 64) {
-                    entry_scale[d][0] = row == kNowhere ? 0.0f : a.pool.key_scales[row];
-                    entry_scale[d][1] = row == kNowhere ? 0.0f : a.pool.value_scales[row];
-                } else {
-                    entry_scale[d][0] = row == kNowhere ? 0.0f : (lane < 32 ? a.pool.key_scales : a.pool.value_scales)[row];
-                }
+                entry_scale[d] =
+                    from_row == kNowhere ? 0.0f : (lane < 32 ? a.pool.key_scales : a.pool.value_scales)[from_row];
             }
         };
+        uint32_t tile = tile_0 * kKeys;
+        uint32_t pages[kAhead], next_page[2];  // of the first tiles, and of the next ones to fetch
+        const auto find_pages = [&]() {
+            tile = tile_0 * kKeys;
+            each<kAhead>([&](auto n) { pages[n.value] = page_at(tile + n.value * kKeys); });
+            next_page[0] = page_at(tile + kAhead * kKeys);
+            next_page[1] = page_at(tile + (kAhead + 1) * kKeys);
+        };
+        const auto fetch_first = [&]() {
+            each<kAhead>([&](auto n) { fetch(n, row_at(tile + n.value * kKeys, pages[n.value])); });
+        };
+        find_pages();
+
+        // ---- queries -------------------------------------------------------------------
+        uint4 queries[kOperands];
+        const S* from = static_cast<const S*>(a.query) + token * a.query_steps.token + head * a.query_steps.head;
+#pragma unroll
+        for (int n = 0; n < kOperands; n++) {
+            const int word = element_of((4 * n + quarter) * E) / E;
+            queries[n] = real ? head_word(from, word, a.pool.size) : make_uint4(0, 0, 0, 0);
+        }
+        fetch_first();
+        float factor = a.scale * attention::kLog2e;  // of the scores, in powers of two
+        if constexpr (kScaled && !std::is_same_v<S, M>) {
+            // The row's largest to 2^8 and above, an infinity or a NaN as it is:
+            // what f16 then loses is below 2^-32 of the largest.
+            float largest = 0.0f;
+#pragma unroll
+            for (int n = 0; n < kOperands; n++) {
+                const Words<S, E> words{{queries[n]}};
+#pragma unroll
+                for (int e = 0; e < E; e++) largest = fmaxf(largest, fabsf(words.at(e)));
+            }
+            largest = quarters<Largest>(largest);
+            int power = largest > 0.0f && largest < INFINITY ? 8 - ilogbf(largest) : 0;
+            power = power > 126 ? 126 : power;
+            factor = ldexpf(factor, -power);
+            const float grown = ldexpf(1.0f, power);
+#pragma unroll
+            for (int n = 0; n < kOperands; n++) {
+                const Words<S, E> words{{queries[n]}};
+                Words<M, E> to;
+                float v[E];
+#pragma unroll
+                for (int e = 0; e < E; e++) v[e] = words.at(e) * grown;
+                to.put(v);
+                queries[n] = to.w[0];
+            }
+        }
+
+        // ---- a sweep over the part's tiles -----------------------------------------
+        f32x4 acc[SIZE / 16];
+        float most, total;
+        [[maybe_unused]] float unit = 0x1p-126f;  // above every value's scale so far, and a power of two
+        // Where the lane's first word of a tile lands, of which the others' places
+        // follow if a row's words and the rows a step has are powers of two.
+        constexpr int kStepRows = kMovers / kRowWords;
+        constexpr bool kRegular = (kRowWords & (kRowWords - 1)) == 0 && kMovers % kRowWords == 0 &&
+                                  kKeys * kRowWords % kMovers == 0;
+        const uint32_t mover_place = TileOf::Base::place(mover / kRowWords, mover % kRowWords);
         const auto land = [&](auto set, const TileOf& key_tile, const TileOf& value_tile) {
             constexpr int d = decltype(set)::value;
+            const auto place_in = [&](const TileOf& to, int k, int w) {
+                if constexpr (kRegular) return to.from(mover_place, k * kStepRows, w * kRowWords);
+                const int i = k * kMovers + mover;
+                return to.word(i / kRowWords, i % kRowWords + w * kRowWords);
+            };
 #pragma unroll
             for (int k = 0; k < kEach; k++) {
-                const int i = k * kMovers + (SHARED ? threadIdx.x : lane);
-                if (kKeys * kRowWords % kMovers != 0 && i >= kKeys * kRowWords) continue;
-                const int row = i / kRowWords, word = i % kRowWords;
+                if (kKeys * kRowWords % kMovers != 0 && k * kMovers + mover >= kKeys * kRowWords) continue;
                 if constexpr (QUANT) {
                     Words<M, 16> keys, values;
                     widened(key_words[d][k], keys);
                     widened(value_words[d][k], values);
 #pragma unroll
-                    for (int w = 0; w < 16 / E; w++) {
-                        *reinterpret_cast<uint4*>(key_tile.word(row, word + w * kRowWords)) = keys.w[w];
-                        *reinterpret_cast<uint4*>(value_tile.word(row, word + w * kRowWords)) = values.w[w];
+                    for (int w = 0; w < kSpread; w++) {
+                        *reinterpret_cast<uint4*>(place_in(key_tile, k, w)) = keys.w[w];
+                        *reinterpret_cast<uint4*>(place_in(value_tile, k, w)) = values.w[w];
                     }
                 } else {
-                    *reinterpret_cast<uint4*>(key_tile.word(row, word)) = key_words[d][k];
-                    *reinterpret_cast<uint4*>(value_tile.word(row, word)) = value_words[d][k];
+                    *reinterpret_cast<uint4*>(place_in(key_tile, k, 0)) = key_words[d][k];
+                    *reinterpret_cast<uint4*>(place_in(value_tile, k, 0)) = value_words[d][k];
                 }
             }
             if constexpr (QUANT) {
-                if (!SHARED || wave == 0) {
-#pragma unroll
-                    for (int n = 0; n < kScaleWords; n++) scales[stage][64 * n + lane] = entry_scale[d][n];
-                }
+                if (!SHARED || wave == 0) scales[stage][lane] = entry_scale[d];
             }
         };
-        uint32_t next_page[2];  // of the next tiles to fetch
         [[maybe_unused]] int pick = kFinite;
-        // The tile that is in `set`; of every `parity`-th page of the two.
+        // The tile that is in `set`; its next one's page is the `parity`-th.
         const auto turn = [&](auto set, auto parity, auto is_slow) {
             constexpr bool SLOW = decltype(is_slow)::value;
+            constexpr int d = decltype(set)::value, p = decltype(parity)::value;
+            // (Keys past `key_end` are seen by no row, or by none that is real.)
             const bool masked = tile + kKeys > least || tile + kKeys > key_end;
             const TileOf key_tile{tiles[stage]};
             const TileOf value_tile{tiles[stage] + TileOf::kBytes};
             if constexpr (kScaled) {
-                const auto& entry = entry_scale[decltype(set)::value];
-                const float high = wave64<Largest>(kKeys == 64 ? entry[kScaleWords - 1] : lane < 32 ? 0.0f : entry[0]);
+                const float high = wave64<Largest>(lane < 32 ? 0.0f : entry_scale[d]);
                 if (high >= unit && high < INFINITY) {
                     const float grown = ldexpf(1.0f, ilogbf(high) + 3);
-                    const float factor = unit / grown;
+                    const float kept = unit / grown;
                     unit = grown;
 #pragma unroll
-                    for (int r = 0; r < RB; r++) {
-#pragma unroll
-                        for (int t = 0; t < SIZE / 16; t++) acc[r][t] *= factor;
-                    }
+                    for (int t = 0; t < SIZE / 16; t++) acc[t] *= kept;
                 }
             }
             // A stage that a block shares was read before the last barrier; a
@@ -660,143 +666,106 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             else wave_order();
             const uint32_t next = tile + kAhead * kKeys;
             if (next < key_end) {
-                fetch(set, row_at(next, next_page[decltype(parity)::value]));
-                next_page[decltype(parity)::value] = page_at(next + 2 * kKeys);
+                fetch(set, row_at(next, next_page[p]));
+                next_page[p] = page_at(next + 2 * kKeys);
             }
             // Scores, and their maximum over the tile.
-            f32x4 scores[RB][kBlocks16];
+            f32x4 scores[kBlocks16];
+#pragma unroll
+            for (int b = 0; b < kBlocks16; b++) {
+                scores[b] = f32x4{};
+#pragma unroll
+                for (int n = 0; n < kOperands; n++) {
+                    scores[b] = product16<M>(key_tile.by_row(row_place, b, n), queries[n], scores[b]);
+                }
+                if constexpr (QUANT) scores[b] *= *reinterpret_cast<const f32x4*>(&scales[stage][16 * b + 4 * quarter]);
+            }
+            const auto sees = [&](int b, int i) { return tile + 16 * b + 4 * quarter + i < seen; };
+            if (masked) {
+#pragma unroll
+                for (int b = 0; b < kBlocks16; b++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) scores[b][i] = sees(b, i) ? scores[b][i] : -INFINITY;
+                }
+            }
+            float high = -INFINITY;
 #pragma unroll
             for (int b = 0; b < kBlocks16; b++) {
 #pragma unroll
-                for (int r = 0; r < RB; r++) scores[r][b] = f32x4{};
+                for (int i = 0; i < 4; i++) high = fmaxf(high, scores[b][i]);
+            }
+            high = quarters<Largest>(high) * factor;
+            // The maximum only moves when it grows past 2^8: the weights stay
+            // that small, and the sums are rarely rescaled.
+            const bool grows = high > most + 8.0f;
+            if (__ballot(grows) != 0) {
+                const float kept = grows ? power2(most - high) : 1.0f;
+                if (grows) most = high;
+                total *= kept;
 #pragma unroll
-                for (int n = 0; n < kOperands; n++) {
-                    const uint4 keys = key_tile.by_row(row_place, b, n);
+                for (int t = 0; t < SIZE / 16; t++) acc[t] *= kept;
+            }
+            const float origin = (most == -INFINITY ? 0.0f : most) - kPower;
 #pragma unroll
-                    for (int r = 0; r < RB; r++) scores[r][b] = product16<M>(keys, queries[r][n], scores[r][b]);
+            for (int b = 0; b < kBlocks16; b++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    scores[b][i] = power2(fmaf(scores[b][i], factor, -origin));
+                    total += scores[b][i];
                 }
                 if constexpr (QUANT) {
-                    const f32x4 scale = *reinterpret_cast<const f32x4*>(&scales[stage][16 * b + 4 * quarter]);
+                    f32x4 scale = *reinterpret_cast<const f32x4*>(&scales[stage][32 + 16 * b + 4 * quarter]);
+                    if constexpr (kScaled) scale *= 1.0f / unit;
+                    scores[b] *= scale;
+                    if (masked) {
+                        // (A scale may be a NaN.)
 #pragma unroll
-                    for (int r = 0; r < RB; r++) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) scores[r][b][i] *= scale[i];
-                    }
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < RB; r++) {
-                if (masked) {
-#pragma unroll
-                    for (int b = 0; b < kBlocks16; b++) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            if (tile + 16 * b + 4 * quarter + i >= seen[r]) scores[r][b][i] = -INFINITY;
-                        }
-                    }
-                }
-                float high = -INFINITY;
-#pragma unroll
-                for (int b = 0; b < kBlocks16; b++) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) high = fmaxf(high, scores[r][b][i]);
-                }
-                high = quarters<Largest>(high) * factors[r];
-                // The maximum only moves when it grows past 2^8: the weights
-                // stay that small, and the sums are rarely rescaled.
-                const bool grows = high > most[r] + 8.0f;
-                if (__ballot(grows) != 0) {
-                    const float factor = grows ? power2(most[r] - high) : 1.0f;
-                    if (grows) most[r] = high;
-                    total[r] *= factor;
-#pragma unroll
-                    for (int t = 0; t < SIZE / 16; t++) acc[r][t] *= factor;
-                }
-                const float origin = (most[r] == -INFINITY ? 0.0f : most[r]) - kPower;
-#pragma unroll
-                for (int b = 0; b < kBlocks16; b++) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        scores[r][b][i] = power2(fmaf(scores[r][b][i], factors[r], -origin));
-                        total[r] += scores[r][b][i];
-                    }
-                    if constexpr (QUANT) {
-                        const f32x4 scale = *reinterpret_cast<const f32x4*>(&scales[stage][(kKeys == 64 ? 64 : 32) + 16 * b + 4 * quarter]);
-                        const float against = kScaled ? 1.0f / unit : 1.0f;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) scores[r][b][i] *= scale[i] * against;
-                        if (masked) {
-                            // (A scale may be a NaN.)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                if (tile + 16 * b + 4 * quarter + i >= seen[r]) scores[r][b][i] = 0.0f;
-                            }
-                        }
+                        for (int i = 0; i < 4; i++) scores[b][i] = sees(b, i) ? scores[b][i] : 0.0f;
                     }
                 }
             }
             // The weights as operands, and their products with the values.
+            float v[E];
 #pragma unroll
-            for (int deep = 0; deep < kDeeps; deep++) {
-                uint4 high_part[RB], low_part[RB];
-#pragma unroll
-                for (int r = 0; r < RB; r++) {
-                    float v[E];
-#pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        const int b = deep * (kDeepKeys / 16) + e / 4;
-                        v[e] = scores[r][b][e % 4];
-                        if (SLOW && pick != kFinite) {
-                            const bool sees = tile + 16 * b + 4 * quarter + e % 4 < seen[r];
-                            v[e] = (pick == kNaN ? sees : pick == kZero ? sees && v[e] == 0.0f : v[e] != 0.0f) ? 1.0f : 0.0f;
-                        }
-                    }
-                    Words<M, E> high, low;
-                    high.put(v);
-                    high_part[r] = high.w[0];
-                    if constexpr (kTwoParts) {
-#pragma unroll
-                        for (int e = 0; e < E; e++) v[e] -= high.at(e);
-                        low.put(v);
-                        low_part[r] = low.w[0];
-                    }
+            for (int e = 0; e < E; e++) {
+                v[e] = scores[e / 4][e % 4];
+                if (SLOW && pick != kFinite) {
+                    const bool one = pick == kNaN    ? sees(e / 4, e % 4)
+                                     : pick == kZero ? sees(e / 4, e % 4) && v[e] == 0.0f
+                                                     : v[e] != 0.0f;
+                    v[e] = one ? 1.0f : 0.0f;
                 }
+            }
+            Words<M, E> high_part, low_part;
+            high_part.put(v);
+            if constexpr (kTwoParts) {
 #pragma unroll
-                for (int t = 0; t < SIZE / 16; t++) {
-                    uint4 values = value_tile.by_column(column_place, deep * kDeepKeys, t);
-                    if constexpr (SLOW) {
-                        values = make_uint4(picked(values.x, pick), picked(values.y, pick), picked(values.z, pick),
-                                            picked(values.w, pick));
-                    }
+                for (int e = 0; e < E; e++) v[e] -= high_part.at(e);
+                low_part.put(v);
+            }
 #pragma unroll
-                    for (int r = 0; r < RB; r++) {
-                        acc[r][t] = product16<M>(values, high_part[r], acc[r][t]);
-                        if constexpr (kTwoParts) acc[r][t] = product16<M>(values, low_part[r], acc[r][t]);
-                    }
+            for (int t = 0; t < SIZE / 16; t++) {
+                uint4 values = value_tile.by_column(column_place, t);
+                if constexpr (SLOW) {
+                    values = make_uint4(picked(values.x, pick), picked(values.y, pick), picked(values.z, pick),
+                                        picked(values.w, pick));
                 }
+                acc[t] = product16<M>(values, high_part.w[0], acc[t]);
+                if constexpr (kTwoParts) acc[t] = product16<M>(values, low_part.w[0], acc[t]);
             }
             tile += kKeys;
             if constexpr (SHARED) stage ^= 1;
         };
+        // Over the tiles, of which the first are on their way.
         const auto sweep = [&](auto is_slow) {
+            most = -INFINITY, total = 0.0f;
 #pragma unroll
-            for (int r = 0; r < RB; r++) {
-                most[r] = -INFINITY, total[r] = 0.0f;
-#pragma unroll
-                for (int t = 0; t < SIZE / 16; t++) acc[r][t] = f32x4{};
-            }
-            tile = tile_0 * kKeys;
-            // (Keys past `key_end` are seen by no row, or by none that is real.)
-            uint32_t pages[kAhead];
-            each<kAhead>([&](auto n) { pages[n.value] = page_at(tile + n.value * kKeys); });
-            next_page[0] = page_at(tile + kAhead * kKeys);
-            next_page[1] = page_at(tile + (kAhead + 1) * kKeys);
-            each<kAhead>([&](auto n) { fetch(n, row_at(tile + n.value * kKeys, pages[n.value])); });
+            for (int t = 0; t < SIZE / 16; t++) acc[t] = f32x4{};
             while (tile < key_end) {
                 each<(kAhead > 2 ? kAhead : 2)>([&](auto n) {
-                    constexpr int set = n.value % kAhead, parity = n.value % 2;
                     if (n.value == 0 || tile < key_end) {
-                        turn(std::integral_constant<int, set>(), std::integral_constant<int, parity>(), is_slow);
+                        turn(std::integral_constant<int, n.value % kAhead>(), std::integral_constant<int, n.value % 2>(),
+                             is_slow);
                     }
                 });
             }
@@ -809,77 +778,63 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             // that are seen, and at last without them.
             bool spoiled = false;
 #pragma unroll
-            for (int r = 0; r < RB; r++) {
+            for (int t = 0; t < SIZE / 16; t++) {
 #pragma unroll
-                for (int t = 0; t < SIZE / 16; t++) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) spoiled |= !(fabsf(acc[r][t][i]) < INFINITY);
-                }
+                for (int i = 0; i < 4; i++) spoiled |= !(fabsf(acc[t][i]) < INFINITY);
             }
             const bool any = SHARED ? __syncthreads_or(spoiled) != 0 : __ballot(spoiled) != 0;
             if (__builtin_expect(any, false)) {
-                uint32_t up[RB] = {}, down[RB] = {};  // a bit an element, both for a NaN
+                uint32_t up = 0, down = 0;  // a bit an element, both for a NaN
 #pragma unroll 1
                 for (pick = kZero; pick >= kFinite; pick--) {
+                    find_pages();
+                    fetch_first();
                     sweep(std::true_type());
                     if (pick == kFinite) break;
-#pragma unroll
-                    for (int r = 0; r < RB; r++) {
-                        uint32_t bits = 0;
-#pragma unroll
-                        for (int t = 0; t < SIZE / 16; t++) {
-#pragma unroll
-                            for (int i = 0; i < 4; i++) bits |= acc[r][t][i] > 0.0f ? 1u << (4 * t + i) : 0u;
-                        }
-                        if (pick != kMinus) up[r] |= bits;
-                        if (pick != kPlus) down[r] |= bits;
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < RB; r++) {
+                    uint32_t bits = 0;
 #pragma unroll
                     for (int t = 0; t < SIZE / 16; t++) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            if (up[r] >> (4 * t + i) & 1) acc[r][t][i] += INFINITY;
-                            if (down[r] >> (4 * t + i) & 1) acc[r][t][i] -= INFINITY;
-                        }
+                        for (int i = 0; i < 4; i++) bits |= acc[t][i] > 0.0f ? 1u << (4 * t + i) : 0u;
+                    }
+                    if (pick != kMinus) up |= bits;
+                    if (pick != kPlus) down |= bits;
+                }
+#pragma unroll
+                for (int t = 0; t < SIZE / 16; t++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (up >> (4 * t + i) & 1) acc[t][i] += INFINITY;
+                        if (down >> (4 * t + i) & 1) acc[t][i] -= INFINITY;
                     }
                 }
             }
         }
 
         // ---- the part's sums stored ----------------------------------------------------
+        const float all = quarters<Added>(total);
+        const float back = kScaled ? unit : 1.0f;
+        if (real && whole && final) {
+            // (A sum of 0 over keys that are seen is of scores of -infinity alone:
+            // 0 / 0.)
+            const float scale = back / all;
+            S* const to = static_cast<S*>(a.out) + token * a.out_steps.token + head * a.out_steps.head;
 #pragma unroll
-        for (int r = 0; r < RB; r++) {
-            const float all = quarters<Added>(total[r]);
-            const uint32_t row = row_of_lane(r);
-            if (row >= rows) continue;
-            const uint32_t number = first_row + row, place = a.group_of.div(number);
-            const uint32_t token = s.first + place, head = key_head * a.group + number - place * a.group;
-            const float back = kScaled ? unit : 1.0f;
-            if (whole && final) {
-                // (A sum of 0 over keys that are seen is of scores of -infinity
-                // alone: 0 / 0.)
-                const float scale = back / all;
-                S* const to = static_cast<S*>(a.out) + token * a.out_steps.token + head * a.out_steps.head;
-#pragma unroll
-                for (int t = 0; t < SIZE / 16; t++) {
-                    store_four(to, element_of(16 * t + 4 * quarter), a.pool.size, seen[r] > 0 ? acc[r][t] * scale : f32x4{});
-                }
-                if (quarter == 0 && a.normalizers != nullptr) {
-                    a.normalizers[uint64_t{head} * a.batch.tokens + token] =
-                        all == 0.0f ? -INFINITY : (most[r] + log2f(all) - kPower) * attention::kLn2;
-                }
-            } else {
-                const uint64_t to = whole ? uint64_t{token} * a.query_heads + head : uint64_t{slot} * ROWS + row;
-                float* const values = (whole ? parts.rows : parts.slots) + to * SIZE;
-#pragma unroll
-                for (int t = 0; t < SIZE / 16; t++) {
-                    *reinterpret_cast<f32x4*>(values + element_of(16 * t + 4 * quarter)) = acc[r][t] * back;
-                }
-                if (quarter == 0) (whole ? parts.row_stats : parts.slot_stats)[to] = make_float2(most[r], all);
+            for (int t = 0; t < SIZE / 16; t++) {
+                store_four(to, element_of(16 * t + 4 * quarter), a.pool.size, seen > 0 ? acc[t] * scale : f32x4{});
             }
+            if (quarter == 0 && a.normalizers != nullptr) {
+                a.normalizers[uint64_t{head} * a.batch.tokens + token] =
+                    all == 0.0f ? -INFINITY : (most + log2f(all) - kPower) * attention::kLn2;
+            }
+        } else if (real) {
+            const uint64_t to = whole ? uint64_t{token} * a.query_heads + head : uint64_t{slot} * ROWS + row;
+            float* const values = (whole ? parts.rows : parts.slots) + to * SIZE;
+#pragma unroll
+            for (int t = 0; t < SIZE / 16; t++) {
+                *reinterpret_cast<f32x4*>(values + element_of(16 * t + 4 * quarter)) = acc[t] * back;
+            }
+            if (quarter == 0) (whole ? parts.row_stats : parts.slot_stats)[to] = make_float2(most, all);
         }
         at += tile_1 - tile_0;
     }
@@ -899,44 +854,30 @@ __global__ void __launch_bounds__(kAttendThreads)
     for (uint64_t at = uint64_t{blockIdx.x} * kRows + threadIdx.x / 64 / WAVES; at < all_rows; at += apart) {
         const uint32_t row = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at));
         const uint32_t token = row / a.query_heads, head = row % a.query_heads;
-        const uint32_t key_head = a.group_of.div(head), within = head - key_head * a.group;
+        // What is read of a row that no worker had is not used: its sequence has
+        // no keys.
+        const Found mine = own.found[row];
+        const Found shared = a.batch.prefix > 0 ? prefix.found[row] : Found{1, 0, 0, 0};
         Span span{0, 0};
         const uint32_t sequence = wave_sequence_of(a.batch, token, &span);
-
-        // A line's parts of the row: n of them, the first in `first_slot`, or
-        // the one of a whole item.
-        struct Found {
-            uint32_t n = 0, first_worker = 0, first_slot = 0, line = 0, within = 0;
-            bool whole = false;
-        } mine, shared;
+        uint32_t mine_count = 0, count = 0;
         bool sees = false;
         if (sequence != kNowhere) {
             const Sequence s = sequence_at<false>(a, sequence);
-            const uint32_t place = token - s.first, left = s.tokens - place;
-            const auto find = [&](const Parts& parts, uint32_t rows, uint32_t workers, uint64_t first, uint32_t number,
-                                  uint32_t tokens) {
-                Found f;
-                const uint32_t row_blocks = static_cast<uint32_t>((uint64_t{tokens} * a.group + rows - 1) / rows);
-                const Plan plan = parts.plans[first + uint64_t{key_head} * row_blocks + number / rows];
-                f.whole = plan.whole != 0;
-                f.n = f.whole ? 1 : plan.first <= plan.last && plan.last < workers ? plan.last - plan.first + 1 : 0;
-                f.first_worker = plan.first, f.first_slot = plan.slot;
-                f.line = rows, f.within = number % rows;
-                return f;
+            const uint32_t left = s.first + s.tokens - token;
+            const auto count_of = [](const Found& f, uint32_t workers) {
+                return f.whole ? 1 : f.first <= f.last && f.last < workers ? f.last - f.first + 1 : 0;
             };
-            if (s.keys > 0) {
-                mine = find(own, own_rows, own_workers, first_item(a, own_rows, sequence, s.first),
-                            place * a.group + within, s.tokens);
-                sees = seen_of(s.length, left, 0, s.keys) > 0;
-            }
+            if (s.keys > 0) mine_count = count_of(mine, own_workers);
+            count = mine_count;
+            sees = seen_of(s.length, left, 0, s.keys) > 0;
             if (a.batch.prefix > 0) {
-                shared = find(prefix, prefix_rows, prefix_workers, 0, token * a.group + within, a.batch.tokens);
+                count += count_of(shared, prefix_workers);
                 sees = sees || seen_of(s.length, left, a.batch.prefix, a.batch.prefix) > 0;
             }
         }
-        const uint32_t count = mine.n + shared.n;
         // A whole item without a prefix is a result already.
-        if (count == 1 && mine.whole && a.batch.prefix == 0) continue;
+        if (count == 1 && mine_count == 1 && mine.whole && a.batch.prefix == 0) continue;
 
         const uint32_t half = threadIdx.x % 64 / 32, column = threadIdx.x % 32 * 4;
         float top = -INFINITY, total = 0.0f;
@@ -952,12 +893,11 @@ __global__ void __launch_bounds__(kAttendThreads)
                 stats[k] = make_float2(-INFINITY, 0.0f);
                 values[k] = f32x4{};
                 if (i >= count) continue;
-                const bool is_mine = i < mine.n;
+                const bool is_mine = i < mine_count;
                 const Found& f = is_mine ? mine : shared;
                 const Parts& parts = is_mine ? own : prefix;
-                const uint32_t n = is_mine ? i : i - mine.n;
-                const uint64_t slot = n == 0 ? f.first_slot : uint64_t{2} * (f.first_worker + n);
-                const uint64_t place = f.whole ? row : slot * f.line + f.within;
+                const uint32_t n = is_mine ? i : i - mine_count, line = is_mine ? own_rows : prefix_rows;
+                const uint64_t place = f.whole ? row : n == 0 ? f.place : uint64_t{2 * (f.first + n)} * line + f.place % line;
                 stats[k] = (f.whole ? parts.row_stats : parts.slot_stats)[place];
                 if (column < SIZE) {
                     values[k] =
@@ -1018,52 +958,41 @@ __global__ void __launch_bounds__(kAttendThreads)
         constexpr int SIZE = 128; __VA_ARGS__;          \
     }
 
-template <int SIZE, int FORM, bool QUANT>
-void attend_form(const Attention& a, const Parts& parts, bool prefix, bool final, uint32_t blocks, hipStream_t s) {
-    if (prefix) {
-        attend_kernel<SIZE, FORM, QUANT, true><<<blocks, kAttendThreads, 0, s>>>(a, parts, false);
-    } else {
-        attend_kernel<SIZE, FORM, QUANT, false><<<blocks, kAttendThreads, 0, s>>>(a, parts, final);
-    }
-}
-
 template <int SIZE, bool QUANT>
-void attend_size(const Attention& a, const Parts& parts, bool prefix, bool final, int form, uint32_t blocks,
-                 hipStream_t s) {
-    if (form == kRows16) {
-        attend_form<SIZE, kRows16, QUANT>(a, parts, prefix, final, blocks, s);
-    } else if (form == kRows32) {
-        attend_form<SIZE, kRows32, QUANT>(a, parts, prefix, final, blocks, s);
-    } else {
-        attend_form<SIZE, kRows128, QUANT>(a, parts, prefix, final, blocks, s);
-    }
+void attend_size(const Attention& a, const Parts& parts, bool prefix, bool final, bool shared, hipStream_t s) {
+    const uint32_t blocks = static_cast<uint32_t>(compute_units()) * blocks_of_form(shared);
+    const auto kernel = shared ? prefix ? attend_kernel<SIZE, true, QUANT, true> : attend_kernel<SIZE, true, QUANT, false>
+                        : prefix ? attend_kernel<SIZE, false, QUANT, true>
+                                 : attend_kernel<SIZE, false, QUANT, false>;
+    kernel<<<blocks, kAttendThreads, 0, s>>>(a, parts, final);
 }
 
-int attend(const Attention& a, const Parts& parts, bool quant, bool prefix, bool final, int form, uint32_t blocks) {
+int attend(const Attention& a, const Parts& parts, bool quant, bool prefix, bool final, bool shared) {
     TC_STREAM(s);
     TC_CACHE_SIZE(a.pool.size, {
         if (quant) {
-            attend_size<SIZE, true>(a, parts, prefix, final, form, blocks, s);
+            attend_size<SIZE, true>(a, parts, prefix, final, shared, s);
         } else {
-            attend_size<SIZE, false>(a, parts, prefix, final, form, blocks, s);
+            attend_size<SIZE, false>(a, parts, prefix, final, shared, s);
         }
     })
     return check_launch("cache attention");
 }
 
-int join(const Attention& a, const Parts& own, const Parts& prefix, bool quant, int own_form, int prefix_form,
-         uint32_t blocks) {
+int join(const Attention& a, const Parts& own, const Parts& prefix, bool quant, bool own_shared, bool prefix_shared) {
     TC_STREAM(s);
+    const uint32_t units = static_cast<uint32_t>(compute_units());
     const uint64_t rows = uint64_t{a.batch.tokens} * a.query_heads;
     // A block a row where rows are few and their parts, therefore, many.
-    const bool few = rows <= static_cast<uint64_t>(compute_units()) * 4;
+    const bool few = rows <= uint64_t{units} * 4;
     const uint64_t turns = few ? rows : (rows + kAttendWaves - 1) / kAttendWaves;
     const uint32_t grid = turns < (1u << 20) ? static_cast<uint32_t>(turns) : 1u << 20;
     const float power = sizeof(S) == 2 && (quant || kHalf) ? kHalfPower : 0.0f;
     TC_CACHE_SIZE(a.pool.size, {
         const auto kernel = few ? join_kernel<SIZE, kAttendWaves> : join_kernel<SIZE, 1>;
-        kernel<<<grid, kAttendThreads, 0, s>>>(a, own, prefix, rows_of_form(own_form), rows_of_form(prefix_form),
-                                               workers_of(own_form, blocks), workers_of(prefix_form, blocks), power);
+        kernel<<<grid, kAttendThreads, 0, s>>>(a, own, prefix, rows_of_form(own_shared), rows_of_form(prefix_shared),
+                                               units * workers_of_form(own_shared),
+                                               units * workers_of_form(prefix_shared), power);
     })
     return check_launch("cache attention");
 }
