@@ -9,8 +9,8 @@
 // three bits of fraction by up to |x| / 16.)
 //
 // Bound by memory, or for a few tokens by the chain of reads that finds a
-// row's place (offsets, length, page).  A wave takes a token's rows, so that
-// this chain is walked once for several of them: 16 lanes hold a row, 8
+// row's place (offsets, length, page).  A block takes a few tokens' rows, so
+// that this chain is walked once for many of them: 16 lanes hold a row, 8
 // elements each, and the largest magnitude is taken in registers.
 
 #include "cache.hpp"
@@ -30,6 +30,9 @@ int check_pool(const std::string& what, const tc_cache* given, Pool* pool) {
     if (c.key_heads == 0 || c.head_size == 0) return fail(TC_INVALID, what + ": heads of no elements");
     if (c.head_size > 128) {
         return fail(TC_UNSUPPORTED, what + ": heads of " + std::to_string(c.head_size) + " elements, more than 128");
+    }
+    if (c.key_heads > (1u << 24)) {  // twice as many rows of a block's tokens are counted in 32 bits
+        return fail(TC_UNSUPPORTED, what + ": " + std::to_string(c.key_heads) + " key heads");
     }
     if (c.page_size == 0) return fail(TC_INVALID, what + ": pages of no tokens");
     uint64_t rows = 0;
@@ -82,7 +85,8 @@ int check_batch(const std::string& what, const tc_cache_batch* given, const Pool
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kAtOnce = 4;  // rows whose loads a lane has in flight
+constexpr int kGroups = kThreads / 16;  // rows that a block holds at a time
+constexpr int kAtOnce = 2;  // pairs of rows whose loads a lane has in flight
 
 // Where the call's rows lie outside the cache.
 template <typename P>
@@ -122,165 +126,243 @@ __device__ __forceinline__ void store_eight(S* row, uint32_t lane, uint32_t size
     }
 }
 
-// A wave's token and its share of the token's rows, keys before values.
-struct Share {
-    uint32_t token, part;
-};
-__device__ __forceinline__ Share share_of(uint64_t unit, uint32_t parts) {
-    return {static_cast<uint32_t>(unit / parts), static_cast<uint32_t>(unit % parts)};
-}
-
-// The place of the token's position in its sequence: the sequence and the
-// position, or kNowhere.
-struct Place {
-    uint32_t sequence, at;
-};
-__device__ __forceinline__ Place place_of(const Batch& batch, uint32_t token) {
-    Span span;
-    const uint32_t sequence = wave_sequence_of(batch, token, &span);
-    if (sequence == kNowhere) return {kNowhere, 0};
+// The row of a token's first head in the pool, kNowhere if the token has no
+// place; `sequence` has it, `end` is past the sequence's last token here.
+__device__ __forceinline__ uint32_t row_of_token(const Pool& pool, const Batch& batch, uint32_t sequence, uint32_t token,
+                                                 uint32_t end) {
+    if (sequence == kNowhere) return kNowhere;
     // The sequence's tokens here are its last.
-    const uint32_t length = batch.lengths[sequence], left = span.end - token;
-    return length < left ? Place{kNowhere, 0} : Place{sequence, length - left};
+    const uint32_t length = batch.lengths[sequence], left = end - token;
+    if (length < left) return kNowhere;
+    return row_of(pool, batch.pages + uint64_t{sequence} * batch.most_pages, batch.most_pages, 0, length - left);
 }
 
+constexpr uint32_t kMostTokens = 8;  // of a block at a time
+
+// A block's tokens at a time, and the row in the pool of each one's first head:
+// of a single token found by each wave, of several by a thread each, which goes
+// on from the first token's sequence (each step a read that the next one waits
+// for, so that few of them count more than many lanes).
+struct Tokens {
+    uint64_t first;
+    uint32_t here;
+
+    __device__ __forceinline__ void find(const Pool& pool, const Batch& batch, uint32_t per_block, uint32_t* found,
+                                         uint32_t* only) const {
+        Span span{0, 0};
+        uint32_t token = static_cast<uint32_t>(first);
+        if (per_block == 1) {
+            const uint32_t sequence = wave_sequence_of(batch, token, &span);
+            *only = row_of_token(pool, batch, sequence, token, span.end);
+            return;
+        }
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            uint32_t sequence = wave_sequence_of(batch, token, &span);
+            if (threadIdx.x < here) {
+                token += threadIdx.x;
+                if (sequence != kNowhere && token >= span.end && sequence + 1 < batch.sequences) {
+                    sequence++;
+                    span = span_of(batch, sequence);
+                }
+                if (sequence == kNowhere || token < span.first || token >= span.end) {
+                    sequence = sequence_of(batch, token, &span);
+                }
+                found[threadIdx.x] = row_of_token(pool, batch, sequence, token, span.end);
+            }
+        }
+        __syncthreads();
+    }
+};
+
+// The largest magnitude's bits of 8 elements, in 32 bits: past those of the
+// largest finite number where one is an infinity or a NaN.
+template <typename S>
+__device__ __forceinline__ float largest_of(const Words<S, 8>& words) {
+    const uint32_t* const w = reinterpret_cast<const uint32_t*>(words.w);
+    if constexpr (sizeof(S) == 2) {
+        typedef uint16_t pair __attribute__((ext_vector_type(2)));
+        pair most = __builtin_bit_cast(pair, w[0] & 0x7fff7fffu);
+#pragma unroll
+        for (int n = 1; n < 4; n++) most = __builtin_elementwise_max(most, __builtin_bit_cast(pair, w[n] & 0x7fff7fffu));
+        const uint16_t bits = most.x > most.y ? most.x : most.y;
+        return Elem<S>::widen(__builtin_bit_cast(S, bits));
+    } else {
+        float most = 0.0f;
+#pragma unroll
+        for (int n = 0; n < 8; n++) most = LargestBits::join(most, __uint_as_float(w[n] & 0x7fffffffu));
+        return most;
+    }
+}
+
+// round(v / scale) as 8 whole numbers of 8 bits.  The quotients' nearest whole
+// numbers are those of the products with an approximate reciprocal, which are
+// off by less than 127 * 2^-22, unless one lies next to the middle of two: then,
+// and where the reciprocal is no number, the quotients themselves are rounded.
+// Adding 1.5 * 2^23 rounds to a whole number, ties to even, and leaves it in the
+// sum's last bits.  (Quotients alone took 56 us for 16001 tokens of 16 rows of
+// 128 f16 elements.)
+__device__ __forceinline__ uint2 quantised(const float (&v)[8], float scale) {
+    constexpr float kWhole = 12582912.0f;
+    const float reciprocal = __builtin_amdgcn_rcpf(scale);
+    uint32_t bits[8];
+    float off = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float t = v[e] * reciprocal, sum = t + kWhole;
+        bits[e] = __float_as_uint(sum);
+        off = fmaxf(off, fabsf(t - (sum - kWhole)));
+    }
+    // (With a scale of 2^-120 or more the reciprocal is a normal number.)
+    if (!(scale >= 0x1p-120f) || off > 0.49995f) {
+        const bool some = scale > 0.0f;  // neither 0 nor a NaN
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float q = some ? fminf(fmaxf(rintf(v[e] / scale), -127.0f), 127.0f) : 0.0f;
+            bits[e] = static_cast<uint32_t>(static_cast<int>(q));
+        }
+    }
+    // The last bytes of four, in order.
+    const auto four = [&](int n) {
+        return __builtin_amdgcn_perm(bits[n + 1], bits[n], 0x0c0c0400u) |
+               __builtin_amdgcn_perm(bits[n + 3], bits[n + 2], 0x04000c0cu);
+    };
+    return make_uint2(four(0), four(4));
+}
+
+// Both rows of a token's head at a time, that of its key and that of its value:
+// their place in the pool is the same.
 template <typename S, bool QUANT>
 __global__ void __launch_bounds__(kThreads)
-    write_kernel(const Pool pool, const Batch batch, const Rows<const S*> rows, uint32_t parts) {
-    const uint32_t lane = threadIdx.x % 16, turn = threadIdx.x % 64 / 16;
-    const uint64_t units = uint64_t{batch.tokens} * parts, waves = uint64_t{gridDim.x} * (kThreads / 64);
-    for (uint64_t unit = uint64_t{blockIdx.x} * (kThreads / 64) + threadIdx.x / 64; unit < units; unit += waves) {
-        const Share share = share_of(unit, parts);
-        const Place place = place_of(batch, share.token);
-        if (place.sequence == kNowhere) continue;
-        const uint32_t first = row_of(pool, batch.pages + uint64_t{place.sequence} * batch.most_pages,
-                                      batch.most_pages, 0, place.at);
-        if (first == kNowhere) continue;
-        for (uint32_t base = share.part * 4; base < 2 * pool.heads; base += parts * 4 * kAtOnce) {
-            Words<S, 8> words[kAtOnce];
+    write_kernel(const Pool pool, const Batch batch, const Rows<const S*> rows, uint32_t per_block) {
+    __shared__ uint32_t found[kMostTokens];
+    const uint32_t lane = threadIdx.x % 16, group = threadIdx.x / 16;
+    const Steps steps[2] = {rows.key_steps, rows.value_steps};
+    for (uint64_t first = uint64_t{blockIdx.x} * per_block; first < batch.tokens; first += uint64_t{gridDim.x} * per_block) {
+        const Tokens tokens{first, static_cast<uint32_t>(batch.tokens - first < per_block ? batch.tokens - first : per_block)};
+        uint32_t only = kNowhere;
+        RowWalk<2, kGroups> from(pool.heads, steps, group, first), to = from;
+        Words<S, 8> keys[kAtOnce], values[kAtOnce];
+        const auto load = [&]() {
 #pragma unroll
-            for (int k = 0; k < kAtOnce; k++) {
-                const uint32_t n = base + k * parts * 4 + turn;
-                if (n >= 2 * pool.heads) continue;
-                const bool key = n < pool.heads;
-                const uint32_t head = key ? n : n - pool.heads;
-                const Steps steps = key ? rows.key_steps : rows.value_steps;
-                load_eight((key ? rows.key : rows.value) + share.token * steps.token + head * steps.head, lane,
-                           pool.size, words[k]);
+            for (int k = 0; k < kAtOnce; k++, from.move()) {
+                if (from.token >= tokens.here) continue;
+                load_eight(rows.key + from.at[0], lane, pool.size, keys[k]);
+                load_eight(rows.value + from.at[1], lane, pool.size, values[k]);
             }
+        };
+        const auto put = [&](const Words<S, 8>& words, void* entries, float* scales, uint32_t row) {
+            if constexpr (QUANT) {
+                const float most = row16<LargestBits>(largest_of(words));
+                const bool finite = __float_as_uint(most) < 0x7f800000u;
+                const float scale = finite ? most / 127.0f : __uint_as_float(0x7fc00000u);
+                float v[8];
+                words.get(v);
+                const uint2 packed = quantised(v, scale);
+                if (8 * lane < pool.row) {
+                    *reinterpret_cast<uint2*>(static_cast<char*>(entries) + uint64_t{row} * pool.row + 8 * lane) = packed;
+                }
+                if (lane == 0) scales[row] = scale;
+            } else {
+                S* const at_row = static_cast<S*>(entries) + uint64_t{row} * pool.row + 8 * lane;
 #pragma unroll
-            for (int k = 0; k < kAtOnce; k++) {
-                const uint32_t n = base + k * parts * 4 + turn;
-                if (n >= 2 * pool.heads) continue;
-                const bool key = n < pool.heads;
-                const uint32_t row = first + (key ? n : n - pool.heads) * pool.page_size;
-                void* const entries = key ? pool.keys : pool.values;
-                if constexpr (QUANT) {
-                    float v[8], most = 0.0f;
-                    words[k].get(v);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) most = LargestBits::join(most, fabsf(v[e]));
-                    most = row16<LargestBits>(most);
-                    // Bits past the largest finite number's: an infinity or a NaN.
-                    const bool finite = __float_as_uint(most) < 0x7f800000u;
-                    const float scale = finite ? most / 127.0f : __uint_as_float(0x7fc00000u);
-                    uint32_t packed[2] = {0, 0};
-                    if (finite && scale > 0.0f) {
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const float q = fminf(fmaxf(rintf(v[e] / scale), -127.0f), 127.0f);
-                            packed[e / 4] |= (static_cast<uint32_t>(static_cast<int>(q)) & 0xffu) << (8 * (e % 4));
-                        }
-                    }
-                    if (8 * lane < pool.row) {
-                        *reinterpret_cast<uint2*>(static_cast<char*>(entries) + uint64_t{row} * pool.row + 8 * lane) =
-                            make_uint2(packed[0], packed[1]);
-                    }
-                    if (lane == 0) (key ? pool.key_scales : pool.value_scales)[row] = scale;
-                } else {
-                    S* const to = static_cast<S*>(entries) + uint64_t{row} * pool.row + 8 * lane;
-#pragma unroll
-                    for (int w = 0; w < Words<S, 8>::kCount; w++) {
-                        if (8 * lane + w * kWordElements<S> < pool.row) {
-                            store_word<false>(to + w * kWordElements<S>, words[k].w[w]);
-                        }
+                for (int w = 0; w < Words<S, 8>::kCount; w++) {
+                    if (8 * lane + w * kWordElements<S> < pool.row) {
+                        store_word<false>(at_row + w * kWordElements<S>, words.w[w]);
                     }
                 }
             }
+        };
+        // (The places are found while the first rows are on their way.)
+        load();
+        tokens.find(pool, batch, per_block, found, &only);
+        while (to.token < tokens.here) {
+#pragma unroll
+            for (int k = 0; k < kAtOnce; k++, to.move()) {
+                if (to.token >= tokens.here) continue;
+                const uint32_t at = per_block == 1 ? only : found[to.token];
+                if (at == kNowhere) continue;
+                const uint32_t row = at + to.head * pool.page_size;
+                put(keys[k], pool.keys, pool.key_scales, row);
+                put(values[k], pool.values, pool.value_scales, row);
+            }
+            if (to.token < tokens.here) load();
         }
     }
 }
 
 template <typename S, bool QUANT>
 __global__ void __launch_bounds__(kThreads)
-    read_kernel(const Pool pool, const Batch batch, const Rows<S*> rows, uint32_t parts) {
-    const uint32_t lane = threadIdx.x % 16, turn = threadIdx.x % 64 / 16;
-    const uint64_t units = uint64_t{batch.tokens} * parts, waves = uint64_t{gridDim.x} * (kThreads / 64);
-    for (uint64_t unit = uint64_t{blockIdx.x} * (kThreads / 64) + threadIdx.x / 64; unit < units; unit += waves) {
-        const Share share = share_of(unit, parts);
-        const Place place = place_of(batch, share.token);
-        const uint32_t first = place.sequence == kNowhere
-                                   ? kNowhere
-                                   : row_of(pool, batch.pages + uint64_t{place.sequence} * batch.most_pages,
-                                            batch.most_pages, 0, place.at);
-        for (uint32_t base = share.part * 4; base < 2 * pool.heads; base += parts * 4 * kAtOnce) {
-            Words<S, 8> words[kAtOnce];
-            uint2 packed[kAtOnce];
-            float scales[kAtOnce];
+    read_kernel(const Pool pool, const Batch batch, const Rows<S*> rows, uint32_t per_block) {
+    __shared__ uint32_t found[kMostTokens];
+    const uint32_t lane = threadIdx.x % 16, group = threadIdx.x / 16;
+    const Steps steps[2] = {rows.key_steps, rows.value_steps};
+    struct Entries {
+        Words<S, 8> words;
+        uint2 packed;
+        float scale;
+    };
+    const auto get = [&](const void* entries, const float* scales, uint32_t row, bool some, Entries& out) {
+        out.packed = make_uint2(0, 0), out.scale = 0.0f;
 #pragma unroll
-            for (int k = 0; k < kAtOnce; k++) {
-                const uint32_t n = base + k * parts * 4 + turn;
-                packed[k] = make_uint2(0, 0), scales[k] = 0.0f;
+        for (int w = 0; w < Words<S, 8>::kCount; w++) out.words.w[w] = make_uint4(0, 0, 0, 0);
+        if (!some) return;
+        if constexpr (QUANT) {
+            if (8 * lane < pool.row) {
+                out.packed = *reinterpret_cast<const uint2*>(static_cast<const char*>(entries) + uint64_t{row} * pool.row +
+                                                             8 * lane);
+            }
+            out.scale = scales[row];
+        } else {
+            const S* const at_row = static_cast<const S*>(entries) + uint64_t{row} * pool.row + 8 * lane;
 #pragma unroll
-                for (int w = 0; w < Words<S, 8>::kCount; w++) words[k].w[w] = make_uint4(0, 0, 0, 0);
-                if (n >= 2 * pool.heads || first == kNowhere) continue;
-                const bool key = n < pool.heads;
-                const uint32_t row = first + (key ? n : n - pool.heads) * pool.page_size;
-                const void* const entries = key ? pool.keys : pool.values;
-                if constexpr (QUANT) {
-                    if (8 * lane < pool.row) {
-                        packed[k] = *reinterpret_cast<const uint2*>(static_cast<const char*>(entries) +
-                                                                    uint64_t{row} * pool.row + 8 * lane);
-                    }
-                    scales[k] = (key ? pool.key_scales : pool.value_scales)[row];
-                } else {
-                    const S* const from = static_cast<const S*>(entries) + uint64_t{row} * pool.row + 8 * lane;
-#pragma unroll
-                    for (int w = 0; w < Words<S, 8>::kCount; w++) {
-                        if (8 * lane + w * kWordElements<S> < pool.row) {
-                            words[k].w[w] = load_word<false>(from + w * kWordElements<S>);
-                        }
-                    }
+            for (int w = 0; w < Words<S, 8>::kCount; w++) {
+                if (8 * lane + w * kWordElements<S> < pool.row) {
+                    out.words.w[w] = load_word<false>(at_row + w * kWordElements<S>);
                 }
             }
+        }
+    };
+    const auto put = [&](Entries& in, S* row) {
+        if constexpr (QUANT) {
+            float v[8];
 #pragma unroll
-            for (int k = 0; k < kAtOnce; k++) {
-                const uint32_t n = base + k * parts * 4 + turn;
-                if (n >= 2 * pool.heads) continue;
-                if constexpr (QUANT) {
-                    float v[8];
+            for (int e = 0; e < 8; e++) {
+                const uint32_t four = e < 4 ? in.packed.x : in.packed.y;
+                v[e] = static_cast<float>(static_cast<int8_t>(four >> (8 * (e % 4)))) * in.scale;
+            }
+            in.words.put(v);
+        }
+        store_eight(row, lane, pool.size, in.words);
+    };
+    for (uint64_t first = uint64_t{blockIdx.x} * per_block; first < batch.tokens; first += uint64_t{gridDim.x} * per_block) {
+        const Tokens tokens{first, static_cast<uint32_t>(batch.tokens - first < per_block ? batch.tokens - first : per_block)};
+        uint32_t only = kNowhere;
+        tokens.find(pool, batch, per_block, found, &only);
+        RowWalk<2, kGroups> from(pool.heads, steps, group, first), to = from;
+        while (to.token < tokens.here) {
+            Entries keys[kAtOnce], values[kAtOnce];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const uint32_t four = e < 4 ? packed[k].x : packed[k].y;
-                        v[e] = static_cast<float>(static_cast<int8_t>(four >> (8 * (e % 4)))) * scales[k];
-                    }
-                    words[k].put(v);
-                }
-                const bool key = n < pool.heads;
-                const uint32_t head = key ? n : n - pool.heads;
-                const Steps steps = key ? rows.key_steps : rows.value_steps;
-                store_eight((key ? rows.key : rows.value) + share.token * steps.token + head * steps.head, lane,
-                            pool.size, words[k]);
+            for (int k = 0; k < kAtOnce; k++, from.move()) {
+                const uint32_t at = from.token >= tokens.here ? kNowhere : per_block == 1 ? only : found[from.token];
+                const uint32_t row = at + from.head * pool.page_size;
+                get(pool.keys, pool.key_scales, row, at != kNowhere, keys[k]);
+                get(pool.values, pool.value_scales, row, at != kNowhere, values[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < kAtOnce; k++, to.move()) {
+                if (to.token >= tokens.here) continue;
+                put(keys[k], rows.key + to.at[0]);
+                put(values[k], rows.value + to.at[1]);
             }
         }
     }
 }
 
-// The waves that share a token's rows: all that can where tokens are few, one
-// where they fill the chip.
-uint32_t parts_of(const Pool& pool, const Batch& batch) {
-    const uint32_t most = (2 * pool.heads + 3) / 4;
-    return batch.tokens >= static_cast<uint32_t>(compute_units()) * 8 ? 1 : most;
+// The tokens of a block at a time: one where tokens are few, several where
+// blocks of them fill the chip.
+uint32_t per_block_of(const Batch& batch) {
+    return batch.tokens >= static_cast<uint32_t>(compute_units()) * 2 * kMostTokens ? kMostTokens : 1;
 }
 
 // What both calls check; `*nothing` if there is nothing to do.
@@ -341,15 +423,15 @@ int tc_cache_write(const tc_cache* cache, const tc_cache_batch* batch, const voi
     if (status == TC_OK) status = cache::check_storage(what, *cache, pool);
     if (status != TC_OK || nothing) return status;
     TC_STREAM(s);
-    const uint32_t parts = cache::parts_of(pool, checked);
-    const uint32_t blocks = grid_for(uint64_t{checked.tokens} * parts, cache::kThreads / 64, 32);
+    const uint32_t per_block = cache::per_block_of(checked);
+    const uint32_t blocks = grid_for(checked.tokens, per_block, 32);
     TC_DISPATCH_FLOAT(cache->dtype, what, S, {
         const cache::Rows<const S*> rows{static_cast<const S*>(key), static_cast<const S*>(value), key_steps,
                                          value_steps};
         if (cache->format == TC_CACHE_INT8) {
-            cache::write_kernel<S, true><<<blocks, cache::kThreads, 0, s>>>(pool, checked, rows, parts);
+            cache::write_kernel<S, true><<<blocks, cache::kThreads, 0, s>>>(pool, checked, rows, per_block);
         } else {
-            cache::write_kernel<S, false><<<blocks, cache::kThreads, 0, s>>>(pool, checked, rows, parts);
+            cache::write_kernel<S, false><<<blocks, cache::kThreads, 0, s>>>(pool, checked, rows, per_block);
         }
     })
     return check_launch(what);
@@ -366,14 +448,14 @@ int tc_cache_read(const tc_cache* cache, const tc_cache_batch* batch, void* key,
     if (status == TC_OK) status = cache::check_storage(what, *cache, pool);
     if (status != TC_OK || nothing) return status;
     TC_STREAM(s);
-    const uint32_t parts = cache::parts_of(pool, checked);
-    const uint32_t blocks = grid_for(uint64_t{checked.tokens} * parts, cache::kThreads / 64, 32);
+    const uint32_t per_block = cache::per_block_of(checked);
+    const uint32_t blocks = grid_for(checked.tokens, per_block, 32);
     TC_DISPATCH_FLOAT(cache->dtype, what, S, {
         const cache::Rows<S*> rows{static_cast<S*>(key), static_cast<S*>(value), key_steps, value_steps};
         if (cache->format == TC_CACHE_INT8) {
-            cache::read_kernel<S, true><<<blocks, cache::kThreads, 0, s>>>(pool, checked, rows, parts);
+            cache::read_kernel<S, true><<<blocks, cache::kThreads, 0, s>>>(pool, checked, rows, per_block);
         } else {
-            cache::read_kernel<S, false><<<blocks, cache::kThreads, 0, s>>>(pool, checked, rows, parts);
+            cache::read_kernel<S, false><<<blocks, cache::kThreads, 0, s>>>(pool, checked, rows, per_block);
         }
     })
     return check_launch(what);

@@ -39,7 +39,7 @@ int run(const AttentionLaunches& launches, const Attention& a, bool quant) {
     const uint64_t sequences = a.batch.sequences;
     const bool own_shared = shares(tokens * a.group / (sequences > 0 ? sequences : 1));
     const bool prefix_shared = shares(tokens * a.group);
-    const auto slot_rows = [&](bool form) { return 2 * units * workers_of_form(form) * rows_of_form(form); };
+    const auto slot_rows = [&](bool form) { return 2 * units * blocks_of_form(form) * rows_of_form(form); };
     const Storage own(slot_rows(own_shared), prefix ? rows : 0, rows, size);
     const Storage shared(prefix ? slot_rows(prefix_shared) : 0, prefix ? rows : 0, prefix ? rows : 0, size);
     if (own.status() != TC_OK) return own.status();

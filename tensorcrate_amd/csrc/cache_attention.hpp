@@ -16,22 +16,24 @@
 // of query rows as all tokens' heads fill: its keys are read once for each of
 // those and not for each sequence.
 //
-// A wave holds 16 query rows (token and head of a key head's group) or 32 as
-// the columns of 16 x 16 products.  s transposed is k . q^T, so that a lane has
-// 4 keys of a row in each product's result, and those registers are the operand
-// of o^T = v^T . p^T.  Keys and values go through registers to the wave's own
-// tile in LDS, since rows on pages have no step between them and 8-bit entries
-// are widened on the way; the next tile's rows are in flight meanwhile.  Where
-// more rows than 32 share keys, a block's four waves hold 128 of them and share
-// each tile (SHARED): the widening is done once for all of them.
+// A wave holds 16 query rows (token and head of a key head's group) as the
+// columns of 16 x 16 products.  s transposed is k . q^T, so that a lane has 4
+// keys of a row in each product's result, and those registers are the operand of
+// o^T = v^T . p^T.  Keys and values go through registers to a tile in LDS, since
+// rows on pages have no step between them and 8-bit entries are widened on the
+// way; the next tiles' rows are in flight meanwhile.  Where at most 16 rows share
+// keys, each of a block's four waves has its own tiles, every fourth one, and the
+// waves join at a part's end; where more do, the waves have 16 rows each and
+// share every tile (SHARED), so that keys are read and widened once for 64 rows.
 //
-// The weights are multiplied with the values in two parts of 16 bits, their
-// rounding and the rounding of what that leaves, so that they keep 16 bits of
-// bf16 or 22 of f16: twice the products of a kernel that waits for memory.
-// 8-bit entries under 16-bit queries are multiplied as f16, where whole numbers
-// to 127 are exact: their scales go into the scores and, against a power of two
-// that no scale so far has reached, into the weights, and queries in bf16 are
-// brought into range by a power of two a row.
+// The weights are rounded to 16 bits for the products with the values: in f16
+// once (2^-11 of each), in bf16 in two parts, their rounding and the rounding of
+// what that leaves, which keep 16 bits; f32 keeps all.  8-bit entries under
+// 16-bit queries are multiplied as f16, where whole numbers to 127 are exact:
+// their scales go into the scores and, against a power of two that no scale so
+// far has reached, into the weights, and queries in bf16 are brought into range
+// by a power of two a row.
+//
 #pragma once
 
 #include "attention_tiles.hpp"
@@ -42,13 +44,12 @@ namespace cache {
 
 constexpr int kAttendThreads = 256;
 constexpr int kAttendWaves = kAttendThreads / 64;
-// The first kernel's two forms: waves by themselves of 16 query rows each, or
-// blocks of 64 rows that share their tiles (SHARED).
+// The first kernel's two forms: blocks of 16 query rows, whose waves take a tile
+// each and join at the end of a part, or of 64 rows, 16 a wave, that share each
+// tile (SHARED).
 constexpr uint32_t rows_of_form(bool shared) { return shared ? 64 : 16; }
-// Blocks of a compute unit at a time, as registers allow, and whose parts are
-// one behind another on the line: waves, or blocks.
+// Blocks of a compute unit at a time, as registers allow.
 constexpr uint32_t blocks_of_form(bool shared) { return shared ? 3 : 2; }
-constexpr uint32_t workers_of_form(bool shared) { return blocks_of_form(shared) * (shared ? 1 : kAttendWaves); }
 
 // One launch's operands.
 struct Attention {
@@ -64,17 +65,19 @@ struct Attention {
     float* normalizers;
 };
 
-// Where a query row's parts over a line are: whole in the row's own place, or
-// with the workers first to last, the first one's at `place` of the slots, the
-// others' in their first slot.
+// Where a query row's parts over a line are: in the row's own place if it is
+// kWhole, or with the blocks first to last (none if last is less), the first
+// one's at `place` of the slots, the others' in their first slot.  kSees: the
+// row sees keys of the line; kOutside: it is of no sequence.
+enum { kWhole = 1, kSees = 2, kOutside = 4 };
 struct Found {
-    uint32_t first, last, place, whole;
+    uint32_t first, last, place, marks;
 };
 
-// Partial results.  A worker has two slots, for parts at its two ends.
+// Partial results.  A block has two slots, for parts at its two ends.
 struct Parts {
-    float* slots;        // [2 workers][rows][size]
-    float2* slot_stats;  // [2 workers][rows] (maximum, in powers of two; sum)
+    float* slots;        // [2 blocks][rows][size]
+    float2* slot_stats;  // [2 blocks][rows] (maximum, in powers of two; sum)
     float* rows;         // [token][query head][size], of whole items
     float2* row_stats;
     Found* found;   // [token][query head]
@@ -317,7 +320,6 @@ template <int SIZE, bool SHARED, bool QUANT, bool PREFIX>
 __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_per_eu(blocks_of_form(SHARED))))
     attend_kernel(const Attention a, const Parts parts, bool final) {
     constexpr int ROWS = rows_of_form(SHARED);
-    constexpr int kWorkers = SHARED ? 1 : kAttendWaves;  // of a block
     constexpr int kMovers = SHARED ? kAttendThreads : 64;  // threads that move a tile
     using LineOf = Line<ROWS>;
     using TileOf = KeyTile<SIZE>;
@@ -339,17 +341,21 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
         return (word % kRowWords * kSpread + word / kRowWords) * E + column % E;
     };
     constexpr int kStages = SHARED ? 2 : kAttendWaves;
+    constexpr uint32_t kStep = kKeys * (SHARED ? 1 : kAttendWaves);  // from one tile of a wave to the next
+    constexpr int kStride = SIZE + 4;  // of a row where waves join
     // Tiles in flight, of 8 kEach registers each.
     constexpr int kMostAhead = SHARED ? 2 : 4;
     constexpr int kAhead = 8 / kEach < 1 ? 1 : 8 / kEach > kMostAhead ? kMostAhead : 8 / kEach;
 
     __shared__ __attribute__((aligned(1024))) char tiles[kStages][2 * TileOf::kBytes];
     __shared__ __attribute__((aligned(16))) float scales[QUANT ? kStages : 1][64];
-    __shared__ uint64_t sums[kAttendWaves], found[kWorkers][2];
+    __shared__ uint64_t sums[kAttendWaves], found[2];
+    __shared__ float2 stats[SHARED ? 1 : kAttendWaves][16];
+    static_assert(SHARED || sizeof(tiles) >= kAttendWaves * 16 * kStride * sizeof(float), "waves join in the tiles' place");
 
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, quarter = lane / 16;
 
-    // ---- this worker's tiles -----------------------------------------------------
+    // ---- this block's tiles -----------------------------------------------------
     const uint32_t sequences = PREFIX ? 1 : a.batch.sequences;
     uint64_t total_tiles = 0;
     [[maybe_unused]] uint64_t count_here = 0, upto_here = 0;  // of this thread's sequence, and with those before
@@ -364,6 +370,21 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             count_here = LineOf::count(a, s);
             cut = cut || s.length < s.tokens;
             mine += count_here;
+            // What is no block's item is said by the block whose turn the sequence is.
+            if (s.keys == 0 && n % gridDim.x == blockIdx.x) {
+                const uint64_t from = uint64_t{s.first} * a.query_heads, count = uint64_t{s.tokens} * a.query_heads;
+                for (uint64_t i = 0; i < count; i++) parts.found[from + i] = {1, 0, 0, 0};
+            }
+        }
+        if (sequences == 0 || a.batch.offsets != nullptr) {
+            const uint64_t all = uint64_t{a.batch.tokens} * a.query_heads;
+            const auto upto = [&](uint32_t n) {
+                const uint32_t token = sequences == 0 ? a.batch.tokens : a.batch.offsets[n];
+                return uint64_t{token < a.batch.tokens ? token : a.batch.tokens} * a.query_heads;
+            };
+            const uint64_t step = uint64_t{gridDim.x} * kAttendThreads, mine_first = uint64_t{blockIdx.x} * kAttendThreads + threadIdx.x;
+            for (uint64_t i = mine_first; i < upto(0); i += step) parts.found[i] = {1, 0, 0, kOutside};
+            for (uint64_t i = upto(sequences) + mine_first; i < all; i += step) parts.found[i] = {1, 0, 0, kOutside};
         }
         upto_here = mine;
         for (int offset = 1; offset < 64; offset *= 2) {
@@ -379,29 +400,17 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
         total_tiles = uniform(total_tiles);
         if (blockIdx.x == 0 && threadIdx.x == 0) *parts.cut = cut;
     }
-    // No worker has nothing, so that every one between two parts of an item has
+    // No block has nothing, so that every one between two parts of an item has
     // a part of it.
-    const uint64_t most_workers = uint64_t{gridDim.x} * kWorkers;
-    const uint64_t workers = total_tiles < most_workers ? total_tiles : most_workers;
-    const uint32_t first_worker = blockIdx.x * kWorkers;
-    if (first_worker >= workers) return;
-    const auto begin_of = [&](uint64_t worker) { return worker * total_tiles / workers; };
+    const uint64_t blocks = total_tiles < gridDim.x ? total_tiles : gridDim.x;
+    if (blockIdx.x >= blocks) return;
+    const uint64_t begin = blockIdx.x * total_tiles / blocks, end = (blockIdx.x + uint64_t{1}) * total_tiles / blocks;
 
-    const uint32_t worker = uniform(first_worker + (SHARED ? 0 : wave));
     uint32_t sequence = 0;
     uint64_t before = 0;  // tiles of the sequences before
     if constexpr (!PREFIX) {
-        uint64_t begins[kWorkers];
-#pragma unroll
-        for (int w = 0; w < kWorkers; w++) {
-            // (Of a worker past the last one: the last one's.)
-            begins[w] = begin_of(first_worker + w < workers ? first_worker + w : workers - 1);
-        }
         const auto find = [&](uint32_t n, uint64_t start, uint64_t count) {
-#pragma unroll
-            for (int w = 0; w < kWorkers; w++) {
-                if (begins[w] >= start && begins[w] - start < count) found[w][0] = n, found[w][1] = start;
-            }
+            if (begin >= start && begin - start < count) found[0] = n, found[1] = start;
         };
         if (sequences <= kAttendThreads) find(threadIdx.x, upto_here - count_here, count_here);
         __syncthreads();
@@ -422,16 +431,14 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             }
             find(n, before + upto - count, count);
             __syncthreads();
-            if (begins[kWorkers - 1] - before < all) break;  // the same for the whole block
+            if (begin - before < all) break;  // the same for the whole block
             before += all;
         }
-        sequence = uniform(static_cast<uint32_t>(found[SHARED ? 0 : wave][0]));
-        before = uniform(found[SHARED ? 0 : wave][1]);
+        sequence = uniform(static_cast<uint32_t>(found[0]));
+        before = uniform(found[1]);
     }
     [[maybe_unused]] bool cut = false;
-    if constexpr (PREFIX) cut = __builtin_amdgcn_readfirstlane(*parts.cut) != 0;
-    if (worker >= workers) return;  // (a wave by itself: no barrier follows)
-    const uint64_t begin = begin_of(worker), end = begin_of(worker + uint64_t{1});
+    if constexpr (PREFIX) cut = uniform(*parts.cut) != 0;
 
     const uint32_t row_place = TileOf::row_place(lane), column_place = TileOf::column_place(lane);
     int stage = SHARED ? 0 : wave;
@@ -453,8 +460,8 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
         const uint32_t tile_1 = end - at < tile_count - tile_0 ? tile_0 + static_cast<uint32_t>(end - at) : tile_count;
         const uint32_t key_head = item / row_blocks, row_block = item % row_blocks;
         const bool whole = tile_0 == 0 && tile_1 == tile_count;
-        // (An item's first part is the worker's first if both begin together.)
-        const uint32_t slot = 2 * worker + (at > begin);
+        // (An item's first part is the block's first if both begin together.)
+        const uint32_t slot = 2 * blockIdx.x + (at > begin);
 
         // ---- this lane's query row ---------------------------------------------------
         const uint32_t first_row = row_block * ROWS, left_rows = s.tokens * a.group - first_row;
@@ -473,10 +480,11 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             } else {
                 seen = seen_of(s.length, s.tokens - place, 0, s.keys);
             }
-            if (tile_0 == 0 && quarter == 0) {
-                const uint64_t last = ((at + tile_count) * workers - 1) / total_tiles;
-                parts.found[uint64_t{token} * a.query_heads + head] = {worker, static_cast<uint32_t>(last),
-                                                                       slot * ROWS + row, whole};
+            if (tile_0 == 0 && quarter == 0 && (SHARED || wave == 0)) {
+                const uint64_t last = ((at + tile_count) * blocks - 1) / total_tiles;
+                parts.found[uint64_t{token} * a.query_heads + head] = {
+                    blockIdx.x, static_cast<uint32_t>(last), slot * ROWS + row,
+                    static_cast<uint32_t>((whole ? kWhole : 0) | (seen > 0 ? kSees : 0))};
             }
         }
         // Keys that every, and that any, row of the block sees.
@@ -551,16 +559,16 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                     from_row == kNowhere ? 0.0f : (lane < 32 ? a.pool.key_scales : a.pool.value_scales)[from_row];
             }
         };
-        uint32_t tile = tile_0 * kKeys;
+        uint32_t tile = 0;
         uint32_t pages[kAhead], next_page[2];  // of the first tiles, and of the next ones to fetch
         const auto find_pages = [&]() {
-            tile = tile_0 * kKeys;
-            each<kAhead>([&](auto n) { pages[n.value] = page_at(tile + n.value * kKeys); });
-            next_page[0] = page_at(tile + kAhead * kKeys);
-            next_page[1] = page_at(tile + (kAhead + 1) * kKeys);
+            tile = (tile_0 + (SHARED ? 0 : wave)) * kKeys;
+            each<kAhead>([&](auto n) { pages[n.value] = page_at(tile + n.value * kStep); });
+            next_page[0] = page_at(tile + kAhead * kStep);
+            next_page[1] = page_at(tile + (kAhead + 1) * kStep);
         };
         const auto fetch_first = [&]() {
-            each<kAhead>([&](auto n) { fetch(n, row_at(tile + n.value * kKeys, pages[n.value])); });
+            each<kAhead>([&](auto n) { fetch(n, row_at(tile + n.value * kStep, pages[n.value])); });
         };
         find_pages();
 
@@ -664,10 +672,10 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             land(set, key_tile, value_tile);
             if constexpr (SHARED) __syncthreads();
             else wave_order();
-            const uint32_t next = tile + kAhead * kKeys;
+            const uint32_t next = tile + kAhead * kStep;
             if (next < key_end) {
                 fetch(set, row_at(next, next_page[p]));
-                next_page[p] = page_at(next + 2 * kKeys);
+                next_page[p] = page_at(next + 2 * kStep);
             }
             // Scores, and their maximum over the tile.
             f32x4 scores[kBlocks16];
@@ -753,7 +761,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                 acc[t] = product16<M>(values, high_part.w[0], acc[t]);
                 if constexpr (kTwoParts) acc[t] = product16<M>(values, low_part.w[0], acc[t]);
             }
-            tile += kKeys;
+            tile += kStep;
             if constexpr (SHARED) stage ^= 1;
         };
         // Over the tiles, of which the first are on their way.
@@ -812,40 +820,77 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
         }
 
         // ---- the part's sums stored ----------------------------------------------------
+        const auto store = [&](uint32_t of_token, uint32_t of_head, uint32_t slot_row, bool any, uint32_t column, f32x4 v,
+                               float top, float all, float times) {
+            if (whole && final) {
+                // (A sum of 0 over keys that are seen is of scores of -infinity
+                // alone: 0 / 0.)
+                S* const to = static_cast<S*>(a.out) + of_token * a.out_steps.token + of_head * a.out_steps.head;
+                store_four(to, column, a.pool.size, any ? v * (times / all) : f32x4{});
+                if (column == 0 && a.normalizers != nullptr) {
+                    a.normalizers[uint64_t{of_head} * a.batch.tokens + of_token] =
+                        all == 0.0f ? -INFINITY : (top + log2f(all) - kPower) * attention::kLn2;
+                }
+            } else {
+                const uint64_t to = whole ? uint64_t{of_token} * a.query_heads + of_head : uint64_t{slot} * ROWS + slot_row;
+                *reinterpret_cast<f32x4*>((whole ? parts.rows : parts.slots) + to * SIZE + column) = v * times;
+                if (column == 0) (whole ? parts.row_stats : parts.slot_stats)[to] = make_float2(top, all);
+            }
+        };
         const float all = quarters<Added>(total);
         const float back = kScaled ? unit : 1.0f;
-        if (real && whole && final) {
-            // (A sum of 0 over keys that are seen is of scores of -infinity alone:
-            // 0 / 0.)
-            const float scale = back / all;
-            S* const to = static_cast<S*>(a.out) + token * a.out_steps.token + head * a.out_steps.head;
+        if constexpr (SHARED) {
+            if (real) {
+#pragma unroll
+                for (int t = 0; t < SIZE / 16; t++) {
+                    store(token, head, row, seen > 0, element_of(16 * t + 4 * quarter), acc[t], most, all, back);
+                }
+            }
+        } else {
+            // The waves' sums joined, each against the largest maximum.
+            if (lane < 16) stats[wave][lane] = make_float2(most, all);
+            __syncthreads();
+            const auto joined = [&](uint32_t of_row, float* top, float* sum) {
+                *top = -INFINITY, *sum = 0.0f;
+                for (int w = 0; w < kAttendWaves; w++) *top = fmaxf(*top, stats[w][of_row].x);
+                const float origin = *top == -INFINITY ? 0.0f : *top;
+                for (int w = 0; w < kAttendWaves; w++) *sum += power2(stats[w][of_row].x - origin) * stats[w][of_row].y;
+            };
+            float top, sum;
+            joined(lane % 16, &top, &sum);
+            const float kept = power2(most - (top == -INFINITY ? 0.0f : top)) * back;
+            float* const joint = reinterpret_cast<float*>(&tiles[0][0]);
 #pragma unroll
             for (int t = 0; t < SIZE / 16; t++) {
-                store_four(to, element_of(16 * t + 4 * quarter), a.pool.size, seen > 0 ? acc[t] * scale : f32x4{});
+                *reinterpret_cast<f32x4*>(joint + (wave * 16 + lane % 16) * kStride + element_of(16 * t + 4 * quarter)) =
+                    acc[t] * kept;
             }
-            if (quarter == 0 && a.normalizers != nullptr) {
-                a.normalizers[uint64_t{head} * a.batch.tokens + token] =
-                    all == 0.0f ? -INFINITY : (most + log2f(all) - kPower) * attention::kLn2;
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < 16 * SIZE / 4; i += kAttendThreads) {
+                const uint32_t of_row = i / (SIZE / 4), column = i % (SIZE / 4) * 4;
+                if (of_row >= rows) continue;
+                f32x4 v = *reinterpret_cast<const f32x4*>(joint + of_row * kStride + column);
+                for (int w = 1; w < kAttendWaves; w++) {
+                    v += *reinterpret_cast<const f32x4*>(joint + (w * 16 + of_row) * kStride + column);
+                }
+                joined(of_row, &top, &sum);
+                const uint32_t of_place = a.group_of.div(first_row + of_row);
+                const bool any = PREFIX || seen_of(s.length, s.tokens - of_place, 0, s.keys) > 0;
+                store(s.first + of_place, key_head * a.group + first_row + of_row - of_place * a.group, of_row, any, column,
+                      v, top, sum, 1.0f);
             }
-        } else if (real) {
-            const uint64_t to = whole ? uint64_t{token} * a.query_heads + head : uint64_t{slot} * ROWS + row;
-            float* const values = (whole ? parts.rows : parts.slots) + to * SIZE;
-#pragma unroll
-            for (int t = 0; t < SIZE / 16; t++) {
-                *reinterpret_cast<f32x4*>(values + element_of(16 * t + 4 * quarter)) = acc[t] * back;
-            }
-            if (quarter == 0) (whole ? parts.row_stats : parts.slot_stats)[to] = make_float2(most, all);
+            __syncthreads();
         }
         at += tile_1 - tile_0;
     }
 }
 
 // Each row's parts joined, by WAVES waves: the row's own sequence's and the
-// prefix's, in the order of their workers, two a wave at a time.
+// prefix's, in the order of their blocks, two a wave at a time.
 template <int SIZE, int WAVES>
 __global__ void __launch_bounds__(kAttendThreads)
     join_kernel(const Attention a, const Parts own, const Parts prefix, uint32_t own_rows, uint32_t prefix_rows,
-                uint32_t own_workers, uint32_t prefix_workers, float power) {
+                uint32_t own_blocks, uint32_t prefix_blocks, float power) {
     constexpr int kRows = kAttendWaves / WAVES;  // of a block
     __shared__ f32x4 sums[WAVES > 1 ? WAVES : 1][32];
     __shared__ float2 stats_of[WAVES > 1 ? WAVES : 1];
@@ -854,30 +899,21 @@ __global__ void __launch_bounds__(kAttendThreads)
     for (uint64_t at = uint64_t{blockIdx.x} * kRows + threadIdx.x / 64 / WAVES; at < all_rows; at += apart) {
         const uint32_t row = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at));
         const uint32_t token = row / a.query_heads, head = row % a.query_heads;
-        // What is read of a row that no worker had is not used: its sequence has
-        // no keys.
         const Found mine = own.found[row];
         const Found shared = a.batch.prefix > 0 ? prefix.found[row] : Found{1, 0, 0, 0};
-        Span span{0, 0};
-        const uint32_t sequence = wave_sequence_of(a.batch, token, &span);
-        uint32_t mine_count = 0, count = 0;
-        bool sees = false;
-        if (sequence != kNowhere) {
-            const Sequence s = sequence_at<false>(a, sequence);
-            const uint32_t left = s.first + s.tokens - token;
-            const auto count_of = [](const Found& f, uint32_t workers) {
-                return f.whole ? 1 : f.first <= f.last && f.last < workers ? f.last - f.first + 1 : 0;
-            };
-            if (s.keys > 0) mine_count = count_of(mine, own_workers);
-            count = mine_count;
-            sees = seen_of(s.length, left, 0, s.keys) > 0;
-            if (a.batch.prefix > 0) {
-                count += count_of(shared, prefix_workers);
-                sees = sees || seen_of(s.length, left, a.batch.prefix, a.batch.prefix) > 0;
-            }
-        }
+        // (Offsets that do not rise leave rows that no item has: what is found
+        // for them is none of the slots, or any.)
+        const auto count_of = [](const Found& f, uint32_t blocks, uint32_t line) {
+            return f.marks & kWhole                                                               ? 1
+                   : f.first <= f.last && f.last < blocks && f.place < 2 * uint64_t{blocks} * line ? f.last - f.first + 1
+                                                                                                   : 0;
+        };
+        const bool outside = (mine.marks & kOutside) != 0;
+        const uint32_t mine_count = outside ? 0 : count_of(mine, own_blocks, own_rows);
+        const uint32_t count = outside ? 0 : mine_count + count_of(shared, prefix_blocks, prefix_rows);
+        const bool sees = !outside && ((mine.marks | shared.marks) & kSees) != 0;
         // A whole item without a prefix is a result already.
-        if (count == 1 && mine_count == 1 && mine.whole && a.batch.prefix == 0) continue;
+        if (mine_count == 1 && (mine.marks & kWhole) && a.batch.prefix == 0) continue;
 
         const uint32_t half = threadIdx.x % 64 / 32, column = threadIdx.x % 32 * 4;
         float top = -INFINITY, total = 0.0f;
@@ -897,11 +933,13 @@ __global__ void __launch_bounds__(kAttendThreads)
                 const Found& f = is_mine ? mine : shared;
                 const Parts& parts = is_mine ? own : prefix;
                 const uint32_t n = is_mine ? i : i - mine_count, line = is_mine ? own_rows : prefix_rows;
-                const uint64_t place = f.whole ? row : n == 0 ? f.place : uint64_t{2 * (f.first + n)} * line + f.place % line;
-                stats[k] = (f.whole ? parts.row_stats : parts.slot_stats)[place];
+                // (`line` is a power of two.)
+                const bool whole = (f.marks & kWhole) != 0;
+                const uint32_t place = whole ? row : n == 0 ? f.place : 2 * (f.first + n) * line + (f.place & (line - 1));
+                stats[k] = (whole ? parts.row_stats : parts.slot_stats)[place];
                 if (column < SIZE) {
                     values[k] =
-                        *reinterpret_cast<const f32x4*>((f.whole ? parts.rows : parts.slots) + place * SIZE + column);
+                        *reinterpret_cast<const f32x4*>((whole ? parts.rows : parts.slots) + uint64_t{place} * SIZE + column);
                 }
             }
 #pragma unroll
@@ -991,8 +1029,8 @@ int join(const Attention& a, const Parts& own, const Parts& prefix, bool quant, 
     TC_CACHE_SIZE(a.pool.size, {
         const auto kernel = few ? join_kernel<SIZE, kAttendWaves> : join_kernel<SIZE, 1>;
         kernel<<<grid, kAttendThreads, 0, s>>>(a, own, prefix, rows_of_form(own_shared), rows_of_form(prefix_shared),
-                                               units * workers_of_form(own_shared),
-                                               units * workers_of_form(prefix_shared), power);
+                                               units * blocks_of_form(own_shared),
+                                               units * blocks_of_form(prefix_shared), power);
     })
     return check_launch("cache attention");
 }

@@ -33,4 +33,34 @@ inline int check_heads(const std::string& what, const char* name, Steps steps, u
     return TC_OK;
 }
 
+// The rows of a tensor [token][head] that one of a block's GROUPS groups of lanes
+// takes, every GROUPS-th from token `first` on: token (from there) and head, and
+// the row's place in each of some layouts, moved on by sums that are the same
+// for the block.
+template <int LAYOUTS, int GROUPS>
+struct RowWalk {
+    uint32_t heads, tokens_on, heads_on;
+    uint64_t on[LAYOUTS], wrap[LAYOUTS];
+    uint32_t token, head;
+    uint64_t at[LAYOUTS];
+
+    __device__ __forceinline__ RowWalk(uint32_t count, const Steps (&steps)[LAYOUTS], uint32_t group, uint64_t first)
+        : heads(count), tokens_on(GROUPS / count), heads_on(GROUPS % count), token(group / count), head(group % count) {
+#pragma unroll
+        for (int n = 0; n < LAYOUTS; n++) {
+            on[n] = tokens_on * steps[n].token + heads_on * steps[n].head;
+            wrap[n] = steps[n].token - heads * steps[n].head;
+            at[n] = (first + token) * steps[n].token + head * steps[n].head;
+        }
+    }
+    __device__ __forceinline__ void move() {
+        token += tokens_on, head += heads_on;
+        const bool over = head >= heads;
+        token += over;
+        head -= over ? heads : 0;
+#pragma unroll
+        for (int n = 0; n < LAYOUTS; n++) at[n] += on[n] + (over ? wrap[n] : 0);
+    }
+};
+
 }  // namespace tc

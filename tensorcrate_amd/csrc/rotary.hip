@@ -157,35 +157,6 @@ struct Lane {
     }
 };
 
-// The rows of one of the two tensors that a group of 16 lanes takes in a
-// block's turn, every kGroups-th: token and head, and the row's place in each
-// of up to three layouts, moved on by sums that are the same for the block.
-template <int LAYOUTS>
-struct RowWalk {
-    uint32_t heads, tokens_on, heads_on;
-    uint64_t on[LAYOUTS], wrap[LAYOUTS];
-    uint32_t token, head;
-    uint64_t at[LAYOUTS];
-
-    __device__ __forceinline__ RowWalk(uint32_t count, const Steps (&steps)[LAYOUTS], uint32_t group, uint64_t first)
-        : heads(count), tokens_on(kGroups / count), heads_on(kGroups % count), token(group / count), head(group % count) {
-#pragma unroll
-        for (int n = 0; n < LAYOUTS; n++) {
-            on[n] = tokens_on * steps[n].token + heads_on * steps[n].head;
-            wrap[n] = steps[n].token - heads * steps[n].head;
-            at[n] = (first + token) * steps[n].token + head * steps[n].head;
-        }
-    }
-    __device__ __forceinline__ void move() {
-        token += tokens_on, head += heads_on;
-        const bool over = head >= heads;
-        token += over;
-        head -= over ? heads : 0;
-#pragma unroll
-        for (int n = 0; n < LAYOUTS; n++) at[n] += on[n] + (over ? wrap[n] : 0);
-    }
-};
-
 // 1 / sqrt(v), by the instruction, which takes no subnormal number.
 __device__ __forceinline__ float reciprocal_root(float v) {
     const bool small = v < 0x1p-100f;
@@ -236,9 +207,9 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(B
     const auto walk_of = [&](auto which, uint64_t first) {
         constexpr int n = decltype(which)::value;
         const Steps steps[3] = {r.from_steps[n], r.to_steps[n], r.x_steps[n]};
-        return RowWalk<LAYOUTS>(r.heads[n], reinterpret_cast<const Steps(&)[LAYOUTS]>(steps), group, first);
+        return RowWalk<LAYOUTS, kGroups>(r.heads[n], reinterpret_cast<const Steps(&)[LAYOUTS]>(steps), group, first);
     };
-    const auto fetch = [&](auto which, const RowWalk<LAYOUTS>& walk, Fetched& out) {
+    const auto fetch = [&](auto which, const RowWalk<LAYOUTS, kGroups>& walk, Fetched& out) {
         constexpr int n = decltype(which)::value;
         at.template load<NT>(r.from[n] + walk.at[0], out.row);
         if constexpr (BACK) {
@@ -247,7 +218,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(B
     };
     // The rows of queries or keys of `here` tokens, the first of them in `next`
     // and each one's successor in flight.
-    const auto rows_of = [&](auto which, int stage, RowWalk<LAYOUTS>& walk, uint32_t here, Fetched& next) {
+    const auto rows_of = [&](auto which, int stage, RowWalk<LAYOUTS, kGroups>& walk, uint32_t here, Fetched& next) {
         constexpr int n = decltype(which)::value;
         while (walk.token < here) {
             const uint32_t token = walk.token;
@@ -300,7 +271,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(B
     const auto begin = [&](auto which, uint64_t from, Fetched& out) {
         constexpr int n = decltype(which)::value;
         if (r.heads[n] == 0) return;
-        const RowWalk<LAYOUTS> walk = walk_of(which, from);
+        const RowWalk<LAYOUTS, kGroups> walk = walk_of(which, from);
         if (walk.token < tokens_at(from)) fetch(which, walk, out);
     };
     begin(queries, first, next_query);
@@ -313,12 +284,12 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(B
         begin(keys, first, next_key);
         find_turns(stage ^ 1, first + apart);
         if (r.heads[0] > 0) {
-            RowWalk<LAYOUTS> walk = walk_of(queries, first);
+            RowWalk<LAYOUTS, kGroups> walk = walk_of(queries, first);
             rows_of(queries, stage, walk, here, next_query);
         }
         begin(queries, first + apart, next_query);
         if (r.heads[1] > 0) {
-            RowWalk<LAYOUTS> walk = walk_of(keys, first);
+            RowWalk<LAYOUTS, kGroups> walk = walk_of(keys, first);
             rows_of(keys, stage, walk, here, next_key);
         }
     }
