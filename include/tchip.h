@@ -896,8 +896,9 @@ int tc_cache_read(const tc_cache* cache, const tc_cache_batch* batch, void* key,
  * Element e of head h of token t is at t * token_step + h * head_step + e of
  * queries and results.  `normalizers` [query_heads][tokens] (f32; may be null)
  * receives the log of each query's sum of exponentials.
- *   Sums and softmax are f32; the weights are rounded to `dtype` in f16 and to
- * 16 bits in two parts in bf16 and over 8-bit entries.  A query that attends to
+ *   Sums and softmax are f32.  For the products with the values the weights are
+ * rounded to f16 in f16, and over 8-bit entries in bf16 too; in bf16 over plain
+ * entries to two parts of 8 bits of fraction; in f32 not at all.  A query that attends to
  * nothing (a token in no sequence, or before its first) gets zeros and the
  * normalizer -infinity.  Keys and values of no page are zeros; no other row
  * than those a query attends to reaches its result (of those, an infinite value

@@ -17,6 +17,11 @@
 // block computes those of a few tokens into LDS and then walks their heads.
 // An angle is a product in 64 bits, reduced to a part of a turn there, so that
 // far positions lose nothing; the functions of that part are taken in 32.
+//
+// Measured: 16384 tokens of 40 heads of 128 in bf16 forward 62 us (5.4 TB/s), of 36
+// backward with both weights 91 us (5.0), of which the weights' second launch is
+// some 5; 16 tokens 4.9 us, a launch's time.  With one row of a lane's on its way
+// those were 115, 145 and 6.8 us.
 
 #include <type_traits>
 
