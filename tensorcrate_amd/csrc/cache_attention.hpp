@@ -1027,7 +1027,9 @@ int join(const Attention& a, const Parts& own, const Parts& prefix, bool quant, 
     TC_STREAM(s);
     const uint32_t units = static_cast<uint32_t>(compute_units());
     const uint64_t rows = uint64_t{a.batch.tokens} * a.query_heads;
-    // A block a row where rows are few and their parts, therefore, many.
+    // A block a row where rows are few and their parts, therefore, many.  (One
+    // sequence of 1000 tokens 13.1 us, with a wave a row 17.1, four of 100000 113
+    // and 118; the other way 64 sequences of 32 heads 226 instead of 220.)
     const bool few = rows <= uint64_t{units} * 4;
     const uint64_t turns = few ? rows : (rows + kAttendWaves - 1) / kAttendWaves;
     const uint32_t grid = turns < (1u << 20) ? static_cast<uint32_t>(turns) : 1u << 20;

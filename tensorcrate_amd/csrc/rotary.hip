@@ -346,7 +346,10 @@ int rotary(const tc_rotary_shape& a, Rotary<S, W> r, W* d_query_weight, W* d_key
     r.epsilon = a.epsilon;
     r.tokens = a.tokens;
     r.positions = a.positions, r.frequencies = a.frequencies;
-    // As many blocks as run at once, walking the tokens together.
+    // As many blocks as run at once, walking the tokens together: several at a
+    // time where there are many (gradients of 7001 tokens of 24 heads of 80 29 us,
+    // one at a time 36; 16384 of 36 heads 91 and 94, forward of 40 heads 62 and 60),
+    // else one (16 tokens 4.9 us, four at a time 8.5).
     const uint32_t per_unit = BACK ? kBackPerUnit : kForwardPerUnit;
     const uint64_t units = static_cast<uint64_t>(compute_units());
     r.chunk = a.tokens >= units * per_unit * 2 ? kMostTokens : 1;
