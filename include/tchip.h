@@ -897,13 +897,13 @@ int tc_cache_read(const tc_cache* cache, const tc_cache_batch* batch, void* key,
  * queries and results.  `normalizers` [query_heads][tokens] (f32; may be null)
  * receives the log of each query's sum of exponentials.
  *   Sums and softmax are f32.  For the products with the values the weights are
- * rounded to f16 in f16, and over 8-bit entries in bf16 too; in bf16 over plain
- * entries to two parts of 8 bits of fraction; in f32 not at all.  A query that attends to
- * nothing (a token in no sequence, or before its first) gets zeros and the
- * normalizer -infinity.  Keys and values of no page are zeros; no other row
- * than those a query attends to reaches its result (of those, an infinite value
- * makes a NaN where its weight is 0).  A query all of whose
- * scores are -infinity has the normalizer -infinity and, as 0 / 0, a NaN
+ * rounded to f16 in f16; in bf16, and over 8-bit entries (times the values'
+ * scales) in f16 too, to two parts of bf16, which keep 16 bits; in f32 not at
+ * all.  A query that attends to nothing (a token in no sequence, or before its
+ * first) gets zeros and the normalizer -infinity.  Keys and values of no page
+ * are zeros; no other row than those a query attends to reaches its result (of
+ * those, an infinite value makes a NaN where its weight is 0).  A query all of
+ * whose scores are -infinity has the normalizer -infinity and, as 0 / 0, a NaN
  * result.  The order of every sum depends on the batch's counts and lengths
  * alone. */
 int tc_cache_attention(const tc_cache* cache, const tc_cache_batch* batch, uint32_t query_heads, float scale,

@@ -28,11 +28,11 @@
 //
 // The weights are rounded to 16 bits for the products with the values: in f16
 // once (2^-11 of each), in bf16 in two parts, their rounding and the rounding of
-// what that leaves, which keep 16 bits; f32 keeps all.  8-bit entries under
-// 16-bit queries are multiplied as f16, where whole numbers to 127 are exact:
-// their scales go into the scores and, against a power of two that no scale so
-// far has reached, into the weights, and queries in bf16 are brought into range
-// by a power of two a row.
+// what that leaves, which keep 16 bits; f32 keeps all.  8-bit entries, whole
+// numbers to 127 that every type holds, are widened to the queries' type for
+// the scores, which take the keys' scales afterwards.  The values' scales go
+// into the weights, so that under 16-bit queries weights and values are
+// multiplied as bf16 (`Weighed`).
 //
 // Measured: 64 sequences to 8192 tokens, 32 heads on 8 of 128, bf16: 221 us (5.7
 // TB/s in the first kernel); 4 to 100000 in 8 bits 114 us; 24 to 3000 with 5 new
@@ -206,9 +206,8 @@ struct KeyTile : attention::Tile<SIZE, kKeys> {
 template <typename T>
 __device__ __forceinline__ void widened(uint4 bytes, Words<T, 16>& out) {
     const uint32_t four[4] = {bytes.x, bytes.y, bytes.z, bytes.w};
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (Elem<T>::dtype == TC_F16) {
         // Behind the upper byte of 1024 in f16, whose step is 1: 1024 + 128 + q.
-        static_assert(Elem<T>::dtype == TC_F16, "8 bits are widened to f16 or f32");
         typedef _Float16 pair __attribute__((ext_vector_type(2)));
         uint32_t* const to = reinterpret_cast<uint32_t*>(out.w);
 #pragma unroll
@@ -318,9 +317,17 @@ __device__ __forceinline__ void store_four(S* row, uint32_t first, uint32_t size
     }
 }
 
+// The type that weights and values are multiplied in.  With 8-bit entries the
+// values' scales go into the weights, which then have a range that f16 lacks:
+// a value whose scale is 2^30 times the others' and its weight next to nothing
+// took the others' weights below f16's smallest number.  bf16 has f32's range,
+// and 8-bit numbers are exact in it.
+template <bool QUANT>
+using Weighed = std::conditional_t<QUANT && kHalf, bf16_t, S>;
+
 // Power of two that weights are rounded times in f16, whose least normal is
 // 2^-14: the largest, which may reach 2^8, stay below 2^15.
-constexpr float kHalfPower = 6.0f;
+constexpr float power_of(bool quant) { return kHalf && !quant ? 6.0f : 0.0f; }
 
 template <int SIZE, bool SHARED, bool QUANT, bool PREFIX>
 __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_per_eu(blocks_of_form(SHARED))))
@@ -329,11 +336,10 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
     constexpr int kMovers = SHARED ? kAttendThreads : 64;  // threads that move a tile
     using LineOf = Line<ROWS>;
     using TileOf = KeyTile<SIZE>;
-    // The type that is multiplied in.
-    constexpr bool kScaled = QUANT && sizeof(S) == 2;
-    using M = std::conditional_t<kScaled, _Float16, S>;
-    constexpr bool kTwoParts = sizeof(M) == 2 && Elem<M>::dtype == TC_BF16;
-    constexpr float kPower = sizeof(M) == 2 && Elem<M>::dtype == TC_F16 ? kHalfPower : 0.0f;
+    // The type that weights and values are multiplied in.
+    using V = Weighed<QUANT>;
+    constexpr bool kTwoParts = sizeof(V) == 2 && Elem<V>::dtype == TC_BF16;
+    constexpr float kPower = power_of(QUANT);
     constexpr int kOperands = SIZE / kDeep16;
     constexpr int kEntry = QUANT ? 1 : static_cast<int>(sizeof(S));
     constexpr int kRowWords = SIZE * kEntry / 16;
@@ -587,38 +593,11 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             queries[n] = real ? head_word(from, word, a.pool.size) : make_uint4(0, 0, 0, 0);
         }
         fetch_first();
-        float factor = a.scale * attention::kLog2e;  // of the scores, in powers of two
-        if constexpr (kScaled && !std::is_same_v<S, M>) {
-            // The row's largest to 2^8 and above, an infinity or a NaN as it is:
-            // what f16 then loses is below 2^-32 of the largest.
-            float largest = 0.0f;
-#pragma unroll
-            for (int n = 0; n < kOperands; n++) {
-                const Words<S, E> words{{queries[n]}};
-#pragma unroll
-                for (int e = 0; e < E; e++) largest = fmaxf(largest, fabsf(words.at(e)));
-            }
-            largest = quarters<Largest>(largest);
-            int power = largest > 0.0f && largest < INFINITY ? 8 - ilogbf(largest) : 0;
-            power = power > 126 ? 126 : power;
-            factor = ldexpf(factor, -power);
-            const float grown = ldexpf(1.0f, power);
-#pragma unroll
-            for (int n = 0; n < kOperands; n++) {
-                const Words<S, E> words{{queries[n]}};
-                Words<M, E> to;
-                float v[E];
-#pragma unroll
-                for (int e = 0; e < E; e++) v[e] = words.at(e) * grown;
-                to.put(v);
-                queries[n] = to.w[0];
-            }
-        }
+        const float factor = a.scale * attention::kLog2e;  // of the scores, in powers of two
 
         // ---- a sweep over the part's tiles -----------------------------------------
         f32x4 acc[SIZE / 16];
         float most, total;
-        [[maybe_unused]] float unit = 0x1p-126f;  // above every value's scale so far, and a power of two
         // Where the lane's first word of a tile lands, of which the others' places
         // follow if a row's words and the rows a step has are powers of two.
         constexpr int kStepRows = kMovers / kRowWords;
@@ -636,7 +615,8 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             for (int k = 0; k < kEach; k++) {
                 if (kKeys * kRowWords % kMovers != 0 && k * kMovers + mover >= kKeys * kRowWords) continue;
                 if constexpr (QUANT) {
-                    Words<M, 16> keys, values;
+                    Words<S, 16> keys;
+                    Words<V, 16> values;
                     widened(key_words[d][k], keys);
                     widened(value_words[d][k], values);
 #pragma unroll
@@ -657,21 +637,11 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
         // The tile that is in `set`; its next one's page is the `parity`-th.
         const auto turn = [&](auto set, auto parity, auto is_slow) {
             constexpr bool SLOW = decltype(is_slow)::value;
-            constexpr int d = decltype(set)::value, p = decltype(parity)::value;
+            constexpr int p = decltype(parity)::value;
             // (Keys past `key_end` are seen by no row, or by none that is real.)
             const bool masked = tile + kKeys > least || tile + kKeys > key_end;
             const TileOf key_tile{tiles[stage]};
             const TileOf value_tile{tiles[stage] + TileOf::kBytes};
-            if constexpr (kScaled) {
-                const float high = wave64<Largest>(lane < 32 ? 0.0f : entry_scale[d]);
-                if (high >= unit && high < INFINITY) {
-                    const float grown = ldexpf(1.0f, ilogbf(high) + 3);
-                    const float kept = unit / grown;
-                    unit = grown;
-#pragma unroll
-                    for (int t = 0; t < SIZE / 16; t++) acc[t] *= kept;
-                }
-            }
             // A stage that a block shares was read before the last barrier; a
             // wave's own is in the order of the program.
             if constexpr (!SHARED) wave_order();
@@ -690,7 +660,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                 scores[b] = f32x4{};
 #pragma unroll
                 for (int n = 0; n < kOperands; n++) {
-                    scores[b] = product16<M>(key_tile.by_row(row_place, b, n), queries[n], scores[b]);
+                    scores[b] = product16<S>(key_tile.by_row(row_place, b, n), queries[n], scores[b]);
                 }
                 if constexpr (QUANT) scores[b] *= *reinterpret_cast<const f32x4*>(&scales[stage][16 * b + 4 * quarter]);
             }
@@ -728,9 +698,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                     total += scores[b][i];
                 }
                 if constexpr (QUANT) {
-                    f32x4 scale = *reinterpret_cast<const f32x4*>(&scales[stage][32 + 16 * b + 4 * quarter]);
-                    if constexpr (kScaled) scale *= 1.0f / unit;
-                    scores[b] *= scale;
+                    scores[b] *= *reinterpret_cast<const f32x4*>(&scales[stage][32 + 16 * b + 4 * quarter]);
                     if (masked) {
                         // (A scale may be a NaN.)
 #pragma unroll
@@ -750,7 +718,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                     v[e] = one ? 1.0f : 0.0f;
                 }
             }
-            Words<M, E> high_part, low_part;
+            Words<V, E> high_part, low_part;
             high_part.put(v);
             if constexpr (kTwoParts) {
 #pragma unroll
@@ -764,8 +732,8 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                     values = make_uint4(picked(values.x, pick), picked(values.y, pick), picked(values.z, pick),
                                         picked(values.w, pick));
                 }
-                acc[t] = product16<M>(values, high_part.w[0], acc[t]);
-                if constexpr (kTwoParts) acc[t] = product16<M>(values, low_part.w[0], acc[t]);
+                acc[t] = product16<V>(values, high_part.w[0], acc[t]);
+                if constexpr (kTwoParts) acc[t] = product16<V>(values, low_part.w[0], acc[t]);
             }
             tile += kStep;
             if constexpr (SHARED) stage ^= 1;
@@ -827,29 +795,28 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
 
         // ---- the part's sums stored ----------------------------------------------------
         const auto store = [&](uint32_t of_token, uint32_t of_head, uint32_t slot_row, bool any, uint32_t column, f32x4 v,
-                               float top, float all, float times) {
+                               float top, float all) {
             if (whole && final) {
                 // (A sum of 0 over keys that are seen is of scores of -infinity
                 // alone: 0 / 0.)
                 S* const to = static_cast<S*>(a.out) + of_token * a.out_steps.token + of_head * a.out_steps.head;
-                store_four(to, column, a.pool.size, any ? v * (times / all) : f32x4{});
+                store_four(to, column, a.pool.size, any ? v * (1.0f / all) : f32x4{});
                 if (column == 0 && a.normalizers != nullptr) {
                     a.normalizers[uint64_t{of_head} * a.batch.tokens + of_token] =
                         all == 0.0f ? -INFINITY : (top + log2f(all) - kPower) * attention::kLn2;
                 }
             } else {
                 const uint64_t to = whole ? uint64_t{of_token} * a.query_heads + of_head : uint64_t{slot} * ROWS + slot_row;
-                *reinterpret_cast<f32x4*>((whole ? parts.rows : parts.slots) + to * SIZE + column) = v * times;
+                *reinterpret_cast<f32x4*>((whole ? parts.rows : parts.slots) + to * SIZE + column) = v;
                 if (column == 0) (whole ? parts.row_stats : parts.slot_stats)[to] = make_float2(top, all);
             }
         };
         const float all = quarters<Added>(total);
-        const float back = kScaled ? unit : 1.0f;
         if constexpr (SHARED) {
             if (real) {
 #pragma unroll
                 for (int t = 0; t < SIZE / 16; t++) {
-                    store(token, head, row, seen > 0, element_of(16 * t + 4 * quarter), acc[t], most, all, back);
+                    store(token, head, row, seen > 0, element_of(16 * t + 4 * quarter), acc[t], most, all);
                 }
             }
         } else {
@@ -864,7 +831,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             };
             float top, sum;
             joined(lane % 16, &top, &sum);
-            const float kept = power2(most - (top == -INFINITY ? 0.0f : top)) * back;
+            const float kept = power2(most - (top == -INFINITY ? 0.0f : top));
             float* const joint = reinterpret_cast<float*>(&tiles[0][0]);
 #pragma unroll
             for (int t = 0; t < SIZE / 16; t++) {
@@ -883,7 +850,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                 const uint32_t of_place = a.group_of.div(first_row + of_row);
                 const bool any = PREFIX || seen_of(s.length, s.tokens - of_place, 0, s.keys) > 0;
                 store(s.first + of_place, key_head * a.group + first_row + of_row - of_place * a.group, of_row, any, column,
-                      v, top, sum, 1.0f);
+                      v, top, sum);
             }
             __syncthreads();
         }
@@ -1033,7 +1000,7 @@ int join(const Attention& a, const Parts& own, const Parts& prefix, bool quant, 
     const bool few = rows <= uint64_t{units} * 4;
     const uint64_t turns = few ? rows : (rows + kAttendWaves - 1) / kAttendWaves;
     const uint32_t grid = turns < (1u << 20) ? static_cast<uint32_t>(turns) : 1u << 20;
-    const float power = sizeof(S) == 2 && (quant || kHalf) ? kHalfPower : 0.0f;
+    const float power = power_of(quant);
     TC_CACHE_SIZE(a.pool.size, {
         const auto kernel = few ? join_kernel<SIZE, kAttendWaves> : join_kernel<SIZE, 1>;
         kernel<<<grid, kAttendThreads, 0, s>>>(a, own, prefix, rows_of_form(own_shared), rows_of_form(prefix_shared),

@@ -1,0 +1,73 @@
+"""Attention over a cache where rows differ widely: what one row holds may not
+cost another's precision.
+
+Every bound here goes by what the query itself sees: by the sum of p |v| of each
+element.  A weight is off relatively by its score's error and some roundings of
+32 bits (`loose`, as in test_gpu_cache_attention.py), and by its own rounding
+for the product with the values: none in f32, 2^-16 in two parts of bf16 (two
+roundings of 2^-8)."""
+
+import numpy as np
+import pytest
+
+from tensorcrate_amd import lib
+from tests import generation
+from tests.common import KIND_NAMES, KINDS
+from tests.generation import World
+from tests.language import EPSILON_32, ROUNDING, TINY, near
+from tests.test_gpu_cache_attention import queries, run
+
+pytestmark = pytest.mark.gpu
+
+SIZE, SCALE = 40, 0.2
+
+
+def check(world, q, got, weight):
+    out, normalizers, sizes = generation.cache_attention(world, q, SCALE)
+    keys = [world.rows(0, h, s) for h in range(world.key_heads) for s in range(len(world.lengths))]
+    score = SCALE * max(np.sqrt((k ** 2).sum(1)).max(initial=0) for k in keys) * np.sqrt((q ** 2).sum(2)).max()
+    loose = EPSILON_32 * (64 + max(map(len, keys)) / 8 + 2 * (SIZE + 6) * score)
+    near(got[0], out, (weight + loose) * sizes + ROUNDING[world.kind] * np.abs(out) + TINY[world.kind], "out")
+    near(got[1], normalizers, loose + 4 * EPSILON_32 * np.abs(normalizers), "normalizers")
+
+
+# Of common and of uncommon values, 2^30 apart (f16, whose results have to be
+# in its range, 2^22).
+SPREAD = {lib.F32: (1.0, 2.0**30), lib.BF16: (1.0, 2.0**30), lib.F16: (2.0**-8, 2.0**14)}
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=KIND_NAMES.get)
+@pytest.mark.parametrize("lengths,new,prefix,heads", [([70, 40], [4, 3], 0, 2), ([33, 200], [3, 8], 50, 2),
+                                                      ([90], [40], 0, 4), ([45, 60], [30, 30], 70, 4)])
+def test_large_values_that_are_not_seen(kind, lengths, new, prefix, heads):
+    # The last token's value in 8 bits, which those before it do not see.
+    world = World(kind, lib.CACHE_INT8, 1, SIZE, 16, lengths, new, prefix)
+    rng = np.random.default_rng(1)
+    low, high = SPREAD[kind]
+    world.fill(rng)
+    world.scales[1] *= np.float32(low)
+    for s, n in enumerate(lengths):
+        world.put(world.slot(world.table[s], n - 1), 1, high * rng.standard_normal((1, SIZE)))
+    world.upload()
+    q = queries(world, heads)
+    check(world, q, run(world, q, SCALE), 0.0 if kind == lib.F32 else 2.0**-16)
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=KIND_NAMES.get)
+@pytest.mark.parametrize("length,prefix", [(100, 0), (9, 200), (600, 0)])
+def test_large_values_of_little_weight(kind, length, prefix):
+    # Rows that a query sees with a score far below the others', so that they
+    # add nothing, or about as much as these.
+    world = World(kind, lib.CACHE_INT8, 2, SIZE, 16, [length], prefix=prefix)
+    rng = np.random.default_rng(2)
+    low, high = SPREAD[kind]
+    world.fill(rng)
+    world.scales[1] *= np.float32(low)
+    q = queries(world, 2)
+    pages, count = (world.prefix_pages, prefix) if prefix else (world.table[0], length)
+    for at, score in ((5, -60.0), (count // 2, -np.log(high / low)), (count - 3, -90.0)):
+        place = world.slot(pages, at)
+        world.put(place, 0, score * q[0] / (SCALE * (q[0] ** 2).sum(1, keepdims=True)))
+        world.put(place, 1, high * rng.standard_normal((2, SIZE)))
+    world.upload()
+    check(world, q, run(world, q, SCALE), 0.0 if kind == lib.F32 else 2.0**-16)
