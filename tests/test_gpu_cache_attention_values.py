@@ -15,6 +15,7 @@ from tests import generation
 from tests.common import KIND_NAMES, KINDS
 from tests.generation import World
 from tests.language import EPSILON_32, ROUNDING, TINY, near
+from tests.test_gpu_cache_attention import check as attention_check
 from tests.test_gpu_cache_attention import queries, run
 
 pytestmark = pytest.mark.gpu
@@ -71,3 +72,47 @@ def test_large_values_of_little_weight(kind, length, prefix):
         world.put(place, 1, high * rng.standard_normal((2, SIZE)))
     world.upload()
     check(world, q, run(world, q, SCALE), 0.0 if kind == lib.F32 else 2.0**-16)
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=KIND_NAMES.get)
+@pytest.mark.parametrize("fmt", [lib.CACHE_PLAIN, lib.CACHE_INT8])
+@pytest.mark.parametrize("what", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("lengths,new,prefix", [([90], [40], 0), ([45, 80], [30, 30], 70)])
+def test_what_later_tokens_hold_where_many_rows_share_keys(kind, fmt, what, lengths, new, prefix):
+    world = World(kind, fmt, 1, SIZE, 16, lengths, new, prefix)
+    rng = np.random.default_rng(4)
+    world.fill(rng)
+    for s, (n, own) in enumerate(zip(lengths, new)):
+        for pool, at, element in ((0, n - 1, 5), (1, n - 1, 6), (1, n - 9, 9), (1, n - own // 2, 11)):
+            rows = rng.standard_normal((1, SIZE))
+            rows[0, element] = what
+            world.put(world.slot(world.table[s], at), pool, rows)
+    world.upload()
+    q = queries(world, 4)
+    got = run(world, q, SCALE)
+    first = np.cumsum([0] + new)
+    for s, own in enumerate(new):
+        mine = got[0][first[s]:first[s + 1]]
+        assert np.isfinite(mine[:own // 2]).all() and not np.isfinite(mine[-9:]).all((1, 2)).any()
+    attention_check(world, q, SCALE, got)
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=KIND_NAMES.get)
+@pytest.mark.parametrize("fmt", [lib.CACHE_PLAIN, lib.CACHE_INT8])
+@pytest.mark.parametrize("what", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("heads", [2, 8])
+def test_what_a_prefix_holds(kind, fmt, what, heads):
+    # 6 rows over the prefix, and 24.
+    world = World(kind, fmt, 1, SIZE, 16, [20, 5, 40], prefix=150)
+    rng = np.random.default_rng(5)
+    world.fill(rng)
+    for at, element in ((0, 3), (70, 7), (149, 7)):
+        rows = rng.standard_normal((1, SIZE))
+        rows[0, element] = what
+        world.put(world.slot(world.prefix_pages, at), 1, rows)
+    world.upload()
+    q = queries(world, heads)
+    got = run(world, q, SCALE)
+    attention_check(world, q, SCALE, got)
+    if fmt == lib.CACHE_PLAIN:
+        assert not np.isfinite(got[0][..., [3, 7]]).any() and np.isfinite(np.delete(got[0], [3, 7], 2)).all()
