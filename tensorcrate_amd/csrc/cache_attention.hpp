@@ -740,7 +740,8 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
         };
         // Over the tiles, of which the first are on their way.
         const auto sweep = [&](auto is_slow) {
-            most = -INFINITY, total = 0.0f;
+            if constexpr (!decltype(is_slow)::value) most = -INFINITY;
+            total = 0.0f;
 #pragma unroll
             for (int t = 0; t < SIZE / 16; t++) acc[t] = f32x4{};
             while (tile < key_end) {
@@ -757,7 +758,9 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             // A value that is an infinity or a NaN has spoiled every row, its
             // weight being 0 in those that do not see it, or 0 in the second of
             // two parts.  So once more for each kind of them, counting those
-            // that are seen, and at last without them.
+            // that are seen, and at last without them; against the maximum that
+            // the first sweep ended with, so that what it counts is not scaled
+            // down by scores that come later.
             bool spoiled = false;
 #pragma unroll
             for (int t = 0; t < SIZE / 16; t++) {

@@ -74,6 +74,56 @@ def test_large_values_of_little_weight(kind, length, prefix):
     check(world, q, run(world, q, SCALE), 0.0 if kind == lib.F32 else 2.0**-16)
 
 
+class Alike(World):
+    """`count` sequences on the same pages, `new` tokens of each a call's: many
+    tiles for a block, of few rows in the cache."""
+
+    def __init__(self, kind, fmt, key_heads, size, page, length, count, new=1, seed=0):
+        super().__init__(kind, fmt, key_heads, size, page, [length], [new], seed=seed)
+        self.lengths, self.new = [length] * count, [new] * count
+        self.table = np.repeat(self.table, count, 0)
+        self.offsets = (new * np.arange(count + 1)).astype(np.uint32)
+        self.tokens = new * count
+        self.held = {}
+
+    def fill(self, rng, spread=1.0):
+        self.lengths, whole = self.lengths[:1], self.lengths
+        super().fill(rng, spread)
+        self.lengths = whole
+
+    def rows(self, n, head, sequence):
+        if (n, head) not in self.held:
+            self.held[n, head] = super().rows(n, head, 0)
+        return self.held[n, head]
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=KIND_NAMES.get)
+@pytest.mark.parametrize("fmt", [lib.CACHE_PLAIN, lib.CACHE_INT8])
+@pytest.mark.parametrize("new,heads,count", [(1, 2, 40), (8, 8, 40)])
+def test_infinities_and_nans_that_later_scores_outweigh(kind, fmt, new, heads, count):
+    # Rows of 4 and of 64 queries, several tiles a wave.  A score 800 below the
+    # largest has a weight of 0 in 64 bits too: what is infinite there is a NaN.
+    world = Alike(kind, fmt, 2, SIZE, 16, 1024, count, new)
+    rng = np.random.default_rng(3)
+    world.fill(rng)
+    one = queries(world, 2)[0]
+    q = np.broadcast_to(np.repeat(one, heads // 2, 0), (world.tokens, heads, SIZE)).copy()
+    for at in range(32, 300, 16):
+        rows = 800.0 * one / (SCALE * (one ** 2).sum(1, keepdims=True))
+        world.put(world.slot(world.table[0], at + 2), 0, rows + 0.01 * rng.standard_normal(rows.shape))
+    for at, what in ((3, np.nan), (4, np.inf), (5, -np.inf)):
+        rows = rng.standard_normal((2, SIZE))
+        rows[:, 2 * at] = what
+        world.put(world.slot(world.table[0], at), 1, rows)
+    world.upload()
+    got = run(world, q, SCALE)
+    assert np.isnan(got[0][..., [6, 8, 10]]).all()
+    if fmt == lib.CACHE_PLAIN:
+        # One rounding of f16, and of 2^-25 at 2^6 what is below its numbers.
+        assert np.isfinite(got[0]).sum() == world.tokens * heads * (SIZE - 3)
+        check(world, q, got, {lib.F32: 0.0, lib.F16: 2.0**-11, lib.BF16: 2.0**-16}[kind])
+
+
 @pytest.mark.parametrize("kind", KINDS, ids=KIND_NAMES.get)
 @pytest.mark.parametrize("fmt", [lib.CACHE_PLAIN, lib.CACHE_INT8])
 @pytest.mark.parametrize("what", [np.inf, -np.inf, np.nan])
