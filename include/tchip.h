@@ -897,9 +897,9 @@ int tc_cache_read(const tc_cache* cache, const tc_cache_batch* batch, void* key,
  * queries and results.  `normalizers` [query_heads][tokens] (f32; may be null)
  * receives the log of each query's sum of exponentials.
  *   Sums and softmax are f32.  For the products with the values the weights are
- * rounded to f16 in f16; in bf16, and over 8-bit entries (times the values'
- * scales) in f16 too, to two parts of bf16, which keep 16 bits; in f32 not at
- * all.  A query that attends to nothing (a token in no sequence, or before its
+ * rounded to two parts: of f16 in f16, which keep 22 bits; of bf16 in bf16 and,
+ * times the values' scales, over 8-bit entries under 16-bit queries, which keep
+ * 16; in f32 not at all.  A query that attends to nothing (a token in no sequence, or before its
  * first) gets zeros and the normalizer -infinity.  Keys and values of no page
  * are zeros; no other row than those a query attends to reaches its result (of
  * those, an infinite value makes a NaN where its weight is 0).  A query all of

@@ -26,9 +26,10 @@
 // waves join at a part's end; where more do, the waves have 16 rows each and
 // share every tile (SHARED), so that keys are read and widened once for 64 rows.
 //
-// The weights are rounded to 16 bits for the products with the values: in f16
-// once (2^-11 of each), in bf16 in two parts, their rounding and the rounding of
-// what that leaves, which keep 16 bits; f32 keeps all.  8-bit entries, whole
+// For the products with the values the weights are taken in two parts where
+// those have 16 bits, their rounding and the rounding of what that leaves: bf16
+// keeps 16 bits so, f16 22; f32 keeps all.  (In f16 one part alone, 2^-11 of each
+// weight, took as long, and results in f16 were off by up to 1.4 times as much.)  8-bit entries, whole
 // numbers to 127 that every type holds, are widened to the queries' type for
 // the scores, which take the keys' scales afterwards.  The values' scales go
 // into the weights, so that under 16-bit queries weights and values are
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
     using TileOf = KeyTile<SIZE>;
     // The type that weights and values are multiplied in.
     using V = Weighed<QUANT>;
-    constexpr bool kTwoParts = sizeof(V) == 2 && Elem<V>::dtype == TC_BF16;
+    constexpr bool kTwoParts = sizeof(V) == 2;
     constexpr float kPower = power_of(QUANT);
     constexpr int kOperands = SIZE / kDeep16;
     constexpr int kEntry = QUANT ? 1 : static_cast<int>(sizeof(S));
