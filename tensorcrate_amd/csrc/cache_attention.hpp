@@ -29,11 +29,11 @@
 // For the products with the values the weights are taken in two parts where
 // those have 16 bits, their rounding and the rounding of what that leaves: bf16
 // keeps 16 bits so, f16 22; f32 keeps all.  (In f16 one part alone, 2^-11 of each
-// weight, took as long, and results in f16 were off by up to 1.4 times as much.)  8-bit entries, whole
-// numbers to 127 that every type holds, are widened to the queries' type for
-// the scores, which take the keys' scales afterwards.  The values' scales go
-// into the weights, so that under 16-bit queries weights and values are
-// multiplied as bf16 (`Weighed`).
+// weight, took as long, and results in f16 were off by up to 1.4 times as much.)
+// 8-bit entries, whole numbers to 127 that every type holds, are widened to the
+// queries' type for the scores, which take the keys' scales afterwards.  The
+// values' scales go into the weights, so that under 16-bit queries weights and
+// values are multiplied as bf16 (`Weighed`).
 //
 // Measured: 64 sequences to 8192 tokens, 32 heads on 8 of 128, bf16: 221 us (5.7
 // TB/s in the first kernel); 4 to 100000 in 8 bits 114 us; 24 to 3000 with 5 new
@@ -383,11 +383,6 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
             count_here = LineOf::count(a, s);
             cut = cut || s.length < s.tokens;
             mine += count_here;
-            // What is no block's item is said by the block whose turn the sequence is.
-            if (s.keys == 0 && n % gridDim.x == blockIdx.x) {
-                const uint64_t from = uint64_t{s.first} * a.query_heads, count = uint64_t{s.tokens} * a.query_heads;
-                for (uint64_t i = 0; i < count; i++) parts.found[from + i] = {1, 0, 0, 0};
-            }
         }
         if (sequences == 0 || a.batch.offsets != nullptr) {
             const uint64_t all = uint64_t{a.batch.tokens} * a.query_heads;
@@ -406,6 +401,16 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
         }
         if (lane == 63) sums[wave] = upto_here;
         cut = __syncthreads_or(cut);
+        if (cut || a.batch.most_pages == 0) {
+            // The rows of sequences without keys are no block's item: they are
+            // marked by the block whose turn the sequence is.
+            for (uint32_t n = blockIdx.x; n < sequences; n += gridDim.x) {
+                const Sequence s = sequence_at<false>(a, n);
+                if (s.keys != 0) continue;
+                const uint64_t from = uint64_t{s.first} * a.query_heads, count = uint64_t{s.tokens} * a.query_heads;
+                for (uint64_t i = threadIdx.x; i < count; i += kAttendThreads) parts.found[from + i] = {1, 0, 0, 0};
+            }
+        }
         for (int w = 0; w < kAttendWaves; w++) {
             if (w < wave) upto_here += sums[w];
             total_tiles += sums[w];

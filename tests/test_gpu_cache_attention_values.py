@@ -195,3 +195,16 @@ def test_weights_keep_their_bits(kind, fmt, lengths, new, prefix, heads):
     out, _, _ = generation.cache_attention(world, q, SCALE)
     half_step = ROUNDING[kind] * 2.0 ** np.floor(np.log2(np.abs(out)))
     assert ((got - out) ** 2).mean() ** 0.5 < 1.1 * (half_step ** 2 / 3).mean() ** 0.5
+
+
+@pytest.mark.parametrize("prefix", [0, 90])
+def test_a_prompt_without_pages_of_its_own(prefix):
+    # It sees the prefix alone, and where there is none nothing.
+    world = World(lib.BF16, lib.CACHE_PLAIN, 1, SIZE, 16, [0, 0], [700, 30], prefix, extra=0)
+    world.fill(np.random.default_rng(7))
+    world.lengths = [700, 30]
+    world.upload()
+    q = queries(world, 4)
+    got = run(world, q, SCALE)
+    attention_check(world, q, SCALE, got)
+    assert prefix or ((got[0] == 0).all() and (got[1] == -np.inf).all())
