@@ -801,10 +801,11 @@ typedef struct tc_rotary_shape {
  *   y = x / sqrt(mean of x^2 + epsilon) * weight
  * (or x itself without `normalize`), its pairs (a, b) turned to
  * (a cos - b sin, b cos + a sin), in f32 and rounded to `dtype` once.  The
- * weights, `head_size` elements for all heads of the queries and of the keys,
- * may each be null (1), and are refused without `normalize`.  The results may
- * take the operands' place (the same pointer with the same steps), and must
- * not otherwise overlap them. */
+ * squares too are f32: the norm of elements past 2^60, or without an epsilon
+ * below 2^-56, is not that of the formula.  The weights, `head_size` elements
+ * for all heads of the queries and of the keys, may each be null (1), and are
+ * refused without `normalize`.  The results may take the operands' place (the
+ * same pointer with the same steps), and must not otherwise overlap them. */
 int tc_rotary_norm(const tc_rotary_shape* shape, const void* query, const void* key, const void* query_weight,
                    const void* key_weight, void* query_out, void* key_out);
 
@@ -854,8 +855,8 @@ typedef struct tc_cache {
  * sequence's token j is at slot j % page_size of page
  * pages[s * most_pages + j / page_size].  Tokens before the first or past the
  * last offset are in no sequence.
- *   A page number of `page_count` or more is no page, and neither is one past
- * `most_pages`.
+ *   A page number of `page_count` or more is no page.  A sequence holds no more
+ * than its `most_pages` pages do: tokens behind them have no place.
  *   Where `prefix_length` is not 0, every sequence begins with that many tokens
  * more, the same for all and kept once, on the pages `prefix_pages`;
  * `lengths` and `pages` are those of the tokens behind it. */
@@ -896,16 +897,23 @@ int tc_cache_read(const tc_cache* cache, const tc_cache_batch* batch, void* key,
  * Element e of head h of token t is at t * token_step + h * head_step + e of
  * queries and results.  `normalizers` [query_heads][tokens] (f32; may be null)
  * receives the log of each query's sum of exponentials.
+ *   A query attends to nothing where its token is in no sequence, or comes
+ * before its sequence's first (the sequence's length being less than its tokens
+ * here) and there is no prefix: it gets zeros and the normalizer -infinity.
+ * Behind a prefix such a token attends to the part of it that ends as far
+ * before the prefix's end.  Keys and values on no page are zeros, which count;
+ * those past a sequence's `most_pages` pages are not attended to.  No other row
+ * than those a query attends to reaches its result; of those, an infinite value
+ * makes a NaN where its weight is 0.  A query all of whose scores are -infinity
+ * has the normalizer -infinity and, as 0 / 0, a NaN result.
  *   Sums and softmax are f32.  For the products with the values the weights are
- * rounded to two parts: of f16 in f16, which keep 22 bits; of bf16 in bf16 and,
- * times the values' scales, over 8-bit entries under 16-bit queries, which keep
- * 16; in f32 not at all.  A query that attends to nothing (a token in no sequence, or before its
- * first) gets zeros and the normalizer -infinity.  Keys and values of no page
- * are zeros; no other row than those a query attends to reaches its result (of
- * those, an infinite value makes a NaN where its weight is 0).  A query all of
- * whose scores are -infinity has the normalizer -infinity and, as 0 / 0, a NaN
- * result.  The order of every sum depends on the batch's counts and lengths
- * alone. */
+ * rounded to two parts: of f16 in f16, which keep 22 bits (and 2^-31 of the
+ * largest weight); of bf16 in bf16 and, times the values' scales, over 8-bit
+ * entries under 16-bit queries, which keep 16 (fewer under values below 2^-110);
+ * in f32 not at all.  A weight is at most 2^8 before the sums are divided: these
+ * are finite while the number of keys times the largest value times 2^8 is, and
+ * q . k, without the scale and in 8 bits without the entries' scales, has to be.
+ * The order of every sum depends on the batch's counts and lengths alone. */
 int tc_cache_attention(const tc_cache* cache, const tc_cache_batch* batch, uint32_t query_heads, float scale,
                        const void* query, uint64_t query_token_step, uint64_t query_head_step, void* out,
                        uint64_t out_token_step, uint64_t out_head_step, float* normalizers);

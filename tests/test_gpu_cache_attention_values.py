@@ -208,3 +208,24 @@ def test_a_prompt_without_pages_of_its_own(prefix):
     got = run(world, q, SCALE)
     attention_check(world, q, SCALE, got)
     assert prefix or ((got[0] == 0).all() and (got[1] == -np.inf).all())
+
+
+@pytest.mark.parametrize("fmt", [lib.CACHE_PLAIN, lib.CACHE_INT8])
+def test_keys_on_no_page_count_and_keys_behind_all_pages_do_not(fmt):
+    # A sequence of 48 tokens on two pages of 16 and one that is none, and with a
+    # table of the two alone.
+    world = World(lib.F32, fmt, 1, SIZE, 16, [32], [1], extra=0)
+    world.fill(np.random.default_rng(8))
+    q = queries(world, 2)
+    results, totals = [], []
+    for most in (3, 2):
+        world.table = np.concatenate([world.table[:, :2], np.full((1, most - 2), world.page_count, np.uint32)], 1)
+        world.most, world.lengths = most, [48]
+        world.upload()
+        got, normalizers = run(world, q, SCALE)
+        results.append(got[0])
+        totals.append(np.exp(normalizers))
+    # 16 keys of score 0 more, in f32: some 100 roundings of the sums.
+    assert np.abs(totals[0] - totals[1] - 16).max() < 100 * EPSILON_32 * totals[0].max()
+    sums = [r * t for r, t in zip(results, totals)]
+    assert np.abs(sums[0] - sums[1]).max() < 100 * EPSILON_32 * 4 * totals[0].max()  # values to 4
