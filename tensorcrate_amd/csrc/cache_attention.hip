@@ -7,9 +7,10 @@ namespace cache {
 namespace {
 
 // Whether blocks share tiles, where `rows` query rows share keys.  (320 rows over
-// a prefix of 8000 tokens in 8 bits: 41 us so, 59 with 16 rows a block.  4 or 5
-// rows the other way: 4 sequences to 100000 tokens 176 us instead of 114, heads
-// of 80 in f16 65 instead of 47.)
+// a prefix of 8000 tokens in 8 bits: 40 us so, 59 with 16 rows a block.  4 or 5
+// rows the other way: 4 sequences to 100000 tokens 176 us instead of 113, heads
+// of 80 in f16 65 instead of 47.)  For own keys it is the mean of a call's
+// sequences that tells: a prompt among many single tokens goes by these.
 bool shares(uint64_t rows) { return rows > 16; }
 
 // The storage of one line's parts.

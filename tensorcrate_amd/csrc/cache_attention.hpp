@@ -11,7 +11,9 @@
 // the few query heads that share a key head.  So the tiles of all sequences and
 // key heads are one line, cut evenly over as many waves as the chip holds,
 // whatever the lengths are (`Line`); parts of a sequence that lie in several
-// waves are joined by a second kernel.
+// waves are joined by a second kernel.  (Every block of a sequence's query rows
+// counts as all of its keys: of a prompt's first rows, which see few, most tiles
+// are passed over, so that for prompts the cut is not even.)
 //   A prefix that all sequences share is a line of its own, of as many blocks
 // of query rows as all tokens' heads fill: its keys are read once for each of
 // those and not for each sequence.
@@ -35,10 +37,11 @@
 // values' scales go into the weights, so that under 16-bit queries weights and
 // values are multiplied as bf16 (`Weighed`).
 //
-// Measured: 64 sequences to 8192 tokens, 32 heads on 8 of 128, bf16: 221 us (5.7
-// TB/s in the first kernel); 4 to 100000 in 8 bits 114 us; 24 to 3000 with 5 new
+// Measured: 64 sequences to 8192 tokens, 32 heads on 8 of 128, bf16: 220 us (5.7
+// TB/s in the first kernel); 4 to 100000 in 8 bits 113 us; 24 to 3000 with 5 new
 // tokens of 12 heads of 80, f16, 47; one of 1000 13, of which 4 are the join; 80
-// to 500 behind 8000 shared tokens in 8 bits 79 (own keys 33, prefix 41, join).
+// to 500 behind 8000 shared tokens in 8 bits 77 (own keys 31, prefix 40, join);
+// 512 new of 8704 tokens 159 us (445 TFLOP/s), a prompt of 2048 152.
 // With waves that each stored parts of their own, instead of joining in LDS, the
 // last case's own keys took 10 us less, and the longer ones more.
 #pragma once
@@ -55,7 +58,8 @@ constexpr int kAttendWaves = kAttendThreads / 64;
 // each and join at the end of a part, or of 64 rows, 16 a wave, that share each
 // tile (SHARED).
 constexpr uint32_t rows_of_form(bool shared) { return shared ? 64 : 16; }
-// Blocks of a compute unit at a time, as registers allow.
+// Blocks of a compute unit at a time.  (Registers just allow them: over plain
+// entries of 65 elements and more a lane keeps 2 to 17 values in memory.)
 constexpr uint32_t blocks_of_form(bool shared) { return shared ? 3 : 2; }
 
 // One launch's operands.

@@ -229,3 +229,19 @@ def test_keys_on_no_page_count_and_keys_behind_all_pages_do_not(fmt):
     assert np.abs(totals[0] - totals[1] - 16).max() < 100 * EPSILON_32 * totals[0].max()
     sums = [r * t for r, t in zip(results, totals)]
     assert np.abs(sums[0] - sums[1]).max() < 100 * EPSILON_32 * 4 * totals[0].max()  # values to 4
+
+
+@pytest.mark.parametrize("kind", [lib.F32, lib.BF16], ids=KIND_NAMES.get)
+@pytest.mark.parametrize("fmt", [lib.CACHE_PLAIN, lib.CACHE_INT8])
+@pytest.mark.parametrize("power", [-100, 100])
+def test_values_near_the_ends_of_the_range(kind, fmt, power):
+    # 100 keys of values to some 2^102, times the weights' 2^8: below 2^117.
+    world = World(kind, fmt, 1, SIZE, 16, [100, 17], [2, 1])
+    rng = np.random.default_rng(9)
+    world.fill(rng)
+    for s, n in enumerate(world.lengths):
+        for at in range(n):
+            world.put(world.slot(world.table[s], at), 1, rng.standard_normal((1, SIZE)) * 2.0**power)
+    world.upload()
+    q = queries(world, 2)
+    check(world, q, run(world, q, SCALE), WEIGHT[kind])
