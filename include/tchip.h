@@ -907,7 +907,7 @@ int tc_cache_read(const tc_cache* cache, const tc_cache_batch* batch, void* key,
  * makes a NaN where its weight is 0.  A query all of whose scores are -infinity
  * has the normalizer -infinity and, as 0 / 0, a NaN result.
  *   Sums and softmax are f32.  For the products with the values the weights are
- * rounded to two parts: of f16 in f16, which keep 22 bits (and 2^-31 of the
+ * rounded to two parts: of f16 in f16, which keep 21 bits (and 2^-31 of the
  * largest weight); of bf16 in bf16 and, times the values' scales, over 8-bit
  * entries under 16-bit queries, which keep 16 (fewer under values below 2^-110);
  * in f32 not at all.  A weight is at most 2^8 before the sums are divided: these

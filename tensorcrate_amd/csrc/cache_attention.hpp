@@ -29,9 +29,10 @@
 // share every tile (SHARED), so that keys are read and widened once for 64 rows.
 //
 // For the products with the values the weights are taken in two parts where
-// those have 16 bits, their rounding and the rounding of what that leaves: bf16
-// keeps 16 bits so, f16 22; f32 keeps all.  (In f16 one part alone, 2^-11 of each
-// weight, took as long, and results in f16 were off by up to 1.4 times as much.)
+// those have 16 bits, 16 bits of each and the rounding of what that leaves: bf16
+// keeps 16 bits so, f16 21; f32 keeps all.  (In f16 one part alone, 2^-11 of each
+// weight, took 155 instead of 170 us for 512 new of 8704 tokens, and as long
+// where memory bounds; results in f16 were off by up to 1.4 times as much.)
 // 8-bit entries, whole numbers to 127 that every type holds, are widened to the
 // queries' type for the scores, which take the keys' scales afterwards.  The
 // values' scales go into the weights, so that under 16-bit queries weights and
@@ -41,7 +42,7 @@
 // TB/s in the first kernel); 4 to 100000 in 8 bits 113 us; 24 to 3000 with 5 new
 // tokens of 12 heads of 80, f16, 47; one of 1000 13, of which 4 are the join; 80
 // to 500 behind 8000 shared tokens in 8 bits 77 (own keys 31, prefix 40, join);
-// 512 new of 8704 tokens 159 us (445 TFLOP/s), a prompt of 2048 152.
+// 512 new of 8704 tokens 163 us (435 TFLOP/s), a prompt of 2048 155.
 // With waves that each stored parts of their own, instead of joining in LDS, the
 // last case's own keys took 10 us less, and the longer ones more.
 #pragma once
@@ -59,7 +60,7 @@ constexpr int kAttendWaves = kAttendThreads / 64;
 // tile (SHARED).
 constexpr uint32_t rows_of_form(bool shared) { return shared ? 64 : 16; }
 // Blocks of a compute unit at a time.  (Registers just allow them: over plain
-// entries of 65 elements and more a lane keeps 2 to 17 values in memory.)
+// entries of 65 elements and more a lane keeps 2 to 16 values in memory.)
 constexpr uint32_t blocks_of_form(bool shared) { return shared ? 3 : 2; }
 
 // One launch's operands.
@@ -729,7 +730,17 @@ __global__ void __launch_bounds__(kAttendThreads) __attribute__((amdgpu_waves_pe
                 }
             }
             Words<V, E> high_part, low_part;
-            high_part.put(v);
+            if constexpr (Elem<V>::dtype == TC_F16) {
+                // Cut off, two by one instruction: the second part takes what is
+                // left (512 new of 8704 tokens 170 us so, 181 rounded).
+                uint32_t* const to = reinterpret_cast<uint32_t*>(high_part.w);
+#pragma unroll
+                for (int e = 0; e < E; e += 2) {
+                    to[e / 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(v[e], v[e + 1]));
+                }
+            } else {
+                high_part.put(v);
+            }
             if constexpr (kTwoParts) {
 #pragma unroll
                 for (int e = 0; e < E; e++) v[e] -= high_part.at(e);
